@@ -296,6 +296,77 @@ int vitk_fourier_features_bwd(const float* grid, const float* w, const void* g, 
  * aligned).  Called with the dropped samples before the residual epilogue (or the norm backward) writes the kept ones. */
 int vitk_copy_samples(const void* src, void* dst, const int64_t* idx, int64_t n, int64_t sample_bytes, void* stream);
 
+/* ---- per-head normalisation of q and k with the rotation in the same pass ---------------------------------------------
+ * vit/attention.py:25-41 (applied at :95-105) followed by vit/rope.py:139-163, and the backward of the two together.
+ *   xhat = (x - mean) * rstd (RMSNorm: mean 0, eps inside the root), n = xhat * w (+ b),
+ *   y = n cos + rotate_half(n) sin for the rows l >= prefix of every sample, y = n for the others (all, without a table).
+ * A section is q or k: heads addressed as ptr[b*sb + l*ss + h*sh + d], d contiguous; sec[1].w = NULL: one section only.
+ * fwd reads x and writes y (may be x itself).  bwd reads x and g = dL/dy and writes y = dL/dx (may be g itself) and the
+ * weight gradients dw / db [Dh] (NULL where not wanted), summed in a fixed order through `workspace`.
+ * head_dim: a multiple of 8, at most 128; strides: multiples of 4 elements, pointers aligned to 4 elements.
+ * round_norm = 1 rounds n (backward: the un-rotated gradient) to the tensors' dtype between the two steps, and
+ * emulate_bf16 = 1 rounds the products of the rotation to bf16, as separate passes do; 0: one rounding, at the store. */
+typedef struct VitkQkSection {
+  const void *x, *g;
+  void* y;
+  const void *w, *b;            /* [Dh], w_dtype; b NULL without a bias */
+  void *dw, *db;
+  const float* table;           /* [2, (B,) L - prefix, Dh] sin, cos; 16-byte aligned; or NULL */
+  int64_t x_sb, x_ss, x_sh, g_sb, g_ss, g_sh, y_sb, y_ss, y_sh;
+  int64_t L, H, prefix;
+  int32_t per_sample;           /* 1: one table per sample */
+  int32_t reserved;
+} VitkQkSection;
+typedef struct VitkQkNormRope {
+  VitkQkSection sec[2];
+  int64_t B, Dh;
+  void* workspace;              /* bwd with dw / db: vitk_qk_norm_rope_workspace_bytes */
+  float eps;
+  int32_t dtype, w_dtype, is_layernorm, round_norm, emulate_bf16;
+} VitkQkNormRope;
+size_t vitk_qk_norm_rope_workspace_bytes(const VitkQkNormRope* a);
+int vitk_qk_norm_rope_fwd(const VitkQkNormRope* a, void* stream);
+int vitk_qk_norm_rope_bwd(const VitkQkNormRope* a, void* stream);
+
+/* ---- attention with a learned relative position bias and / or per-sample key counts -----------------------------------
+ * No counterpart in the reference, whose attention functions take an attn_mask that its layers never pass
+ * (vit/attention.py:177, :233).
+ *   S[i,j] = scale * q_i k_j + table[index[i,j], h],  j < kv_len[b];   P = softmax(S) (dropout on P);   o_i = sum_j P v_j
+ * bias_table [num_buckets, H] and bias_index [Lq, Lk] may be NULL (no bias), kv_len [B] may be NULL (all Lk keys); counts
+ * are clamped to [0, Lk].  Keys at or beyond the count are never read; their dk and dv are written as zeros.  A row that
+ * has no key left, or only keys with a bias of -inf, gives o = 0 and zero gradients (lse = +inf).  Finite table entries
+ * beyond +-1e37 count as +-1e37.
+ * Every operand has (batch, head, row) strides of its own, d contiguous.  head_dim <= 128.
+ * bwd: dbias_table [num_buckets, H] (or NULL) is summed over the pairs of a bucket in a fixed order given by the plan
+ * order / piece / bucket_piece: `order` holds the pair numbers i * Lk + j sorted by bucket, piece p covers order[piece[p]
+ * .. piece[p+1]) inside one bucket, bucket n owns the pieces bucket_piece[n] .. bucket_piece[n+1).
+ * workspace: vitk_attn_var_workspace_bytes(a, bwd), 256-byte aligned; nothing in it outlives the call. */
+typedef struct VitkAttnVar {
+  const void *q, *k, *v;
+  void* o;
+  const void* dout;
+  void *dq, *dk, *dv;
+  float* lse;                   /* [B, H, Lq] */
+  const int32_t* kv_len;
+  const void* bias_table;       /* [num_buckets, H], dtype */
+  const uint16_t* bias_index;   /* [Lq, Lk] */
+  void* dbias_table;
+  const int32_t *order, *piece, *bucket_piece;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t B, H, Lq, Lk, Dh, num_buckets, num_pieces;
+  int64_t st[24];               /* sb, sh, ss of q, k, v, o, dout, dq, dk, dv */
+  uint64_t seed;
+  float scale, drop_p;
+  int32_t dtype;
+  int32_t dbias_dtype;          /* of dbias_table */
+  int32_t algo;                 /* 0 auto, 1 portable, 2 MFMA */
+  int32_t reserved;
+} VitkAttnVar;
+size_t vitk_attn_var_workspace_bytes(const VitkAttnVar* a, int bwd);
+int vitk_attn_var_fwd(const VitkAttnVar* a, void* stream);
+int vitk_attn_var_bwd(const VitkAttnVar* a, void* stream);
+
 /* Diagnostics (no counterpart in the reference): `blocks` idle workgroups that hold their CUs for about `cycles` shader
  * clocks, to measure what a launch loses when another stream's kernel occupies part of the chip. */
 int vitk_debug_hold_cus(int blocks, long long cycles, void* stream);

@@ -1,0 +1,217 @@
+"""Host side of the relative position bias, the key counts and the per-head normalisation pass: bucket plans against brute
+force, and the refusals, which need no GPU."""
+import ctypes
+import itertools
+import math
+import os
+import re
+
+import pytest
+import torch
+
+from vit_amd import KVMemory, RelativeBuckets, ViTConfig, _lib, qk_norm_rope
+from vit_amd.attention import CrossAttention, SelfAttention, attention
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def unsigned(index16):
+    return index16.to(torch.int64) & 0xFFFF
+
+
+@pytest.mark.parametrize("shape,nb", [((1, 1), 1), ((3, 5), 7), ((40, 61), 3), ((200, 300), 65536)])
+def test_plan_covers_every_pair_once_in_bucket_order(shape, nb):
+    g = torch.Generator().manual_seed(shape[0])
+    idx = torch.randint(0, nb, shape, generator=g)
+    if nb > 1000:
+        idx[0, 0] = nb - 1   # a number that does not fit a signed 16-bit integer
+    plan = RelativeBuckets(idx, nb)
+    assert plan.shape == shape and plan.num_buckets == nb
+    assert torch.equal(unsigned(plan.index16), idx)
+    order = plan.order.long()
+    assert torch.equal(order.sort().values, torch.arange(idx.numel()))
+    flat = idx.reshape(-1)
+    assert torch.equal(plan.piece[[0, -1]].long(), torch.tensor([0, idx.numel()])) and plan.piece.numel() == plan.num_pieces + 1
+    assert plan.bucket_piece.numel() == nb + 1 and int(plan.bucket_piece[-1]) == plan.num_pieces
+    sizes = plan.piece.diff()
+    assert int(sizes.min()) >= 1 and int(sizes.max()) <= RelativeBuckets.PIECE
+    used = torch.unique(flat).tolist()
+    for n in used[:50]:
+        a, b = int(plan.bucket_piece[n]), int(plan.bucket_piece[n + 1])
+        mine = order[int(plan.piece[a]):int(plan.piece[b])]
+        assert torch.equal(mine, (flat == n).nonzero()[:, 0])   # all pairs of the bucket, in rising order
+    for n in set(range(min(nb, 50))) - set(used):
+        assert plan.bucket_piece[n] == plan.bucket_piece[n + 1]
+
+
+@pytest.mark.parametrize("dims,prefix,table", [((3, 4), 0, None), ((3, 4), 2, None), ((5,), 1, None), ((2, 3, 2), 0, (4, 3, 3)), ((1, 1), 1, None)])
+def test_grid_buckets_are_one_per_offset(dims, prefix, table):
+    plan = RelativeBuckets.grid(dims, prefix, table_dims=table)
+    idx = unsigned(plan.index16)
+    n = math.prod(dims)
+    assert plan.shape == (n + prefix,) * 2
+    table = table or dims
+    assert plan.num_buckets == math.prod(2 * t - 1 for t in table) + (3 if prefix else 0)
+    pos = list(itertools.product(*[range(d) for d in dims]))
+    seen = {}
+    for i, a in enumerate(pos):
+        for j, b in enumerate(pos):
+            off = tuple(x - y for x, y in zip(a, b))
+            assert seen.setdefault(off, int(idx[prefix + i, prefix + j])) == int(idx[prefix + i, prefix + j])
+    assert len(set(seen.values())) == len(seen)   # different offsets, different buckets
+    if prefix:
+        special = {int(idx[0, prefix]), int(idx[prefix, 0]), int(idx[0, 0])}
+        assert len(special) == 3 and not special & set(seen.values())
+        assert bool((idx[:prefix, prefix:] == idx[0, prefix]).all()) and bool((idx[prefix:, :prefix] == idx[prefix, 0]).all())
+
+
+def test_log_distance_buckets():
+    plan = RelativeBuckets.log_distance(50, 400, num_buckets=32, max_distance=128)
+    idx = unsigned(plan.index16)
+    assert plan.num_buckets == 32
+    for d in range(8):   # the first half of the buckets are single distances
+        assert int(idx[49, 49 - d]) == d and (d == 0 or int(idx[0, d]) == 16 + d)
+    # 8 further buckets grow by (128 / 8)^(1/8) each: their borders, by hand
+    for d in range(8, 400):
+        want = min(15, 8 + sum(d >= 8 * 16 ** (k / 8) - 1e-6 for k in range(1, 9)))
+        assert int(idx[0, d]) == 16 + want, d
+    assert bool((idx[0, 1:].diff() >= 0).all())
+
+
+def test_plan_refusals():
+    with pytest.raises(ValueError, match=r"\[0, 4\)"):
+        RelativeBuckets(torch.tensor([[0, 4]]), 4)
+    with pytest.raises(ValueError, match=r"\[0, 4\)"):
+        RelativeBuckets(torch.tensor([[-1, 3]]), 4)
+    with pytest.raises(ValueError, match="empty"):
+        RelativeBuckets(torch.zeros((0, 3), dtype=torch.int64), 4)
+    with pytest.raises(ValueError, match="num_buckets"):
+        RelativeBuckets(torch.zeros((1, 3), dtype=torch.int64), 65537)
+    with pytest.raises(ValueError, match="integer"):
+        RelativeBuckets(torch.zeros((1, 3)), 4)
+    with pytest.raises(ValueError, match="integer"):
+        RelativeBuckets(torch.zeros((3,), dtype=torch.int64), 4)
+    with pytest.raises(ValueError, match="cover"):
+        RelativeBuckets.grid((5, 5), table_dims=(4, 5))
+    with pytest.raises(ValueError, match="multiple of 4"):
+        RelativeBuckets.log_distance(4, 4, num_buckets=6)
+
+
+def test_attention_refusals():
+    q, k = torch.zeros(2, 3, 4, 8), torch.zeros(2, 5, 4, 8)
+    plan = RelativeBuckets(torch.zeros((3, 5), dtype=torch.int64), 2)
+    table = torch.zeros(2, 4)
+    bad = [
+        (dict(q=q[0]), "must be"), (dict(k=torch.zeros(2, 5, 2, 8)), "go with"), (dict(k=torch.zeros(3, 5, 4, 8)), "go with"),
+        (dict(v=torch.zeros(2, 6, 4, 8)), "differ"), (dict(bias_table=table), "both"), (dict(buckets=plan), "both"),
+        (dict(bias_table=torch.zeros(3, 4), buckets=plan), "bias_table must be"),
+        (dict(bias_table=table, buckets=RelativeBuckets(torch.zeros((5, 3), dtype=torch.int64), 2)), "buckets cover"),
+        (dict(kv_lengths=torch.zeros(3, dtype=torch.int32)), "kv_lengths"), (dict(kv_lengths=[1, 2]), "kv_lengths"),
+        (dict(kv_lengths=torch.zeros(2)), "kv_lengths"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
+        (dict(dropout=1.0, training=True), "dropout"), (dict(q=torch.zeros(2, 3, 4, 136), k=torch.zeros(2, 5, 4, 136)), "head_dim"),
+    ]
+    for change, match in bad:
+        kw = dict(q=q, k=k, v=None) | change
+        kw["v"] = kw["k"] if kw["v"] is None else kw["v"]
+        with pytest.raises(ValueError, match=match):
+            attention(**kw)
+    with pytest.raises(TypeError, match="float16"):
+        attention(q.half(), k.half(), k.half())
+    with pytest.raises(TypeError, match="queries"):
+        attention(q, k.bfloat16(), k.bfloat16())
+    with pytest.raises(RuntimeError, match="no CPU fallback|MI355X"):
+        attention(q, k, k)
+
+
+def test_qk_norm_rope_refusals():
+    q, w = torch.zeros(2, 3, 4, 16), torch.ones(16)
+    for kw, match in [(dict(q=torch.zeros(2, 3, 4, 12), w=torch.ones(12)), "multiples of 8"), (dict(w=torch.ones(8)), "q_norm_weight"),
+                      (dict(k=q), "k_norm_weight"), (dict(rope_q=torch.zeros(2, 4, 16)), "rope_q"),
+                      (dict(rope_q=torch.zeros(2, 3, 1, 2, 16)), "rope_q"), (dict(eps=-1.0), "eps"),
+                      (dict(q_norm_bias=torch.zeros(16, dtype=torch.bfloat16)), "q_norm_bias")]:
+        kw = dict(kw)
+        with pytest.raises(ValueError, match=match):
+            qk_norm_rope(kw.pop("q", q), kw.pop("k", None), kw.pop("w", w), **kw)
+    with pytest.raises(RuntimeError, match="no CPU fallback|MI355X"):
+        qk_norm_rope(q, None, w)
+
+
+def test_layer_refusals():
+    x = torch.zeros(1, 5, 32)
+    plan = RelativeBuckets(torch.zeros((5, 5), dtype=torch.int64), 3)
+    with pytest.raises(ValueError, match="relative position bias"):
+        SelfAttention(32, 2, relative_buckets=3)(x)
+    with pytest.raises(ValueError, match="relative position bias"):
+        SelfAttention(32, 2)(x, buckets=plan)
+    with pytest.raises(ValueError, match="sequence of 4"):
+        SelfAttention(32, 2, relative_buckets=3)(x[:, :4], buckets=plan)
+    with pytest.raises(NotImplementedError, match="relative"):
+        SelfAttention(32, 2, relative_buckets=3).forward_weights(x)
+    layer = CrossAttention(32, 2).eval()
+    memory = KVMemory(torch.zeros(1, 7, 2, 2, 16), None)
+    with torch.no_grad(), pytest.raises(ValueError, match="project_kv"):
+        layer(x, memory, kv_lengths=torch.tensor([1]))
+    with torch.no_grad(), pytest.raises(ValueError, match="go with"):
+        layer(x, KVMemory(torch.zeros(2, 7, 2, 2, 16), None))
+    with pytest.raises(RuntimeError, match="inference"):
+        layer(x, memory)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="inference"):
+        layer.train()(x, memory)
+    with pytest.raises(ValueError, match="kv_lengths"):
+        layer(x, x, kv_lengths=torch.tensor([1, 2]))
+
+
+def test_relative_vit_has_a_table_per_block_and_refuses_masks():
+    cfg = ViTConfig(in_channels=3, patch_size=(8, 8), img_size=(32, 24), depth=2, hidden_size=64, ffn_hidden_size=128,
+                    num_attention_heads=2, num_register_tokens=2, pos_enc="relative", dtype=torch.float32)
+    model = cfg.instantiate()
+    names = [n for n in model.state_dict() if "relative" in n]
+    assert names == [f"blocks.{i}.self_attention.relative_bias" for i in range(2)]
+    assert tuple(model.state_dict()[names[0]].shape) == (7 * 5 + 3, 2)
+    assert ViTConfig.from_yaml(cfg.to_yaml()) == cfg
+    assert model.prepare_buckets((4, 3)).shape == (14, 14)
+    assert model.prepare_buckets((2, 3)).num_buckets == 38 and model.prepare_buckets((4, 3)) is model.prepare_buckets((4, 3))
+    with pytest.raises(ValueError, match="cover"):
+        model.prepare_buckets((5, 3))
+    with pytest.raises(NotImplementedError, match="masks"):
+        model(torch.zeros(1, 3, 32, 24), mask=torch.ones(1, 12, dtype=torch.bool))
+    assert not [n for n in ViTConfig(**{**cfg.__dict__, "pos_enc": "rope"}).instantiate().state_dict() if "relative" in n]
+
+
+@pytest.mark.parametrize("cname", ["VitkQkSection", "VitkQkNormRope", "VitkAttnVar"])
+def test_descriptor_layout_matches_the_header(cname):
+    header = open(os.path.join(ROOT, "include", "vitk.h")).read()
+    body = header[header.index(f"typedef struct {cname} {{"):header.index(f"}} {cname};")]
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    names = []
+    for stmt in body.split("{", 1)[1].split(";"):
+        if stmt.strip():
+            names += [re.sub(r"\[\d+\]|[*\s]", "", piece.split()[-1]) for piece in stmt.split(",")]
+    assert names == [f[0] for f in getattr(_lib, cname)._fields_]
+
+
+def test_entry_points_refuse_bad_descriptors():
+    """Errors of the C entry points come back as a code and a text; nothing is launched for them."""
+    lib = _lib.load()
+
+    def err(rc):
+        return lib.vitk_last_error().decode() if rc else ""
+
+    a = _lib.VitkAttnVar()
+    a.B, a.H, a.Lq, a.Lk, a.Dh, a.scale = 1, 1, 1, 1, 129, 1.0
+    assert "bad shape" in err(lib.vitk_attn_var_fwd(ctypes.byref(a), None)) and "null" in err(lib.vitk_attn_var_fwd(None, None))
+    a.Dh = 64
+    assert "null pointer" in err(lib.vitk_attn_var_fwd(ctypes.byref(a), None))
+    a.Lq = 1 << 22
+    assert "at most" in err(lib.vitk_attn_var_bwd(ctypes.byref(a), None))
+    a.Lq, a.scale = 1, 0.0
+    assert "scale" in err(lib.vitk_attn_var_fwd(ctypes.byref(a), None))
+    a.scale, a.drop_p = 1.0, 1.0
+    assert "dropout" in err(lib.vitk_attn_var_fwd(ctypes.byref(a), None))
+    a.drop_p, a.dtype = 0.0, 7
+    assert "dtype" in err(lib.vitk_attn_var_fwd(ctypes.byref(a), None))
+    n = _lib.VitkQkNormRope()
+    n.B, n.Dh = 1, 20
+    assert "multiple of 8" in err(lib.vitk_qk_norm_rope_fwd(ctypes.byref(n), None)) and "null" in err(lib.vitk_qk_norm_rope_bwd(None, None))
+    n.Dh = 16
+    assert "null pointer" in err(lib.vitk_qk_norm_rope_fwd(ctypes.byref(n), None))

@@ -5,10 +5,13 @@
     tokens = model(x).visual_tokens                        # every kernel in forward/backward is libvitk.so
 
 Importing the package does not load the extension; the first kernel call does, and raises if it is missing."""
+from .attention import KVMemory, qk_norm_rope
 from .config import ViTConfig
 from .features import ViTFeatures
 from .head import AttentivePoolHead, AttentivePoolHeadConfig, Head, HeadConfig
+from .pos_enc import RelativeBuckets
 from .vit import ViT
 
-__all__ = ["ViT", "ViTConfig", "ViTFeatures", "Head", "HeadConfig", "AttentivePoolHead", "AttentivePoolHeadConfig"]
+__all__ = ["ViT", "ViTConfig", "ViTFeatures", "Head", "HeadConfig", "AttentivePoolHead", "AttentivePoolHeadConfig",
+           "RelativeBuckets", "KVMemory", "qk_norm_rope"]
 __version__ = "0.1.0"

@@ -22,6 +22,8 @@ EXPORTS = [
     "vitk_act_bwd", "vitk_im2col", "vitk_col2im", "vitk_colsum", "vitk_colsum_static", "vitk_colsum_workspace_bytes", "vitk_scale_cast",
     "vitk_scale_cast_dgamma", "vitk_scale_cast_dgamma_workspace_bytes",
     "vitk_prefix_fill", "vitk_copy_samples", "vitk_fourier_features", "vitk_fourier_features_bwd",
+    "vitk_qk_norm_rope_fwd", "vitk_qk_norm_rope_bwd", "vitk_qk_norm_rope_workspace_bytes",
+    "vitk_attn_var_fwd", "vitk_attn_var_bwd", "vitk_attn_var_workspace_bytes",
 ]
 
 
@@ -62,6 +64,38 @@ class VitkAttn(C.Structure):
     ]
 
 
+class VitkQkSection(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("g", C.c_void_p), ("y", C.c_void_p), ("w", C.c_void_p), ("b", C.c_void_p),
+        ("dw", C.c_void_p), ("db", C.c_void_p), ("table", C.c_void_p),
+        ("x_sb", C.c_int64), ("x_ss", C.c_int64), ("x_sh", C.c_int64), ("g_sb", C.c_int64), ("g_ss", C.c_int64),
+        ("g_sh", C.c_int64), ("y_sb", C.c_int64), ("y_ss", C.c_int64), ("y_sh", C.c_int64),
+        ("L", C.c_int64), ("H", C.c_int64), ("prefix", C.c_int64), ("per_sample", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class VitkQkNormRope(C.Structure):
+    _fields_ = [
+        ("sec", VitkQkSection * 2), ("B", C.c_int64), ("Dh", C.c_int64), ("workspace", C.c_void_p), ("eps", C.c_float),
+        ("dtype", C.c_int32), ("w_dtype", C.c_int32), ("is_layernorm", C.c_int32), ("round_norm", C.c_int32),
+        ("emulate_bf16", C.c_int32),
+    ]
+
+
+class VitkAttnVar(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("dout", C.c_void_p),
+        ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("lse", C.c_void_p), ("kv_len", C.c_void_p),
+        ("bias_table", C.c_void_p), ("bias_index", C.c_void_p), ("dbias_table", C.c_void_p),
+        ("order", C.c_void_p), ("piece", C.c_void_p), ("bucket_piece", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("B", C.c_int64), ("H", C.c_int64), ("Lq", C.c_int64), ("Lk", C.c_int64), ("Dh", C.c_int64),
+        ("num_buckets", C.c_int64), ("num_pieces", C.c_int64), ("st", C.c_int64 * 24),
+        ("seed", C.c_uint64), ("scale", C.c_float), ("drop_p", C.c_float),
+        ("dtype", C.c_int32), ("dbias_dtype", C.c_int32), ("algo", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
 _lib: Optional[C.CDLL] = None
 
 
@@ -84,6 +118,11 @@ def load() -> C.CDLL:
         getattr(lib, name).argtypes = [C.c_int64]
     lib.vitk_gemm_workspace_bytes.restype = C.c_size_t
     lib.vitk_gemm_workspace_bytes.argtypes = [C.POINTER(VitkGemm)]
+    if hasattr(lib, "vitk_attn_var_fwd"):
+        lib.vitk_qk_norm_rope_workspace_bytes.restype = C.c_size_t
+        lib.vitk_qk_norm_rope_workspace_bytes.argtypes = [C.POINTER(VitkQkNormRope)]
+        lib.vitk_attn_var_workspace_bytes.restype = C.c_size_t
+        lib.vitk_attn_var_workspace_bytes.argtypes = [C.POINTER(VitkAttnVar), C.c_int]
     vp, i32, i64, f32, u64 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_uint64
     sigs = {
         "vitk_norm_fwd": [vp, i32, vp, vp, i32, vp, i32, vp, vp, vp, i64, i64, f32, i32, vp],
@@ -93,6 +132,10 @@ def load() -> C.CDLL:
         "vitk_attn_fwd": [C.POINTER(VitkAttn), vp],
         "vitk_attn_bwd": [C.POINTER(VitkAttn), vp],
         "vitk_attn_weights": [C.POINTER(VitkAttn), vp, vp],
+        "vitk_qk_norm_rope_fwd": [C.POINTER(VitkQkNormRope), vp],
+        "vitk_qk_norm_rope_bwd": [C.POINTER(VitkQkNormRope), vp],
+        "vitk_attn_var_fwd": [C.POINTER(VitkAttnVar), vp],
+        "vitk_attn_var_bwd": [C.POINTER(VitkAttnVar), vp],
         "vitk_debug_hold_cus": [i32, C.c_longlong, vp],
         "vitk_rope_qk": [vp, i32, vp, i64, i64, i64, i64, i64, i32, i32, i32, vp],
         "vitk_rope_rows": [vp, i32, vp, i64, i64, i64, i64, i64, i64, i64, i32, i32, i32, vp],

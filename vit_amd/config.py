@@ -1,6 +1,7 @@
 """ViTConfig: the reference's configuration dataclass, field for field (vit/vit.py:67-152), including the
 YAML round trip and the validation errors.  ``rope_normalize_coords`` is kept although the reference never
-forwards it to the RoPE module (vit/vit.py:284-292): the model always uses "separate"."""
+forwards it to the RoPE module (vit/vit.py:284-292): the model always uses "separate".  ``pos_enc`` takes one value the
+reference does not have: "relative", a learned relative position bias in every block's attention."""
 from __future__ import annotations
 
 from dataclasses import dataclass, field

@@ -1,0 +1,428 @@
+// Attention with a learned relative position bias and / or a key count per sample, forward and backward.
+//
+//   S = scale Q K^T + T[bucket(i, j), h] over the keys j < len(b),  P = softmax(S),  O = P V
+//   dV = P^T dO,  dP = dO V^T,  dS = P (dP - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q,
+//   dT[n, h] = sum over samples and over the pairs (i, j) of bucket n of dS
+//
+// Portable kernels (any dtype, head_dim <= 128, any strides, fp32 math): 64 stationary rows per workgroup, 4 threads per row.
+#include "attn_tile.h"
+
+struct VarP {
+  const void *q, *k, *v, *dout;
+  void *o, *dq, *dk, *dv;
+  float *lse, *delta;
+  const int32_t* kv_len;
+  const void* table;
+  const uint16_t* index;
+  float* dbias;   // [splits][H][Lq][Lk]
+  int64_t q_sb, q_sh, q_ss, k_sb, k_sh, k_ss, v_sb, v_sh, v_ss, o_sb, o_sh, o_ss, g_sb, g_sh, g_ss;
+  int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
+  int B, H, Lq, Lk, Dh;
+  uint64_t seed;
+  float scale, keep_scale;
+  uint32_t thr;
+};
+
+__device__ __forceinline__ int key_count(const VarP& p, int64_t b) {
+  if (!p.kv_len) return p.Lk;
+  const int n = p.kv_len[b];
+  return n < 0 ? 0 : n > p.Lk ? p.Lk : n;
+}
+// Finite entries beyond +-1e37 are pulled in so that a bias keeps its order against the scores after the multiplication by
+// 1 / scale; -inf, +inf and NaN pass.
+__device__ __forceinline__ float clamp_bias(float x) {
+  const float a = fabsf(x);
+  return a > 1e37f && a < INFINITY ? copysignf(1e37f, x) : x;
+}
+// dropout counter of (row, key): as in attn.hip, row * (Lk rounded up to even) + key
+__device__ __forceinline__ uint64_t var_drop_ld(const VarP& p) { return (uint64_t)((p.Lk + 1) & ~1); }
+
+constexpr int VMAXI = 32;  // head_dim <= 128
+constexpr int VT = 32;     // streamed rows per LDS tile
+
+template <class T>
+__device__ __forceinline__ void vload_tile(float* dst, const T* src, int64_t ss, int64_t row0, int64_t nrows, int Dh, int tid) {
+  for (int i = tid; i < VT * Dh; i += 256) {
+    const int r = i / Dh, d = i % Dh;
+    dst[i] = (row0 + r < nrows) ? to_f<T>(src[(row0 + r) * ss + d]) : 0.f;
+  }
+}
+__device__ __forceinline__ float vquad_sum(float v) {
+  v += __shfl_xor(v, 1, 64);
+  v += __shfl_xor(v, 2, 64);
+  return v;
+}
+template <class T> __device__ __forceinline__ float var_bias(const VarP& p, int64_t i, int64_t j, int64_t h) {
+  return p.table ? clamp_bias(to_f<T>(((const T*)p.table)[(int64_t)p.index[i * p.Lk + j] * p.H + h])) : 0.f;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void var_fwd_simple_k(VarP p) {
+  extern __shared__ __attribute__((aligned(16))) float sm[];
+  const int Dh = p.Dh, tid = threadIdx.x, part = tid & 3;
+  const int64_t b = blockIdx.z, h = blockIdx.y, qrow = (int64_t)blockIdx.x * 64 + (tid >> 2);
+  float* Ks = sm;
+  float* Vs = sm + VT * Dh;
+  const T* qp = (const T*)p.q + b * p.q_sb + h * p.q_sh;
+  const T* kp = (const T*)p.k + b * p.k_sb + h * p.k_sh;
+  const T* vp = (const T*)p.v + b * p.v_sb + h * p.v_sh;
+  const bool qv = qrow < p.Lq;
+  const int len = key_count(p, b);
+  float q[VMAXI], o[VMAXI];
+#pragma unroll
+  for (int i = 0; i < VMAXI; i++) {
+    const int d = part + 4 * i;
+    q[i] = (qv && d < Dh) ? to_f<T>(qp[qrow * p.q_ss + d]) : 0.f;
+    o[i] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  const int64_t srow = (b * p.H + h) * p.Lq + qrow;
+  const uint64_t rbase = (uint64_t)srow * var_drop_ld(p);
+  for (int64_t k0 = 0; k0 < len; k0 += VT) {
+    __syncthreads();
+    vload_tile<T>(Ks, kp, p.k_ss, k0, len, Dh, tid);
+    vload_tile<T>(Vs, vp, p.v_ss, k0, len, Dh, tid);
+    __syncthreads();
+    const int nk = (int)(len - k0 < VT ? len - k0 : VT);
+    for (int kk = 0; kk < nk; kk++) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < VMAXI; i++) {
+        const int d = part + 4 * i;
+        if (d < Dh) s = fmaf(q[i], Ks[kk * Dh + d], s);
+      }
+      s = vquad_sum(s) * p.scale;
+      if (qv) s += var_bias<T>(p, qrow, k0 + kk, h);
+      if (s == -INFINITY) continue;   // nothing of this key (the whole quad skips together)
+      const float mn = fmaxf(m, s);
+      const float a = expf(m - mn), pr = expf(s - mn);
+      l = l * a + pr;
+      m = mn;
+      float pd = pr;
+      if (p.thr) pd = rng_u32(p.seed, rbase + (uint64_t)(k0 + kk)) >= p.thr ? pr * p.keep_scale : 0.f;
+#pragma unroll
+      for (int i = 0; i < VMAXI; i++) {
+        const int d = part + 4 * i;
+        if (d < Dh) o[i] = fmaf(pd, Vs[kk * Dh + d], o[i] * a);
+      }
+    }
+  }
+  if (!qv) return;
+  T* op = (T*)p.o + b * p.o_sb + h * p.o_sh + qrow * p.o_ss;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < VMAXI; i++) {
+    const int d = part + 4 * i;
+    if (d < Dh) op[d] = from_f<T>(o[i] * inv);
+  }
+  if (part == 0) p.lse[srow] = l == 0.f ? INFINITY : m + logf(l);
+}
+
+// delta[b,h,i] = sum_d dO O   (a wave per row)
+template <class T>
+__global__ __launch_bounds__(256) void var_delta_k(VarP p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)p.B * p.H * p.Lq) return;
+  const int64_t s = row % p.Lq, h = (row / p.Lq) % p.H, b = row / ((int64_t)p.Lq * p.H);
+  const T* o = (const T*)p.o + b * p.o_sb + h * p.o_sh + s * p.o_ss;
+  const T* g = (const T*)p.dout + b * p.g_sb + h * p.g_sh + s * p.g_ss;
+  float acc = 0.f;
+  for (int d = lane; d < p.Dh; d += 64) acc += to_f<T>(o[d]) * to_f<T>(g[d]);
+  acc = wave_sum(acc);
+  if (lane == 0) p.delta[row] = acc;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void var_dq_simple_k(VarP p) {
+  extern __shared__ __attribute__((aligned(16))) float sm[];
+  const int Dh = p.Dh, tid = threadIdx.x, part = tid & 3;
+  const int64_t b = blockIdx.z, h = blockIdx.y, qrow = (int64_t)blockIdx.x * 64 + (tid >> 2);
+  float* Ks = sm;
+  float* Vs = sm + VT * Dh;
+  const T* qp = (const T*)p.q + b * p.q_sb + h * p.q_sh;
+  const T* kp = (const T*)p.k + b * p.k_sb + h * p.k_sh;
+  const T* vp = (const T*)p.v + b * p.v_sb + h * p.v_sh;
+  const T* gp = (const T*)p.dout + b * p.g_sb + h * p.g_sh;
+  const bool qv = qrow < p.Lq;
+  const int len = key_count(p, b);
+  float q[VMAXI], g[VMAXI], dq[VMAXI];
+#pragma unroll
+  for (int i = 0; i < VMAXI; i++) {
+    const int d = part + 4 * i;
+    q[i] = (qv && d < Dh) ? to_f<T>(qp[qrow * p.q_ss + d]) : 0.f;
+    g[i] = (qv && d < Dh) ? to_f<T>(gp[qrow * p.g_ss + d]) : 0.f;
+    dq[i] = 0.f;
+  }
+  const int64_t srow = (b * p.H + h) * p.Lq + qrow;
+  const float lse = qv ? p.lse[srow] : 0.f, delta = qv ? p.delta[srow] : 0.f;
+  const uint64_t rbase = (uint64_t)srow * var_drop_ld(p);
+  for (int64_t k0 = 0; k0 < len; k0 += VT) {
+    __syncthreads();
+    vload_tile<T>(Ks, kp, p.k_ss, k0, len, Dh, tid);
+    vload_tile<T>(Vs, vp, p.v_ss, k0, len, Dh, tid);
+    __syncthreads();
+    const int nk = (int)(len - k0 < VT ? len - k0 : VT);
+    for (int kk = 0; kk < nk; kk++) {
+      float s = 0.f, dp = 0.f;
+#pragma unroll
+      for (int i = 0; i < VMAXI; i++) {
+        const int d = part + 4 * i;
+        if (d < Dh) { s = fmaf(q[i], Ks[kk * Dh + d], s); dp = fmaf(g[i], Vs[kk * Dh + d], dp); }
+      }
+      s = vquad_sum(s) * p.scale;
+      dp = vquad_sum(dp);
+      if (qv) s += var_bias<T>(p, qrow, k0 + kk, h);
+      const float pr = expf(s - lse);
+      if (p.thr) dp = rng_u32(p.seed, rbase + (uint64_t)(k0 + kk)) >= p.thr ? dp * p.keep_scale : 0.f;
+      const float ds = pr * (dp - delta);
+#pragma unroll
+      for (int i = 0; i < VMAXI; i++) {
+        const int d = part + 4 * i;
+        if (d < Dh) dq[i] = fmaf(ds, Ks[kk * Dh + d], dq[i]);
+      }
+    }
+  }
+  if (!qv) return;
+  T* op = (T*)p.dq + b * p.dq_sb + h * p.dq_sh + qrow * p.dq_ss;
+#pragma unroll
+  for (int i = 0; i < VMAXI; i++) {
+    const int d = part + 4 * i;
+    if (d < Dh) op[d] = from_f<T>(dq[i] * p.scale);
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void var_dkdv_simple_k(VarP p) {
+  extern __shared__ __attribute__((aligned(16))) float sm[];
+  const int Dh = p.Dh, tid = threadIdx.x, part = tid & 3;
+  const int64_t b = blockIdx.z, h = blockIdx.y, krow = (int64_t)blockIdx.x * 64 + (tid >> 2);
+  float* Qs = sm;
+  float* Gs = sm + VT * Dh;
+  float* Ls = sm + 2 * VT * Dh;   // lse[VT], delta[VT]
+  const T* qp = (const T*)p.q + b * p.q_sb + h * p.q_sh;
+  const T* kp = (const T*)p.k + b * p.k_sb + h * p.k_sh;
+  const T* vp = (const T*)p.v + b * p.v_sb + h * p.v_sh;
+  const T* gp = (const T*)p.dout + b * p.g_sb + h * p.g_sh;
+  const int len = key_count(p, b);
+  const bool kv = krow < len;
+  float k[VMAXI], v[VMAXI], dk[VMAXI], dv[VMAXI];
+#pragma unroll
+  for (int i = 0; i < VMAXI; i++) {
+    const int d = part + 4 * i;
+    k[i] = (kv && d < Dh) ? to_f<T>(kp[krow * p.k_ss + d]) : 0.f;
+    v[i] = (kv && d < Dh) ? to_f<T>(vp[krow * p.v_ss + d]) : 0.f;
+    dk[i] = 0.f; dv[i] = 0.f;
+  }
+  const int64_t sbase = (b * p.H + h) * p.Lq;
+  const bool any = (int64_t)blockIdx.x * 64 < len;   // otherwise the whole block of keys is padding
+  for (int64_t q0 = 0; any && q0 < p.Lq; q0 += VT) {
+    __syncthreads();
+    vload_tile<T>(Qs, qp, p.q_ss, q0, p.Lq, Dh, tid);
+    vload_tile<T>(Gs, gp, p.g_ss, q0, p.Lq, Dh, tid);
+    if (tid < VT) {
+      const bool ok = q0 + tid < p.Lq;
+      Ls[tid] = ok ? p.lse[sbase + q0 + tid] : 0.f;
+      Ls[VT + tid] = ok ? p.delta[sbase + q0 + tid] : 0.f;
+    }
+    __syncthreads();
+    const int nq = (int)(p.Lq - q0 < VT ? p.Lq - q0 : VT);
+    for (int qq = 0; qq < nq; qq++) {
+      float s = 0.f, dp = 0.f;
+#pragma unroll
+      for (int i = 0; i < VMAXI; i++) {
+        const int d = part + 4 * i;
+        if (d < Dh) { s = fmaf(k[i], Qs[qq * Dh + d], s); dp = fmaf(v[i], Gs[qq * Dh + d], dp); }
+      }
+      s = vquad_sum(s) * p.scale;
+      dp = vquad_sum(dp);
+      if (kv) s += var_bias<T>(p, q0 + qq, krow, h);
+      const float pr = kv ? expf(s - Ls[qq]) : 0.f;
+      float pd = pr;
+      if (p.thr) {
+        const bool keep = rng_u32(p.seed, (uint64_t)(sbase + q0 + qq) * var_drop_ld(p) + (uint64_t)krow) >= p.thr;
+        pd = keep ? pr * p.keep_scale : 0.f;
+        dp = keep ? dp * p.keep_scale : 0.f;
+      }
+      const float ds = pr * (dp - Ls[VT + qq]);
+#pragma unroll
+      for (int i = 0; i < VMAXI; i++) {
+        const int d = part + 4 * i;
+        if (d < Dh) { dv[i] = fmaf(pd, Gs[qq * Dh + d], dv[i]); dk[i] = fmaf(ds, Qs[qq * Dh + d], dk[i]); }
+      }
+    }
+  }
+  if (krow >= p.Lk) return;
+  T* okp = (T*)p.dk + b * p.dk_sb + h * p.dk_sh + krow * p.dk_ss;
+  T* ovp = (T*)p.dv + b * p.dv_sb + h * p.dv_sh + krow * p.dv_ss;
+#pragma unroll
+  for (int i = 0; i < VMAXI; i++) {
+    const int d = part + 4 * i;
+    if (d < Dh) { okp[d] = from_f<T>(kv ? dk[i] * p.scale : 0.f); ovp[d] = from_f<T>(kv ? dv[i] : 0.f); }
+  }
+}
+
+// dbias[h][i][j] = sum_b dS   (a thread per pair)
+template <class T>
+__global__ __launch_bounds__(256) void var_dbias_simple_k(VarP p) {
+  const int64_t pair = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t h = blockIdx.y;
+  if (pair >= (int64_t)p.Lq * p.Lk) return;
+  const int64_t i = pair / p.Lk, j = pair - i * p.Lk;
+  const float bias = var_bias<T>(p, i, j, h);
+  float sum = 0.f;
+  for (int64_t b = 0; b < p.B; b++) {
+    if (j >= key_count(p, b)) continue;
+    const T* q = (const T*)p.q + b * p.q_sb + h * p.q_sh + i * p.q_ss;
+    const T* k = (const T*)p.k + b * p.k_sb + h * p.k_sh + j * p.k_ss;
+    const T* v = (const T*)p.v + b * p.v_sb + h * p.v_sh + j * p.v_ss;
+    const T* g = (const T*)p.dout + b * p.g_sb + h * p.g_sh + i * p.g_ss;
+    float s = 0.f, dp = 0.f;
+    for (int d = 0; d < p.Dh; d++) { s = fmaf(to_f<T>(q[d]), to_f<T>(k[d]), s); dp = fmaf(to_f<T>(g[d]), to_f<T>(v[d]), dp); }
+    const int64_t srow = (b * p.H + h) * p.Lq + i;
+    const float pr = expf(fmaf(s, p.scale, bias) - p.lse[srow]);
+    if (p.thr) dp = rng_u32(p.seed, (uint64_t)srow * var_drop_ld(p) + (uint64_t)j) >= p.thr ? dp * p.keep_scale : 0.f;
+    sum += pr * (dp - p.delta[srow]);
+  }
+  p.dbias[h * p.Lq * p.Lk + pair] = sum;
+}
+
+// ---- bucket sums of dbias: pieces of at most a few thousand pairs, then the pieces of a bucket, both in a fixed order ----
+__global__ __launch_bounds__(256) void var_piece_sum_k(const float* __restrict__ dbias, const int32_t* __restrict__ order,
+                                                       const int32_t* __restrict__ piece, float* __restrict__ part,
+                                                       int64_t pairs, int H, int npieces, int splits) {
+  const int lane = threadIdx.x & 63, pc = (int)blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y;
+  if (pc >= npieces) return;
+  const int b = piece[pc], e = piece[pc + 1];
+  float a = 0.f;
+  for (int i = b + lane; i < e; i += 64) {
+    const int64_t at = order[i];
+    for (int s = 0; s < splits; s++) a += dbias[((int64_t)s * H + h) * pairs + at];
+  }
+  a = wave_sum(a);
+  if (lane == 0) part[(int64_t)h * npieces + pc] = a;
+}
+template <class T>
+__global__ __launch_bounds__(256) void var_bucket_sum_k(const float* __restrict__ part, const int32_t* __restrict__ bucket_piece,
+                                                        T* __restrict__ out, int H, int npieces, int nbuckets) {
+  const int lane = threadIdx.x & 63, n = (int)blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y;
+  if (n >= nbuckets) return;
+  float a = 0.f;
+  for (int i = bucket_piece[n] + lane; i < bucket_piece[n + 1]; i += 64) a += part[(int64_t)h * npieces + i];
+  a = wave_sum(a);
+  if (lane == 0) out[(int64_t)n * H + h] = from_f<T>(a);
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+static VarP make_varp(const VitkAttnVar* a) {
+  VarP p;
+  p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->o; p.dout = a->dout; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
+  p.lse = a->lse; p.delta = nullptr; p.kv_len = a->kv_len; p.table = a->bias_table; p.index = a->bias_index; p.dbias = nullptr;
+  const int64_t* s = a->st;
+  p.q_sb = s[0]; p.q_sh = s[1]; p.q_ss = s[2]; p.k_sb = s[3]; p.k_sh = s[4]; p.k_ss = s[5];
+  p.v_sb = s[6]; p.v_sh = s[7]; p.v_ss = s[8]; p.o_sb = s[9]; p.o_sh = s[10]; p.o_ss = s[11];
+  p.g_sb = s[12]; p.g_sh = s[13]; p.g_ss = s[14]; p.dq_sb = s[15]; p.dq_sh = s[16]; p.dq_ss = s[17];
+  p.dk_sb = s[18]; p.dk_sh = s[19]; p.dk_ss = s[20]; p.dv_sb = s[21]; p.dv_sh = s[22]; p.dv_ss = s[23];
+  p.B = (int)a->B; p.H = (int)a->H; p.Lq = (int)a->Lq; p.Lk = (int)a->Lk; p.Dh = (int)a->Dh;
+  p.seed = a->seed; p.scale = a->scale;
+  p.thr = a->drop_p > 0.f ? drop_threshold(a->drop_p) : 0;
+  p.keep_scale = 1.f / (1.f - a->drop_p);
+  return p;
+}
+static int var_validate(const VitkAttnVar* a, bool bwd) {
+  VITK_REQUIRE(a, "attn_var: null descriptor");
+  VITK_REQUIRE(a->B >= 0 && a->B <= 65535 && a->H > 0 && a->H <= 65535 && a->Lq >= 0 && a->Lk >= 0 && a->Dh > 0 && a->Dh <= 128,
+               "attn_var: bad shape B=%lld H=%lld Lq=%lld Lk=%lld Dh=%lld", (long long)a->B, (long long)a->H, (long long)a->Lq,
+               (long long)a->Lk, (long long)a->Dh);
+  VITK_REQUIRE(a->Lq < (1 << 22) && a->Lk < (1 << 24), "attn_var: at most 2^22 queries and 2^24 keys");
+  VITK_REQUIRE(a->dtype == VITK_F32 || a->dtype == VITK_BF16, "attn_var: bad dtype");
+  VITK_REQUIRE(!a->dbias_table || a->dbias_dtype == VITK_F32 || a->dbias_dtype == VITK_BF16, "attn_var: bad dtype of the bias gradient");
+  VITK_REQUIRE(a->drop_p >= 0.f && a->drop_p < 1.f, "attn_var: dropout p=%f out of range", a->drop_p);
+  VITK_REQUIRE(a->scale > 0.f && a->scale < 1e10f, "attn_var: scale=%g must be positive", a->scale);
+  if (a->B * a->Lq * a->Lk > 0) VITK_REQUIRE(a->q && a->k && a->v && a->o && a->lse, "attn_var: null pointer");
+  VITK_REQUIRE(!a->bias_table == !a->bias_index, "attn_var: a bias needs its table and its index");
+  if (a->bias_table) {
+    VITK_REQUIRE(a->num_buckets > 0 && a->num_buckets <= 65536, "attn_var: num_buckets=%lld outside [1, 65536]", (long long)a->num_buckets);
+    VITK_REQUIRE(a->Lq * a->Lk < (1ll << 31), "attn_var: a bias over %lld x %lld pairs is not supported", (long long)a->Lq, (long long)a->Lk);
+  }
+  if (bwd) {
+    VITK_REQUIRE(a->B * a->Lq == 0 || (a->dout && a->dq), "attn_var_bwd: null pointer");
+    VITK_REQUIRE(a->B * a->Lk == 0 || (a->dk && a->dv), "attn_var_bwd: null pointer");
+    if (a->dbias_table)
+      VITK_REQUIRE(a->bias_table && a->order && a->piece && a->bucket_piece && a->num_pieces >= 0, "attn_var_bwd: the bias gradient needs the bias and its plan");
+  }
+  return 0;
+}
+static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+struct VarWs { size_t delta, dbias, part, total; int splits; };
+static VarWs var_ws(const VitkAttnVar* a, bool bwd) {
+  VarWs w = {0, 0, 0, 0, 1};
+  if (!bwd) return w;
+  size_t at = 0;
+  w.delta = at; at += up256((size_t)(a->B * a->H * a->Lq) * 4);
+  if (a->dbias_table) {
+    w.dbias = at; at += up256((size_t)w.splits * a->H * a->Lq * a->Lk * 4);
+    w.part = at; at += up256((size_t)a->H * a->num_pieces * 4);
+  }
+  w.total = at;
+  return w;
+}
+extern "C" size_t vitk_attn_var_workspace_bytes(const VitkAttnVar* a, int bwd) {
+  if (!a || var_validate(a, bwd != 0)) return 0;
+  return var_ws(a, bwd != 0).total;
+}
+#define VAR_T(T, ...) do { if (a->dtype == VITK_F32) { typedef float T; __VA_ARGS__; } else { typedef bf16 T; __VA_ARGS__; } } while (0)
+
+extern "C" int vitk_attn_var_fwd(const VitkAttnVar* a, void* stream) {
+  if (int rc = var_validate(a, false)) return rc;
+  if (a->B == 0 || a->Lq == 0) return 0;
+  hipStream_t st = (hipStream_t)stream;
+  const VarP p = make_varp(a);
+  const VarWs w = var_ws(a, false);
+  VITK_REQUIRE(w.total == 0 || (a->workspace && a->workspace_bytes >= (int64_t)w.total), "attn_var_fwd: workspace too small");
+  dim3 grid((unsigned)ceil_div(a->Lq, 64), (unsigned)a->H, (unsigned)a->B);
+  const size_t lds = (size_t)2 * VT * a->Dh * sizeof(float);
+  VAR_T(T, hipLaunchKernelGGL((var_fwd_simple_k<T>), grid, dim3(256), lds, st, p));
+  VITK_LAUNCH_CHECK("attn_var_fwd");
+  return 0;
+}
+
+extern "C" int vitk_attn_var_bwd(const VitkAttnVar* a, void* stream) {
+  if (int rc = var_validate(a, true)) return rc;
+  if (a->B * (a->Lq + a->Lk) == 0 && !a->dbias_table) return 0;
+  hipStream_t st = (hipStream_t)stream;
+  VarP p = make_varp(a);
+  const VarWs w = var_ws(a, true);
+  VITK_REQUIRE(w.total == 0 || (a->workspace && a->workspace_bytes >= (int64_t)w.total), "attn_var_bwd: workspace too small");
+  p.delta = (float*)((char*)a->workspace + w.delta);
+  p.dbias = (float*)((char*)a->workspace + w.dbias);
+  const int64_t rows = a->B * a->H * a->Lq;
+  const size_t lds = (size_t)2 * VT * a->Dh * sizeof(float);
+  if (rows > 0) {
+    VAR_T(T, hipLaunchKernelGGL((var_delta_k<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, p));
+    VAR_T(T, hipLaunchKernelGGL((var_dq_simple_k<T>), dim3((unsigned)ceil_div(a->Lq, 64), (unsigned)a->H, (unsigned)a->B), dim3(256), lds, st, p));
+  }
+  if (a->B * a->Lk > 0)
+    VAR_T(T, hipLaunchKernelGGL((var_dkdv_simple_k<T>), dim3((unsigned)ceil_div(a->Lk, 64), (unsigned)a->H, (unsigned)a->B), dim3(256), lds + 512, st, p));
+  if (a->dbias_table) {
+    float* part = (float*)((char*)a->workspace + w.part);
+    const int64_t pairs = a->Lq * a->Lk;
+    if (pairs > 0) {
+      VAR_T(T, hipLaunchKernelGGL((var_dbias_simple_k<T>), dim3((unsigned)ceil_div(pairs, 256), (unsigned)a->H), dim3(256), 0, st, p));
+      if (a->num_pieces > 0)
+        hipLaunchKernelGGL(var_piece_sum_k, dim3((unsigned)ceil_div(a->num_pieces, 4), (unsigned)a->H), dim3(256), 0, st, p.dbias,
+                           a->order, a->piece, part, pairs, (int)a->H, (int)a->num_pieces, w.splits);
+    }
+    const dim3 bgrid((unsigned)ceil_div(a->num_buckets, 4), (unsigned)a->H);
+    if (a->dbias_dtype == VITK_F32)
+      hipLaunchKernelGGL((var_bucket_sum_k<float>), bgrid, dim3(256), 0, st, part, a->bucket_piece, (float*)a->dbias_table, (int)a->H,
+                         (int)a->num_pieces, (int)a->num_buckets);
+    else
+      hipLaunchKernelGGL((var_bucket_sum_k<bf16>), bgrid, dim3(256), 0, st, part, a->bucket_piece, (bf16*)a->dbias_table, (int)a->H,
+                         (int)a->num_pieces, (int)a->num_buckets);
+  }
+  VITK_LAUNCH_CHECK("attn_var_bwd");
+  return 0;
+}

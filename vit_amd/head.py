@@ -53,8 +53,9 @@ class AttentivePoolHead(nn.Module):
         self.pool.reset_parameters()
         self.proj.reset_parameters()
 
-    def forward(self, x: Tensor) -> Tensor:
-        return self.proj(self.pool(x))
+    def forward(self, x: Tensor, lengths: Optional[Tensor] = None) -> Tensor:
+        """``lengths`` [B]: the tokens each sample has; rows of x behind them are padding."""
+        return self.proj(self.pool(x, lengths))
 
     def forward_weights(self, x: Tensor) -> Tensor:
         return self.pool.forward_weights(x)

@@ -230,13 +230,15 @@ def can_fuse_activation(dtype: torch.dtype, D: int, F: int) -> bool:
 
 
 def _attn_desc(qkv: Tensor, o: Tensor, lse: Tensor, B: int, S: int, H: int, Dh: int, scale: float, drop_p: float,
-               seed: int, algo: Optional[int]) -> L.VitkAttn:
-    """qkv is the packed projection [B*S, 3*H*Dh]; o is [B*S, H*Dh]."""
+               seed: int, algo: Optional[int], v_src: Optional[Tensor] = None) -> L.VitkAttn:
+    """qkv is the packed projection [B*S, 3*H*Dh]; o is [B*S, H*Dh].  ``v_src``: v is read from the last third of this
+    buffer of the same layout instead (q and k then come from a buffer of their own)."""
     D = H * Dh
     es = qkv.element_size()
     a = L.VitkAttn()
     base = qkv.data_ptr()
-    a.q, a.k, a.v = base, base + D * es, base + 2 * D * es
+    assert v_src is None or (v_src.is_contiguous() and v_src.shape == qkv.shape and v_src.dtype == qkv.dtype)
+    a.q, a.k, a.v = base, base + D * es, (base if v_src is None else v_src.data_ptr()) + 2 * D * es
     a.o, a.lse = L.ptr(o), L.ptr(lse)
     a.B, a.H, a.S, a.Dh = B, H, S, Dh
     a.q_sb, a.q_sh, a.q_ss = S * 3 * D, Dh, 3 * D
@@ -248,20 +250,20 @@ def _attn_desc(qkv: Tensor, o: Tensor, lse: Tensor, B: int, S: int, H: int, Dh: 
 
 
 def attn_fwd(qkv: Tensor, B: int, S: int, H: int, Dh: int, scale: float, drop_p: float = 0.0, seed: int = 0,
-             algo: Optional[int] = None):
+             algo: Optional[int] = None, v_src: Optional[Tensor] = None):
     lib = L.load()
-    L.require_gpu(qkv)
+    L.require_gpu(qkv, v_src)
     assert qkv.is_contiguous() and qkv.shape == (B * S, 3 * H * Dh)
     o = torch.empty((B * S, H * Dh), dtype=qkv.dtype, device=qkv.device)
     lse = torch.empty((B, H, S), dtype=torch.float32, device=qkv.device)
-    a = _attn_desc(qkv, o, lse, B, S, H, Dh, scale, drop_p, seed, algo)
+    a = _attn_desc(qkv, o, lse, B, S, H, Dh, scale, drop_p, seed, algo, v_src)
     L.check(lib.vitk_attn_fwd(C.byref(a), L.stream()))
     return o, lse
 
 
 def attn_bwd(qkv: Tensor, o: Tensor, lse: Tensor, dout: Tensor, B: int, S: int, H: int, Dh: int, scale: float,
              drop_p: float = 0.0, seed: int = 0, algo: Optional[int] = None, rope: Optional[Tensor] = None,
-             rope_emulate_bf16: bool = False, qk_norm: Optional[dict] = None) -> Tensor:
+             rope_emulate_bf16: bool = False, qk_norm: Optional[dict] = None, v_src: Optional[Tensor] = None) -> Tensor:
     """Returns dqkv in the packed layout of qkv.  ``rope`` (fp32 [2, S - prefix, 64]): q and k were rotated with this
     table before the attention; dq and dk come back through the transposed rotation."""
     lib = L.load()
@@ -270,7 +272,7 @@ def attn_bwd(qkv: Tensor, o: Tensor, lse: Tensor, dout: Tensor, B: int, S: int, 
     D = H * Dh
     dqkv = torch.empty_like(qkv)
     delta = torch.empty((B, H, S), dtype=torch.float32, device=qkv.device)
-    a = _attn_desc(qkv, o, lse, B, S, H, Dh, scale, drop_p, seed, algo)
+    a = _attn_desc(qkv, o, lse, B, S, H, Dh, scale, drop_p, seed, algo, v_src)
     es = qkv.element_size()
     a.dout, a.delta = L.ptr(dout), L.ptr(delta)
     base = dqkv.data_ptr()
@@ -285,11 +287,12 @@ def attn_bwd(qkv: Tensor, o: Tensor, lse: Tensor, dout: Tensor, B: int, S: int, 
 
 
 def _cross_desc(q: Tensor, kv: Tensor, o: Tensor, lse: Tensor, B: int, Sq: int, Sk: int, H: int, Dh: int, scale: float,
-                drop_p: float, seed: int, algo: Optional[int] = None) -> L.VitkAttn:
-    """q [B*Sq, H*Dh]; kv [B*Sk, 2*H*Dh] = [k | v]; o [B*Sq, H*Dh]."""
+                drop_p: float, seed: int, algo: Optional[int] = None, v_src: Optional[Tensor] = None) -> L.VitkAttn:
+    """q [B*Sq, H*Dh]; kv [B*Sk, 2*H*Dh] = [k | v] (v from ``v_src`` of the same layout, if given); o [B*Sq, H*Dh]."""
     D = H * Dh
     a = L.VitkAttn()
-    a.q, a.k, a.v = q.data_ptr(), kv.data_ptr(), kv.data_ptr() + D * kv.element_size()
+    assert v_src is None or (v_src.is_contiguous() and v_src.shape == kv.shape and v_src.dtype == kv.dtype)
+    a.q, a.k, a.v = q.data_ptr(), kv.data_ptr(), (kv if v_src is None else v_src).data_ptr() + D * kv.element_size()
     a.o, a.lse = L.ptr(o), L.ptr(lse)
     a.B, a.H, a.S, a.Dh, a.Sk = B, H, Sq, Dh, Sk
     a.q_sb, a.q_sh, a.q_ss = Sq * D, Dh, D
@@ -302,7 +305,7 @@ def _cross_desc(q: Tensor, kv: Tensor, o: Tensor, lse: Tensor, B: int, Sq: int, 
 
 
 def attn_cross_fwd(q: Tensor, kv: Tensor, B: int, Sq: int, Sk: int, H: int, Dh: int, scale: float, drop_p: float = 0.0,
-                   seed: int = 0, algo: Optional[int] = None):
+                   seed: int = 0, algo: Optional[int] = None, v_src: Optional[Tensor] = None):
     """Attention of Sq queries over Sk keys per sample (vit/attention.py:269-273 with Lq != Lk)."""
     lib = L.load()
     L.require_gpu(q, kv)
@@ -311,13 +314,14 @@ def attn_cross_fwd(q: Tensor, kv: Tensor, B: int, Sq: int, Sk: int, H: int, Dh: 
     assert q.dtype == kv.dtype
     o = torch.empty_like(q)
     lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
-    a = _cross_desc(q, kv, o, lse, B, Sq, Sk, H, Dh, scale, drop_p, seed, algo)
+    a = _cross_desc(q, kv, o, lse, B, Sq, Sk, H, Dh, scale, drop_p, seed, algo, v_src)
     L.check(lib.vitk_attn_fwd(C.byref(a), L.stream()))
     return o, lse
 
 
 def attn_cross_bwd(q: Tensor, kv: Tensor, o: Tensor, lse: Tensor, dout: Tensor, B: int, Sq: int, Sk: int, H: int, Dh: int,
-                   scale: float, drop_p: float = 0.0, seed: int = 0, algo: Optional[int] = None):
+                   scale: float, drop_p: float = 0.0, seed: int = 0, algo: Optional[int] = None,
+                   v_src: Optional[Tensor] = None):
     """Returns (dq [B*Sq, D], dkv [B*Sk, 2D])."""
     lib = L.load()
     L.require_gpu(q, kv, o, lse, dout)
@@ -325,7 +329,7 @@ def attn_cross_bwd(q: Tensor, kv: Tensor, o: Tensor, lse: Tensor, dout: Tensor, 
     D = H * Dh
     dq, dkv = torch.empty_like(q), torch.empty_like(kv)
     delta = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
-    a = _cross_desc(q, kv, o, lse, B, Sq, Sk, H, Dh, scale, drop_p, seed, algo)
+    a = _cross_desc(q, kv, o, lse, B, Sq, Sk, H, Dh, scale, drop_p, seed, algo, v_src)
     a.dout, a.delta = L.ptr(dout), L.ptr(delta)
     a.dq, a.dk, a.dv = dq.data_ptr(), dkv.data_ptr(), dkv.data_ptr() + D * dkv.element_size()
     a.dq_sb, a.dq_sh, a.dq_ss = Sq * D, Dh, D
@@ -512,3 +516,182 @@ def prefix_fill_(out: Tensor, cls_tokens: Tensor, register_tokens: Tensor) -> Te
     L.check(lib.vitk_prefix_fill(L.ptr(cls_tokens) if ncls else None, ncls, L.ptr(register_tokens) if nreg else None, nreg,
                                  L.dt(cls_tokens), L.ptr(out), L.dt(out), B, S, D, L.stream()))
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# per-head normalisation with the rotation in the same pass
+# ------------------------------------------------------------------------------------------------
+def can_qk_norm_rope(dtype: torch.dtype, Dh: int) -> bool:
+    """Head sizes and types of the normalisation + rotation pass."""
+    return Dh % 8 == 0 and 8 <= Dh <= 128 and dtype in (torch.float32, torch.bfloat16)
+
+
+def head_rows(t: Tensor) -> Tensor:
+    """``t`` [B, L, H, Dh] with d contiguous and heads on 4-element boundaries (a view that is not is copied once)."""
+    sb, ss, sh, sd = t.stride()
+    if sd == 1 and not (sb % 4 or ss % 4 or sh % 4 or t.data_ptr() % (4 * t.element_size())):
+        return t
+    return t.contiguous()
+
+
+def _qk_section(sec: L.VitkQkSection, x: Tensor, g: Optional[Tensor], y: Tensor, w: Tensor, b: Optional[Tensor],
+                dw: Optional[Tensor], db: Optional[Tensor], table: Optional[Tensor]) -> None:
+    B, Ln, H, Dh = x.shape
+    sec.x, sec.y, sec.w = x.data_ptr(), y.data_ptr(), w.data_ptr()
+    sec.x_sb, sec.x_ss, sec.x_sh, _ = x.stride()
+    sec.y_sb, sec.y_ss, sec.y_sh, _ = y.stride()
+    if b is not None:
+        sec.b = b.data_ptr()
+    if g is not None:
+        sec.g = g.data_ptr()
+        sec.g_sb, sec.g_ss, sec.g_sh, _ = g.stride()
+    sec.dw, sec.db = L.ptr(dw), L.ptr(db)
+    sec.L, sec.H = Ln, H
+    if table is not None:   # fp32 [2, N, Dh] or [2, B, N, Dh], contiguous (ops._rope_table)
+        sec.table, sec.prefix, sec.per_sample = table.data_ptr(), Ln - table.shape[-2], int(table.dim() == 4)
+    else:
+        sec.prefix = Ln
+
+
+def _qk_check(x: Tensor, w: Tensor, b: Optional[Tensor], table: Optional[Tensor]) -> None:
+    B, Ln, _, Dh = x.shape
+    assert x.stride(-1) == 1 and w.is_contiguous() and w.numel() == Dh
+    assert b is None or (b.is_contiguous() and b.numel() == Dh and b.dtype == w.dtype)
+    if table is not None:
+        n = table.shape[-2]
+        assert table.dtype == torch.float32 and table.is_contiguous() and n <= Ln
+        assert tuple(table.shape) in ((2, n, Dh), (2, B, n, Dh)), f"rope table {tuple(table.shape)} for {tuple(x.shape)}"
+
+
+def qk_norm_rope_fwd(q: Tensor, k: Optional[Tensor], q_out: Tensor, k_out: Optional[Tensor], w: tuple, b: tuple, tables: tuple,
+                     eps: float, layernorm: bool, round_norm: bool = False, emulate_bf16: bool = False) -> None:
+    """q [B, Lq, H, Dh] (and k [B, Lk, Hk, Dh]) -> q_out, k_out, same shapes, any strides with d contiguous: every head
+    normalised, scaled by w = (w_q, w_k), shifted by b, and rotated with tables = (table_q, table_k)."""
+    lib = L.load()
+    L.require_gpu(q, k, q_out, k_out, *w, *b, *tables)
+    a = L.VitkQkNormRope()
+    for i, (x, y) in enumerate(((q, q_out), (k, k_out))):
+        if x is not None:
+            _qk_check(x, w[i], b[i], tables[i])
+            assert y.dtype == x.dtype == q.dtype and y.shape == x.shape and y.stride(-1) == 1
+            _qk_section(a.sec[i], x, None, y, w[i], b[i], None, None, tables[i])
+    a.B, a.Dh, a.eps, a.dtype, a.w_dtype = q.shape[0], q.shape[-1], eps, L.dt(q), L.dt(w[0])
+    a.is_layernorm, a.round_norm, a.emulate_bf16 = int(layernorm), int(round_norm), int(emulate_bf16)
+    L.check(lib.vitk_qk_norm_rope_fwd(C.byref(a), L.stream()))
+
+
+def qk_norm_rope_bwd(xs: tuple, gs: tuple, dxs: tuple, w: tuple, tables: tuple, eps: float,
+                     layernorm: bool, want: tuple, round_norm: bool = False, emulate_bf16: bool = False) -> tuple:
+    """xs = (q, k or None) the heads before the normalisation, gs the gradients of the outputs, dxs where the gradients of
+    xs go (may be gs).  ``want`` = flags of (dw_q, db_q, dw_k, db_k); returns those four (or None) in the weights' dtype."""
+    lib = L.load()
+    L.require_gpu(*xs, *gs, *dxs, *w, *tables)
+    a = L.VitkQkNormRope()
+    outs = [torch.empty_like(w[i // 2]) if f and xs[i // 2] is not None else None for i, f in enumerate(want)]
+    for i in range(2):
+        if xs[i] is not None:
+            _qk_check(xs[i], w[i], None, tables[i])
+            for t in (gs[i], dxs[i]):
+                assert t.dtype == xs[i].dtype and t.shape == xs[i].shape and t.stride(-1) == 1
+            _qk_section(a.sec[i], xs[i], gs[i], dxs[i], w[i], None, outs[2 * i], outs[2 * i + 1], tables[i])
+    x = xs[0]
+    a.B, a.Dh, a.eps, a.dtype, a.w_dtype = x.shape[0], x.shape[-1], eps, L.dt(x), L.dt(w[0])
+    a.is_layernorm, a.round_norm, a.emulate_bf16 = int(layernorm), int(round_norm), int(emulate_bf16)
+    if any(t is not None for t in outs):
+        ws = torch.empty(lib.vitk_qk_norm_rope_workspace_bytes(C.byref(a)), dtype=torch.uint8, device=x.device)
+        a.workspace = ws.data_ptr()
+    L.check(lib.vitk_qk_norm_rope_bwd(C.byref(a), L.stream()))
+    return tuple(outs)
+
+
+# ------------------------------------------------------------------------------------------------
+# attention with a relative position bias and / or key counts
+# ------------------------------------------------------------------------------------------------
+def attn_operand(t: Tensor) -> Tensor:
+    """``t`` [B, L, H, Dh] as the kernels take it: d contiguous, and rows on 16-byte boundaries where head_dim allows it
+    (the kernels on the matrix units load 16 bytes at a time; a view that is not laid out so is copied once)."""
+    if t.stride(3) == 1:
+        n = 16 // t.element_size()
+        sb, ss, sh, _ = t.stride()
+        if t.shape[3] % n or not (sb % n or ss % n or sh % n or t.data_ptr() % 16):
+            return t
+    return t.contiguous()
+
+
+def _var_strides(ts) -> "C.Array":
+    vals = []
+    for t in ts:
+        if t is None:
+            vals += (0, 0, 0)
+        else:
+            sb, ss, sh, _ = t.stride()
+            vals += (sb, sh, ss)
+    return (C.c_int64 * 24)(*vals)
+
+
+def _var_desc(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, table: Optional[Tensor], buckets, kv_len: Optional[Tensor],
+              scale: float, drop_p: float, seed: int, algo: Optional[int]) -> L.VitkAttnVar:
+    B, Lq, H, Dh = q.shape
+    Lk = k.shape[1]
+    assert k.shape == (B, Lk, H, Dh) == v.shape and o.shape == q.shape and q.dtype == k.dtype == v.dtype == o.dtype
+    assert q.stride(3) == k.stride(3) == v.stride(3) == o.stride(3) == 1
+    a = L.VitkAttnVar()
+    a.q, a.k, a.v, a.o, a.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr()
+    if kv_len is not None:
+        assert kv_len.dtype == torch.int32 and kv_len.is_contiguous() and kv_len.numel() == B
+        a.kv_len = kv_len.data_ptr()
+    if table is not None:
+        assert table.dtype == q.dtype and table.is_contiguous() and tuple(table.shape) == (buckets.num_buckets, H)
+        assert buckets.shape == (Lq, Lk)
+        a.bias_table, a.bias_index, a.num_buckets = table.data_ptr(), buckets.index16.data_ptr(), buckets.num_buckets
+        a.num_pieces = buckets.num_pieces
+    a.B, a.H, a.Lq, a.Lk, a.Dh = B, H, Lq, Lk, Dh
+    a.seed, a.scale, a.drop_p = seed & 0xFFFFFFFFFFFFFFFF, scale, drop_p
+    a.dtype, a.algo = L.dt(q), _ALGO if algo is None else algo
+    return a
+
+
+def attn_var_fwd(q: Tensor, k: Tensor, v: Tensor, *, table: Optional[Tensor] = None, buckets=None,
+                 kv_len: Optional[Tensor] = None, scale: float, drop_p: float = 0.0, seed: int = 0,
+                 algo: Optional[int] = None, out: Optional[Tensor] = None):
+    """q [B, Lq, H, Dh], k / v [B, Lk, H, Dh] (strided views, d contiguous) -> o [B, Lq, H, Dh], lse [B, H, Lq]."""
+    lib = L.load()
+    L.require_gpu(q, k, v, table, kv_len, None if buckets is None else buckets.index16)
+    B, Lq, H, Dh = q.shape
+    o = torch.empty((B, Lq, H, Dh), dtype=q.dtype, device=q.device) if out is None else out
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device)
+    a = _var_desc(q, k, v, o, lse, table, buckets, kv_len, scale, drop_p, seed, algo)
+    a.st = _var_strides((q, k, v, o, None, None, None, None))
+    need = lib.vitk_attn_var_workspace_bytes(C.byref(a), 0)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    L.check(lib.vitk_attn_var_fwd(C.byref(a), L.stream()))
+    return o, lse
+
+
+def attn_var_bwd(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, dout: Tensor, *, dq: Tensor, dk: Tensor, dv: Tensor,
+                 table: Optional[Tensor] = None, buckets=None, kv_len: Optional[Tensor] = None, scale: float,
+                 drop_p: float = 0.0, seed: int = 0, dtable_dtype: Optional[torch.dtype] = None,
+                 algo: Optional[int] = None) -> Optional[Tensor]:
+    """Fills dq, dk, dv (strided views, d contiguous; padded keys get zeros) and returns the gradient of the bias table in
+    ``dtable_dtype`` (None: not wanted)."""
+    lib = L.load()
+    L.require_gpu(q, k, v, o, lse, dout, dq, dk, dv, table, kv_len, None if buckets is None else buckets.index16)
+    assert dout.shape == q.shape == dq.shape and dk.shape == k.shape == dv.shape
+    assert dout.dtype == dq.dtype == dk.dtype == dv.dtype == q.dtype
+    assert dout.stride(3) == dq.stride(3) == dk.stride(3) == dv.stride(3) == 1
+    a = _var_desc(q, k, v, o, lse, table, buckets, kv_len, scale, drop_p, seed, algo)
+    a.dout, a.dq, a.dk, a.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    a.st = _var_strides((q, k, v, o, dout, dq, dk, dv))
+    dtable = None
+    if dtable_dtype is not None:
+        dtable = torch.empty(table.shape, dtype=dtable_dtype, device=q.device)
+        a.dbias_table, a.dbias_dtype = dtable.data_ptr(), L.dt(dtable)
+        a.order, a.piece, a.bucket_piece = buckets.order.data_ptr(), buckets.piece.data_ptr(), buckets.bucket_piece.data_ptr()
+    need = lib.vitk_attn_var_workspace_bytes(C.byref(a), 1)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    L.check(lib.vitk_attn_var_bwd(C.byref(a), L.stream()))
+    return dtable

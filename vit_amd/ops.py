@@ -15,6 +15,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import ddp as _ddp
@@ -444,12 +445,79 @@ def _qk_norm_params(qw: Tensor, qb: Optional[Tensor], kw: Tensor, kb: Optional[T
     return w2, b2
 
 
+def _qkv_views(qkv: Tensor, v_src: Optional[Tensor], B: int, S: int, H: int, Dh: int):
+    """(q, k, v) as [B, S, H, Dh] views of the packed projection; v from ``v_src`` where the q / k buffer is another one."""
+    p = qkv.view(B, S, 3, H, Dh)
+    return p[:, :, 0], p[:, :, 1], (p if v_src is None else v_src.view(B, S, 3, H, Dh))[:, :, 2]
+
+
+def _kv_views(kv: Tensor, v_src: Optional[Tensor], B: int, Lk: int, H: int, Dh: int):
+    """(k, v) as [B, Lk, H, Dh] views of the packed [k | v] projection."""
+    p = kv.view(B, Lk, 2, H, Dh)
+    return p[:, :, 0], (p if v_src is None else v_src.view(B, Lk, 2, H, Dh))[:, :, 1]
+
+
+class QkNormRopeFn(torch.autograd.Function):
+    """Heads of q [B, Lq, H, Dh] and k [B, Lk, Hk, Dh] (or None): normalised, scaled, shifted and rotated in one pass; the
+    backward takes the statistics from the saved inputs again."""
+
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, qb, kb, table_q, table_k, eps, layernorm):
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        K.qk_norm_rope_fwd(q, k, qo, ko, (qw, kw), (qb, kb), (table_q, table_k), eps, layernorm)
+        ctx.save_for_backward(q, k, qw, kw, table_q, table_k)
+        ctx.meta = (eps, layernorm, qb is not None, kb is not None)
+        return qo, ko
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, qw, kw, table_q, table_k = ctx.saved_tensors
+        eps, layernorm, has_qb, has_kb = ctx.meta
+        need = ctx.needs_input_grad
+        dq = torch.zeros_like(q) if dq is None else K.head_rows(dq)
+        gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        gk = None
+        if k is not None:
+            dk = torch.zeros_like(k) if dk is None else K.head_rows(dk)
+            gk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dw = K.qk_norm_rope_bwd((q, k), (dq, dk if k is not None else None), (gq, gk), (qw, kw), (table_q, table_k),
+                                eps, layernorm, (need[2], has_qb and need[4], need[3], has_kb and need[5]))
+        return (gq if need[0] else None, gk if need[1] else None, dw[0], dw[2], dw[1], dw[3], None, None, None, None)
+
+
+class AttentionFn(torch.autograd.Function):
+    """softmax(scale q k^T + bias) v with a relative position bias and / or key counts (K.attn_var_fwd / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, buckets, kv_len, scale, drop_p, seed):
+        tab = None if table is None else table.detach().to(q.dtype).contiguous()
+        o, lse = K.attn_var_fwd(q, k, v, table=tab, buckets=buckets, kv_len=kv_len, scale=scale, drop_p=drop_p, seed=seed)
+        ctx.save_for_backward(q, k, v, o, lse, tab, kv_len)
+        ctx.meta = (buckets, scale, drop_p, seed, None if table is None else table.dtype)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, o, lse, tab, kv_len = ctx.saved_tensors
+        buckets, scale, drop_p, seed, table_dtype = ctx.meta
+        need = ctx.needs_input_grad
+        dout = K.attn_operand(dout)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dtab = K.attn_var_bwd(q, k, v, o, lse, dout, dq=dq, dk=dk, dv=dv, table=tab, buckets=buckets, kv_len=kv_len, scale=scale,
+                              drop_p=drop_p, seed=seed, dtable_dtype=table_dtype if need[3] else None)
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtab, None, None, None, None, None)
+
+
 class AttentionSublayerFn(torch.autograd.Function):
     """x -> x (+) alpha * gamma * dropout(out_proj(SDPA(rope(qkv_proj(norm(x))))))   (vit/attention.py:163-215)."""
 
     @staticmethod
-    def forward(ctx, x, norm_w, norm_b, w_qkv, b_qkv, w_out, b_out, gamma, rope, keep_idx, qn_w, qn_b, kn_w, kn_b, opt):
-        L.require_gpu(x, norm_w, w_qkv, w_out)
+    def forward(ctx, x, norm_w, norm_b, w_qkv, b_qkv, w_out, b_out, gamma, rope, keep_idx, qn_w, qn_b, kn_w, kn_b, opt,
+                rel_table=None):
+        L.require_gpu(x, norm_w, w_qkv, w_out, rel_table)
         B, S, D = x.shape
         Dh = opt["head_dim"]
         H = D // Dh
@@ -494,9 +562,18 @@ class AttentionSublayerFn(torch.autograd.Function):
         else:
             fuse_rope = False
             K.gemm(xn, wq, trans_a=False, trans_b=False, M=M, N=3 * D, K=D, out=qkv, bias=bq, tag="qkv")
-        # otherwise the heads of q (and of k) are copied out as a contiguous [M*H, Dh] matrix, which is what the row-norm
-        # kernels take and what their backward needs; the normalised rows go back into the packed buffer.
-        if qn_w is not None and not fuse_norm:
+        # otherwise the heads are normalised (and rotated in the same pass) from the projection into the q and k sections of a
+        # second packed buffer, whose v section stays unused: the attention takes v from the projection itself
+        v_src = None
+        fuse_pass = qn_w is not None and not fuse_norm and K.can_qk_norm_rope(tc, Dh) and qn_w.dtype == kn_w.dtype
+        if fuse_pass:
+            v_src, qkv = qkv, torch.empty_like(qkv)
+            src, dst = v_src.view(Bk, S, 3, H, Dh), qkv.view(Bk, S, 3, H, Dh)
+            K.qk_norm_rope_fwd(src[:, :, 0], src[:, :, 1], dst[:, :, 0], dst[:, :, 1], (qn_w.detach(), kn_w.detach()),
+                               (_cast(qn_b, qn_w.dtype), _cast(kn_b, kn_w.dtype)), (table, table), opt["qk_eps"],
+                               opt["qk_layernorm"], True, emu)
+            qk_saved = (v_src,) + (None,) * 5
+        elif qn_w is not None and not fuse_norm:   # head sizes the pass does not take: heads copied out, normalised, copied back
             qk_saved = []
             for which, (w_, b_) in enumerate(((qn_w, qn_b), (kn_w, kn_b))):
                 pre = qkv[:, which * D:(which + 1) * D].contiguous().view(M * H, Dh)
@@ -504,10 +581,17 @@ class AttentionSublayerFn(torch.autograd.Function):
                                          opt["qk_layernorm"], tc)
                 qkv[:, which * D:(which + 1) * D].copy_(nrm.view(M, D))
                 qk_saved += [pre, r_, m_]
-        if table is not None and not fuse_rope:
+        if table is not None and not fuse_rope and not fuse_pass:
             K.rope_qk_(qkv, table, Bk, S, H, Dh, S - table.shape[-2], False, emu)
         seed_a = next_seed(x.device) if p_attn > 0 else 0
-        o, lse = K.attn_fwd(qkv, Bk, S, H, Dh, Dh ** -0.5, p_attn, seed_a)
+        rel = None
+        if rel_table is not None:
+            rel = _cast_param(rel_table, tc)
+            o, lse = K.attn_var_fwd(*_qkv_views(qkv, v_src, Bk, S, H, Dh), table=rel, buckets=opt["buckets"], scale=Dh ** -0.5,
+                                    drop_p=p_attn, seed=seed_a)
+            o = o.view(M, D)
+        else:
+            o, lse = K.attn_fwd(qkv, Bk, S, H, Dh, Dh ** -0.5, p_attn, seed_a, v_src=v_src)
         seed_h = next_seed(x.device) if p_hid > 0 else 0
         g = _cast(gamma, tr)
         if residual:
@@ -518,19 +602,21 @@ class AttentionSublayerFn(torch.autograd.Function):
             zero = torch.zeros((M, D), dtype=tc, device=x.device)
             out, aux = _residual_gemm(o, wo, bo, zero, None, None, 1.0, p_hid, seed_h, want_aux=False)
             y = out.view(Bk, S, D)
-        ctx.save_for_backward(x2, norm_w, rstd, mean, xn, qkv, o, lse, wq, wo, g, aux, table, rows, qn_w, kn_w, *qk_saved)
+        ctx.save_for_backward(x2, norm_w, rstd, mean, xn, qkv, o, lse, wq, wo, g, aux, table, rows, qn_w, kn_w, rel, *qk_saved)
         ctx.meta = (B, S, D, H, Dh, Bk, tc, tr, p_attn, p_hid, seed_a, seed_h, emu, opt, x.dtype, w_qkv.dtype,
-                    norm_b is not None, b_qkv is not None, b_out is not None, qn_b is not None, kn_b is not None, fuse_rope)
+                    norm_b is not None, b_qkv is not None, b_out is not None, qn_b is not None, kn_b is not None, fuse_rope, fuse_pass,
+                    None if rel_table is None else rel_table.dtype)
         ctx.ptrs = _ptrs(w_qkv, b_qkv, w_out, b_out)
         ctx.dropped = _dropped_samples(keep_idx)
         return y
 
     @staticmethod
     def backward(ctx, dnew):
-        (x2, norm_w, rstd, mean, xn, qkv, o, lse, wq, wo, g, aux, table, rows, qn_w, kn_w, pre_q, rstd_q, mean_q, pre_k,
+        (x2, norm_w, rstd, mean, xn, qkv, o, lse, wq, wo, g, aux, table, rows, qn_w, kn_w, rel, pre_q, rstd_q, mean_q, pre_k,
          rstd_k, mean_k) = ctx.saved_tensors
         (B, S, D, H, Dh, Bk, tc, tr, p_attn, p_hid, seed_a, seed_h, emu, opt, xdtype, wdtype, has_nb, has_bq,
-         has_bo, has_qnb, has_knb, fuse_rope) = ctx.meta
+         has_bo, has_qnb, has_knb, fuse_rope, fuse_pass, rel_dtype) = ctx.meta
+        v_src = pre_q if fuse_pass else None   # the projection output: heads before the pass, and v
         need = ctx.needs_input_grad
         ptrs = ctx.ptrs
         M = Bk * S
@@ -539,12 +625,29 @@ class AttentionSublayerFn(torch.autograd.Function):
         dy, dgamma = _residual_grad(dnew2, tc, g if residual else None, rows if residual else None, M,
                                     opt["alpha"] if residual else 1.0, p_hid, seed_h, aux, need[7], _carried_bf16(dnew, D))
         do, dwo, dbo = _linear_bwd(dy, o, wo, True, need[5], has_bo and need[6], wdtype, tag="out", w_ptr=ptrs[2], b_ptr=ptrs[3])
-        dqkv = K.attn_bwd(qkv, o, lse, do, Bk, S, H, Dh, Dh ** -0.5, p_attn, seed_a, rope=table if fuse_rope else None,
-                          rope_emulate_bf16=emu)
-        if table is not None and not fuse_rope:
+        drel = None
+        if rel is not None:
+            dqkv = torch.empty_like(qkv)
+            gq, gk, gv = _qkv_views(dqkv, None, Bk, S, H, Dh)
+            hd = (Bk, S, H, Dh)
+            drel = K.attn_var_bwd(*_qkv_views(qkv, v_src, Bk, S, H, Dh), o.view(hd), lse, do.contiguous().view(hd), dq=gq, dk=gk,
+                                  dv=gv, table=rel, buckets=opt["buckets"], scale=Dh ** -0.5, drop_p=p_attn, seed=seed_a,
+                                  dtable_dtype=rel_dtype if need[15] else None)
+            if fuse_rope:   # the projection's epilogue rotated q and k
+                K.rope_qk_(dqkv, table, Bk, S, H, Dh, S - table.shape[-2], True, emu)
+        else:
+            dqkv = K.attn_bwd(qkv, o, lse, do, Bk, S, H, Dh, Dh ** -0.5, p_attn, seed_a, rope=table if fuse_rope else None,
+                              rope_emulate_bf16=emu, v_src=v_src)
+        if table is not None and not fuse_rope and not fuse_pass:
             K.rope_qk_(dqkv, table, Bk, S, H, Dh, S - table.shape[-2], True, emu)
         dqn = [None, None, None, None]   # d q_norm.weight, d q_norm.bias, d k_norm.weight, d k_norm.bias
-        if qn_w is not None and K.can_qk_norm_bwd_inplace(dqkv, Dh) and pre_q.dtype == dqkv.dtype and qn_w.dtype == kn_w.dtype:
+        if fuse_pass:   # rotation and normalisation backward in place on the packed gradient
+            gq, gk, _ = _qkv_views(dqkv, None, Bk, S, H, Dh)
+            xq, xk, _ = _qkv_views(v_src, None, Bk, S, H, Dh)
+            dqn = list(K.qk_norm_rope_bwd((xq, xk), (gq, gk), (gq, gk), (qn_w.detach(), kn_w.detach()),
+                                          (table, table), opt["qk_eps"], opt["qk_layernorm"],
+                                          (need[10], has_qnb and need[11], need[12], has_knb and need[13]), True, emu))
+        elif qn_w is not None and K.can_qk_norm_bwd_inplace(dqkv, Dh) and pre_q.dtype == dqkv.dtype and qn_w.dtype == kn_w.dtype:
             # per-head normalisation backward in place on the packed gradient: no head is copied out or back
             dqn = list(K.qk_norm_bwd_(dqkv, pre_q, pre_k, rstd_q, rstd_k, mean_q, mean_k, qn_w.detach(), kn_w.detach(), H, Dh,
                                       opt["qk_layernorm"], (need[10], has_qnb and need[11], need[12], has_knb and need[13])))
@@ -577,7 +680,7 @@ class AttentionSublayerFn(torch.autograd.Function):
             _attach_bf16(dx, shadow)
         if dgamma is not None and dgamma.dtype != g.dtype:
             dgamma = dgamma.to(g.dtype)
-        return (dx if need[0] else None, dnw, dnb, dwq, dbq, dwo, dbo, dgamma, None, None, *dqn, None)
+        return (dx if need[0] else None, dnw, dnb, dwq, dbq, dwo, dbo, dgamma, None, None, *dqn, None, drel)
 
 
 class CrossAttentionFn(torch.autograd.Function):
@@ -587,8 +690,8 @@ class CrossAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, kv, norm_w, norm_b, w_q, b_q, w_kv, b_kv, w_out, b_out, qn_w, qn_b, kn_w, kn_b, gamma, keep_idx,
-                rope_q, rope_k, opt):
-        L.require_gpu(q, kv, norm_w, w_q, w_kv, w_out)
+                rope_q, rope_k, opt, kv_len=None):
+        L.require_gpu(q, kv, norm_w, w_q, w_kv, w_out, kv_len)
         B, Lq, D = q.shape
         Lk = kv.shape[1]
         if kv.shape[0] != B or kv.shape[2] != D:
@@ -616,7 +719,23 @@ class CrossAttentionFn(torch.autograd.Function):
         kvp = torch.empty((Mk, 2 * D), dtype=tc, device=q.device)
         K.gemm(kv2, wkv, trans_a=False, trans_b=False, M=Mk, N=2 * D, K=D, out=kvp, bias=bkv)
         qk_saved = (None,) * 6
-        if qn_w is not None:   # per-head normalisation of q and k (vit/attention.py:25-41)
+        tq, emu_q = _rope_table(rope_q, keep_idx, B, Bk, tc)   # vit/attention.py:156-159
+        tk, emu_k = _rope_table(rope_k, keep_idx, B, Bk, tc)
+        if kv_len is not None and keep_idx is not None:
+            kv_len = kv_len.index_select(0, keep_idx)
+        # per-head normalisation and rotation of q and k in one pass into buffers of their own (v stays in the projection)
+        emus = {e for t, e in ((tq, emu_q), (tk, emu_k)) if t is not None}
+        fuse_pass = qn_w is not None and K.can_qk_norm_rope(tc, Dh) and qn_w.dtype == kn_w.dtype and len(emus) < 2
+        v_src = None
+        if fuse_pass:
+            raw_q, qp = qp, torch.empty_like(qp)
+            v_src, kvp = kvp, torch.empty_like(kvp)
+            K.qk_norm_rope_fwd(raw_q.view(Bk, Lq, H, Dh), v_src.view(Bk, Lk, 2, H, Dh)[:, :, 0], qp.view(Bk, Lq, H, Dh),
+                               kvp.view(Bk, Lk, 2, H, Dh)[:, :, 0], (qn_w.detach(), kn_w.detach()),
+                               (_cast(qn_b, qn_w.dtype), _cast(kn_b, kn_w.dtype)), (tq, tk), opt["qk_eps"], opt["qk_layernorm"],
+                               True, True in emus)
+            qk_saved = (raw_q, None, None, v_src, None, None)
+        elif qn_w is not None:   # per-head normalisation of q and k (vit/attention.py:25-41)
             pre_q = qp.view(Mq * H, Dh)
             nq, rq, mq = K.norm_fwd(pre_q, qn_w.detach(), None if qn_b is None else qn_b.detach(), opt["qk_eps"],
                                     opt["qk_layernorm"], tc)
@@ -626,16 +745,19 @@ class CrossAttentionFn(torch.autograd.Function):
                                     opt["qk_layernorm"], tc)
             kvp[:, :D].copy_(nk.view(Mk, D))
             qk_saved = (pre_q, rq, mq, pre_k, rk, mk)
-        tq, emu_q = _rope_table(rope_q, keep_idx, B, Bk, tc)   # vit/attention.py:156-159
-        tk, emu_k = _rope_table(rope_k, keep_idx, B, Bk, tc)
-        if tq is not None:
+        if tq is not None and not fuse_pass:
             if not qp.is_contiguous():
                 qp = qp.contiguous()
             K.rope_rows_(qp, tq, Bk, Lq, H, Dh, False, emu_q)
-        if tk is not None:
+        if tk is not None and not fuse_pass:
             K.rope_rows_(kvp, tk, Bk, Lk, H, Dh, False, emu_k)
         seed_a = next_seed(q.device) if p_attn > 0 else 0
-        o, lse = K.attn_cross_fwd(qp, kvp, Bk, Lq, Lk, H, Dh, Dh ** -0.5, p_attn, seed_a)
+        if kv_len is not None:
+            o, lse = K.attn_var_fwd(qp.view(Bk, Lq, H, Dh), *_kv_views(kvp, v_src, Bk, Lk, H, Dh), kv_len=kv_len,
+                                    scale=Dh ** -0.5, drop_p=p_attn, seed=seed_a)
+            o = o.view(Mq, D)
+        else:
+            o, lse = K.attn_cross_fwd(qp, kvp, Bk, Lq, Lk, H, Dh, Dh ** -0.5, p_attn, seed_a, v_src=v_src)
         seed_h = next_seed(q.device) if p_hid > 0 else 0
         g = _cast(gamma, tr)
         if residual:
@@ -646,8 +768,9 @@ class CrossAttentionFn(torch.autograd.Function):
             out, aux = _residual_gemm(o, wo, bo, zero, None, None, 1.0, p_hid, seed_h, want_aux=False)
             y = out.view(Bk, Lq, D)
         ctx.save_for_backward(q2, norm_w, rstd, mean, qn, kv2, qp, kvp, o, lse, wq, wkv, wo, g, aux, rows, keep_idx, qn_w, kn_w,
-                              tq, tk, *qk_saved)
+                              tq, tk, kv_len, *qk_saved)
         ctx.emu = (emu_q, emu_k)
+        ctx.fuse_pass = fuse_pass
         ctx.meta = (B, Bk, Lq, Lk, D, H, Dh, tc, tr, p_attn, p_hid, seed_a, seed_h, opt, q.dtype, kv.dtype, w_q.dtype,
                     norm_b is not None, b_q is not None, b_kv is not None, b_out is not None, qn_b is not None,
                     kn_b is not None)
@@ -655,8 +778,10 @@ class CrossAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dnew):
-        (q2, norm_w, rstd, mean, qn, kv2, qp, kvp, o, lse, wq, wkv, wo, g, aux, rows, keep_idx, qn_w, kn_w, tq, tk, pre_q,
+        (q2, norm_w, rstd, mean, qn, kv2, qp, kvp, o, lse, wq, wkv, wo, g, aux, rows, keep_idx, qn_w, kn_w, tq, tk, kv_len, pre_q,
          rstd_q, mean_q, pre_k, rstd_k, mean_k) = ctx.saved_tensors
+        fuse_pass = ctx.fuse_pass
+        v_src = pre_k if fuse_pass else None   # the projection of kv: keys before the pass, and the values
         (B, Bk, Lq, Lk, D, H, Dh, tc, tr, p_attn, p_hid, seed_a, seed_h, opt, qdtype, kvdtype, wdtype, has_nb, has_bq,
          has_bkv, has_bo, has_qnb, has_knb) = ctx.meta
         need = ctx.needs_input_grad
@@ -666,13 +791,27 @@ class CrossAttentionFn(torch.autograd.Function):
         dy, dgamma = _residual_grad(dnew2, tc, g if residual else None, rows if residual else None, Mq,
                                     opt["alpha"] if residual else 1.0, p_hid, seed_h, aux, need[14])
         do, dwo, dbo = _linear_bwd(dy, o, wo, True, need[8], has_bo and need[9], wdtype)
-        dqp, dkvp = K.attn_cross_bwd(qp, kvp, o, lse, do, Bk, Lq, Lk, H, Dh, Dh ** -0.5, p_attn, seed_a)
-        if tq is not None:
+        if kv_len is not None:
+            dqp, dkvp = torch.empty_like(qp), torch.empty_like(kvp)
+            gk, gv = _kv_views(dkvp, None, Bk, Lk, H, Dh)
+            hd = (Bk, Lq, H, Dh)
+            K.attn_var_bwd(qp.view(hd), *_kv_views(kvp, v_src, Bk, Lk, H, Dh), o.view(hd), lse, do.contiguous().view(hd),
+                           dq=dqp.view(hd), dk=gk, dv=gv, kv_len=kv_len, scale=Dh ** -0.5, drop_p=p_attn, seed=seed_a)
+        else:
+            dqp, dkvp = K.attn_cross_bwd(qp, kvp, o, lse, do, Bk, Lq, Lk, H, Dh, Dh ** -0.5, p_attn, seed_a, v_src=v_src)
+        if tq is not None and not fuse_pass:
             K.rope_rows_(dqp, tq, Bk, Lq, H, Dh, True, ctx.emu[0])
-        if tk is not None:
+        if tk is not None and not fuse_pass:
             K.rope_rows_(dkvp, tk, Bk, Lk, H, Dh, True, ctx.emu[1])
         dqn = [None, None, None, None]
-        if qn_w is not None:
+        if fuse_pass:
+            hq, gk = dqp.view(Bk, Lq, H, Dh), _kv_views(dkvp, None, Bk, Lk, H, Dh)[0]
+            dqn = list(K.qk_norm_rope_bwd((pre_q.view(Bk, Lq, H, Dh), _kv_views(v_src, None, Bk, Lk, H, Dh)[0]), (hq, gk), (hq, gk),
+                                          (qn_w.detach(), kn_w.detach()), (tq, tk), opt["qk_eps"],
+                                          opt["qk_layernorm"],
+                                          (need[10], has_qnb and need[11], need[12], has_knb and need[13]), True,
+                                          (ctx.emu[0] and tq is not None) or (ctx.emu[1] and tk is not None)))
+        elif qn_w is not None:
             dpre = torch.empty_like(dqp)
             dqn[0], dqn[1] = K.norm_bwd(dqp.view(Mq * H, Dh), pre_q, qn_w.detach(), rstd_q, mean_q, opt["qk_layernorm"], None,
                                         dpre.view(Mq * H, Dh), need[10], has_qnb and need[11])
@@ -706,7 +845,66 @@ class CrossAttentionFn(torch.autograd.Function):
         if dgamma is not None and dgamma.dtype != g.dtype:
             dgamma = dgamma.to(g.dtype)
         return (dq_in if need[0] else None, dkv_in, dnw, dnb, dwq, dbq, dwkv, dbkv, dwo, dbo, *dqn, dgamma, None, None, None,
-                None)
+                None, None)
+
+
+@torch.no_grad()
+def project_memory(kv, w_kv, b_kv, kn_w, kn_b, rope_k, head_dim, qk_eps, layernorm) -> Tensor:
+    """Keys (normalised and rotated where asked) and values of a memory [B, Lk, D] as [B, Lk, 2, H, Dh]: the kv half of
+    vit/attention.py:112-162, kept by callers for later queries."""
+    L.require_gpu(kv, w_kv, b_kv)
+    B, Lk, D = kv.shape
+    H = D // head_dim
+    tc = compute_dtype(w_kv.dtype)
+    kvp = torch.empty((B * Lk, 2 * D), dtype=tc, device=kv.device)
+    K.gemm(_cast(kv.reshape(B * Lk, D), tc), _cast(w_kv, tc), trans_a=False, trans_b=False, M=B * Lk, N=2 * D, K=D, out=kvp,
+           bias=_cast(b_kv, tc))
+    table, emu = _rope_table(rope_k, None, B, B, tc)
+    keys = kvp.view(B, Lk, 2, H, head_dim)[:, :, 0]
+    _norm_rope_(keys, kvp, kn_w, kn_b, table, emu, qk_eps, layernorm)
+    return kvp.view(B, Lk, 2, H, head_dim)
+
+
+def _norm_rope_(heads: Tensor, rows: Tensor, w, b, table, emu, eps, layernorm) -> None:
+    """In place on ``heads`` [B, L, H, Dh], the first H * Dh columns of ``rows`` [B * L, ...]: per-head normalisation
+    (w not None), then rotation (table not None), as the layers' forward does it."""
+    B, Ln, H, Dh = heads.shape
+    if w is not None and K.can_qk_norm_rope(heads.dtype, Dh):
+        K.qk_norm_rope_fwd(heads, None, heads, None, (w.detach(), None), (_cast(b, w.dtype), None), (table, None), eps, layernorm,
+                           True, emu)
+        return
+    if w is not None:
+        pre = heads.reshape(B * Ln * H, Dh).contiguous()
+        nrm = K.norm_fwd(pre, w.detach(), None if b is None else b.detach(), eps, layernorm, heads.dtype)[0]
+        heads.copy_(nrm.view(B, Ln, H, Dh))
+    if table is not None:
+        K.rope_rows_(rows, table, B, Ln, H, Dh, False, emu)
+
+
+@torch.no_grad()
+def cross_attention_from_memory(q, memory, kv_len, norm_w, norm_b, eps, w_q, b_q, w_out, b_out, qn_w, qn_b, qk_eps, layernorm,
+                                rope_q, gamma, residual) -> Tensor:
+    """q -> (q +) gamma * out_proj(attention(q_proj(norm(q)), memory)) over a memory of ``project_memory``; inference."""
+    L.require_gpu(q, memory, norm_w, w_q, w_out, kv_len)
+    B, Lq, D = q.shape
+    Lk, H, Dh = memory.shape[1], memory.shape[3], memory.shape[4]
+    tc = compute_dtype(w_q.dtype)
+    if memory.dtype != tc:
+        raise TypeError(f"vit_amd: the memory was projected in {memory.dtype}, this call computes in {tc}")
+    tr = _residual_dtype(q, gamma, tc) if residual else tc
+    M = B * Lq
+    q2 = _cast(q.reshape(M, D), tr if residual else q.dtype)
+    qn = K.norm_fwd(q2, norm_w.detach(), None if norm_b is None else norm_b.detach(), eps, layernorm, tc)[0]
+    qp = torch.empty((M, D), dtype=tc, device=q.device)
+    K.gemm(qn, _cast_param(w_q, tc), trans_a=False, trans_b=False, M=M, N=D, K=D, out=qp, bias=_cast_param(b_q, tc))
+    table, emu = _rope_table(rope_q, None, B, B, tc)
+    heads = qp.view(B, Lq, H, Dh)
+    _norm_rope_(heads, qp, qn_w, qn_b, table, emu, qk_eps, layernorm)
+    o = K.attn_var_fwd(heads, memory[:, :, 0], memory[:, :, 1], kv_len=kv_len, scale=Dh ** -0.5)[0].view(M, D)
+    res = q2 if residual else torch.zeros((M, D), dtype=tc, device=q.device)
+    out, _ = _residual_gemm(o, _cast_param(w_out, tc), _cast_param(b_out, tc), res, _cast(gamma, tr) if residual else None, None, 1.0,
+                            0.0, 0, want_aux=False)
+    return out.view(B, Lq, D)
 
 
 def _weights_dtype(tc: torch.dtype) -> torch.dtype:

@@ -112,3 +112,97 @@ def create_position_encoder(pos_enc: str, hidden_size: int, spatial_size: Sequen
     if pos_enc == "rope":
         raise ValueError("Please create RoPE position encoder manually")
     raise ValueError(f"Invalid position encoder: {pos_enc}")
+
+
+# ------------------------------------------------------------------------------------------------------------------------
+# relative positions
+# ------------------------------------------------------------------------------------------------------------------------
+class RelativeBuckets:
+    """Bucket number of every (query, key) pair, and the order in which the gradient of a bias table sums the pairs.
+
+    ``index`` [Lq, Lk] holds integers in [0, num_buckets), num_buckets <= 65536.  The plan is built once (it reads the
+    index on the host) and used by every call of every layer with these positions: ``index16`` the numbers in 16 bits,
+    ``order`` the pairs sorted by bucket, ``piece`` / ``bucket_piece`` the runs of at most ``PIECE`` pairs that are summed
+    at a time and the runs of each bucket."""
+
+    PIECE = 2048
+
+    def __init__(self, index: Tensor, num_buckets: int):
+        if index.dim() != 2 or index.dtype in (torch.bool, torch.uint16, torch.uint32, torch.uint64) or index.is_floating_point() \
+                or index.is_complex():
+            raise ValueError(f"bucket index must be an integer tensor [Lq, Lk], got {index.dtype} {tuple(index.shape)}")
+        if index.numel() == 0:
+            raise ValueError("bucket index is empty")
+        if index.numel() >= 2 ** 31:
+            raise ValueError(f"bucket index of {index.numel()} pairs is too large (2^31)")
+        if not 1 <= num_buckets <= 65536:
+            raise ValueError(f"num_buckets must be in [1, 65536], got {num_buckets}")
+        flat = index.detach().reshape(-1).to(torch.int32)
+        lo, hi = (int(v) for v in torch.stack([index.min(), index.max()]).tolist())
+        if lo < 0 or hi >= num_buckets:
+            raise ValueError(f"bucket numbers must be in [0, {num_buckets}), got {lo} .. {hi}")
+        self.shape = tuple(index.shape)
+        self.num_buckets = int(num_buckets)
+        self.index16 = torch.where(flat >= 32768, flat - 65536, flat).to(torch.int16).view(self.shape)
+        self.order = torch.sort(flat, stable=True).indices.to(torch.int32)
+        counts = torch.bincount(flat, minlength=num_buckets).cpu()
+        pieces = (counts + self.PIECE - 1) // self.PIECE
+        bucket_piece = torch.cat([pieces.new_zeros(1), pieces.cumsum(0)])
+        starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+        owner = torch.repeat_interleave(torch.arange(num_buckets), pieces)          # bucket of every piece
+        within = torch.arange(int(bucket_piece[-1])) - bucket_piece[owner]
+        piece = torch.cat([starts[owner] + within * self.PIECE, starts[-1:]])
+        self.num_pieces = int(bucket_piece[-1])
+        self.piece = piece.to(torch.int32).to(index.device)
+        self.bucket_piece = bucket_piece.to(torch.int32).to(index.device)
+
+    @property
+    def device(self) -> torch.device:
+        return self.index16.device
+
+    def to(self, device) -> "RelativeBuckets":
+        """The same plan on another device."""
+        new = object.__new__(RelativeBuckets)
+        new.__dict__.update({k: v.to(device) if isinstance(v, Tensor) else v for k, v in self.__dict__.items()})
+        return new
+
+    @classmethod
+    def grid(cls, dims: Sequence[int], num_prefix_tokens: int = 0, device=None, table_dims: Optional[Sequence[int]] = None):
+        """Tokens of a grid behind ``num_prefix_tokens`` prefix tokens: a bucket for every offset between two grid tokens of
+        a ``table_dims`` grid (default: ``dims`` itself), and with a prefix three more, for grid token after prefix token
+        (query, key) pairs: prefix to grid, grid to prefix, prefix to prefix."""
+        dims = tuple(int(d) for d in dims)
+        table_dims = tuple(int(d) for d in (table_dims or dims))
+        if len(dims) != len(table_dims) or any(d < 1 or d > t for d, t in zip(dims, table_dims)):
+            raise ValueError(f"a table for grids up to {table_dims} does not cover a {dims} grid")
+        pos = torch.stack(torch.meshgrid([torch.arange(d) for d in dims], indexing="ij"), dim=-1).view(-1, len(dims))
+        num = cls.grid_buckets(table_dims, num_prefix_tokens)
+        idx = torch.zeros((pos.shape[0], pos.shape[0]), dtype=torch.int64)
+        for axis, t in enumerate(table_dims):
+            idx = idx * (2 * t - 1) + (pos[:, None, axis] - pos[None, :, axis] + t - 1)
+        n = int(num_prefix_tokens)
+        if n:
+            full = torch.empty((n + pos.shape[0],) * 2, dtype=torch.int64)
+            full[n:, n:], full[:n, n:], full[n:, :n], full[:n, :n] = idx, num - 3, num - 2, num - 1
+            idx = full
+        return cls(idx.to(device) if device is not None else idx, num)
+
+    @staticmethod
+    def grid_buckets(table_dims: Sequence[int], num_prefix_tokens: int = 0) -> int:
+        return math.prod(2 * int(t) - 1 for t in table_dims) + (3 if num_prefix_tokens else 0)
+
+    @classmethod
+    def log_distance(cls, num_queries: int, num_keys: int, num_buckets: int = 32, max_distance: int = 128, device=None):
+        """Buckets of the signed distance key - query in a sequence: half of them for keys behind the query; of each half
+        the first half are single distances, the others grow logarithmically up to ``max_distance``."""
+        half = num_buckets // 2
+        exact = half // 2
+        if num_buckets % 4 or num_buckets < 4 or max_distance <= exact:
+            raise ValueError(f"log_distance needs num_buckets a multiple of 4 and max_distance > num_buckets / 4, got "
+                             f"{num_buckets}, {max_distance}")
+        far = max(num_queries, num_keys)
+        d = torch.arange(max(far, 1), dtype=torch.float64)
+        log = exact + torch.floor(torch.log(d.clamp_min(1) / exact) / math.log(max_distance / exact) * (half - exact) + 1e-9)
+        table = torch.where(d < exact, d, log.clamp_max(half - 1)).to(torch.int64).to(device)
+        rel = torch.arange(num_keys, device=device)[None, :] - torch.arange(num_queries, device=device)[:, None]
+        return cls(table[rel.abs()] + half * (rel > 0), num_buckets)

@@ -7,16 +7,17 @@ fused into the norm kernel's load and the scaled scatter-add into the out_proj /
 from __future__ import annotations
 
 import collections
-from typing import Any, Optional
+from typing import Any, Optional, Union
 
 import torch
 import torch.nn as nn
 from torch import Tensor
 
-from .attention import CrossAttention, SelfAttention
+from .attention import CrossAttention, KVMemory, SelfAttention
 from .fused import NormMLP
 from .initialization import zero_bias_if_present
 from .layer_scale import LayerScale
+from .pos_enc import RelativeBuckets
 
 
 def drop_path_keep_count(batch_size: int, drop_path_rate: float) -> int:
@@ -86,13 +87,13 @@ class TransformerEncoderLayer(nn.Module):
                  layer_scale: Optional[float] = None, glu_limit: Optional[float] = None,
                  glu_extra_bias: Optional[float] = None, mlp_quantization_config: Any = None,
                  qkv_quantization_config: Any = None, attn_quantization_config: Any = None, device=None, dtype=None,
-                 norm_type: str = "rmsnorm", qk_normalization: bool = False):
+                 norm_type: str = "rmsnorm", qk_normalization: bool = False, relative_buckets: int = 0):
         super().__init__()
         kw = {"device": device, "dtype": dtype}
         self.drop_path_rate = drop_path_rate
         self.self_attention = SelfAttention(hidden_size, num_attention_heads, hidden_dropout, attention_dropout,
                                             bias=attention_bias, eps=eps, norm_type=norm_type,
-                                            qk_normalization=qk_normalization, **kw)
+                                            qk_normalization=qk_normalization, relative_buckets=relative_buckets, **kw)
         self.mlp = NormMLP(hidden_size, ffn_hidden_size, bias=mlp_bias, activation=activation, eps=eps,
                            dropout=hidden_dropout, limit=glu_limit, extra_bias=glu_extra_bias, norm_type=norm_type, **kw)
         if layer_scale is not None:
@@ -109,11 +110,12 @@ class TransformerEncoderLayer(nn.Module):
         if any(c is not None for c in (mlp_quantization_config, qkv_quantization_config, attn_quantization_config)):
             raise NotImplementedError("vit_amd: torchao quantization is outside the encoder hot path")
 
-    def forward(self, x: Tensor, rope: Optional[Tensor] = None) -> Tensor:
+    def forward(self, x: Tensor, rope: Optional[Tensor] = None, buckets: Optional[RelativeBuckets] = None) -> Tensor:
+        """``buckets``: the plan of the relative position bias, for a layer built with ``relative_buckets``."""
         g_attn = getattr(self.layer_scale_attn, "gamma", None)
         g_mlp = getattr(self.layer_scale_mlp, "gamma", None)
         idx, scale = _select_keep_indices(x, self.drop_path_rate, self.training)
-        x = self.self_attention.fused_residual(x, rope, g_attn, idx, scale)
+        x = self.self_attention.fused_residual(x, rope, g_attn, idx, scale, buckets)
         idx, scale = _select_keep_indices(x, self.drop_path_rate, self.training)
         return self.mlp.fused_residual(x, g_mlp, idx, scale)
 
@@ -132,13 +134,13 @@ class TransformerDecoderLayer(nn.Module):
                  layer_scale: Optional[float] = None, glu_limit: Optional[float] = None,
                  glu_extra_bias: Optional[float] = None, mlp_quantization_config: Any = None,
                  qkv_quantization_config: Any = None, attn_quantization_config: Any = None, device=None, dtype=None,
-                 norm_type: str = "rmsnorm", qk_normalization: bool = False):
+                 norm_type: str = "rmsnorm", qk_normalization: bool = False, relative_buckets: int = 0):
         super().__init__()
         kw = {"device": device, "dtype": dtype}
         self.drop_path_rate = drop_path_rate
         self.self_attention = SelfAttention(hidden_size, num_attention_heads, hidden_dropout, attention_dropout,
                                             bias=attention_bias, eps=eps, norm_type=norm_type,
-                                            qk_normalization=qk_normalization, **kw)
+                                            qk_normalization=qk_normalization, relative_buckets=relative_buckets, **kw)
         self.cross_attention = CrossAttention(hidden_size, num_attention_heads, hidden_dropout, attention_dropout,
                                               bias=attention_bias, eps=eps, norm_type=norm_type,
                                               qk_normalization=qk_normalization, **kw)
@@ -155,12 +157,16 @@ class TransformerDecoderLayer(nn.Module):
         if any(c is not None for c in (mlp_quantization_config, qkv_quantization_config, attn_quantization_config)):
             raise NotImplementedError("vit_amd: torchao quantization is outside the encoder hot path")
 
-    def forward(self, x: Tensor, kv: Tensor, rope_q: Optional[Tensor] = None, rope_k: Optional[Tensor] = None) -> Tensor:
+    def forward(self, x: Tensor, kv: Union[Tensor, KVMemory], rope_q: Optional[Tensor] = None,
+                rope_k: Optional[Tensor] = None, kv_lengths: Optional[Tensor] = None,
+                buckets: Optional[RelativeBuckets] = None) -> Tensor:
+        """``kv_lengths`` [B]: the rows of ``kv`` each sample has, the others are padding.  ``kv`` may be what
+        ``cross_attention.project_kv`` made of it (inference).  ``buckets``: the relative position bias of x's tokens."""
         idx, scale = _select_keep_indices(x, self.drop_path_rate, self.training)
-        x = self.self_attention.fused_residual(x, rope_q, getattr(self.layer_scale_attn, "gamma", None), idx, scale)
+        x = self.self_attention.fused_residual(x, rope_q, getattr(self.layer_scale_attn, "gamma", None), idx, scale, buckets)
         idx, scale = _select_keep_indices(x, self.drop_path_rate, self.training)
         x = self.cross_attention.fused_residual(x, kv, getattr(self.layer_scale_cross, "gamma", None), idx, scale,
-                                                rope_q, rope_k)
+                                                rope_q, rope_k, kv_lengths)
         idx, scale = _select_keep_indices(x, self.drop_path_rate, self.training)
         return self.mlp.fused_residual(x, getattr(self.layer_scale_mlp, "gamma", None), idx, scale)
 
@@ -193,9 +199,10 @@ class CrossAttentionTransformer(nn.Module):
         if any(c is not None for c in (mlp_quantization_config, qkv_quantization_config, attn_quantization_config)):
             raise NotImplementedError("vit_amd: torchao quantization is outside the encoder hot path")
 
-    def forward(self, x: Tensor, kv: Tensor, rope_q: Optional[Tensor] = None, rope_k: Optional[Tensor] = None) -> Tensor:
+    def forward(self, x: Tensor, kv: Union[Tensor, KVMemory], rope_q: Optional[Tensor] = None,
+                rope_k: Optional[Tensor] = None, kv_lengths: Optional[Tensor] = None) -> Tensor:
         idx, scale = _select_keep_indices(x, self.drop_path_rate, self.training)
         x = self.cross_attention.fused_residual(x, kv, getattr(self.layer_scale_cross, "gamma", None), idx, scale,
-                                                rope_q, rope_k)
+                                                rope_q, rope_k, kv_lengths)
         idx, scale = _select_keep_indices(x, self.drop_path_rate, self.training)
         return self.mlp.fused_residual(x, getattr(self.layer_scale_mlp, "gamma", None), idx, scale)

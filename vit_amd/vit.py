@@ -21,6 +21,7 @@ from .head import AttentivePoolHeadConfig, HeadConfig
 from .initialization import trunc_normal_
 from .norm import make_norm
 from .patch_embed import PatchEmbed2d, PatchEmbed3d
+from .pos_enc import RelativeBuckets
 from .rope import RopePositionEmbedding
 from .tokens import apply_mask, create_mask
 from .transformer import CrossAttentionTransformer, TransformerDecoderLayer, TransformerEncoderLayer
@@ -42,10 +43,11 @@ class ViT(nn.Module):
             raise NotImplementedError("vit_amd: torchao quantization is outside the encoder hot path")
         kw = {"device": device, "dtype": config.dtype}
         self._config = config
+        self._bucket_plans: dict = {}   # (token grid, device) -> RelativeBuckets
         D = config.hidden_size
         stem_type = PatchEmbed2d if len(config.patch_size) == 2 else PatchEmbed3d
         self.stem = stem_type(config.in_channels, D, config.patch_size, config.img_size,
-                                 pos_enc="none" if config.pos_enc == "rope" else config.pos_enc, **kw)
+                                 pos_enc="none" if config.pos_enc in ("rope", "relative") else config.pos_enc, **kw)
         self.patch_embed_norm = make_norm(D, config.norm_type, **kw) if config.patch_embed_normalization else None
         self.rope = None
         if config.pos_enc == "rope":
@@ -70,7 +72,29 @@ class ViT(nn.Module):
     def config(self) -> ViTConfig:
         return self._config
 
-    def _layer(self, layer_type, mlp_quantization_config, qkv_quantization_config, attn_quantization_config, device, dtype):
+    @property
+    def _num_prefix(self) -> int:
+        return self._config.num_cls_tokens + self._config.num_register_tokens
+
+    def _relative_buckets(self) -> int:
+        """Rows of every block's relative bias table (pos_enc "relative": learned, one per offset in the configured grid)."""
+        if self._config.pos_enc != "relative":
+            return 0
+        return RelativeBuckets.grid_buckets(self.stem.tokenized_size(tuple(self._config.img_size)), self._num_prefix)
+
+    def prepare_buckets(self, tokenized_size: Sequence[int]) -> RelativeBuckets:
+        """Plan of the relative position bias for a token grid up to the configured one; kept per grid and device."""
+        full = tuple(self.stem.tokenized_size(tuple(self._config.img_size)))
+        key = (tuple(tokenized_size), self.cls_tokens.device)
+        plan = self._bucket_plans.get(key)
+        if plan is None:
+            plan = RelativeBuckets.grid(key[0], self._num_prefix, device=key[1], table_dims=full)
+            while len(self._bucket_plans) >= 8:
+                self._bucket_plans.pop(next(iter(self._bucket_plans)))
+            self._bucket_plans[key] = plan
+        return plan
+
+    def _layer(self, layer_type, mlp_quantization_config, qkv_quantization_config, attn_quantization_config, device, dtype, **extra):
         c = self._config
         return layer_type(
             c.hidden_size, c.ffn_hidden_size, c.num_attention_heads, hidden_dropout=c.hidden_dropout,
@@ -79,12 +103,12 @@ class ViT(nn.Module):
             drop_path_rate=c.drop_path_rate, layer_scale=c.layer_scale, glu_limit=c.glu_limit,
             glu_extra_bias=c.glu_extra_bias, mlp_quantization_config=mlp_quantization_config,
             qkv_quantization_config=qkv_quantization_config, attn_quantization_config=attn_quantization_config,
-            device=device, dtype=c.dtype if dtype is None else dtype)
+            device=device, dtype=c.dtype if dtype is None else dtype, **extra)
 
     def create_encoder_layer(self, mlp_quantization_config: Any = None, qkv_quantization_config: Any = None,
                              attn_quantization_config: Any = None, device=None, dtype=None) -> TransformerEncoderLayer:
         return self._layer(TransformerEncoderLayer, mlp_quantization_config, qkv_quantization_config,
-                           attn_quantization_config, device, dtype)
+                           attn_quantization_config, device, dtype, relative_buckets=self._relative_buckets())
 
     def create_decoder_layer(self, mlp_quantization_config: Any = None, qkv_quantization_config: Any = None,
                              attn_quantization_config: Any = None, device=None, dtype=None) -> TransformerDecoderLayer:
@@ -158,6 +182,11 @@ class ViT(nn.Module):
                 output_norm: bool = True) -> ViTFeatures:
         c = self._config
         grid = self.stem.tokenized_size(x.shape[2:])
+        buckets = None
+        if c.pos_enc == "relative":
+            if mask is not None:
+                raise NotImplementedError("vit_amd: token masks with a relative position bias (a plan per sample)")
+            buckets = self.prepare_buckets(grid)
         if mask is None and self.patch_embed_norm is None:
             # nothing stands between the patch embedding and the concatenation: its GEMM writes the patch rows straight
             # into the sequence, behind the prefix tokens
@@ -172,9 +201,9 @@ class ViT(nn.Module):
         for block in self.blocks:
             assert isinstance(block, TransformerEncoderLayer)
             if c.activation_checkpointing and self.training:
-                x = checkpoint(block, x, rope, use_reentrant=False)
+                x = checkpoint(block, x, rope, buckets, use_reentrant=False)
             else:
-                x = block(x, rope=rope)
+                x = block(x, rope=rope, buckets=buckets)
         if output_norm:
             x = self.output_norm(x)
         return ViTFeatures(x, c.num_register_tokens, c.num_cls_tokens, grid)
