@@ -334,8 +334,9 @@ int vitk_qk_norm_rope_bwd(const VitkQkNormRope* a, void* stream);
  *   S[i,j] = scale * q_i k_j + table[index[i,j], h],  j < kv_len[b];   P = softmax(S) (dropout on P);   o_i = sum_j P v_j
  * bias_table [num_buckets, H] and bias_index [Lq, Lk] may be NULL (no bias), kv_len [B] may be NULL (all Lk keys); counts
  * are clamped to [0, Lk].  Keys at or beyond the count are never read; their dk and dv are written as zeros.  A row that
- * has no key left, or only keys with a bias of -inf, gives o = 0 and zero gradients (lse = +inf).  Finite table entries
- * beyond +-1e37 count as +-1e37.
+ * has no key left, or only keys with a bias of -inf, gives o = 0 and zero gradients.  Finite table entries beyond
+ * +-min(1e37, 1e38 scale) count as that limit.  `stat` receives two values per row that bwd takes back: the maximum the
+ * exponentials were taken with, in units of 1 / scale, and -log2 of their sum (0 and -inf for a row without keys).
  * Every operand has (batch, head, row) strides of its own, d contiguous.  head_dim <= 128.
  * bwd: dbias_table [num_buckets, H] (or NULL) is summed over the pairs of a bucket in a fixed order given by the plan
  * order / piece / bucket_piece: `order` holds the pair numbers i * Lk + j sorted by bucket, piece p covers order[piece[p]
@@ -346,7 +347,7 @@ typedef struct VitkAttnVar {
   void* o;
   const void* dout;
   void *dq, *dk, *dv;
-  float* lse;                   /* [B, H, Lq] */
+  float* stat;                  /* [B, H, Lq, 2] */
   const int32_t* kv_len;
   const void* bias_table;       /* [num_buckets, H], dtype */
   const uint16_t* bias_index;   /* [Lq, Lk] */

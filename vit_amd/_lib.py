@@ -85,7 +85,7 @@ class VitkQkNormRope(C.Structure):
 class VitkAttnVar(C.Structure):
     _fields_ = [
         ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("dout", C.c_void_p),
-        ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("lse", C.c_void_p), ("kv_len", C.c_void_p),
+        ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("stat", C.c_void_p), ("kv_len", C.c_void_p),
         ("bias_table", C.c_void_p), ("bias_index", C.c_void_p), ("dbias_table", C.c_void_p),
         ("order", C.c_void_p), ("piece", C.c_void_p), ("bucket_piece", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),

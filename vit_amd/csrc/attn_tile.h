@@ -22,7 +22,7 @@ template <int DHP> struct Strides {
 // a 16-byte chunk beyond the head dimension is given an offset past any size (the host keeps S * stride below 2^30 B).
 constexpr uint32_t OOB_OFF = 0xC0000000u;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const bf16* g, int64_t ss, int S, int Dh) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)g, 0, (int)(((int64_t)(S - 1) * ss + Dh) * 2), 0x00020000);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)g, 0, S > 0 ? (int)(((int64_t)(S - 1) * ss + Dh) * 2) : 0, 0x00020000);
 }
 __device__ __forceinline__ uint4 buf_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
   return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));

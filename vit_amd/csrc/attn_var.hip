@@ -4,38 +4,9 @@
 //   dV = P^T dO,  dP = dO V^T,  dS = P (dP - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q,
 //   dT[n, h] = sum over samples and over the pairs (i, j) of bucket n of dS
 //
-// Portable kernels (any dtype, head_dim <= 128, any strides, fp32 math): 64 stationary rows per workgroup, 4 threads per row.
-#include "attn_tile.h"
-
-struct VarP {
-  const void *q, *k, *v, *dout;
-  void *o, *dq, *dk, *dv;
-  float *lse, *delta;
-  const int32_t* kv_len;
-  const void* table;
-  const uint16_t* index;
-  float* dbias;   // [splits][H][Lq][Lk]
-  int64_t q_sb, q_sh, q_ss, k_sb, k_sh, k_ss, v_sb, v_sh, v_ss, o_sb, o_sh, o_ss, g_sb, g_sh, g_ss;
-  int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
-  int B, H, Lq, Lk, Dh;
-  uint64_t seed;
-  float scale, keep_scale;
-  uint32_t thr;
-};
-
-__device__ __forceinline__ int key_count(const VarP& p, int64_t b) {
-  if (!p.kv_len) return p.Lk;
-  const int n = p.kv_len[b];
-  return n < 0 ? 0 : n > p.Lk ? p.Lk : n;
-}
-// Finite entries beyond +-1e37 are pulled in so that a bias keeps its order against the scores after the multiplication by
-// 1 / scale; -inf, +inf and NaN pass.
-__device__ __forceinline__ float clamp_bias(float x) {
-  const float a = fabsf(x);
-  return a > 1e37f && a < INFINITY ? copysignf(1e37f, x) : x;
-}
-// dropout counter of (row, key): as in attn.hip, row * (Lk rounded up to even) + key
-__device__ __forceinline__ uint64_t var_drop_ld(const VarP& p) { return (uint64_t)((p.Lk + 1) & ~1); }
+// This file: the portable kernels (any dtype, head_dim <= 128, any strides, fp32 math; 64 stationary rows per workgroup, 4
+// threads per row), the bucket sums and the entry points.  attn_var_fwd.hip, attn_var_bwd.hip: bf16 on the matrix units.
+#include "attn_var.h"
 
 constexpr int VMAXI = 32;  // head_dim <= 128
 constexpr int VT = 32;     // streamed rows per LDS tile
@@ -52,8 +23,9 @@ __device__ __forceinline__ float vquad_sum(float v) {
   v += __shfl_xor(v, 2, 64);
   return v;
 }
+// bias of a pair in units of 1 / scale
 template <class T> __device__ __forceinline__ float var_bias(const VarP& p, int64_t i, int64_t j, int64_t h) {
-  return p.table ? clamp_bias(to_f<T>(((const T*)p.table)[(int64_t)p.index[i * p.Lk + j] * p.H + h])) : 0.f;
+  return p.table ? clamp_bias(to_f<T>(((const T*)p.table)[(int64_t)p.index[i * p.Lk + j] * p.H + h]), p.bias_lim) * p.inv_scale : 0.f;
 }
 
 template <class T>
@@ -76,6 +48,7 @@ __global__ __launch_bounds__(256) void var_fwd_simple_k(VarP p) {
     o[i] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
+  const float c = p.scale * LOG2E;
   const int64_t srow = (b * p.H + h) * p.Lq + qrow;
   const uint64_t rbase = (uint64_t)srow * var_drop_ld(p);
   for (int64_t k0 = 0; k0 < len; k0 += VT) {
@@ -91,11 +64,11 @@ __global__ __launch_bounds__(256) void var_fwd_simple_k(VarP p) {
         const int d = part + 4 * i;
         if (d < Dh) s = fmaf(q[i], Ks[kk * Dh + d], s);
       }
-      s = vquad_sum(s) * p.scale;
+      s = vquad_sum(s);
       if (qv) s += var_bias<T>(p, qrow, k0 + kk, h);
       if (s == -INFINITY) continue;   // nothing of this key (the whole quad skips together)
       const float mn = fmaxf(m, s);
-      const float a = expf(m - mn), pr = expf(s - mn);
+      const float a = exp2f(__fmul_rn(m - mn, c)), pr = exp2f(__fmul_rn(s - mn, c));
       l = l * a + pr;
       m = mn;
       float pd = pr;
@@ -115,7 +88,7 @@ __global__ __launch_bounds__(256) void var_fwd_simple_k(VarP p) {
     const int d = part + 4 * i;
     if (d < Dh) op[d] = from_f<T>(o[i] * inv);
   }
-  if (part == 0) p.lse[srow] = l == 0.f ? INFINITY : m + logf(l);
+  if (part == 0) { p.stat[2 * srow] = l == 0.f ? 0.f : m; p.stat[2 * srow + 1] = l == 0.f ? -INFINITY : -log2f(l); }
 }
 
 // delta[b,h,i] = sum_d dO O   (a wave per row)
@@ -155,7 +128,8 @@ __global__ __launch_bounds__(256) void var_dq_simple_k(VarP p) {
     dq[i] = 0.f;
   }
   const int64_t srow = (b * p.H + h) * p.Lq + qrow;
-  const float lse = qv ? p.lse[srow] : 0.f, delta = qv ? p.delta[srow] : 0.f;
+  const float m = qv ? p.stat[2 * srow] : 0.f, lr = qv ? p.stat[2 * srow + 1] : 0.f, delta = qv ? p.delta[srow] : 0.f;
+  const float c = p.scale * LOG2E;
   const uint64_t rbase = (uint64_t)srow * var_drop_ld(p);
   for (int64_t k0 = 0; k0 < len; k0 += VT) {
     __syncthreads();
@@ -170,10 +144,10 @@ __global__ __launch_bounds__(256) void var_dq_simple_k(VarP p) {
         const int d = part + 4 * i;
         if (d < Dh) { s = fmaf(q[i], Ks[kk * Dh + d], s); dp = fmaf(g[i], Vs[kk * Dh + d], dp); }
       }
-      s = vquad_sum(s) * p.scale;
+      s = vquad_sum(s);
       dp = vquad_sum(dp);
       if (qv) s += var_bias<T>(p, qrow, k0 + kk, h);
-      const float pr = expf(s - lse);
+      const float pr = exp2f(__fmul_rn(s - m, c) + lr);
       if (p.thr) dp = rng_u32(p.seed, rbase + (uint64_t)(k0 + kk)) >= p.thr ? dp * p.keep_scale : 0.f;
       const float ds = pr * (dp - delta);
 #pragma unroll
@@ -199,7 +173,8 @@ __global__ __launch_bounds__(256) void var_dkdv_simple_k(VarP p) {
   const int64_t b = blockIdx.z, h = blockIdx.y, krow = (int64_t)blockIdx.x * 64 + (tid >> 2);
   float* Qs = sm;
   float* Gs = sm + VT * Dh;
-  float* Ls = sm + 2 * VT * Dh;   // lse[VT], delta[VT]
+  float* Ls = sm + 2 * VT * Dh;   // m[VT], lr[VT], delta[VT]
+  const float c = p.scale * LOG2E;
   const T* qp = (const T*)p.q + b * p.q_sb + h * p.q_sh;
   const T* kp = (const T*)p.k + b * p.k_sb + h * p.k_sh;
   const T* vp = (const T*)p.v + b * p.v_sb + h * p.v_sh;
@@ -222,8 +197,9 @@ __global__ __launch_bounds__(256) void var_dkdv_simple_k(VarP p) {
     vload_tile<T>(Gs, gp, p.g_ss, q0, p.Lq, Dh, tid);
     if (tid < VT) {
       const bool ok = q0 + tid < p.Lq;
-      Ls[tid] = ok ? p.lse[sbase + q0 + tid] : 0.f;
-      Ls[VT + tid] = ok ? p.delta[sbase + q0 + tid] : 0.f;
+      Ls[tid] = ok ? p.stat[2 * (sbase + q0 + tid)] : 0.f;
+      Ls[VT + tid] = ok ? p.stat[2 * (sbase + q0 + tid) + 1] : 0.f;
+      Ls[2 * VT + tid] = ok ? p.delta[sbase + q0 + tid] : 0.f;
     }
     __syncthreads();
     const int nq = (int)(p.Lq - q0 < VT ? p.Lq - q0 : VT);
@@ -234,17 +210,17 @@ __global__ __launch_bounds__(256) void var_dkdv_simple_k(VarP p) {
         const int d = part + 4 * i;
         if (d < Dh) { s = fmaf(k[i], Qs[qq * Dh + d], s); dp = fmaf(v[i], Gs[qq * Dh + d], dp); }
       }
-      s = vquad_sum(s) * p.scale;
+      s = vquad_sum(s);
       dp = vquad_sum(dp);
       if (kv) s += var_bias<T>(p, q0 + qq, krow, h);
-      const float pr = kv ? expf(s - Ls[qq]) : 0.f;
+      const float pr = kv ? exp2f(__fmul_rn(s - Ls[qq], c) + Ls[VT + qq]) : 0.f;
       float pd = pr;
       if (p.thr) {
         const bool keep = rng_u32(p.seed, (uint64_t)(sbase + q0 + qq) * var_drop_ld(p) + (uint64_t)krow) >= p.thr;
         pd = keep ? pr * p.keep_scale : 0.f;
         dp = keep ? dp * p.keep_scale : 0.f;
       }
-      const float ds = pr * (dp - Ls[VT + qq]);
+      const float ds = pr * (dp - Ls[2 * VT + qq]);
 #pragma unroll
       for (int i = 0; i < VMAXI; i++) {
         const int d = part + 4 * i;
@@ -280,7 +256,7 @@ __global__ __launch_bounds__(256) void var_dbias_simple_k(VarP p) {
     float s = 0.f, dp = 0.f;
     for (int d = 0; d < p.Dh; d++) { s = fmaf(to_f<T>(q[d]), to_f<T>(k[d]), s); dp = fmaf(to_f<T>(g[d]), to_f<T>(v[d]), dp); }
     const int64_t srow = (b * p.H + h) * p.Lq + i;
-    const float pr = expf(fmaf(s, p.scale, bias) - p.lse[srow]);
+    const float pr = exp2f(__fmul_rn(s + bias - p.stat[2 * srow], p.scale * LOG2E) + p.stat[2 * srow + 1]);
     if (p.thr) dp = rng_u32(p.seed, (uint64_t)srow * var_drop_ld(p) + (uint64_t)j) >= p.thr ? dp * p.keep_scale : 0.f;
     sum += pr * (dp - p.delta[srow]);
   }
@@ -317,19 +293,34 @@ __global__ __launch_bounds__(256) void var_bucket_sum_k(const float* __restrict_
 // host side
 // ------------------------------------------------------------------------------------------------
 static VarP make_varp(const VitkAttnVar* a) {
-  VarP p;
+  VarP p = {};
   p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->o; p.dout = a->dout; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
-  p.lse = a->lse; p.delta = nullptr; p.kv_len = a->kv_len; p.table = a->bias_table; p.index = a->bias_index; p.dbias = nullptr;
+  p.stat = a->stat; p.kv_len = a->kv_len; p.table = a->bias_table; p.index = a->bias_index;
   const int64_t* s = a->st;
   p.q_sb = s[0]; p.q_sh = s[1]; p.q_ss = s[2]; p.k_sb = s[3]; p.k_sh = s[4]; p.k_ss = s[5];
   p.v_sb = s[6]; p.v_sh = s[7]; p.v_ss = s[8]; p.o_sb = s[9]; p.o_sh = s[10]; p.o_ss = s[11];
   p.g_sb = s[12]; p.g_sh = s[13]; p.g_ss = s[14]; p.dq_sb = s[15]; p.dq_sh = s[16]; p.dq_ss = s[17];
   p.dk_sb = s[18]; p.dk_sh = s[19]; p.dk_ss = s[20]; p.dv_sb = s[21]; p.dv_sh = s[22]; p.dv_ss = s[23];
   p.B = (int)a->B; p.H = (int)a->H; p.Lq = (int)a->Lq; p.Lk = (int)a->Lk; p.Dh = (int)a->Dh;
-  p.seed = a->seed; p.scale = a->scale;
+  p.nqt = (int)ceil_div(a->Lq, 32); p.nkt = (int)ceil_div(a->Lk, 64) * 2;
+  p.nkt_t = (int)ceil_div(a->Lk, 32); p.nqt_t = (int)ceil_div(a->Lq, 64) * 2;
+  p.splits = 1;
+  p.seed = a->seed; p.scale = a->scale; p.inv_scale = 1.f / a->scale;
+  p.bias_lim = 1e38f * a->scale < 1e37f ? 1e38f * a->scale : 1e37f;
   p.thr = a->drop_p > 0.f ? drop_threshold(a->drop_p) : 0;
   p.keep_scale = 1.f / (1.f - a->drop_p);
   return p;
+}
+// The stride of an axis of one element is never used; torch leaves anything there.
+static VitkAttnVar var_normal(const VitkAttnVar* a) {
+  VitkAttnVar n = *a;
+  for (int i = 0; i < 8; i++) {
+    const bool key_side = i == 1 || i == 2 || i == 6 || i == 7;   // q, k, v, o, dout, dq, dk, dv
+    if (n.B == 1) n.st[3 * i] = 0;
+    if (n.H == 1) n.st[3 * i + 1] = 0;
+    if ((key_side ? n.Lk : n.Lq) == 1) n.st[3 * i + 2] = 0;
+  }
+  return n;
 }
 static int var_validate(const VitkAttnVar* a, bool bwd) {
   VITK_REQUIRE(a, "attn_var: null descriptor");
@@ -337,11 +328,12 @@ static int var_validate(const VitkAttnVar* a, bool bwd) {
                "attn_var: bad shape B=%lld H=%lld Lq=%lld Lk=%lld Dh=%lld", (long long)a->B, (long long)a->H, (long long)a->Lq,
                (long long)a->Lk, (long long)a->Dh);
   VITK_REQUIRE(a->Lq < (1 << 22) && a->Lk < (1 << 24), "attn_var: at most 2^22 queries and 2^24 keys");
+  VITK_REQUIRE((a->B * a->H + 8) * (ceil_div(a->Lq > a->Lk ? a->Lq : a->Lk, 64) + 1) < (1ll << 31), "attn_var: too many rows for one launch");
   VITK_REQUIRE(a->dtype == VITK_F32 || a->dtype == VITK_BF16, "attn_var: bad dtype");
   VITK_REQUIRE(!a->dbias_table || a->dbias_dtype == VITK_F32 || a->dbias_dtype == VITK_BF16, "attn_var: bad dtype of the bias gradient");
   VITK_REQUIRE(a->drop_p >= 0.f && a->drop_p < 1.f, "attn_var: dropout p=%f out of range", a->drop_p);
-  VITK_REQUIRE(a->scale > 0.f && a->scale < 1e10f, "attn_var: scale=%g must be positive", a->scale);
-  if (a->B * a->Lq * a->Lk > 0) VITK_REQUIRE(a->q && a->k && a->v && a->o && a->lse, "attn_var: null pointer");
+  VITK_REQUIRE(a->scale > 1e-30f && a->scale < 1e10f, "attn_var: scale=%g outside (1e-30, 1e10)", a->scale);
+  if (a->B * a->Lq * a->Lk > 0) VITK_REQUIRE(a->q && a->k && a->v && a->o && a->stat, "attn_var: null pointer");
   VITK_REQUIRE(!a->bias_table == !a->bias_index, "attn_var: a bias needs its table and its index");
   if (a->bias_table) {
     VITK_REQUIRE(a->num_buckets > 0 && a->num_buckets <= 65536, "attn_var: num_buckets=%lld outside [1, 65536]", (long long)a->num_buckets);
@@ -355,66 +347,151 @@ static int var_validate(const VitkAttnVar* a, bool bwd) {
   }
   return 0;
 }
+// The matrix-unit kernels take bf16, head sizes that are multiples of 8, 16-byte aligned rows, and rows of one (sample, head)
+// within 32-bit byte offsets (the tiles asked for ahead of the last one included).
+static bool var_mfma_ok(const VitkAttnVar* a, bool bwd) {
+  if (a->dtype != VITK_BF16 || a->Dh % 8 || a->algo == 1 || a->Lk == 0) return false;
+  for (int i = 0; i < (bwd ? 24 : 12); i++)
+    if (a->st[i] % 8) return false;
+  const void* ps[] = {a->q, a->k, a->v, a->o, a->dout, a->dq, a->dk, a->dv};
+  for (int i = 0; i < (bwd ? 8 : 4); i++)
+    if ((uintptr_t)ps[i] & 15) return false;
+  const int64_t lim = 1ll << 29;   // elements
+  if ((a->Lq + 256) * a->st[2] >= lim || (a->Lk + 256) * a->st[5] >= lim || (a->Lk + 256) * a->st[8] >= lim || (a->Lq + 256) * a->st[11] >= lim) return false;
+  return !bwd || (a->Lq + 256) * a->st[14] < lim;
+}
+// Waves per workgroup, 32 query rows each: 4, or 2 where 64 rows hold all queries.
+static int var_nw(const VitkAttnVar* a) { return a->Lq <= 64 && !(a->drop_p > 0.f) ? 2 : 4; }
+// Workgroups that share the keys of a (sample, head) in the forward pass: 1 where the query blocks alone fill the chip
+// (256 CUs, two workgroups each), otherwise as many as do, each with at least four 64-key tiles.
+static int var_fwd_splits(const VitkAttnVar* a) {
+  if (a->drop_p > 0.f) return 1;
+  const int64_t blocks = a->B * a->H * ceil_div(a->Lq, 32 * var_nw(a)), tiles = ceil_div(a->Lk, 64);
+  if (blocks >= 512 || tiles < 8) return 1;
+  int64_t n = ceil_div(768, blocks);
+  if (n > tiles / 4) n = tiles / 4;
+  return (int)(n < 64 ? n : 64);
+}
+// Shares of the samples in the bias gradient: enough workgroups to fill the chip twice.
+static int var_dbias_splits(const VitkAttnVar* a) {
+  const int64_t blocks = a->H * ceil_div(a->Lq, 128) * ceil_div(a->Lk, 128);
+  int64_t n = ceil_div(512, blocks);
+  if (n > a->B) n = a->B;
+  return (int)(n < 1 ? 1 : n);
+}
+static bool var_few(const VitkAttnVar* a) { return a->Lq <= 32 && !(a->drop_p > 0.f); }
+
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-struct VarWs { size_t delta, dbias, part, total; int splits; };
+struct VarWs { size_t delta, bias_s, bias_t, dbias, pieces, part, pstat, total; int splits; };
 static VarWs var_ws(const VitkAttnVar* a, bool bwd) {
-  VarWs w = {0, 0, 0, 0, 1};
-  if (!bwd) return w;
+  VarWs w = {};
+  w.splits = 1;
+  const bool mfma = var_mfma_ok(a, bwd);
+  const size_t rows = (size_t)(a->B * a->H * a->Lq);
   size_t at = 0;
-  w.delta = at; at += up256((size_t)(a->B * a->H * a->Lq) * 4);
-  if (a->dbias_table) {
-    w.dbias = at; at += up256((size_t)w.splits * a->H * a->Lq * a->Lk * 4);
-    w.part = at; at += up256((size_t)a->H * a->num_pieces * 4);
+  auto take = [&](size_t n) { const size_t here = at; at += up256(n); return here; };
+  if (mfma && a->bias_table) {
+    w.bias_s = take((size_t)a->H * ceil_div(a->Lq, 32) * ceil_div(a->Lk, 64) * 2 * 2048);
+    if (bwd) w.bias_t = take((size_t)a->H * ceil_div(a->Lk, 32) * ceil_div(a->Lq, 64) * 2 * 2048);
+  }
+  if (!bwd) {
+    w.splits = mfma ? var_fwd_splits(a) : 1;
+    if (w.splits > 1) { w.part = take(w.splits * rows * a->Dh * 4); w.pstat = take(w.splits * rows * 8); }
+  } else {
+    w.delta = take(rows * 4);
+    if (mfma && var_few(a)) w.part = take((size_t)ceil_div(a->Lk, 128) * rows * a->Dh * 4);
+    if (a->dbias_table) {
+      w.splits = mfma ? var_dbias_splits(a) : 1;
+      w.dbias = take((size_t)w.splits * a->H * a->Lq * a->Lk * 4);
+      w.pieces = take((size_t)a->H * a->num_pieces * 4);
+    }
   }
   w.total = at;
   return w;
 }
 extern "C" size_t vitk_attn_var_workspace_bytes(const VitkAttnVar* a, int bwd) {
   if (!a || var_validate(a, bwd != 0)) return 0;
-  return var_ws(a, bwd != 0).total;
+  const VitkAttnVar n = var_normal(a);
+  return var_ws(&n, bwd != 0).total;
 }
 #define VAR_T(T, ...) do { if (a->dtype == VITK_F32) { typedef float T; __VA_ARGS__; } else { typedef bf16 T; __VA_ARGS__; } } while (0)
 
-extern "C" int vitk_attn_var_fwd(const VitkAttnVar* a, void* stream) {
-  if (int rc = var_validate(a, false)) return rc;
+extern "C" int vitk_attn_var_fwd(const VitkAttnVar* desc, void* stream) {
+  if (int rc = var_validate(desc, false)) return rc;
+  const VitkAttnVar normal = var_normal(desc), *a = &normal;
   if (a->B == 0 || a->Lq == 0) return 0;
   hipStream_t st = (hipStream_t)stream;
-  const VarP p = make_varp(a);
+  VarP p = make_varp(a);
   const VarWs w = var_ws(a, false);
   VITK_REQUIRE(w.total == 0 || (a->workspace && a->workspace_bytes >= (int64_t)w.total), "attn_var_fwd: workspace too small");
-  dim3 grid((unsigned)ceil_div(a->Lq, 64), (unsigned)a->H, (unsigned)a->B);
-  const size_t lds = (size_t)2 * VT * a->Dh * sizeof(float);
-  VAR_T(T, hipLaunchKernelGGL((var_fwd_simple_k<T>), grid, dim3(256), lds, st, p));
+  const bool mfma = var_mfma_ok(a, false);
+  VITK_REQUIRE(a->algo != 2 || mfma, "attn_var_fwd: the matrix-unit kernels cannot take this problem (dtype, alignment, head size)");
+  if (mfma) {
+    char* ws = (char*)a->workspace;
+    p.splits = w.splits;
+    p.part = (float*)(ws + w.part);
+    p.pstat = (float*)(ws + w.pstat);
+    if (a->bias_table) {
+      p.bias_s = (const bf16*)(ws + w.bias_s);
+      var_launch_expand(p, false, st);
+    }
+    var_launch_fwd(p, a->bias_table != nullptr, var_nw(a), st);
+  } else {
+    dim3 grid((unsigned)ceil_div(a->Lq, 64), (unsigned)a->H, (unsigned)a->B);
+    const size_t lds = (size_t)2 * VT * a->Dh * sizeof(float);
+    VAR_T(T, hipLaunchKernelGGL((var_fwd_simple_k<T>), grid, dim3(256), lds, st, p));
+  }
   VITK_LAUNCH_CHECK("attn_var_fwd");
   return 0;
 }
 
-extern "C" int vitk_attn_var_bwd(const VitkAttnVar* a, void* stream) {
-  if (int rc = var_validate(a, true)) return rc;
+extern "C" int vitk_attn_var_bwd(const VitkAttnVar* desc, void* stream) {
+  if (int rc = var_validate(desc, true)) return rc;
+  const VitkAttnVar normal = var_normal(desc), *a = &normal;
   if (a->B * (a->Lq + a->Lk) == 0 && !a->dbias_table) return 0;
   hipStream_t st = (hipStream_t)stream;
   VarP p = make_varp(a);
   const VarWs w = var_ws(a, true);
   VITK_REQUIRE(w.total == 0 || (a->workspace && a->workspace_bytes >= (int64_t)w.total), "attn_var_bwd: workspace too small");
-  p.delta = (float*)((char*)a->workspace + w.delta);
-  p.dbias = (float*)((char*)a->workspace + w.dbias);
+  char* ws = (char*)a->workspace;
+  p.delta = (float*)(ws + w.delta);
+  p.dbias = (float*)(ws + w.dbias);
+  p.part = (float*)(ws + w.part);
+  p.splits = w.splits;
   const int64_t rows = a->B * a->H * a->Lq;
+  const bool mfma = var_mfma_ok(a, true) && rows > 0, bias = a->bias_table != nullptr;
+  VITK_REQUIRE(a->algo != 2 || mfma, "attn_var_bwd: the matrix-unit kernels cannot take this problem (dtype, alignment, head size)");
   const size_t lds = (size_t)2 * VT * a->Dh * sizeof(float);
-  if (rows > 0) {
-    VAR_T(T, hipLaunchKernelGGL((var_delta_k<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, p));
-    VAR_T(T, hipLaunchKernelGGL((var_dq_simple_k<T>), dim3((unsigned)ceil_div(a->Lq, 64), (unsigned)a->H, (unsigned)a->B), dim3(256), lds, st, p));
-  }
-  if (a->B * a->Lk > 0)
-    VAR_T(T, hipLaunchKernelGGL((var_dkdv_simple_k<T>), dim3((unsigned)ceil_div(a->Lk, 64), (unsigned)a->H, (unsigned)a->B), dim3(256), lds + 512, st, p));
-  if (a->dbias_table) {
-    float* part = (float*)((char*)a->workspace + w.part);
-    const int64_t pairs = a->Lq * a->Lk;
-    if (pairs > 0) {
-      VAR_T(T, hipLaunchKernelGGL((var_dbias_simple_k<T>), dim3((unsigned)ceil_div(pairs, 256), (unsigned)a->H), dim3(256), 0, st, p));
-      if (a->num_pieces > 0)
-        hipLaunchKernelGGL(var_piece_sum_k, dim3((unsigned)ceil_div(a->num_pieces, 4), (unsigned)a->H), dim3(256), 0, st, p.dbias,
-                           a->order, a->piece, part, pairs, (int)a->H, (int)a->num_pieces, w.splits);
+  const int64_t pairs = a->Lq * a->Lk;
+  if (mfma) {
+    if (bias) {
+      p.bias_s = (const bf16*)(ws + w.bias_s);
+      p.bias_t = (const bf16*)(ws + w.bias_t);
+      var_launch_expand(p, false, st);
+      var_launch_expand(p, true, st);
     }
+    if (var_few(a)) {
+      var_launch_few_bwd(p, bias, st);
+    } else {
+      var_launch_dq(p, bias, st);     // writes delta
+      var_launch_dkdv(p, bias, st);   // reads it
+    }
+    if (a->dbias_table) var_launch_dbias(p, st);
+  } else {
+    if (rows > 0) {
+      VAR_T(T, hipLaunchKernelGGL((var_delta_k<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, p));
+      VAR_T(T, hipLaunchKernelGGL((var_dq_simple_k<T>), dim3((unsigned)ceil_div(a->Lq, 64), (unsigned)a->H, (unsigned)a->B), dim3(256), lds, st, p));
+    }
+    if (a->B * a->Lk > 0)
+      VAR_T(T, hipLaunchKernelGGL((var_dkdv_simple_k<T>), dim3((unsigned)ceil_div(a->Lk, 64), (unsigned)a->H, (unsigned)a->B), dim3(256), lds + 512, st, p));
+    if (a->dbias_table && pairs > 0)
+      VAR_T(T, hipLaunchKernelGGL((var_dbias_simple_k<T>), dim3((unsigned)ceil_div(pairs, 256), (unsigned)a->H), dim3(256), 0, st, p));
+  }
+  if (a->dbias_table) {
+    float* part = (float*)(ws + w.pieces);
+    if (a->num_pieces > 0)
+      hipLaunchKernelGGL(var_piece_sum_k, dim3((unsigned)ceil_div(a->num_pieces, 4), (unsigned)a->H), dim3(256), 0, st, p.dbias,
+                         a->order, a->piece, part, pairs, (int)a->H, (int)a->num_pieces, w.splits);
     const dim3 bgrid((unsigned)ceil_div(a->num_buckets, 4), (unsigned)a->H);
     if (a->dbias_dtype == VITK_F32)
       hipLaunchKernelGGL((var_bucket_sum_k<float>), bgrid, dim3(256), 0, st, part, a->bucket_piece, (float*)a->dbias_table, (int)a->H,

@@ -1,0 +1,681 @@
+// Backward pass on the matrix units of attention with a relative position bias and / or key counts.
+//
+//   var_dq_k    queries stationary (32 per wave), K and V stream: S'^T and dP^T with the query on the lane, dQ^T += K^T dS^T
+//   var_dkdv_k  keys stationary, Q and dO stream: S' and dP with the key on the lane, dV^T += dO^T P, dK^T += Q^T dS
+//   var_dbias_k pairs stationary (128 x 128 per workgroup), samples stream: dS summed over the samples in the accumulators, in
+//               32 bits, one 32-bit value per pair and head out; no atomics, so the sums do not depend on the order of anything
+//   var_few_bwd_k up to 32 queries: keys stationary, everything in one pass over K and V (below)
+// P is formed again from the row statistics of the forward pass; delta = rowsum(dO O) comes from var_dq_k / var_few_bwd_k.
+#include "attn_var.h"
+
+template <bool BIAS>
+__device__ __forceinline__ f32x16 init_tile(const bf16x8& lo, const bf16x8& hi, float inv_scale) {
+  f32x16 a = ZERO16;
+  if (BIAS) {
+#pragma unroll
+    for (int r = 0; r < 8; r++) { a[r] = (float)lo[r] * inv_scale; a[8 + r] = (float)hi[r] * inv_scale; }
+  }
+  return a;
+}
+
+// ---- dQ -----------------------------------------------------------------------------------------------------------------
+template <int DHP, int HALVES, bool PARTIAL, bool BIAS, bool DROP, int KS, int VS>
+__device__ __forceinline__ void var_dq_tile(const VarP& p, const char* sK, const char* sV, const bf16x8 (&qf)[DHP / 16],
+                                            const bf16x8 (&gf)[DHP / 16], f32x16 (&sacc)[HALVES], f32x16 (&dqacc)[DHP / 32],
+                                            float m, float nmc, bool big, float delta, float c, int k0, int len, uint32_t xrow,
+                                            int lane) {
+  const f32x16 zero = ZERO16;
+  const int rowoff = 4 * (lane >> 5);
+#pragma unroll
+  for (int st = 0; st < HALVES; st++) {
+    f32x16 pacc = MFMA(frag_rows<VS, 0>(sV, st * 32, 0, lane), gf[0], zero, 0, 0, 0);
+#pragma unroll
+    for (int ks = 0; ks < DHP / 16; ks++) {
+      sacc[st] = MFMA(frag_rows<KS, 1>(sK, st * 32, ks, lane), qf[ks], sacc[st], 0, 0, 0);
+      if (ks) pacc = MFMA(frag_rows<VS, 0>(sV, st * 32, ks, lane), gf[ks], pacc, 0, 0, 0);
+    }
+    if (BIAS && big) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) sacc[st][r] = fast_exp2((sacc[st][r] - m) * c);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; r++) sacc[st][r] = fast_exp2(fmaf(sacc[st][r], c, nmc));
+    }
+#pragma unroll
+    for (int g = 0; g < 4; g++) {   // registers 4 g .. 4 g + 3: four consecutive keys from a multiple of 4
+      uint32_t dr[4] = {0u, 0u, 0u, 0u};
+      if (DROP) rng_lin_run<4>(xrow + (uint32_t)((k0 + st * 32 + acc_row(4 * g)) >> 1) * RNG_C1, dr);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int r = 4 * g + j;
+        float pr = sacc[st][r];
+        if (PARTIAL && st == HALVES - 1) pr = k0 + st * 32 + acc_row(r) + rowoff < len ? pr : 0.f;
+        float dp = pacc[r];
+        if (DROP) dp = dr[j] >= p.thr ? dp * p.keep_scale : 0.f;
+        sacc[st][r] = pr * (dp - delta);
+      }
+    }
+    // dS is rounded to bf16 to be an operand (half a step, 2^-8); its row factor 1 / sum is applied to the 32-bit result
+#pragma unroll
+    for (int s2 = 0; s2 < 2; s2++) {
+      const bf16x8 df = acc_to_frag(sacc[st], s2);
+#pragma unroll
+      for (int dt = 0; dt < DHP / 32; dt++)
+        dqacc[dt] = MFMA(frag_cols<KS, 1>(sK, st * 32, s2, dt * 32, lane), df, dqacc[dt], 0, 0, 0);
+    }
+  }
+}
+
+template <int DHP, bool BIAS, bool DROP> constexpr int var_dq_occ() { return (DHP <= 64 && !DROP && !BIAS) ? 3 : DHP <= 96 ? 2 : 1; }
+template <int DHP, int NW, bool BIAS, bool DROP>
+__global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_dq_k(VarP p) {
+  constexpr int NT = NW * 64, CPR = DHP / 8, NCH = (64 * CPR + NT - 1) / NT;
+  constexpr int KS = Strides<DHP>::COLS, VS = Strides<DHP>::ROWS;   // K is read both ways (swizzled), V row-wise only
+  constexpr int TILE = 64 * KS + 64 * VS;
+  __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, S = p.Lq;
+  const HeadBlock hb = head_block(p.B, p.H, S, NW * 32);
+  if (!hb.valid) return;
+  const int64_t b = hb.b, h = hb.h;
+  const int qrow = hb.xb * (NW * 32) + wid * 32 + (lane & 31);
+  const bool qv = qrow < S;
+  const bool wave_on = hb.xb * (NW * 32) + wid * 32 < S;
+  const bf16* qp = (const bf16*)p.q + b * p.q_sb + h * p.q_sh;
+  const bf16* kp = (const bf16*)p.k + b * p.k_sb + h * p.k_sh;
+  const bf16* vp = (const bf16*)p.v + b * p.v_sb + h * p.v_sh;
+  const bf16* gp = (const bf16*)p.dout + b * p.g_sb + h * p.g_sh;
+  const int len = key_count(p, b);
+  const TileSrc<NCH> ksrc = make_tilesrc<DHP, NT, NCH>(kp, p.k_ss, len, Dh, tid);
+  const TileSrc<NCH> vsrc = make_tilesrc<DHP, NT, NCH>(vp, p.v_ss, len, Dh, tid);
+  const int ntiles = (len + 63) >> 6, nfull = len >> 6;
+  bf16x8 qf[DHP / 16], gf[DHP / 16], of[DHP / 16];
+  load_stationary<DHP>(qf, qp, p.q_ss, qrow, S, Dh, lane);
+  load_stationary<DHP>(gf, gp, p.g_ss, qrow, S, Dh, lane);
+  load_stationary<DHP>(of, (const bf16*)p.o + b * p.o_sb + h * p.o_sh, p.o_ss, qrow, S, Dh, lane);
+  const int64_t srow = (b * p.H + h) * p.Lq + qrow;
+  const float m = qv ? p.stat[2 * srow] : 0.f, lr = qv ? p.stat[2 * srow + 1] : -INFINITY;
+  const int qt = hb.xb * NW + wid;
+  const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc(
+      BIAS ? (void*)(p.bias_s + ((int64_t)h * p.nqt + (wave_on ? qt : 0)) * p.nkt * 1024) : nullptr, 0, BIAS ? p.nkt * 2048 : 0, 0x00020000);
+  bf16x8 bf[4];
+  auto load_bias = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(t * 4096 + i * 1024 + lane * 16)));
+  };
+  if (BIAS) load_bias(0);
+  uint4 rkA[NCH], rvA[NCH], rkB[NCH], rvB[NCH];
+  stage_load(rkA, ksrc, 0);
+  stage_load(rvA, vsrc, 0);
+  stage_load(rkB, ksrc, 1);
+  stage_load(rvB, vsrc, 1);
+  // delta = rowsum(dO * O), each half-wave holds half of the row; published for the kernels launched after this one
+  float delta = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < DHP / 16; ks++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) delta += (float)of[ks][j] * (float)gf[ks][j];
+  delta += __shfl_xor(delta, 32, 64);
+  if (qv && lane < 32) p.delta[srow] = delta;
+  const float c = p.scale * LOG2E, nmc = -m * c;
+  const bool big = BIAS && __any(fabsf(m * c) > BIG_EXP);
+  const uint32_t rbase = var_drop_xrow(p, (uint64_t)srow, lane);
+  const f32x16 zero = ZERO16;
+  f32x16 dqacc[DHP / 32];
+#pragma unroll
+  for (int dt = 0; dt < DHP / 32; dt++) dqacc[dt] = zero;
+  stage_store<DHP, NT, NCH, KS, true>(rkA, smem, tid);
+  stage_store<DHP, NT, NCH, VS, false>(rvA, smem + 64 * KS, tid);
+  __syncthreads();
+
+  auto step = [&](int t, uint4 (&nk)[NCH], uint4 (&nv)[NCH], uint4 (&fk)[NCH], uint4 (&fv)[NCH]) {
+    const char* sK = smem + (t & 1) * TILE;
+    const char* sV = sK + 64 * KS;
+    f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
+    if (BIAS) load_bias(t + 1);   // ahead of the K and V tiles: see var_fwd_k
+    stage_load(fk, ksrc, t + 2);
+    stage_load(fv, vsrc, t + 2);
+    if (wave_on) var_dq_tile<DHP, 2, false, BIAS, DROP, KS, VS>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, c, t * 64, len, rbase, lane);
+    char* nK = smem + ((t + 1) & 1) * TILE;
+    stage_store<DHP, NT, NCH, KS, true>(nk, nK, tid);
+    stage_store<DHP, NT, NCH, VS, false>(nv, nK + 64 * KS, tid);
+    __syncthreads();
+  };
+  for (int t = 0; t < nfull; t += 2) {
+    step(t, rkB, rvB, rkA, rvA);
+    if (t + 1 < nfull) step(t + 1, rkA, rvA, rkB, rvB);
+  }
+  if (nfull < ntiles && wave_on) {
+    const char* sK = smem + (nfull & 1) * TILE;
+    const char* sV = sK + 64 * KS;
+    if (len - nfull * 64 > 32) {
+      f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
+      var_dq_tile<DHP, 2, true, BIAS, DROP, KS, VS>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, c, nfull * 64, len, rbase, lane);
+    } else {
+      f32x16 sacc[1] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale)};
+      var_dq_tile<DHP, 1, true, BIAS, DROP, KS, VS>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, c, nfull * 64, len, rbase, lane);
+    }
+  }
+  if (!qv) return;
+  store_rows<DHP>((bf16*)p.dq + b * p.dq_sb + h * p.dq_sh + (int64_t)qrow * p.dq_ss, dqacc, p.scale * fast_exp2(lr), Dh, lane);
+}
+
+// ---- row constants of a 64-query tile, read by the kernels that stream queries ---------------------------------------------
+// sL: -m c + lr [64] (rows beyond Lq: -inf), delta [64]; with a bias also m [64], lr [64] and a flag: some |m c| > BIG_EXP.
+// Wave 0 fetches the statistics, wave 1 delta; every wave keeps what it fetched until store().
+struct RowConsts {
+  __amdgpu_buffer_rsrc_t srs, drs;
+  float a, b;
+};
+__device__ __forceinline__ void rc_open(RowConsts& rc, const VarP& p, int64_t sbase) {
+  rc.srs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.stat + 2 * sbase), 0, p.Lq * 8, 0x00020000);
+  rc.drs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.delta + sbase), 0, p.Lq * 4, 0x00020000);
+}
+__device__ __forceinline__ void rc_load(RowConsts& rc, int q0, int wid, int lane) {   // branch-free buffer loads
+  const uint32_t at = (uint32_t)(q0 + lane);
+  rc.a = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(wid == 0 ? rc.srs : rc.drs, wid == 0 ? at * 8u : wid == 1 ? at * 4u : OOB_OFF, 0, 0));
+  rc.b = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rc.srs, wid == 0 ? at * 8u + 4u : OOB_OFF, 0, 0));
+}
+template <bool BIAS>
+__device__ __forceinline__ void rc_store(const RowConsts& rc, float* sL, int q0, int Lq, float c, int wid, int lane) {
+  if (wid == 0) {
+    const bool ok = q0 + lane < Lq;
+    const float m = rc.a, lr = ok ? rc.b : -INFINITY;
+    sL[lane] = fmaf(-m, c, lr);
+    if (BIAS) {
+      sL[128 + lane] = m;
+      sL[192 + lane] = lr;
+      const bool big = __any(fabsf(m * c) > BIG_EXP);
+      if (lane == 0) sL[256] = big ? 1.f : 0.f;
+    }
+  } else if (wid == 1) {
+    sL[64 + lane] = rc.a;
+  }
+}
+template <bool BIAS> constexpr int rc_bytes() { return BIAS ? 1040 : 512; }
+
+// ---- dK, dV -----------------------------------------------------------------------------------------------------------------
+// P of a 32 x 32 tile (query r on the accumulator row, key on the lane) from its scores
+template <bool BIAS>
+__device__ __forceinline__ void prob_rows(f32x16& sacc, const float* sL, int st, int rowoff, float c) {
+  const bool big = BIAS && __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sL[256])) != 0;
+  if (BIAS && big) {
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const int ql = st * 32 + 8 * g + rowoff;
+      const f32x4 m4 = *(const f32x4*)(sL + 128 + ql), l4 = *(const f32x4*)(sL + 192 + ql);
+#pragma unroll
+      for (int j = 0; j < 4; j++) sacc[4 * g + j] = fast_exp2((sacc[4 * g + j] - m4[j]) * c + l4[j]);
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const f32x4 n4 = *(const f32x4*)(sL + st * 32 + 8 * g + rowoff);
+#pragma unroll
+      for (int j = 0; j < 4; j++) sacc[4 * g + j] = fast_exp2(fmaf(sacc[4 * g + j], c, n4[j]));
+    }
+  }
+}
+// dS (in pacc) and the P that multiplies dO (in sacc) of a 32 x 32 tile
+template <bool DROP>
+__device__ __forceinline__ void ds_rows(const VarP& p, f32x16& sacc, f32x16& pacc, const float* sL, int st, int rowoff,
+                                        uint32_t xkey, uint32_t xstep, bool kodd, int khalf) {
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
+    const f32x4 d4 = *(const f32x4*)(sL + 64 + st * 32 + 8 * g + rowoff);
+    uint32_t drops[4] = {0u, 0u, 0u, 0u};
+    if (DROP) {   // neighbouring lanes share a pair's hash: each computes two rows' hashes and they swap (see attn.hip)
+#pragma unroll
+      for (int jj = 0; jj < 2; jj++) {
+        const uint32_t mine = rng_fmix(xkey + (uint32_t)(st * 32 + 8 * g + 2 * jj) * xstep);
+        const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)mine, 0xB1, 0xF, 0xF, true);   // quad_perm [1,0,3,2]
+        const uint32_t h0 = kodd ? other : mine, h1 = kodd ? mine : other;
+        drops[2 * jj] = (h0 << khalf) & 0xffff0000u;
+        drops[2 * jj + 1] = (h1 << khalf) & 0xffff0000u;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int r = 4 * g + j;
+      const float pr = sacc[r];
+      float dp = pacc[r];
+      if (DROP) {
+        const bool keep = drops[j] >= p.thr;
+        sacc[r] = keep ? pr * p.keep_scale : 0.f;
+        dp = keep ? dp * p.keep_scale : 0.f;
+      }
+      pacc[r] = pr * (dp - d4[j]);
+    }
+  }
+}
+struct DropKey { uint32_t xstep; bool kodd; int khalf; uint32_t xk; };
+__device__ __forceinline__ DropKey drop_key(const VarP& p, int krow) {
+  DropKey d;
+  d.xstep = (uint32_t)(var_drop_ld(p) >> 1) * RNG_C1;
+  d.kodd = krow & 1;
+  d.khalf = d.kodd ? 0 : 16;
+  d.xk = (uint32_t)(krow >> 1) * RNG_C1 + rng_seedmix(p.seed);
+  return d;
+}
+__device__ __forceinline__ uint32_t drop_xkey(const VarP& p, const DropKey& d, int64_t row0, int rowoff) {
+  return (uint32_t)((uint64_t)(row0 + rowoff + (d.kodd ? 1 : 0)) * (var_drop_ld(p) >> 1)) * RNG_C1 + d.xk;
+}
+
+template <int DHP, int HALVES, bool BIAS, bool DROP, int QS>
+__device__ __forceinline__ void var_dkdv_tile(const VarP& p, const char* sQ, const char* sG, const float* sL,
+                                              const bf16x8 (&kf)[DHP / 16], const bf16x8 (&vf)[DHP / 16], f32x16 (&sacc)[HALVES],
+                                              f32x16 (&dkacc)[DHP / 32], f32x16 (&dvacc)[DHP / 32], float c, int64_t row0,
+                                              const DropKey& dk, int lane) {
+  const f32x16 zero = ZERO16;
+  const int rowoff = 4 * (lane >> 5);
+  const uint32_t xkey = DROP ? drop_xkey(p, dk, row0, rowoff) : 0u;
+#pragma unroll
+  for (int st = 0; st < HALVES; st++) {
+    f32x16 pacc = MFMA(frag_rows<QS, 1>(sG, st * 32, 0, lane), vf[0], zero, 0, 0, 0);
+#pragma unroll
+    for (int ks = 0; ks < DHP / 16; ks++) {
+      sacc[st] = MFMA(frag_rows<QS, 1>(sQ, st * 32, ks, lane), kf[ks], sacc[st], 0, 0, 0);
+      if (ks) pacc = MFMA(frag_rows<QS, 1>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
+    }
+    prob_rows<BIAS>(sacc[st], sL, st, rowoff, c);
+    ds_rows<DROP>(p, sacc[st], pacc, sL, st, rowoff, xkey, dk.xstep, dk.kodd, dk.khalf);
+#pragma unroll
+    for (int s2 = 0; s2 < 2; s2++) {
+      const bf16x8 pf = acc_to_frag(sacc[st], s2);
+      const bf16x8 df = acc_to_frag(pacc, s2);
+#pragma unroll
+      for (int dt = 0; dt < DHP / 32; dt++) {
+        dvacc[dt] = MFMA(frag_cols<QS, 1>(sG, st * 32, s2, dt * 32, lane), pf, dvacc[dt], 0, 0, 0);
+        dkacc[dt] = MFMA(frag_cols<QS, 1>(sQ, st * 32, s2, dt * 32, lane), df, dkacc[dt], 0, 0, 0);
+      }
+    }
+  }
+}
+
+template <int DHP, bool BIAS, bool DROP> constexpr int var_dkdv_occ() { return (DHP <= 64 || (DHP <= 96 && !DROP)) ? 2 : 1; }
+template <int DHP, int NW, bool BIAS, bool DROP>
+__global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void var_dkdv_k(VarP p) {
+  constexpr int NT = NW * 64, CPR = DHP / 8, NCH = (64 * CPR + NT - 1) / NT;
+  constexpr int QS = Strides<DHP>::COLS;   // Q and dO tiles are read both ways (swizzled)
+  constexpr int TILE = 2 * 64 * QS + rc_bytes<BIAS>();
+  __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, S = p.Lq;
+  const HeadBlock hb = head_block(p.B, p.H, p.Lk, NW * 32);
+  if (!hb.valid) return;
+  const int64_t b = hb.b, h = hb.h;
+  const int key0 = hb.xb * (NW * 32), krow = key0 + wid * 32 + (lane & 31);
+  const int len = key_count(p, b);
+  const bool wave_on = key0 + wid * 32 < len;
+  const bf16* qp = (const bf16*)p.q + b * p.q_sb + h * p.q_sh;
+  const bf16* gp = (const bf16*)p.dout + b * p.g_sb + h * p.g_sh;
+  const int64_t sbase = (b * p.H + h) * p.Lq;
+  const f32x16 zero = ZERO16;
+  f32x16 dkacc[DHP / 32], dvacc[DHP / 32];
+#pragma unroll
+  for (int dt = 0; dt < DHP / 32; dt++) { dkacc[dt] = zero; dvacc[dt] = zero; }
+  if (key0 < len) {   // otherwise all of the block's keys are padding
+    const TileSrc<NCH> qsrc = make_tilesrc<DHP, NT, NCH>(qp, p.q_ss, S, Dh, tid);
+    const TileSrc<NCH> gsrc = make_tilesrc<DHP, NT, NCH>(gp, p.g_ss, S, Dh, tid);
+    const int ntiles = (S + 63) >> 6, nfull = S >> 6;
+    RowConsts rc;
+    rc_open(rc, p, sbase);
+    bf16x8 kf[DHP / 16], vf[DHP / 16];
+    load_stationary<DHP>(kf, (const bf16*)p.k + b * p.k_sb + h * p.k_sh, p.k_ss, krow, len, Dh, lane);
+    load_stationary<DHP>(vf, (const bf16*)p.v + b * p.v_sb + h * p.v_sh, p.v_ss, krow, len, Dh, lane);
+    const int kt = hb.xb * NW + wid;
+    const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc(
+        BIAS ? (void*)(p.bias_t + ((int64_t)h * p.nkt_t + (wave_on ? kt : 0)) * p.nqt_t * 1024) : nullptr, 0, BIAS ? p.nqt_t * 2048 : 0, 0x00020000);
+    bf16x8 bf[4];
+    auto load_bias = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(t * 4096 + i * 1024 + lane * 16)));
+    };
+    const float c = p.scale * LOG2E;
+    const DropKey dkey = drop_key(p, krow);
+    uint4 rq[NCH], rg[NCH];
+    if (BIAS) load_bias(0);
+    stage_load(rq, qsrc, 0);
+    stage_load(rg, gsrc, 0);
+    rc_load(rc, 0, wid, lane);
+    stage_store<DHP, NT, NCH, QS, true>(rq, smem, tid);
+    stage_store<DHP, NT, NCH, QS, true>(rg, smem + 64 * QS, tid);
+    rc_store<BIAS>(rc, (float*)(smem + 2 * 64 * QS), 0, S, c, wid, lane);
+    __syncthreads();
+    for (int t = 0; t < nfull; t++) {   // tile t + 1 travels while tile t is multiplied
+      const char* sQ = smem + (t & 1) * TILE;
+      const char* sG = sQ + 64 * QS;
+      const float* sL = (const float*)(sQ + 2 * 64 * QS);
+      f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
+      if (BIAS) load_bias(t + 1);
+      stage_load(rq, qsrc, t + 1);   // tiles beyond the queries read as zeros
+      stage_load(rg, gsrc, t + 1);
+      rc_load(rc, (t + 1) * 64, wid, lane);
+      if (wave_on) var_dkdv_tile<DHP, 2, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, sacc, dkacc, dvacc, c, sbase + t * 64, dkey, lane);
+      char* nQ = smem + ((t + 1) & 1) * TILE;
+      stage_store<DHP, NT, NCH, QS, true>(rq, nQ, tid);
+      stage_store<DHP, NT, NCH, QS, true>(rg, nQ + 64 * QS, tid);
+      rc_store<BIAS>(rc, (float*)(nQ + 2 * 64 * QS), (t + 1) * 64, S, c, wid, lane);
+      __syncthreads();
+    }
+    if (nfull < ntiles && wave_on) {
+      const char* sQ = smem + (nfull & 1) * TILE;
+      const char* sG = sQ + 64 * QS;
+      const float* sL = (const float*)(sQ + 2 * 64 * QS);
+      if (S - nfull * 64 > 32) {
+        f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
+        var_dkdv_tile<DHP, 2, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, sacc, dkacc, dvacc, c, sbase + nfull * 64, dkey, lane);
+      } else {
+        f32x16 sacc[1] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale)};
+        var_dkdv_tile<DHP, 1, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, sacc, dkacc, dvacc, c, sbase + nfull * 64, dkey, lane);
+      }
+    }
+  }
+  if (krow >= p.Lk) return;
+  bf16* dvp = (bf16*)p.dv + b * p.dv_sb + h * p.dv_sh + (int64_t)krow * p.dv_ss;
+  bf16* dkp = (bf16*)p.dk + b * p.dk_sb + h * p.dk_sh + (int64_t)krow * p.dk_ss;
+  if (krow >= len) {   // padding: its columns hold whatever the zero rows gave
+#pragma unroll
+    for (int dt = 0; dt < DHP / 32; dt++) { dkacc[dt] = zero; dvacc[dt] = zero; }
+  }
+  store_rows<DHP>(dvp, dvacc, 1.f, Dh, lane);
+  store_rows<DHP>(dkp, dkacc, p.scale, Dh, lane);
+}
+
+// ---- bias gradient: dS summed over the samples ---------------------------------------------------------------------------------
+// A workgroup owns 128 keys (32 per wave, on the lanes) x 128 queries (two 64-row tiles) of a head and walks the samples of
+// its share (gridDim.y shares); dS of every sample is added to 4 accumulator tiles per wave and leaves as 32-bit values.  It
+// forms S' and dP once more, 4 of the 14 products of a training pass, which costs less than writing dS (2 bytes per sample,
+// head and pair) and reading it back.
+template <int DHP, bool DROP>
+__global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) {
+  constexpr int NT = 256, CPR = DHP / 8, NCH = (64 * CPR + NT - 1) / NT;
+  constexpr int QS = Strides<DHP>::ROWS;   // Q and dO tiles are read row-wise only
+  constexpr int TILE = 2 * 64 * QS + rc_bytes<true>();
+  __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh;
+  const int nkb = (p.Lk + 127) / 128, nqb = (p.Lq + 127) / 128;
+  const int kb = (int)blockIdx.x % nkb, rest = (int)blockIdx.x / nkb;
+  const int qb = rest % nqb, h = rest / nqb;
+  const int key0 = kb * 128, q0 = qb * 128, krow = key0 + wid * 32 + (lane & 31);
+  const int share = (p.B + (int)gridDim.y - 1) / (int)gridDim.y;
+  const int b_end = min(p.B, share * ((int)blockIdx.y + 1));
+  const float c = p.scale * LOG2E;
+  const int rowoff = 4 * (lane >> 5);
+  const f32x16 zero = ZERO16;
+  f32x16 acc[4] = {zero, zero, zero, zero};
+  auto next_live = [&](int b) { while (b < b_end && key_count(p, b) <= key0) b++; return b; };
+  const int kt = key0 / 32 + wid;   // may lie beyond the last key tile: the descriptor then covers nothing
+  const bool tile_on = kt < p.nkt_t;
+  const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.bias_t + ((int64_t)h * p.nkt_t + (tile_on ? kt : 0)) * p.nqt_t * 1024),
+                                                                       0, tile_on ? p.nqt_t * 2048 : 0, 0x00020000);
+  const DropKey dkey = drop_key(p, krow);
+  RowConsts rc;
+  uint4 rq[NCH], rg[NCH];
+  auto load_tile = [&](int b, int qs) {   // 64 rows of Q, dO and their constants
+    const TileSrc<NCH> qsrc = make_tilesrc<DHP, NT, NCH>((const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, p.Lq, Dh, tid);
+    const TileSrc<NCH> gsrc = make_tilesrc<DHP, NT, NCH>((const bf16*)p.dout + b * p.g_sb + h * p.g_sh, p.g_ss, p.Lq, Dh, tid);
+    stage_load(rq, qsrc, qb * 2 + qs);
+    stage_load(rg, gsrc, qb * 2 + qs);
+    rc_open(rc, p, ((int64_t)b * p.H + h) * p.Lq);
+    rc_load(rc, q0 + qs * 64, wid, lane);
+  };
+  auto store_tile = [&](int buf, int qs) {
+    char* s = smem + buf * TILE;
+    stage_store<DHP, NT, NCH, QS, false>(rq, s, tid);
+    stage_store<DHP, NT, NCH, QS, false>(rg, s + 64 * QS, tid);
+    rc_store<true>(rc, (float*)(s + 2 * 64 * QS), q0 + qs * 64, p.Lq, c, wid, lane);
+  };
+  const bool second = q0 + 64 < p.Lq;   // the second 64-query tile has rows
+  int b = next_live(share * (int)blockIdx.y), buf = 0;
+  if (b < b_end) {
+    load_tile(b, 0);
+    store_tile(0, 0);
+    __syncthreads();
+  }
+  while (b < b_end) {
+    const int len = key_count(p, b), bn = next_live(b + 1);
+    const bool wave_on = key0 + wid * 32 < len, live = krow < len;
+    bf16x8 kf[DHP / 16], vf[DHP / 16];
+    load_stationary<DHP>(kf, (const bf16*)p.k + b * p.k_sb + h * p.k_sh, p.k_ss, krow, len, Dh, lane);
+    load_stationary<DHP>(vf, (const bf16*)p.v + b * p.v_sb + h * p.v_sh, p.v_ss, krow, len, Dh, lane);
+#pragma unroll
+    for (int qs = 0; qs < 2; qs++) {
+      if (qs == 1 && !second) break;
+      const bool more = (qs == 0 && second) || bn < b_end;
+      const int nb = (qs == 0 && second) ? b : bn, nqs = (qs == 0 && second) ? 1 : 0;
+      bf16x8 bf[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)((qb * 2 + qs) * 4096 + i * 1024 + lane * 16)));
+      if (more) load_tile(nb, nqs);
+      if (wave_on) {
+        const char* sQ = smem + buf * TILE;
+        const char* sG = sQ + 64 * QS;
+        const float* sL = (const float*)(sQ + 2 * 64 * QS);
+        const uint32_t xkey = DROP ? drop_xkey(p, dkey, ((int64_t)b * p.H + h) * p.Lq + q0 + qs * 64, rowoff) : 0u;
+#pragma unroll
+        for (int st = 0; st < 2; st++) {
+          f32x16 sacc = init_tile<true>(bf[2 * st], bf[2 * st + 1], p.inv_scale);
+          f32x16 pacc = zero;
+#pragma unroll
+          for (int ks = 0; ks < DHP / 16; ks++) {
+            sacc = MFMA(frag_rows<QS, 0>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
+            pacc = MFMA(frag_rows<QS, 0>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
+          }
+          prob_rows<true>(sacc, sL, st, rowoff, c);
+          ds_rows<DROP>(p, sacc, pacc, sL, st, rowoff, xkey, dkey.xstep, dkey.kodd, dkey.khalf);
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[2 * qs + st][r] += live ? pacc[r] : 0.f;
+        }
+      }
+      if (more) store_tile(buf ^ 1, nqs);
+      __syncthreads();
+      buf ^= 1;
+    }
+    b = bn;
+  }
+  if (krow >= p.Lk) return;
+  float* out = p.dbias + ((int64_t)blockIdx.y * p.H + h) * p.Lq * p.Lk + krow;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int row = q0 + i * 32 + acc_row(r) + rowoff;
+      if (row < p.Lq) out[(int64_t)row * p.Lk] = acc[i][r];
+    }
+}
+
+// ---- up to 32 queries -------------------------------------------------------------------------------------------------------------
+// Bound by K, V in and dK, dV out, so K and V are read once: a wave holds 32 keys, forms S' and dP both ways (the query rows'
+// fragments serve as either operand), and writes dK, dV of its keys; dQ^T += K^T dS^T of the workgroup's 128 keys goes to
+// p.part and is summed over the key blocks, in their order, by var_few_sum_k.
+template <int DHP, int STRIDE>
+__device__ __forceinline__ void frags_to_lds(const bf16x8 (&f)[DHP / 16], char* s, int lane) {
+  const int row = lane & 31, hi = lane >> 5;
+#pragma unroll
+  for (int ks = 0; ks < DHP / 16; ks++) *(bf16x8*)(s + row * STRIDE + (((ks * 2) | hi) ^ swz_of<1>(row)) * 16) = f[ks];
+}
+template <int DHP, bool BIAS>
+__global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p) {
+  constexpr int QS = Strides<DHP>::COLS;
+  constexpr int RED = 4 * 32 * (DHP + 4) * 4;   // dQ of the four waves
+  constexpr int LDS = 6 * 32 * QS > RED ? 6 * 32 * QS : RED;
+  __shared__ __attribute__((aligned(16))) char smem[LDS];   // K of each wave, Q, dO; then the dQ sums
+  __shared__ __attribute__((aligned(16))) float sC[4][32];  // -m c + lr, delta, m, lr
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, rowoff = 4 * (lane >> 5);
+  const HeadBlock hb = head_block(p.B, p.H, p.Lk, 128);
+  if (!hb.valid) return;
+  const int64_t b = hb.b, h = hb.h;
+  const int len = key_count(p, b), key0 = hb.xb * 128, krow = key0 + wid * 32 + (lane & 31);
+  bf16* dvp = (bf16*)p.dv + b * p.dv_sb + h * p.dv_sh + (int64_t)krow * p.dv_ss;
+  bf16* dkp = (bf16*)p.dk + b * p.dk_sb + h * p.dk_sh + (int64_t)krow * p.dk_ss;
+  const f32x16 zero = ZERO16;
+  f32x16 dk[DHP / 32], dv[DHP / 32], dq[DHP / 32];
+#pragma unroll
+  for (int dt = 0; dt < DHP / 32; dt++) { dk[dt] = zero; dv[dt] = zero; dq[dt] = zero; }
+  const int qrow = lane & 31;
+  const bool qv = qrow < p.Lq;
+  const int64_t srow = (b * p.H + h) * p.Lq + qrow;
+  if (key0 < len) {   // otherwise padding only: zeros to dK and dV, nothing to dQ (var_few_sum_k does not read it)
+    bf16x8 kf[DHP / 16], vf[DHP / 16], qf[DHP / 16], gf[DHP / 16];
+    load_stationary<DHP>(kf, (const bf16*)p.k + b * p.k_sb + h * p.k_sh, p.k_ss, krow, len, Dh, lane);
+    load_stationary<DHP>(vf, (const bf16*)p.v + b * p.v_sb + h * p.v_sh, p.v_ss, krow, len, Dh, lane);
+    load_stationary<DHP>(qf, (const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, qrow, p.Lq, Dh, lane);
+    load_stationary<DHP>(gf, (const bf16*)p.dout + b * p.g_sb + h * p.g_sh, p.g_ss, qrow, p.Lq, Dh, lane);
+    float delta = 0.f;
+    {
+      bf16x8 of[DHP / 16];
+      load_stationary<DHP>(of, (const bf16*)p.o + b * p.o_sb + h * p.o_sh, p.o_ss, qrow, p.Lq, Dh, lane);
+#pragma unroll
+      for (int ks = 0; ks < DHP / 16; ks++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) delta += (float)of[ks][j] * (float)gf[ks][j];
+      delta += __shfl_xor(delta, 32, 64);
+    }
+    const float m = qv ? p.stat[2 * srow] : 0.f, lr = qv ? p.stat[2 * srow + 1] : -INFINITY;
+    const float c = p.scale * LOG2E, nmc = -m * c;
+    const bool big = BIAS && __any(fabsf(m * c) > BIG_EXP);
+    char* sK = smem + wid * 32 * QS;
+    char* sQ = smem + 4 * 32 * QS;
+    char* sG = smem + 5 * 32 * QS;
+    frags_to_lds<DHP, QS>(kf, sK, lane);
+    if (wid == 0) {
+      frags_to_lds<DHP, QS>(qf, sQ, lane);
+      if (lane < 32) { sC[0][lane] = nmc + lr; sC[1][lane] = delta; sC[2][lane] = m; sC[3][lane] = lr; }
+      if (hb.xb == 0 && qv && lane < 32) p.delta[srow] = delta;   // for the bias gradient
+    }
+    if (wid == 1) frags_to_lds<DHP, QS>(gf, sG, lane);
+    bf16x8 bs[2], bt[2];
+    if (BIAS) {
+      const int kt = key0 / 32 + wid;
+      const bool on = kt < p.nkt_t;
+      const bf16* ps = p.bias_s + ((int64_t)h * p.nqt * p.nkt + (on ? kt : 0)) * 1024 + lane * 8;
+      const bf16* pt = p.bias_t + ((int64_t)h * p.nkt_t + (on ? kt : 0)) * p.nqt_t * 1024 + lane * 8;
+      bs[0] = *(const bf16x8*)ps; bs[1] = *(const bf16x8*)(ps + 512);
+      bt[0] = *(const bf16x8*)pt; bt[1] = *(const bf16x8*)(pt + 512);
+    }
+    __syncthreads();
+    // queries on the rows, key on the lane: P and dS for dV and dK
+    {
+      f32x16 s = init_tile<BIAS>(bt[0], bt[1], p.inv_scale), d = zero;
+#pragma unroll
+      for (int ks = 0; ks < DHP / 16; ks++) {
+        s = MFMA(qf[ks], kf[ks], s, 0, 0, 0);
+        d = MFMA(gf[ks], vf[ks], d, 0, 0, 0);
+      }
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int ql = 8 * g + rowoff;
+        const f32x4 n4 = *(const f32x4*)(sC[0] + ql), d4 = *(const f32x4*)(sC[1] + ql);
+        const f32x4 m4 = *(const f32x4*)(sC[2] + ql), l4 = *(const f32x4*)(sC[3] + ql);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int r = 4 * g + j;
+          s[r] = BIAS && big ? fast_exp2((s[r] - m4[j]) * c + l4[j]) : fast_exp2(fmaf(s[r], c, n4[j]));
+          d[r] = s[r] * (d[r] - d4[j]);
+        }
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; s2++) {
+        const bf16x8 pf = acc_to_frag(s, s2), df = acc_to_frag(d, s2);
+#pragma unroll
+        for (int dt = 0; dt < DHP / 32; dt++) {
+          dv[dt] = MFMA(frag_cols<QS, 1>(sG, 0, s2, dt * 32, lane), pf, dv[dt], 0, 0, 0);
+          dk[dt] = MFMA(frag_cols<QS, 1>(sQ, 0, s2, dt * 32, lane), df, dk[dt], 0, 0, 0);
+        }
+      }
+    }
+    // keys on the rows, query on the lane: dS for dQ
+    {
+      f32x16 s = init_tile<BIAS>(bs[0], bs[1], p.inv_scale), d = zero;
+#pragma unroll
+      for (int ks = 0; ks < DHP / 16; ks++) {
+        s = MFMA(kf[ks], qf[ks], s, 0, 0, 0);
+        d = MFMA(vf[ks], gf[ks], d, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const float pr = BIAS && big ? fast_exp2((s[r] - m) * c) : fast_exp2(fmaf(s[r], c, nmc));
+        d[r] = key0 + wid * 32 + acc_row(r) + rowoff < len ? pr * (d[r] - delta) : 0.f;
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; s2++) {
+        const bf16x8 df = acc_to_frag(d, s2);
+#pragma unroll
+        for (int dt = 0; dt < DHP / 32; dt++) dq[dt] = MFMA(frag_cols<QS, 1>(sK, 0, s2, dt * 32, lane), df, dq[dt], 0, 0, 0);
+      }
+    }
+    // dQ of the four waves, summed in their order; a lane holds d = dt*32 + 8 g + rowoff + 0..3 of its query
+    __syncthreads();
+    float* red = (float*)smem;
+    const float f = p.scale * fast_exp2(lr);
+#pragma unroll
+    for (int dt = 0; dt < DHP / 32; dt++)
+#pragma unroll
+      for (int g = 0; g < 4; g++)
+        *(float4*)(red + (wid * 32 + qrow) * (DHP + 4) + dt * 32 + 8 * g + rowoff) =
+            make_float4(dq[dt][4 * g] * f, dq[dt][4 * g + 1] * f, dq[dt][4 * g + 2] * f, dq[dt][4 * g + 3] * f);
+    __syncthreads();
+    const int64_t rows = (int64_t)p.B * p.H * p.Lq;
+    for (int i = tid; i < p.Lq * Dh; i += 256) {
+      const int q = i / Dh, d = i - q * Dh;
+      float a = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; w++) a += red[(w * 32 + q) * (DHP + 4) + d];
+      p.part[((int64_t)hb.xb * rows + (b * p.H + h) * p.Lq + q) * Dh + d] = a;
+    }
+  } else if (hb.xb == 0 && wid == 0 && qv && lane < 32) {
+    p.delta[srow] = 0.f;   // a sample without keys: o = 0
+  }
+  if (krow >= p.Lk) return;
+  if (krow >= len) {
+#pragma unroll
+    for (int dt = 0; dt < DHP / 32; dt++) { dk[dt] = zero; dv[dt] = zero; }
+  }
+  store_rows<DHP>(dvp, dv, 1.f, Dh, lane);
+  store_rows<DHP>(dkp, dk, p.scale, Dh, lane);
+}
+// dQ = sum of the key blocks' shares; 16 lanes per row
+__global__ __launch_bounds__(256) void var_few_sum_k(VarP p) {
+  const int64_t rows = (int64_t)p.B * p.H * p.Lq;
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int j = threadIdx.x & 15;
+  if (row >= rows || j * 8 >= p.Dh) return;
+  const int64_t i = row % p.Lq, h = (row / p.Lq) % p.H, b = row / ((int64_t)p.Lq * p.H);
+  const int n = (key_count(p, b) + 127) / 128;
+  float a[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) a[k] = 0.f;
+  for (int s = 0; s < n; s++) {
+    const float* src = p.part + ((int64_t)s * rows + row) * p.Dh + j * 8;
+    const float4 x = *(const float4*)src, y = *(const float4*)(src + 4);
+    a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w; a[4] += y.x; a[5] += y.y; a[6] += y.z; a[7] += y.w;
+  }
+  bf16x8 r;
+#pragma unroll
+  for (int k = 0; k < 8; k++) r[k] = (bf16)a[k];
+  *(bf16x8*)((bf16*)p.dq + b * p.dq_sb + h * p.dq_sh + i * p.dq_ss + j * 8) = r;
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------------------------
+#define VAR_DH(FN, ...) do { if (p.Dh <= 64) FN<64, __VA_ARGS__>(p, st); else if (p.Dh <= 96) FN<96, __VA_ARGS__>(p, st); else FN<128, __VA_ARGS__>(p, st); } while (0)
+template <int DHP, bool BIAS> static void dq_dh(const VarP& p, hipStream_t st) {
+  const dim3 grid(head_block_grid(p.B, p.H, p.Lq, 128));
+  if (p.thr) hipLaunchKernelGGL((var_dq_k<DHP, 4, BIAS, true>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((var_dq_k<DHP, 4, BIAS, false>), grid, dim3(256), 0, st, p);
+}
+template <int DHP, bool BIAS> static void dkdv_dh(const VarP& p, hipStream_t st) {
+  const dim3 grid(head_block_grid(p.B, p.H, p.Lk, 128));
+  if (p.thr) hipLaunchKernelGGL((var_dkdv_k<DHP, 4, BIAS, true>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((var_dkdv_k<DHP, 4, BIAS, false>), grid, dim3(256), 0, st, p);
+}
+template <int DHP, bool DROP> static void dbias_dh(const VarP& p, hipStream_t st) {
+  const dim3 grid((unsigned)(ceil_div(p.Lk, 128) * ceil_div(p.Lq, 128) * p.H), (unsigned)p.splits);
+  hipLaunchKernelGGL((var_dbias_k<DHP, DROP>), grid, dim3(256), 0, st, p);
+}
+template <int DHP, bool BIAS> static void few_dh(const VarP& p, hipStream_t st) {
+  hipLaunchKernelGGL((var_few_bwd_k<DHP, BIAS>), dim3(head_block_grid(p.B, p.H, p.Lk, 128)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(var_few_sum_k, dim3((unsigned)ceil_div((int64_t)p.B * p.H * p.Lq, 16)), dim3(256), 0, st, p);
+}
+void var_launch_dq(const VarP& p, bool bias, hipStream_t st) { if (bias) VAR_DH(dq_dh, true); else VAR_DH(dq_dh, false); }
+void var_launch_dkdv(const VarP& p, bool bias, hipStream_t st) { if (bias) VAR_DH(dkdv_dh, true); else VAR_DH(dkdv_dh, false); }
+void var_launch_dbias(const VarP& p, hipStream_t st) { if (p.thr) VAR_DH(dbias_dh, true); else VAR_DH(dbias_dh, false); }
+void var_launch_few_bwd(const VarP& p, bool bias, hipStream_t st) { if (bias) VAR_DH(few_dh, true); else VAR_DH(few_dh, false); }

@@ -1,0 +1,334 @@
+// Forward pass on the matrix units (bf16, v_mfma_f32_32x32x16_bf16) of attention with a relative position bias and / or key
+// counts, and the bias laid out for it.
+//
+//   workgroup = NW waves x 32 queries (Q in registers), 64-key tiles of K and V pass through LDS (double buffer, two tiles in
+//   flight); S'^T = K Q^T has the keys on the accumulator rows and the query on the lane, so the running maximum is a
+//   register reduction and the probabilities are the next product's operand as they stand.  The bias enters as the INITIAL
+//   accumulator of the score product: it costs an unpacking and a multiplication by 1 / scale per element and nothing else.
+#include "attn_var.h"
+
+// ---- bias in accumulator order ----------------------------------------------------------------------------------------
+// T[index[i][j]][h] as tiles of 32 x 32 in the order in which the lanes of an accumulator tile hold them: tile =
+// [2 register halves][64 lanes][8 registers], 16 bytes per lane and half, so that a wave fetches a tile with two coalesced
+// 16-byte loads per lane.  TR = false: keys on the rows, query on the lane (forward, dQ), tiles ordered [H][query tile][key
+// tile]; TR = true: queries on the rows, key on the lane (dK/dV, bias gradient), [H][key tile][query tile].  Gathering once
+// per pair and head here, instead of once per pair, head and sample inside the attention, takes the gather (an LDS or L2
+// access with its own address per element) out of the inner loops.  Bound by its stores.  HV heads are read per access.
+template <int HV> struct HeadVec;
+template <> struct HeadVec<8> { typedef uint4 t; };
+template <> struct HeadVec<4> { typedef uint2 t; };
+template <> struct HeadVec<2> { typedef uint32_t t; };
+template <> struct HeadVec<1> { typedef uint16_t t; };
+
+template <int HV, bool TR>
+__global__ __launch_bounds__(256) void var_expand_k(VarP p, bf16* __restrict__ out) {
+  const int half = (threadIdx.x >> 6) & 1, lane = threadIdx.x & 63, hi = lane >> 5;
+  const int nlt = TR ? p.nkt_t : p.nqt, nrt = TR ? p.nqt_t : p.nkt;   // tiles along the lanes, along the rows
+  const int64_t tiles = (int64_t)nlt * nrt;
+  const int64_t tile = (int64_t)blockIdx.x * 2 + (threadIdx.x >> 7);
+  if (tile >= tiles) return;
+  const int lt = (int)(tile / nrt), rt = (int)(tile - (int64_t)lt * nrt);
+  const int at_lane = lt * 32 + (lane & 31);
+  int n[8];
+  bool ok[8];
+#pragma unroll
+  for (int r = 0; r < 8; r++) {
+    const int at_row = rt * 32 + acc_row(8 * half + r) + 4 * hi;
+    const int i = TR ? at_row : at_lane, j = TR ? at_lane : at_row;
+    ok[r] = i < p.Lq && j < p.Lk;
+    n[r] = ok[r] ? p.index[(int64_t)i * p.Lk + j] : 0;
+  }
+  typedef typename HeadVec<HV>::t V;
+  for (int h = 0; h < p.H; h += HV) {
+    uint16_t e[8][HV];
+#pragma unroll
+    for (int r = 0; r < 8; r++) {
+      const V v = *(const V*)((const bf16*)p.table + (int64_t)n[r] * p.H + h);
+      __builtin_memcpy(e[r], &v, sizeof(V));
+    }
+#pragma unroll
+    for (int hv = 0; hv < HV; hv++) {
+      bf16x8 o;
+#pragma unroll
+      for (int r = 0; r < 8; r++) {
+        const float x = clamp_bias((float)__builtin_bit_cast(bf16, e[r][hv]), p.bias_lim);
+        o[r] = (bf16)(ok[r] ? x : 0.f);
+      }
+      *(bf16x8*)(out + (((int64_t)(h + hv) * tiles + tile) * 2 + half) * 512 + lane * 8) = o;
+    }
+  }
+}
+template <bool TR> static void expand_t(const VarP& p, hipStream_t st) {
+  const int64_t tiles = TR ? (int64_t)p.nkt_t * p.nqt_t : (int64_t)p.nqt * p.nkt;
+  const dim3 grid((unsigned)ceil_div(tiles, 2)), block(256);
+  bf16* out = (bf16*)(TR ? p.bias_t : p.bias_s);
+  const uintptr_t at = (uintptr_t)p.table;
+  if (p.H % 8 == 0 && at % 16 == 0) hipLaunchKernelGGL((var_expand_k<8, TR>), grid, block, 0, st, p, out);
+  else if (p.H % 4 == 0 && at % 8 == 0) hipLaunchKernelGGL((var_expand_k<4, TR>), grid, block, 0, st, p, out);
+  else if (p.H % 2 == 0 && at % 4 == 0) hipLaunchKernelGGL((var_expand_k<2, TR>), grid, block, 0, st, p, out);
+  else hipLaunchKernelGGL((var_expand_k<1, TR>), grid, block, 0, st, p, out);
+}
+void var_launch_expand(const VarP& p, bool transposed, hipStream_t st) {
+  if (transposed) expand_t<true>(p, st);
+  else expand_t<false>(p, st);
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------------
+// The bias of HALVES 32-key tiles as initial accumulators, in units of 1 / scale
+template <int HALVES, bool BIAS>
+__device__ __forceinline__ void var_init(f32x16 (&sacc)[HALVES], const bf16x8 (&bf)[4], float inv_scale) {
+#pragma unroll
+  for (int st = 0; st < HALVES; st++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) sacc[st][r] = BIAS ? (float)bf[2 * st + (r >> 3)][r & 7] * inv_scale : 0.f;
+}
+// One 64-key tile (HALVES = 2) or its first 32 keys (HALVES = 1) against a wave's 32 queries; sacc starts as the bias.
+template <int DHP, int HALVES, bool PARTIAL, bool BIAS, bool DROP, int KS, int VS>
+__device__ __forceinline__ void var_fwd_tile(const VarP& p, const char* sK, const char* sV, const bf16x8 (&qf)[DHP / 16],
+                                             f32x16 (&sacc)[HALVES], f32x16 (&oacc)[DHP / 32], f32x16& lacc, float& m, float c,
+                                             int k0, int len, uint32_t xrow, int lane) {
+  const int rowoff = 4 * (lane >> 5);
+#pragma unroll
+  for (int st = 0; st < HALVES; st++)
+#pragma unroll
+    for (int ks = 0; ks < DHP / 16; ks++) sacc[st] = MFMA(frag_rows<KS, 0>(sK, st * 32, ks, lane), qf[ks], sacc[st], 0, 0, 0);
+  if (PARTIAL) {   // keys at or beyond the count (only in the last half of the last tile)
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+      if (k0 + (HALVES - 1) * 32 + acc_row(r) + rowoff >= len) sacc[HALVES - 1][r] = -INFINITY;
+  }
+  float mx = sacc[0][0];
+#pragma unroll
+  for (int st = 0; st < HALVES; st++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) mx = fmaxf(mx, sacc[st][r]);
+  mx = max_xor32(mx);
+  // m only has to keep the exponentials in range: it is moved (and O, l rescaled) when some query's tile maximum exceeds it
+  // by more than 2^8 in the exponent.  A row without any score yet has m = -inf.
+  if (__any(mx * c > m * c + 8.f)) {
+    const float mnew = fmaxf(m, mx);
+    const float alpha = m == mnew ? 1.f : fast_exp2((m - mnew) * c);
+    lacc[0] *= alpha;   // only element 0 of the sum tile is ever read
+#pragma unroll
+    for (int dt = 0; dt < DHP / 32; dt++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) oacc[dt][r] *= alpha;
+    m = mnew;
+  }
+  const float ms = BIAS && m == -INFINITY ? 0.f : m;   // nothing but -inf so far: the exponentials are 0
+  if (BIAS && __any(fabsf(ms * c) > BIG_EXP)) {
+#pragma unroll
+    for (int st = 0; st < HALVES; st++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) sacc[st][r] = fast_exp2((sacc[st][r] - ms) * c);
+  } else {
+    const float nmc = -ms * c;
+#pragma unroll
+    for (int st = 0; st < HALVES; st++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) sacc[st][r] = fast_exp2(fmaf(sacc[st][r], c, nmc));
+  }
+  bf16x8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; j++) ones[j] = (bf16)1.f;
+  // O^T[d][q] += V^T[d][key] P^T[key][q].  The probabilities are rounded to bf16 to be an operand (half a step, 2^-8); the
+  // row sum is taken of the rounded ones, on the matrix unit, so that the weights of a row add up to 1.
+#pragma unroll
+  for (int st = 0; st < HALVES; st++)
+#pragma unroll
+    for (int s2 = 0; s2 < 2; s2++) {
+      bf16x8 pf = acc_to_frag(sacc[st], s2);
+      lacc = MFMA(ones, pf, lacc, 0, 0, 0);
+      if (DROP) {   // registers 8 s2 + 0..3 and + 4..7 are two runs of four consecutive keys, each from a multiple of 4
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          uint32_t dr[4];
+          rng_lin_run<4>(xrow + (uint32_t)((k0 + st * 32 + acc_row(8 * s2 + 4 * g)) >> 1) * RNG_C1, dr);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const int r = 8 * s2 + 4 * g + j;
+            sacc[st][r] = dr[j] < p.thr ? 0.f : sacc[st][r] * p.keep_scale;
+          }
+        }
+        pf = acc_to_frag(sacc[st], s2);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DHP / 32; dt++)
+        oacc[dt] = MFMA(frag_cols<VS, 0>(sV, st * 32, s2, dt * 32, lane), pf, oacc[dt], 0, 0, 0);
+    }
+}
+
+// waves per SIMD: what the registers of an instance allow without spilling
+template <int DHP, int NW, bool BIAS, bool DROP> constexpr int var_fwd_occ() {
+  return DHP <= 64 ? (NW == 4 && !BIAS ? 3 : 2) : (DHP <= 96 && NW == 4) ? 2 : 1;
+}
+
+// SPLIT: the keys of a (sample, head) are shared by gridDim.y workgroups; each leaves O unnormalised in 32 bits with its m and
+// row sum, and var_combine_k joins them.
+template <int DHP, int NW, bool BIAS, bool DROP, bool SPLIT>
+__global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void var_fwd_k(VarP p) {
+  constexpr int NT = NW * 64, CPR = DHP / 8, NCH = (64 * CPR + NT - 1) / NT;
+  constexpr int KS = Strides<DHP>::ROWS, VS = Strides<DHP>::COLS, TILE = 64 * KS + 64 * VS;
+  __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, S = p.Lq;
+  const HeadBlock hb = head_block(p.B, p.H, S, NW * 32);
+  if (!hb.valid) return;
+  const int64_t b = hb.b, h = hb.h;
+  const int qrow = hb.xb * (NW * 32) + wid * 32 + (lane & 31);
+  const bool wave_on = hb.xb * (NW * 32) + wid * 32 < S;   // else this wave only helps staging
+  const bf16* qp = (const bf16*)p.q + b * p.q_sb + h * p.q_sh;
+  const bf16* kp = (const bf16*)p.k + b * p.k_sb + h * p.k_sh;
+  const bf16* vp = (const bf16*)p.v + b * p.v_sb + h * p.v_sh;
+  const int len_all = key_count(p, b);
+  // this workgroup's keys: [64 tile0, len)
+  int tile0 = 0, len = len_all;
+  if (SPLIT) {
+    const int per = (((len_all + 63) >> 6) + p.splits - 1) / p.splits;
+    tile0 = per * (int)blockIdx.y;
+    const int end = (tile0 + per) * 64;
+    if (end < len) len = end;
+    if (tile0 * 64 >= len_all) len = tile0 * 64;   // nothing left for this share
+  }
+  const int ntiles = (len + 63) >> 6, nfull = len >> 6;
+  const TileSrc<NCH> ksrc = make_tilesrc<DHP, NT, NCH>(kp, p.k_ss, len, Dh, tid);
+  const TileSrc<NCH> vsrc = make_tilesrc<DHP, NT, NCH>(vp, p.v_ss, len, Dh, tid);
+  bf16x8 qf[DHP / 16];
+  load_stationary<DHP>(qf, qp, p.q_ss, qrow, S, Dh, lane);
+  // bias tiles of this wave's query tile; key tiles beyond the row read as zeros
+  const int qt = hb.xb * NW + wid;
+  const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc(
+      BIAS ? (void*)(p.bias_s + ((int64_t)h * p.nqt + (wave_on ? qt : 0)) * p.nkt * 1024) : nullptr, 0, BIAS ? p.nkt * 2048 : 0, 0x00020000);
+  bf16x8 bf[4];
+  auto load_bias = [&](bf16x8 (&d)[4], int t) {   // t-th 64-key tile: two 32 x 32 tiles
+#pragma unroll
+    for (int i = 0; i < 4; i++) d[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(t * 4096 + i * 1024 + lane * 16)));
+  };
+  if (BIAS) load_bias(bf, tile0);
+  uint4 rkA[NCH], rvA[NCH], rkB[NCH], rvB[NCH];
+  stage_load(rkA, ksrc, tile0);
+  stage_load(rvA, vsrc, tile0);
+  stage_load(rkB, ksrc, tile0 + 1);   // tiles beyond the keys read as zeros, so prefetches need no condition
+  stage_load(rvB, vsrc, tile0 + 1);
+  const f32x16 zero = ZERO16;
+  f32x16 oacc[DHP / 32], lacc = zero;
+#pragma unroll
+  for (int dt = 0; dt < DHP / 32; dt++) oacc[dt] = zero;
+  float m = -INFINITY;
+  const float c = p.scale * LOG2E;
+  const uint32_t rbase = var_drop_xrow(p, (uint64_t)(b * p.H + h) * p.Lq + (uint64_t)qrow, lane);
+  stage_store<DHP, NT, NCH, KS, false>(rkA, smem, tid);
+  stage_store<DHP, NT, NCH, VS, false>(rvA, smem + 64 * KS, tid);
+  __syncthreads();
+
+  auto step = [&](int t, uint4 (&nk)[NCH], uint4 (&nv)[NCH], uint4 (&fk)[NCH], uint4 (&fv)[NCH]) {
+    const char* sK = smem + ((t - tile0) & 1) * TILE;
+    const char* sV = sK + 64 * KS;
+    // loads return in order: the next tile's bias is asked for ahead of the K and V tiles behind it, so that waiting for it
+    // leaves those in flight
+    f32x16 sacc[2];
+    var_init<2, BIAS>(sacc, bf, p.inv_scale);
+    if (BIAS) load_bias(bf, t + 1);
+    stage_load(fk, ksrc, t + 2);
+    stage_load(fv, vsrc, t + 2);
+    if (wave_on) var_fwd_tile<DHP, 2, false, BIAS, DROP, KS, VS>(p, sK, sV, qf, sacc, oacc, lacc, m, c, t * 64, len, rbase, lane);
+    char* nK = smem + ((t + 1 - tile0) & 1) * TILE;
+    stage_store<DHP, NT, NCH, KS, false>(nk, nK, tid);
+    stage_store<DHP, NT, NCH, VS, false>(nv, nK + 64 * KS, tid);
+    __syncthreads();
+  };
+  for (int t = tile0; t < nfull; t += 2) {
+    step(t, rkB, rvB, rkA, rvA);
+    if (t + 1 < nfull) step(t + 1, rkA, rvA, rkB, rvB);
+  }
+  if (nfull < ntiles && nfull >= tile0 && wave_on) {
+    const char* sK = smem + ((nfull - tile0) & 1) * TILE;
+    const char* sV = sK + 64 * KS;
+    if (len - nfull * 64 > 32) {
+      f32x16 sacc[2];
+      var_init<2, BIAS>(sacc, bf, p.inv_scale);
+      var_fwd_tile<DHP, 2, true, BIAS, DROP, KS, VS>(p, sK, sV, qf, sacc, oacc, lacc, m, c, nfull * 64, len, rbase, lane);
+    } else {
+      f32x16 sacc[1];
+      var_init<1, BIAS>(sacc, bf, p.inv_scale);
+      var_fwd_tile<DHP, 1, true, BIAS, DROP, KS, VS>(p, sK, sV, qf, sacc, oacc, lacc, m, c, nfull * 64, len, rbase, lane);
+    }
+  }
+  if (qrow >= S) return;
+  const float l = lacc[0];
+  const int64_t srow = (b * p.H + h) * p.Lq + qrow;
+  if (SPLIT) {
+    const int64_t rows = (int64_t)p.B * p.H * p.Lq;
+    const int64_t prow = (int64_t)blockIdx.y * rows + srow;
+    float* dst = p.part + prow * Dh;
+#pragma unroll
+    for (int dt = 0; dt < DHP / 32; dt++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int d = dt * 32 + 8 * g + 4 * (lane >> 5);
+        if (d < Dh) *(float4*)(dst + d) = make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
+      }
+    if (lane < 32) { p.pstat[2 * prow] = m; p.pstat[2 * prow + 1] = l; }
+    return;
+  }
+  store_rows<DHP>((bf16*)p.o + b * p.o_sb + h * p.o_sh + (int64_t)qrow * p.o_ss, oacc, l == 0.f ? 0.f : 1.f / l, Dh, lane);
+  if (lane < 32) {
+    p.stat[2 * srow] = l == 0.f ? 0.f : m;
+    p.stat[2 * srow + 1] = l == 0.f ? -INFINITY : -__log2f(l);
+  }
+}
+
+// Joins the shares of a row: M = max m, O = sum 2^((m - M) c) O_s / sum 2^((m - M) c) l_s.  16 lanes per row.
+__global__ __launch_bounds__(256) void var_combine_k(VarP p) {
+  const int64_t rows = (int64_t)p.B * p.H * p.Lq;
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int j = threadIdx.x & 15;
+  if (row >= rows) return;
+  const float c = p.scale * LOG2E;
+  float M = -INFINITY;
+  for (int s = 0; s < p.splits; s++) M = fmaxf(M, p.pstat[2 * (s * rows + row)]);
+  float l = 0.f, o[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) o[i] = 0.f;
+  const bool on = j * 8 < p.Dh;
+  for (int s = 0; s < p.splits; s++) {
+    const int64_t at = s * rows + row;
+    const float m = p.pstat[2 * at], w = m == M ? (M == -INFINITY ? 0.f : 1.f) : fast_exp2((m - M) * c);
+    l = fmaf(w, p.pstat[2 * at + 1], l);
+    if (on && w != 0.f) {
+      const float4 a = *(const float4*)(p.part + at * p.Dh + j * 8), b = *(const float4*)(p.part + at * p.Dh + j * 8 + 4);
+      o[0] = fmaf(w, a.x, o[0]); o[1] = fmaf(w, a.y, o[1]); o[2] = fmaf(w, a.z, o[2]); o[3] = fmaf(w, a.w, o[3]);
+      o[4] = fmaf(w, b.x, o[4]); o[5] = fmaf(w, b.y, o[5]); o[6] = fmaf(w, b.z, o[6]); o[7] = fmaf(w, b.w, o[7]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t i = row % p.Lq, h = (row / p.Lq) % p.H, b = row / ((int64_t)p.Lq * p.H);
+  if (on) {
+    bf16x8 r;
+#pragma unroll
+    for (int k = 0; k < 8; k++) r[k] = (bf16)(o[k] * inv);
+    *(bf16x8*)((bf16*)p.o + b * p.o_sb + h * p.o_sh + i * p.o_ss + j * 8) = r;
+  }
+  if (j == 0) {
+    p.stat[2 * row] = l == 0.f ? 0.f : M;
+    p.stat[2 * row + 1] = l == 0.f ? -INFINITY : -__log2f(l);
+  }
+}
+
+template <int DHP, bool BIAS> static void fwd_dh(const VarP& p, int nw, hipStream_t st) {
+  const dim3 grid(head_block_grid(p.B, p.H, p.Lq, nw * 32), (unsigned)p.splits);
+  if (p.thr) {
+    hipLaunchKernelGGL((var_fwd_k<DHP, 4, BIAS, true, false>), grid, dim3(256), 0, st, p);
+  } else if (p.splits > 1) {
+    if (nw == 2) hipLaunchKernelGGL((var_fwd_k<DHP, 2, BIAS, false, true>), grid, dim3(128), 0, st, p);
+    else hipLaunchKernelGGL((var_fwd_k<DHP, 4, BIAS, false, true>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL(var_combine_k, dim3((unsigned)ceil_div((int64_t)p.B * p.H * p.Lq, 16)), dim3(256), 0, st, p);
+  } else {
+    if (nw == 2) hipLaunchKernelGGL((var_fwd_k<DHP, 2, BIAS, false, false>), grid, dim3(128), 0, st, p);
+    else hipLaunchKernelGGL((var_fwd_k<DHP, 4, BIAS, false, false>), grid, dim3(256), 0, st, p);
+  }
+}
+void var_launch_fwd(const VarP& p, bool bias, int nw, hipStream_t st) {
+  if (p.Dh <= 64) { if (bias) fwd_dh<64, true>(p, nw, st); else fwd_dh<64, false>(p, nw, st); }
+  else if (p.Dh <= 96) { if (bias) fwd_dh<96, true>(p, nw, st); else fwd_dh<96, false>(p, nw, st); }
+  else { if (bias) fwd_dh<128, true>(p, nw, st); else fwd_dh<128, false>(p, nw, st); }
+}

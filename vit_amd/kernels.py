@@ -629,14 +629,14 @@ def _var_strides(ts) -> "C.Array":
     return (C.c_int64 * 24)(*vals)
 
 
-def _var_desc(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, table: Optional[Tensor], buckets, kv_len: Optional[Tensor],
+def _var_desc(q: Tensor, k: Tensor, v: Tensor, o: Tensor, stat: Tensor, table: Optional[Tensor], buckets, kv_len: Optional[Tensor],
               scale: float, drop_p: float, seed: int, algo: Optional[int]) -> L.VitkAttnVar:
     B, Lq, H, Dh = q.shape
     Lk = k.shape[1]
     assert k.shape == (B, Lk, H, Dh) == v.shape and o.shape == q.shape and q.dtype == k.dtype == v.dtype == o.dtype
     assert q.stride(3) == k.stride(3) == v.stride(3) == o.stride(3) == 1
     a = L.VitkAttnVar()
-    a.q, a.k, a.v, a.o, a.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr()
+    a.q, a.k, a.v, a.o, a.stat = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), stat.data_ptr()
     if kv_len is not None:
         assert kv_len.dtype == torch.int32 and kv_len.is_contiguous() and kv_len.numel() == B
         a.kv_len = kv_len.data_ptr()
@@ -654,34 +654,35 @@ def _var_desc(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, table: Op
 def attn_var_fwd(q: Tensor, k: Tensor, v: Tensor, *, table: Optional[Tensor] = None, buckets=None,
                  kv_len: Optional[Tensor] = None, scale: float, drop_p: float = 0.0, seed: int = 0,
                  algo: Optional[int] = None, out: Optional[Tensor] = None):
-    """q [B, Lq, H, Dh], k / v [B, Lk, H, Dh] (strided views, d contiguous) -> o [B, Lq, H, Dh], lse [B, H, Lq]."""
+    """q [B, Lq, H, Dh], k / v [B, Lk, H, Dh] (strided views, d contiguous) -> o [B, Lq, H, Dh] and the row
+    statistics [B, H, Lq, 2] that attn_var_bwd takes."""
     lib = L.load()
     L.require_gpu(q, k, v, table, kv_len, None if buckets is None else buckets.index16)
     B, Lq, H, Dh = q.shape
     o = torch.empty((B, Lq, H, Dh), dtype=q.dtype, device=q.device) if out is None else out
-    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device)
-    a = _var_desc(q, k, v, o, lse, table, buckets, kv_len, scale, drop_p, seed, algo)
+    stat = torch.empty((B, H, Lq, 2), dtype=torch.float32, device=q.device)
+    a = _var_desc(q, k, v, o, stat, table, buckets, kv_len, scale, drop_p, seed, algo)
     a.st = _var_strides((q, k, v, o, None, None, None, None))
     need = lib.vitk_attn_var_workspace_bytes(C.byref(a), 0)
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     L.check(lib.vitk_attn_var_fwd(C.byref(a), L.stream()))
-    return o, lse
+    return o, stat
 
 
-def attn_var_bwd(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, dout: Tensor, *, dq: Tensor, dk: Tensor, dv: Tensor,
+def attn_var_bwd(q: Tensor, k: Tensor, v: Tensor, o: Tensor, stat: Tensor, dout: Tensor, *, dq: Tensor, dk: Tensor, dv: Tensor,
                  table: Optional[Tensor] = None, buckets=None, kv_len: Optional[Tensor] = None, scale: float,
                  drop_p: float = 0.0, seed: int = 0, dtable_dtype: Optional[torch.dtype] = None,
                  algo: Optional[int] = None) -> Optional[Tensor]:
     """Fills dq, dk, dv (strided views, d contiguous; padded keys get zeros) and returns the gradient of the bias table in
     ``dtable_dtype`` (None: not wanted)."""
     lib = L.load()
-    L.require_gpu(q, k, v, o, lse, dout, dq, dk, dv, table, kv_len, None if buckets is None else buckets.index16)
+    L.require_gpu(q, k, v, o, stat, dout, dq, dk, dv, table, kv_len, None if buckets is None else buckets.index16)
     assert dout.shape == q.shape == dq.shape and dk.shape == k.shape == dv.shape
     assert dout.dtype == dq.dtype == dk.dtype == dv.dtype == q.dtype
     assert dout.stride(3) == dq.stride(3) == dk.stride(3) == dv.stride(3) == 1
-    a = _var_desc(q, k, v, o, lse, table, buckets, kv_len, scale, drop_p, seed, algo)
+    a = _var_desc(q, k, v, o, stat, table, buckets, kv_len, scale, drop_p, seed, algo)
     a.dout, a.dq, a.dk, a.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     a.st = _var_strides((q, k, v, o, dout, dq, dk, dv))
     dtable = None
