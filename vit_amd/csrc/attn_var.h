@@ -54,3 +54,8 @@ void var_launch_dq(const VarP& p, bool bias, hipStream_t st);
 void var_launch_dkdv(const VarP& p, bool bias, hipStream_t st);
 void var_launch_dbias(const VarP& p, hipStream_t st);
 void var_launch_few_bwd(const VarP& p, bool bias, hipStream_t st);
+void var_launch_combine(const VarP& p, bool f32, hipStream_t st);
+// float32 (attn_var_f32.hip)
+void f32_launch_fwd(const VarP& p, hipStream_t st);
+void f32_launch_bwd(const VarP& p, hipStream_t st);
+void f32_launch_dbias(const VarP& p, hipStream_t st);

@@ -5,7 +5,8 @@
 //   dT[n, h] = sum over samples and over the pairs (i, j) of bucket n of dS
 //
 // This file: the portable kernels (any dtype, head_dim <= 128, any strides, fp32 math; 64 stationary rows per workgroup, 4
-// threads per row), the bucket sums and the entry points.  attn_var_fwd.hip, attn_var_bwd.hip: bf16 on the matrix units.
+// threads per row), the bucket sums and the entry points.  On the matrix units: attn_var_fwd.hip, attn_var_bwd.hip (bf16),
+// attn_var_f32.hip (float32).
 #include "attn_var.h"
 
 constexpr int VMAXI = 32;  // head_dim <= 128
@@ -347,16 +348,17 @@ static int var_validate(const VitkAttnVar* a, bool bwd) {
   }
   return 0;
 }
-// The matrix-unit kernels take bf16, head sizes that are multiples of 8, 16-byte aligned rows, and rows of one (sample, head)
+// The matrix-unit kernels take head sizes that are multiples of 8, 16-byte aligned rows, and rows of one (sample, head)
 // within 32-bit byte offsets (the tiles asked for ahead of the last one included).
 static bool var_mfma_ok(const VitkAttnVar* a, bool bwd) {
-  if (a->dtype != VITK_BF16 || a->Dh % 8 || a->algo == 1 || a->Lk == 0) return false;
+  if (a->Dh % 8 || a->algo == 1 || a->Lk == 0) return false;
+  const int es = a->dtype == VITK_BF16 ? 2 : 4;
   for (int i = 0; i < (bwd ? 24 : 12); i++)
-    if (a->st[i] % 8) return false;
+    if (a->st[i] * es % 16) return false;
   const void* ps[] = {a->q, a->k, a->v, a->o, a->dout, a->dq, a->dk, a->dv};
   for (int i = 0; i < (bwd ? 8 : 4); i++)
     if ((uintptr_t)ps[i] & 15) return false;
-  const int64_t lim = 1ll << 29;   // elements
+  const int64_t lim = (1ll << 30) / es;   // elements
   if ((a->Lq + 256) * a->st[2] >= lim || (a->Lk + 256) * a->st[5] >= lim || (a->Lk + 256) * a->st[8] >= lim || (a->Lq + 256) * a->st[11] >= lim) return false;
   return !bwd || (a->Lq + 256) * a->st[14] < lim;
 }
@@ -365,6 +367,13 @@ static int var_nw(const VitkAttnVar* a) { return a->Lq <= 64 && !(a->drop_p > 0.
 // Workgroups that share the keys of a (sample, head) in the forward pass: 1 where the query blocks alone fill the chip
 // (256 CUs, two workgroups each), otherwise as many as do, each with at least four 64-key tiles.
 static int var_fwd_splits(const VitkAttnVar* a) {
+  if (a->dtype == VITK_F32) {   // one wave of 32 queries per workgroup, 32-key tiles
+    const int64_t waves = a->B * a->H * ceil_div(a->Lq, 32), tiles = ceil_div(a->Lk, 32);
+    if (waves >= 1024 || tiles < 4) return 1;
+    int64_t n = ceil_div(1024, waves);
+    if (n > tiles / 2) n = tiles / 2;
+    return (int)(n < 64 ? n : 64);
+  }
   if (a->drop_p > 0.f) return 1;
   const int64_t blocks = a->B * a->H * ceil_div(a->Lq, 32 * var_nw(a)), tiles = ceil_div(a->Lk, 64);
   if (blocks >= 512 || tiles < 8) return 1;
@@ -374,12 +383,12 @@ static int var_fwd_splits(const VitkAttnVar* a) {
 }
 // Shares of the samples in the bias gradient: enough workgroups to fill the chip twice.
 static int var_dbias_splits(const VitkAttnVar* a) {
-  const int64_t blocks = a->H * ceil_div(a->Lq, 128) * ceil_div(a->Lk, 128);
+  const int64_t blocks = a->H * ceil_div(a->Lq, a->dtype == VITK_F32 ? 32 : 128) * ceil_div(a->Lk, 128);
   int64_t n = ceil_div(512, blocks);
   if (n > a->B) n = a->B;
   return (int)(n < 1 ? 1 : n);
 }
-static bool var_few(const VitkAttnVar* a) { return a->Lq <= 32 && !(a->drop_p > 0.f); }
+static bool var_few(const VitkAttnVar* a) { return a->dtype == VITK_BF16 && a->Lq <= 32 && !(a->drop_p > 0.f); }
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 struct VarWs { size_t delta, bias_s, bias_t, dbias, pieces, part, pstat, total; int splits; };
@@ -390,7 +399,7 @@ static VarWs var_ws(const VitkAttnVar* a, bool bwd) {
   const size_t rows = (size_t)(a->B * a->H * a->Lq);
   size_t at = 0;
   auto take = [&](size_t n) { const size_t here = at; at += up256(n); return here; };
-  if (mfma && a->bias_table) {
+  if (mfma && a->bias_table && a->dtype == VITK_BF16) {
     w.bias_s = take((size_t)a->H * ceil_div(a->Lq, 32) * ceil_div(a->Lk, 64) * 2 * 2048);
     if (bwd) w.bias_t = take((size_t)a->H * ceil_div(a->Lk, 32) * ceil_div(a->Lq, 64) * 2 * 2048);
   }
@@ -431,11 +440,16 @@ extern "C" int vitk_attn_var_fwd(const VitkAttnVar* desc, void* stream) {
     p.splits = w.splits;
     p.part = (float*)(ws + w.part);
     p.pstat = (float*)(ws + w.pstat);
-    if (a->bias_table) {
-      p.bias_s = (const bf16*)(ws + w.bias_s);
-      var_launch_expand(p, false, st);
+    if (a->dtype == VITK_F32) {
+      f32_launch_fwd(p, st);
+      if (p.splits > 1) var_launch_combine(p, true, st);
+    } else {
+      if (a->bias_table) {
+        p.bias_s = (const bf16*)(ws + w.bias_s);
+        var_launch_expand(p, false, st);
+      }
+      var_launch_fwd(p, a->bias_table != nullptr, var_nw(a), st);
     }
-    var_launch_fwd(p, a->bias_table != nullptr, var_nw(a), st);
   } else {
     dim3 grid((unsigned)ceil_div(a->Lq, 64), (unsigned)a->H, (unsigned)a->B);
     const size_t lds = (size_t)2 * VT * a->Dh * sizeof(float);
@@ -463,7 +477,10 @@ extern "C" int vitk_attn_var_bwd(const VitkAttnVar* desc, void* stream) {
   VITK_REQUIRE(a->algo != 2 || mfma, "attn_var_bwd: the matrix-unit kernels cannot take this problem (dtype, alignment, head size)");
   const size_t lds = (size_t)2 * VT * a->Dh * sizeof(float);
   const int64_t pairs = a->Lq * a->Lk;
-  if (mfma) {
+  if (mfma && a->dtype == VITK_F32) {
+    f32_launch_bwd(p, st);   // dQ and delta, then dK and dV
+    if (a->dbias_table) f32_launch_dbias(p, st);
+  } else if (mfma) {
     if (bias) {
       p.bias_s = (const bf16*)(ws + w.bias_s);
       p.bias_t = (const bf16*)(ws + w.bias_t);

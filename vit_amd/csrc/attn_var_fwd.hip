@@ -278,7 +278,7 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
 }
 
 // Joins the shares of a row: M = max m, O = sum 2^((m - M) c) O_s / sum 2^((m - M) c) l_s.  16 lanes per row.
-__global__ __launch_bounds__(256) void var_combine_k(VarP p) {
+template <class T> __global__ __launch_bounds__(256) void var_combine_k(VarP p) {
   const int64_t rows = (int64_t)p.B * p.H * p.Lq;
   const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   const int j = threadIdx.x & 15;
@@ -303,10 +303,12 @@ __global__ __launch_bounds__(256) void var_combine_k(VarP p) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t i = row % p.Lq, h = (row / p.Lq) % p.H, b = row / ((int64_t)p.Lq * p.H);
   if (on) {
-    bf16x8 r;
+    T* dst = (T*)p.o + b * p.o_sb + h * p.o_sh + i * p.o_ss + j * 8;
+    Vec4<T> x, y;
 #pragma unroll
-    for (int k = 0; k < 8; k++) r[k] = (bf16)(o[k] * inv);
-    *(bf16x8*)((bf16*)p.o + b * p.o_sb + h * p.o_sh + i * p.o_ss + j * 8) = r;
+    for (int k = 0; k < 4; k++) { x.v[k] = o[k] * inv; y.v[k] = o[4 + k] * inv; }
+    x.store(dst);
+    y.store(dst + 4);
   }
   if (j == 0) {
     p.stat[2 * row] = l == 0.f ? 0.f : M;
@@ -314,6 +316,11 @@ __global__ __launch_bounds__(256) void var_combine_k(VarP p) {
   }
 }
 
+void var_launch_combine(const VarP& p, bool f32, hipStream_t st) {
+  const dim3 grid((unsigned)ceil_div((int64_t)p.B * p.H * p.Lq, 16));
+  if (f32) hipLaunchKernelGGL((var_combine_k<float>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((var_combine_k<bf16>), grid, dim3(256), 0, st, p);
+}
 template <int DHP, bool BIAS> static void fwd_dh(const VarP& p, int nw, hipStream_t st) {
   const dim3 grid(head_block_grid(p.B, p.H, p.Lq, nw * 32), (unsigned)p.splits);
   if (p.thr) {
@@ -321,7 +328,7 @@ template <int DHP, bool BIAS> static void fwd_dh(const VarP& p, int nw, hipStrea
   } else if (p.splits > 1) {
     if (nw == 2) hipLaunchKernelGGL((var_fwd_k<DHP, 2, BIAS, false, true>), grid, dim3(128), 0, st, p);
     else hipLaunchKernelGGL((var_fwd_k<DHP, 4, BIAS, false, true>), grid, dim3(256), 0, st, p);
-    hipLaunchKernelGGL(var_combine_k, dim3((unsigned)ceil_div((int64_t)p.B * p.H * p.Lq, 16)), dim3(256), 0, st, p);
+    var_launch_combine(p, false, st);
   } else {
     if (nw == 2) hipLaunchKernelGGL((var_fwd_k<DHP, 2, BIAS, false, false>), grid, dim3(128), 0, st, p);
     else hipLaunchKernelGGL((var_fwd_k<DHP, 4, BIAS, false, false>), grid, dim3(256), 0, st, p);
