@@ -34,7 +34,7 @@ def test_plan_covers_every_pair_once_in_bucket_order(shape, nb):
     assert torch.equal(plan.piece[[0, -1]].long(), torch.tensor([0, idx.numel()])) and plan.piece.numel() == plan.num_pieces + 1
     assert plan.bucket_piece.numel() == nb + 1 and int(plan.bucket_piece[-1]) == plan.num_pieces
     sizes = plan.piece.diff()
-    assert int(sizes.min()) >= 1 and int(sizes.max()) <= RelativeBuckets.PIECE
+    assert int(sizes.min()) >= 1 and int(sizes.max()) <= plan.piece_length
     used = torch.unique(flat).tolist()
     for n in used[:50]:
         a, b = int(plan.bucket_piece[n]), int(plan.bucket_piece[n + 1])

@@ -47,6 +47,34 @@ __device__ __forceinline__ uint32_t var_drop_xrow(const VarP& p, uint64_t row, i
 // nothing but a mask's lowest value); such tiles take (S' - m) c instead.
 constexpr float BIG_EXP = 16384.f;
 
+// Workgroup -> item for launches whose neighbouring items share data: workgroups go to the 8 XCDs round-robin and every XCD
+// has an L2 of its own, so each XCD takes a contiguous eighth of the items.  Launched with xcd_grid(items) workgroups.
+__device__ __forceinline__ int64_t xcd_item(int64_t L, int64_t items) {
+  const int64_t n = (items + 7) >> 3, i = L >> 3, item = (L & 7) * n + i;
+  return i < n && item < items ? item : -1;
+}
+static inline unsigned xcd_grid(int64_t items) { return (unsigned)(8 * ((items + 7) >> 3)); }
+// Workgroup -> (sample, head, block of stationary rows).  With a bias the samples are neighbours: they read the same bias
+// tiles, which are then fetched once per XCD and not once per sample (ViT-g/14 at 1024 px, 4 samples: 3.6 GB of bias per
+// pass otherwise).  Without one the row blocks of a (sample, head) are: they share its streamed operands (head_block).
+template <bool BIAS>
+__device__ __forceinline__ HeadBlock var_block(const VarP& p, int nrows, int rows_per_block) {
+  if (!BIAS) return head_block(p.B, p.H, nrows, rows_per_block);
+  const int nxb = (nrows + rows_per_block - 1) / rows_per_block;
+  const int64_t it = xcd_item(blockIdx.x, (int64_t)p.H * nxb * p.B);
+  HeadBlock o;
+  o.valid = it >= 0;
+  const int64_t g = it / p.B;
+  o.b = it - g * p.B;
+  o.h = g / nxb;
+  o.xb = (int)(g - o.h * nxb);
+  return o;
+}
+template <bool BIAS> static inline unsigned var_grid(const VarP& p, int nrows, int rows_per_block) {
+  if (!BIAS) return head_block_grid(p.B, p.H, nrows, rows_per_block);
+  return xcd_grid((int64_t)p.H * ceil_div(nrows, rows_per_block) * p.B);
+}
+
 // launches of the matrix-unit kernels (attn_var_fwd.hip, attn_var_bwd.hip); operands checked by the caller
 void var_launch_expand(const VarP& p, bool transposed, hipStream_t st);
 void var_launch_fwd(const VarP& p, bool bias, int nw, hipStream_t st);

@@ -264,30 +264,57 @@ __global__ __launch_bounds__(256) void var_dbias_simple_k(VarP p) {
   p.dbias[h * p.Lq * p.Lk + pair] = sum;
 }
 
-// ---- bucket sums of dbias: pieces of at most a few thousand pairs, then the pieces of a bucket, both in a fixed order ----
+// ---- bucket sums of dbias: pieces of a bucket's pairs, then the pieces of a bucket, both in a fixed order -------------------
+// A wave sums one piece for up to 4 heads: a pair number is read once for them, and 4 pairs x 4 heads are in flight per lane.
 __global__ __launch_bounds__(256) void var_piece_sum_k(const float* __restrict__ dbias, const int32_t* __restrict__ order,
                                                        const int32_t* __restrict__ piece, float* __restrict__ part,
                                                        int64_t pairs, int H, int npieces, int splits) {
-  const int lane = threadIdx.x & 63, pc = (int)blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y;
+  // Neighbouring pieces on one XCD: the pairs of a bucket lie along a diagonal, a value per cache line, and the rest of each
+  // line belongs to the buckets next to it.
+  const int nblk = (npieces + 3) / 4;
+  const int64_t it = xcd_item(blockIdx.x, (int64_t)nblk * ((H + 3) / 4));
+  if (it < 0) return;
+  const int lane = threadIdx.x & 63, pc = (int)(it % nblk) * 4 + (threadIdx.x >> 6), h0 = (int)(it / nblk) * 4;
   if (pc >= npieces) return;
-  const int b = piece[pc], e = piece[pc + 1];
-  float a = 0.f;
-  for (int i = b + lane; i < e; i += 64) {
-    const int64_t at = order[i];
-    for (int s = 0; s < splits; s++) a += dbias[((int64_t)s * H + h) * pairs + at];
+  const int b = piece[pc], e = piece[pc + 1], nh = min(4, H - h0);
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; s++) {
+    const float* src = dbias + ((int64_t)s * H + h0) * pairs;
+    for (int i = b + lane; i < e; i += 256) {
+      float x[4][4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const bool in = i + 64 * u < e;
+        const int64_t at = in ? order[i + 64 * u] : 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[u][k] = in && k < nh ? src[k * pairs + at] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) a[k] += (x[0][k] + x[1][k]) + (x[2][k] + x[3][k]);
+    }
   }
-  a = wave_sum(a);
-  if (lane == 0) part[(int64_t)h * npieces + pc] = a;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const float t = wave_sum(a[k]);
+    if (lane == 0 && k < nh) part[(int64_t)(h0 + k) * npieces + pc] = t;
+  }
 }
+// a workgroup per bucket and head
 template <class T>
 __global__ __launch_bounds__(256) void var_bucket_sum_k(const float* __restrict__ part, const int32_t* __restrict__ bucket_piece,
-                                                        T* __restrict__ out, int H, int npieces, int nbuckets) {
-  const int lane = threadIdx.x & 63, n = (int)blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y;
-  if (n >= nbuckets) return;
+                                                        T* __restrict__ out, int H, int npieces) {
+  __shared__ float red[4];
+  const int n = (int)blockIdx.x, h = blockIdx.y, b = bucket_piece[n], e = bucket_piece[n + 1];
+  if (e - b <= 1) {   // most buckets of a grid: one piece
+    if (threadIdx.x == 0) out[(int64_t)n * H + h] = from_f<T>(e > b ? part[(int64_t)h * npieces + b] : 0.f);
+    return;
+  }
   float a = 0.f;
-  for (int i = bucket_piece[n] + lane; i < bucket_piece[n + 1]; i += 64) a += part[(int64_t)h * npieces + i];
+  for (int i = b + (int)threadIdx.x; i < e; i += 256) a += part[(int64_t)h * npieces + i];
   a = wave_sum(a);
-  if (lane == 0) out[(int64_t)n * H + h] = from_f<T>(a);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+  __syncthreads();
+  if (threadIdx.x == 0) out[(int64_t)n * H + h] = from_f<T>((red[0] + red[1]) + (red[2] + red[3]));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -383,7 +410,8 @@ static int var_fwd_splits(const VitkAttnVar* a) {
 }
 // Shares of the samples in the bias gradient: enough workgroups to fill the chip twice.
 static int var_dbias_splits(const VitkAttnVar* a) {
-  const int64_t blocks = a->H * ceil_div(a->Lq, a->dtype == VITK_F32 ? 32 : 128) * ceil_div(a->Lk, 128);
+  const int rows = a->dtype == VITK_F32 ? 32 : 64;   // queries of a workgroup
+  const int64_t blocks = a->H * ceil_div(a->Lq, rows) * ceil_div(a->Lk, 128);
   int64_t n = ceil_div(512, blocks);
   if (n > a->B) n = a->B;
   return (int)(n < 1 ? 1 : n);
@@ -507,15 +535,12 @@ extern "C" int vitk_attn_var_bwd(const VitkAttnVar* desc, void* stream) {
   if (a->dbias_table) {
     float* part = (float*)(ws + w.pieces);
     if (a->num_pieces > 0)
-      hipLaunchKernelGGL(var_piece_sum_k, dim3((unsigned)ceil_div(a->num_pieces, 4), (unsigned)a->H), dim3(256), 0, st, p.dbias,
-                         a->order, a->piece, part, pairs, (int)a->H, (int)a->num_pieces, w.splits);
-    const dim3 bgrid((unsigned)ceil_div(a->num_buckets, 4), (unsigned)a->H);
+      hipLaunchKernelGGL(var_piece_sum_k, dim3(xcd_grid(ceil_div(a->num_pieces, 4) * ceil_div(a->H, 4))), dim3(256), 0, st, p.dbias, a->order, a->piece, part, pairs, (int)a->H, (int)a->num_pieces, w.splits);
+    const dim3 bgrid((unsigned)a->num_buckets, (unsigned)a->H);
     if (a->dbias_dtype == VITK_F32)
-      hipLaunchKernelGGL((var_bucket_sum_k<float>), bgrid, dim3(256), 0, st, part, a->bucket_piece, (float*)a->dbias_table, (int)a->H,
-                         (int)a->num_pieces, (int)a->num_buckets);
+      hipLaunchKernelGGL((var_bucket_sum_k<float>), bgrid, dim3(256), 0, st, part, a->bucket_piece, (float*)a->dbias_table, (int)a->H, (int)a->num_pieces);
     else
-      hipLaunchKernelGGL((var_bucket_sum_k<bf16>), bgrid, dim3(256), 0, st, part, a->bucket_piece, (bf16*)a->dbias_table, (int)a->H,
-                         (int)a->num_pieces, (int)a->num_buckets);
+      hipLaunchKernelGGL((var_bucket_sum_k<bf16>), bgrid, dim3(256), 0, st, part, a->bucket_piece, (bf16*)a->dbias_table, (int)a->H, (int)a->num_pieces);
   }
   VITK_LAUNCH_CHECK("attn_var_bwd");
   return 0;

@@ -74,7 +74,7 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
   constexpr int TILE = 64 * KS + 64 * VS;
   __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, S = p.Lq;
-  const HeadBlock hb = head_block(p.B, p.H, S, NW * 32);
+  const HeadBlock hb = var_block<BIAS>(p, S, NW * 32);
   if (!hb.valid) return;
   const int64_t b = hb.b, h = hb.h;
   const int qrow = hb.xb * (NW * 32) + wid * 32 + (lane & 31);
@@ -262,25 +262,30 @@ __device__ __forceinline__ uint32_t drop_xkey(const VarP& p, const DropKey& d, i
 
 template <int DHP, int HALVES, bool BIAS, bool DROP, int QS>
 __device__ __forceinline__ void var_dkdv_tile(const VarP& p, const char* sQ, const char* sG, const float* sL,
-                                              const bf16x8 (&kf)[DHP / 16], const bf16x8 (&vf)[DHP / 16], f32x16 (&sacc)[HALVES],
-                                              f32x16 (&dkacc)[DHP / 32], f32x16 (&dvacc)[DHP / 32], float c, int64_t row0,
-                                              const DropKey& dk, int lane) {
+                                              const bf16x8 (&kf)[DHP / 16], const bf16x8 (&vf)[DHP / 16], bf16x8 (&bf)[4],
+                                              __amdgpu_buffer_rsrc_t brs, uint32_t bias_next, f32x16 (&dkacc)[DHP / 32],
+                                              f32x16 (&dvacc)[DHP / 32], float c, int64_t row0, const DropKey& dk, int lane) {
   const f32x16 zero = ZERO16;
   const int rowoff = 4 * (lane >> 5);
   const uint32_t xkey = DROP ? drop_xkey(p, dk, row0, rowoff) : 0u;
 #pragma unroll
   for (int st = 0; st < HALVES; st++) {
-    f32x16 pacc = MFMA(frag_rows<QS, 1>(sG, st * 32, 0, lane), vf[0], zero, 0, 0, 0);
+    // a half's bias becomes its initial scores and the registers take the next tile's
+    f32x16 sacc = init_tile<BIAS>(bf[2 * st], bf[2 * st + 1], p.inv_scale), pacc = zero;
+    if (BIAS) {
+      bf[2 * st] = __builtin_bit_cast(bf16x8, buf_load16(brs, bias_next + (uint32_t)(st * 2048 + lane * 16)));
+      bf[2 * st + 1] = __builtin_bit_cast(bf16x8, buf_load16(brs, bias_next + (uint32_t)(st * 2048 + 1024 + lane * 16)));
+    }
 #pragma unroll
     for (int ks = 0; ks < DHP / 16; ks++) {
-      sacc[st] = MFMA(frag_rows<QS, 1>(sQ, st * 32, ks, lane), kf[ks], sacc[st], 0, 0, 0);
-      if (ks) pacc = MFMA(frag_rows<QS, 1>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
+      sacc = MFMA(frag_rows<QS, 1>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
+      pacc = MFMA(frag_rows<QS, 1>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
     }
-    prob_rows<BIAS>(sacc[st], sL, st, rowoff, c);
-    ds_rows<DROP>(p, sacc[st], pacc, sL, st, rowoff, xkey, dk.xstep, dk.kodd, dk.khalf);
+    prob_rows<BIAS>(sacc, sL, st, rowoff, c);
+    ds_rows<DROP>(p, sacc, pacc, sL, st, rowoff, xkey, dk.xstep, dk.kodd, dk.khalf);
 #pragma unroll
     for (int s2 = 0; s2 < 2; s2++) {
-      const bf16x8 pf = acc_to_frag(sacc[st], s2);
+      const bf16x8 pf = acc_to_frag(sacc, s2);
       const bf16x8 df = acc_to_frag(pacc, s2);
 #pragma unroll
       for (int dt = 0; dt < DHP / 32; dt++) {
@@ -299,7 +304,7 @@ __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void va
   constexpr int TILE = 2 * 64 * QS + rc_bytes<BIAS>();
   __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, S = p.Lq;
-  const HeadBlock hb = head_block(p.B, p.H, p.Lk, NW * 32);
+  const HeadBlock hb = var_block<BIAS>(p, p.Lk, NW * 32);
   if (!hb.valid) return;
   const int64_t b = hb.b, h = hb.h;
   const int key0 = hb.xb * (NW * 32), krow = key0 + wid * 32 + (lane & 31);
@@ -344,12 +349,10 @@ __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void va
       const char* sQ = smem + (t & 1) * TILE;
       const char* sG = sQ + 64 * QS;
       const float* sL = (const float*)(sQ + 2 * 64 * QS);
-      f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
-      if (BIAS) load_bias(t + 1);
       stage_load(rq, qsrc, t + 1);   // tiles beyond the queries read as zeros
       stage_load(rg, gsrc, t + 1);
       rc_load(rc, (t + 1) * 64, wid, lane);
-      if (wave_on) var_dkdv_tile<DHP, 2, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, sacc, dkacc, dvacc, c, sbase + t * 64, dkey, lane);
+      if (wave_on) var_dkdv_tile<DHP, 2, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, bf, brs, (uint32_t)(t + 1) * 4096u, dkacc, dvacc, c, sbase + t * 64, dkey, lane);
       char* nQ = smem + ((t + 1) & 1) * TILE;
       stage_store<DHP, NT, NCH, QS, true>(rq, nQ, tid);
       stage_store<DHP, NT, NCH, QS, true>(rg, nQ + 64 * QS, tid);
@@ -360,13 +363,9 @@ __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void va
       const char* sQ = smem + (nfull & 1) * TILE;
       const char* sG = sQ + 64 * QS;
       const float* sL = (const float*)(sQ + 2 * 64 * QS);
-      if (S - nfull * 64 > 32) {
-        f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
-        var_dkdv_tile<DHP, 2, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, sacc, dkacc, dvacc, c, sbase + nfull * 64, dkey, lane);
-      } else {
-        f32x16 sacc[1] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale)};
-        var_dkdv_tile<DHP, 1, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, sacc, dkacc, dvacc, c, sbase + nfull * 64, dkey, lane);
-      }
+      const uint32_t none = OOB_OFF;
+      if (S - nfull * 64 > 32) var_dkdv_tile<DHP, 2, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, bf, brs, none, dkacc, dvacc, c, sbase + nfull * 64, dkey, lane);
+      else var_dkdv_tile<DHP, 1, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, bf, brs, none, dkacc, dvacc, c, sbase + nfull * 64, dkey, lane);
     }
   }
   if (krow >= p.Lk) return;
@@ -381,27 +380,33 @@ __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void va
 }
 
 // ---- bias gradient: dS summed over the samples ---------------------------------------------------------------------------------
-// A workgroup owns 128 keys (32 per wave, on the lanes) x 128 queries (two 64-row tiles) of a head and walks the samples of
-// its share (gridDim.y shares); dS of every sample is added to 4 accumulator tiles per wave and leaves as 32-bit values.  It
-// forms S' and dP once more, 4 of the 14 products of a training pass, which costs less than writing dS (2 bytes per sample,
-// head and pair) and reading it back.
-template <int DHP, bool DROP>
+// A workgroup owns 128 keys (32 per wave, on the lanes) x 64 QT queries of a head and walks the samples of its share
+// (p.splits shares); dS of every sample is added to 2 QT accumulator tiles per wave and leaves as 32-bit values.  It forms S'
+// and dP once more, 4 of the 14 products of a training pass, which costs less than writing dS (2 bytes per sample, head and
+// pair) and reading it back.  Every load is asked for a step ahead: the next 64 rows of Q and dO while a tile is multiplied,
+// the next sample's keys and values during the last tile of a sample.
+template <int DHP, int QT, bool DROP>
 __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) {
   constexpr int NT = 256, CPR = DHP / 8, NCH = (64 * CPR + NT - 1) / NT;
   constexpr int QS = Strides<DHP>::ROWS;   // Q and dO tiles are read row-wise only
   constexpr int TILE = 2 * 64 * QS + rc_bytes<true>();
   __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh;
-  const int nkb = (p.Lk + 127) / 128, nqb = (p.Lq + 127) / 128;
-  const int kb = (int)blockIdx.x % nkb, rest = (int)blockIdx.x / nkb;
-  const int qb = rest % nqb, h = rest / nqb;
-  const int key0 = kb * 128, q0 = qb * 128, krow = key0 + wid * 32 + (lane & 31);
-  const int share = (p.B + (int)gridDim.y - 1) / (int)gridDim.y;
-  const int b_end = min(p.B, share * ((int)blockIdx.y + 1));
+  const int nkb = (p.Lk + 127) / 128, nqb = (p.Lq + 64 * QT - 1) / (64 * QT);
+  // neighbours: the key blocks of a query block, then the query blocks of a head (and share): they read the same rows
+  const int64_t it = xcd_item(blockIdx.x, (int64_t)nkb * nqb * p.splits * p.H);
+  if (it < 0) return;
+  const int kb = (int)(it % nkb), qb = (int)(it / nkb % nqb);
+  const int part = (int)(it / ((int64_t)nkb * nqb) % p.splits), h = (int)(it / ((int64_t)nkb * nqb * p.splits));
+  const int key0 = kb * 128, q0 = qb * 64 * QT, krow = key0 + wid * 32 + (lane & 31);
+  const int share = (p.B + p.splits - 1) / p.splits;
+  const int b_end = min(p.B, share * (part + 1));
   const float c = p.scale * LOG2E;
   const int rowoff = 4 * (lane >> 5);
   const f32x16 zero = ZERO16;
-  f32x16 acc[4] = {zero, zero, zero, zero};
+  f32x16 acc[2 * QT];
+#pragma unroll
+  for (int i = 0; i < 2 * QT; i++) acc[i] = zero;
   auto next_live = [&](int b) { while (b < b_end && key_count(p, b) <= key0) b++; return b; };
   const int kt = key0 / 32 + wid;   // may lie beyond the last key tile: the descriptor then covers nothing
   const bool tile_on = kt < p.nkt_t;
@@ -410,11 +415,21 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
   const DropKey dkey = drop_key(p, krow);
   RowConsts rc;
   uint4 rq[NCH], rg[NCH];
+  // this thread's chunks of a 64-row tile: the same offsets in every sample
+  uint32_t qoff[NCH], goff[NCH];
+#pragma unroll
+  for (int i = 0; i < NCH; i++) {
+    const int ch = tid + i * NT, row = ch / CPR, d = (ch % CPR) * 8;
+    const bool in = ch < 64 * CPR && d < Dh;
+    qoff[i] = in ? (uint32_t)((row * p.q_ss + d) * 2) : OOB_OFF;
+    goff[i] = in ? (uint32_t)((row * p.g_ss + d) * 2) : OOB_OFF;
+  }
   auto load_tile = [&](int b, int qs) {   // 64 rows of Q, dO and their constants
-    const TileSrc<NCH> qsrc = make_tilesrc<DHP, NT, NCH>((const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, p.Lq, Dh, tid);
-    const TileSrc<NCH> gsrc = make_tilesrc<DHP, NT, NCH>((const bf16*)p.dout + b * p.g_sb + h * p.g_sh, p.g_ss, p.Lq, Dh, tid);
-    stage_load(rq, qsrc, qb * 2 + qs);
-    stage_load(rg, gsrc, qb * 2 + qs);
+    const __amdgpu_buffer_rsrc_t qrs = rows_rsrc((const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, p.Lq, Dh);
+    const __amdgpu_buffer_rsrc_t grs = rows_rsrc((const bf16*)p.dout + b * p.g_sb + h * p.g_sh, p.g_ss, p.Lq, Dh);
+    const uint32_t qbase = (uint32_t)((q0 + qs * 64) * p.q_ss * 2), gbase = (uint32_t)((q0 + qs * 64) * p.g_ss * 2);
+#pragma unroll
+    for (int i = 0; i < NCH; i++) { rq[i] = buf_load16(qrs, qoff[i] + qbase); rg[i] = buf_load16(grs, goff[i] + gbase); }
     rc_open(rc, p, ((int64_t)b * p.H + h) * p.Lq);
     rc_load(rc, q0 + qs * 64, wid, lane);
   };
@@ -424,9 +439,16 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
     stage_store<DHP, NT, NCH, QS, false>(rg, s + 64 * QS, tid);
     rc_store<true>(rc, (float*)(s + 2 * 64 * QS), q0 + qs * 64, p.Lq, c, wid, lane);
   };
-  const bool second = q0 + 64 < p.Lq;   // the second 64-query tile has rows
-  int b = next_live(share * (int)blockIdx.y), buf = 0;
+  bf16x8 kf[DHP / 16], vf[DHP / 16], kn[DHP / 16], vn[DHP / 16];
+  auto load_keys = [&](int b) {
+    const int len = key_count(p, b);
+    load_stationary<DHP>(kn, (const bf16*)p.k + b * p.k_sb + h * p.k_sh, p.k_ss, krow, len, Dh, lane);
+    load_stationary<DHP>(vn, (const bf16*)p.v + b * p.v_sb + h * p.v_sh, p.v_ss, krow, len, Dh, lane);
+  };
+  const bool second = QT == 2 && q0 + 64 < p.Lq;   // the second 64-query tile has rows
+  int b = next_live(share * part), buf = 0;
   if (b < b_end) {
+    load_keys(b);
     load_tile(b, 0);
     store_tile(0, 0);
     __syncthreads();
@@ -434,17 +456,14 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
   while (b < b_end) {
     const int len = key_count(p, b), bn = next_live(b + 1);
     const bool wave_on = key0 + wid * 32 < len, live = krow < len;
-    bf16x8 kf[DHP / 16], vf[DHP / 16];
-    load_stationary<DHP>(kf, (const bf16*)p.k + b * p.k_sb + h * p.k_sh, p.k_ss, krow, len, Dh, lane);
-    load_stationary<DHP>(vf, (const bf16*)p.v + b * p.v_sb + h * p.v_sh, p.v_ss, krow, len, Dh, lane);
 #pragma unroll
-    for (int qs = 0; qs < 2; qs++) {
+    for (int ks = 0; ks < DHP / 16; ks++) { kf[ks] = kn[ks]; vf[ks] = vn[ks]; }
+#pragma unroll
+    for (int qs = 0; qs < QT; qs++) {
       if (qs == 1 && !second) break;
-      const bool more = (qs == 0 && second) || bn < b_end;
-      const int nb = (qs == 0 && second) ? b : bn, nqs = (qs == 0 && second) ? 1 : 0;
-      bf16x8 bf[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)((qb * 2 + qs) * 4096 + i * 1024 + lane * 16)));
+      const bool last = qs == QT - 1 || !second, more = !last || bn < b_end;
+      const int nb = last ? bn : b, nqs = last ? 0 : 1;
+      if (last && more) load_keys(bn);
       if (more) load_tile(nb, nqs);
       if (wave_on) {
         const char* sQ = smem + buf * TILE;
@@ -453,12 +472,13 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
         const uint32_t xkey = DROP ? drop_xkey(p, dkey, ((int64_t)b * p.H + h) * p.Lq + q0 + qs * 64, rowoff) : 0u;
 #pragma unroll
         for (int st = 0; st < 2; st++) {
-          f32x16 sacc = init_tile<true>(bf[2 * st], bf[2 * st + 1], p.inv_scale);
+          const uint32_t at = (uint32_t)(((qb * QT + qs) * 2 + st) * 2048 + lane * 16);
+          f32x16 sacc = init_tile<true>(__builtin_bit_cast(bf16x8, buf_load16(brs, at)), __builtin_bit_cast(bf16x8, buf_load16(brs, at + 1024)), p.inv_scale);
           f32x16 pacc = zero;
 #pragma unroll
           for (int ks = 0; ks < DHP / 16; ks++) {
-            sacc = MFMA(frag_rows<QS, 0>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
             pacc = MFMA(frag_rows<QS, 0>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
+            sacc = MFMA(frag_rows<QS, 0>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
           }
           prob_rows<true>(sacc, sL, st, rowoff, c);
           ds_rows<DROP>(p, sacc, pacc, sL, st, rowoff, xkey, dkey.xstep, dkey.kodd, dkey.khalf);
@@ -473,9 +493,9 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
     b = bn;
   }
   if (krow >= p.Lk) return;
-  float* out = p.dbias + ((int64_t)blockIdx.y * p.H + h) * p.Lq * p.Lk + krow;
+  float* out = p.dbias + ((int64_t)part * p.H + h) * p.Lq * p.Lk + krow;
 #pragma unroll
-  for (int i = 0; i < 4; i++)
+  for (int i = 0; i < 2 * QT; i++)
 #pragma unroll
     for (int r = 0; r < 16; r++) {
       const int row = q0 + i * 32 + acc_row(r) + rowoff;
@@ -501,7 +521,7 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
   __shared__ __attribute__((aligned(16))) char smem[LDS];   // K of each wave, Q, dO; then the dQ sums
   __shared__ __attribute__((aligned(16))) float sC[4][32];  // -m c + lr, delta, m, lr
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, rowoff = 4 * (lane >> 5);
-  const HeadBlock hb = head_block(p.B, p.H, p.Lk, 128);
+  const HeadBlock hb = var_block<BIAS>(p, p.Lk, 128);
   if (!hb.valid) return;
   const int64_t b = hb.b, h = hb.h;
   const int len = key_count(p, b), key0 = hb.xb * 128, krow = key0 + wid * 32 + (lane & 31);
@@ -658,21 +678,22 @@ __global__ __launch_bounds__(256) void var_few_sum_k(VarP p) {
 // ---- launches ------------------------------------------------------------------------------------------------------------------------
 #define VAR_DH(FN, ...) do { if (p.Dh <= 64) FN<64, __VA_ARGS__>(p, st); else if (p.Dh <= 96) FN<96, __VA_ARGS__>(p, st); else FN<128, __VA_ARGS__>(p, st); } while (0)
 template <int DHP, bool BIAS> static void dq_dh(const VarP& p, hipStream_t st) {
-  const dim3 grid(head_block_grid(p.B, p.H, p.Lq, 128));
+  const dim3 grid(var_grid<BIAS>(p, p.Lq, 128));
   if (p.thr) hipLaunchKernelGGL((var_dq_k<DHP, 4, BIAS, true>), grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL((var_dq_k<DHP, 4, BIAS, false>), grid, dim3(256), 0, st, p);
 }
 template <int DHP, bool BIAS> static void dkdv_dh(const VarP& p, hipStream_t st) {
-  const dim3 grid(head_block_grid(p.B, p.H, p.Lk, 128));
+  const dim3 grid(var_grid<BIAS>(p, p.Lk, 128));
   if (p.thr) hipLaunchKernelGGL((var_dkdv_k<DHP, 4, BIAS, true>), grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL((var_dkdv_k<DHP, 4, BIAS, false>), grid, dim3(256), 0, st, p);
 }
 template <int DHP, bool DROP> static void dbias_dh(const VarP& p, hipStream_t st) {
-  const dim3 grid((unsigned)(ceil_div(p.Lk, 128) * ceil_div(p.Lq, 128) * p.H), (unsigned)p.splits);
-  hipLaunchKernelGGL((var_dbias_k<DHP, DROP>), grid, dim3(256), 0, st, p);
+  constexpr int QT = 1;   // 128 queries (QT = 2) spill: ViT-B/14, 64 samples, 191 us
+  const dim3 grid(xcd_grid(ceil_div(p.Lk, 128) * ceil_div(p.Lq, 64 * QT) * p.splits * p.H));
+  hipLaunchKernelGGL((var_dbias_k<DHP, QT, DROP>), grid, dim3(256), 0, st, p);
 }
 template <int DHP, bool BIAS> static void few_dh(const VarP& p, hipStream_t st) {
-  hipLaunchKernelGGL((var_few_bwd_k<DHP, BIAS>), dim3(head_block_grid(p.B, p.H, p.Lk, 128)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((var_few_bwd_k<DHP, BIAS>), dim3(var_grid<BIAS>(p, p.Lk, 128)), dim3(256), 0, st, p);
   hipLaunchKernelGGL(var_few_sum_k, dim3((unsigned)ceil_div((int64_t)p.B * p.H * p.Lq, 16)), dim3(256), 0, st, p);
 }
 void var_launch_dq(const VarP& p, bool bias, hipStream_t st) { if (bias) VAR_DH(dq_dh, true); else VAR_DH(dq_dh, false); }

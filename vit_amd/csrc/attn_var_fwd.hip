@@ -171,7 +171,7 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
   constexpr int KS = Strides<DHP>::ROWS, VS = Strides<DHP>::COLS, TILE = 64 * KS + 64 * VS;
   __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, S = p.Lq;
-  const HeadBlock hb = head_block(p.B, p.H, S, NW * 32);
+  const HeadBlock hb = var_block<BIAS>(p, S, NW * 32);
   if (!hb.valid) return;
   const int64_t b = hb.b, h = hb.h;
   const int qrow = hb.xb * (NW * 32) + wid * 32 + (lane & 31);
@@ -322,7 +322,7 @@ void var_launch_combine(const VarP& p, bool f32, hipStream_t st) {
   else hipLaunchKernelGGL((var_combine_k<bf16>), grid, dim3(256), 0, st, p);
 }
 template <int DHP, bool BIAS> static void fwd_dh(const VarP& p, int nw, hipStream_t st) {
-  const dim3 grid(head_block_grid(p.B, p.H, p.Lq, nw * 32), (unsigned)p.splits);
+  const dim3 grid(var_grid<BIAS>(p, p.Lq, nw * 32), (unsigned)p.splits);
   if (p.thr) {
     hipLaunchKernelGGL((var_fwd_k<DHP, 4, BIAS, true, false>), grid, dim3(256), 0, st, p);
   } else if (p.splits > 1) {

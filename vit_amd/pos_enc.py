@@ -122,10 +122,8 @@ class RelativeBuckets:
 
     ``index`` [Lq, Lk] holds integers in [0, num_buckets), num_buckets <= 65536.  The plan is built once (it reads the
     index on the host) and used by every call of every layer with these positions: ``index16`` the numbers in 16 bits,
-    ``order`` the pairs sorted by bucket, ``piece`` / ``bucket_piece`` the runs of at most ``PIECE`` pairs that are summed
-    at a time and the runs of each bucket."""
-
-    PIECE = 2048
+    ``order`` the pairs sorted by bucket, ``piece`` / ``bucket_piece`` the runs of at most ``piece_length`` pairs that are
+    summed at a time and the runs of each bucket."""
 
     def __init__(self, index: Tensor, num_buckets: int):
         if index.dim() != 2 or index.dtype in (torch.bool, torch.uint16, torch.uint32, torch.uint64) or index.is_floating_point() \
@@ -146,12 +144,14 @@ class RelativeBuckets:
         self.index16 = torch.where(flat >= 32768, flat - 65536, flat).to(torch.int16).view(self.shape)
         self.order = torch.sort(flat, stable=True).indices.to(torch.int32)
         counts = torch.bincount(flat, minlength=num_buckets).cpu()
-        pieces = (counts + self.PIECE - 1) // self.PIECE
+        # short runs keep many waves busy; the number of runs stays within what the second sum takes in a few steps
+        self.piece_length = length = min(4096, max(256, 1 << (flat.numel() // 8192).bit_length()))
+        pieces = (counts + length - 1) // length
         bucket_piece = torch.cat([pieces.new_zeros(1), pieces.cumsum(0)])
         starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
         owner = torch.repeat_interleave(torch.arange(num_buckets), pieces)          # bucket of every piece
         within = torch.arange(int(bucket_piece[-1])) - bucket_piece[owner]
-        piece = torch.cat([starts[owner] + within * self.PIECE, starts[-1:]])
+        piece = torch.cat([starts[owner] + within * length, starts[-1:]])
         self.num_pieces = int(bucket_piece[-1])
         self.piece = piece.to(torch.int32).to(index.device)
         self.bucket_piece = bucket_piece.to(torch.int32).to(index.device)
