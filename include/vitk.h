@@ -303,7 +303,7 @@ int vitk_copy_samples(const void* src, void* dst, const int64_t* idx, int64_t n,
  * A section is q or k: heads addressed as ptr[b*sb + l*ss + h*sh + d], d contiguous; sec[1].w = NULL: one section only.
  * fwd reads x and writes y (may be x itself).  bwd reads x and g = dL/dy and writes y = dL/dx (may be g itself) and the
  * weight gradients dw / db [Dh] (NULL where not wanted), summed in a fixed order through `workspace`.
- * head_dim: a multiple of 8, at most 128; strides: multiples of 4 elements, pointers aligned to 4 elements.
+ * head_dim: a multiple of 8, at most 128; strides multiples of 16 bytes, pointers 16-byte aligned.
  * round_norm = 1 rounds n (backward: the un-rotated gradient) to the tensors' dtype between the two steps, and
  * emulate_bf16 = 1 rounds the products of the rotation to bf16, as separate passes do; 0: one rounding, at the store. */
 typedef struct VitkQkSection {

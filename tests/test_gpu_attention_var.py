@@ -515,9 +515,15 @@ def test_qk_norm_rope(case, dtype, wdtype, ln):
 
 
 def test_qk_norm_rope_in_place_strided_and_wide_batches():
-    """In place on the packed projection, heads on 4-element boundaries only, and enough rows for several walks of the grid."""
+    """In place on the packed projection, heads wider apart than they are long, enough rows for several steps of every wave;
+    heads off the 16-byte boundaries are refused by the kernel and copied by the public call."""
     g = torch.Generator().manual_seed(5)
-    for Dh, pad, B, Ln in ((80, 4, 3, 50), (64, 0, 40, 300)):
+    off = torch.randn(2, 9, 3, 84, generator=g).to(DEV, torch.bfloat16)[..., :80]
+    w80 = torch.ones(80, device=DEV)
+    with pytest.raises(RuntimeError, match="16 bytes"):
+        K.qk_norm_rope_fwd(off, None, torch.empty_like(off), None, (w80, None), (None, None), (None, None), 1e-5, False)
+    check(qk_norm_rope(off, None, w80)[0], norm_rope_reference(off, w80, None, None, False, 1e-5, torch.zeros(2, 9, 3, 80))["y"], "copied")
+    for Dh, pad, B, Ln in ((80, 8, 3, 50), (64, 0, 40, 300), (24, 0, 5, 700), (16, 8, 2, 40)):
         buf = torch.randn(B, Ln, 2, 3, Dh + pad, generator=g).to(DEV, torch.bfloat16)
         x = buf[..., :Dh]
         w = (1 + 0.3 * torch.randn(Dh, generator=g)).to(DEV)

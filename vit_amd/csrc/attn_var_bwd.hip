@@ -393,11 +393,14 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
   __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh;
   const int nkb = (p.Lk + 127) / 128, nqb = (p.Lq + 64 * QT - 1) / (64 * QT);
-  // neighbours: the key blocks of a query block, then the query blocks of a head (and share): they read the same rows
+  // Neighbours: panels of up to 8 key blocks, all query blocks of a panel, then the next panel of the head (and share): the
+  // workgroups that run on an XCD at a time then read few rows between them, which stay in its L2.
   const int64_t it = xcd_item(blockIdx.x, (int64_t)nkb * nqb * p.splits * p.H);
   if (it < 0) return;
-  const int kb = (int)(it % nkb), qb = (int)(it / nkb % nqb);
-  const int part = (int)(it / ((int64_t)nkb * nqb) % p.splits), h = (int)(it / ((int64_t)nkb * nqb * p.splits));
+  const int64_t hp = it / ((int64_t)nkb * nqb);
+  const int part = (int)(hp % p.splits), h = (int)(hp / p.splits), in = (int)(it - hp * nkb * nqb);
+  const int panel = in / (8 * nqb), width = min(8, nkb - panel * 8), rest = in - panel * 8 * nqb;
+  const int kb = panel * 8 + rest % width, qb = rest / width;
   const int key0 = kb * 128, q0 = qb * 64 * QT, krow = key0 + wid * 32 + (lane & 31);
   const int share = (p.B + p.splits - 1) / p.splits;
   const int b_end = min(p.B, share * (part + 1));

@@ -6,9 +6,10 @@
 //   dn   = g * cos + rotate_half^T(g * sin),  dw = sum dn * xhat,  db = sum dn
 //   dx   = rstd * (u - xhat * mean(u * xhat) - mean(u)),  u = dn * w   (RMSNorm without the last mean)
 // The statistics are taken again from x in the backward: the head is in registers anyway, and nothing is kept between the
-// two passes.  A row of a head lies on a group of G lanes; every lane holds V values of the first half of the head and the
-// V values Dh / 2 further on, so that the rotation stays inside the lane.  A wave walks the heads of one token at a time
-// with the token's sines and cosines in registers.  Bound by HBM: x in, y out (forward), g and x in, dx out (backward).
+// two passes.  A lane holds 8 consecutive values of a head (16 bytes in bf16), a wave as many whole rows as fit, so that its
+// loads and stores are one contiguous run where the rows are; the other half of the head that the rotation needs and the
+// row sums go through LDS.  Positions come before samples in a wave's run: their sines and cosines stay in registers.
+// Bound by HBM: x in, y out (forward), g and x in, dx out (backward).
 #include "common.h"
 
 struct QkSec {        // one section: q or k
@@ -30,166 +31,240 @@ struct QkP {
   int ln, round_norm, emu, want_dw;
 };
 
-template <int G> __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+// Eight consecutive values of a head as they lie in memory
+template <class T> struct Raw8;
+template <> struct Raw8<bf16> { uint4 a; };
+template <> struct Raw8<float> { uint4 a, b; };
+template <class T> __device__ __forceinline__ Raw8<T> load8(const T* p) {
+  Raw8<T> r;
+  r.a = *(const uint4*)p;
+  if constexpr (sizeof(T) == 4) r.b = *(const uint4*)(p + 4);
+  return r;
 }
-template <class T, int V> __device__ __forceinline__ void load_n(float (&r)[V], const T* p) {
-  VecN<T, V> t;
-  t.load(p);
+template <class T> __device__ __forceinline__ void unpack8(float (&v)[8], const Raw8<T>& r) {
+  T e[8];
+  __builtin_memcpy(e, &r, sizeof(r));
 #pragma unroll
-  for (int i = 0; i < V; i++) r[i] = t.v[i];
+  for (int i = 0; i < 8; i++) v[i] = to_f<T>(e[i]);
 }
-template <class T, int V> __device__ __forceinline__ void store_n(T* p, const float (&r)[V]) {
-  VecN<T, V> t;
+template <class T> __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  T e[8];
 #pragma unroll
-  for (int i = 0; i < V; i++) t.v[i] = r[i];
-  t.store(p);
-}
-template <class TW> __device__ __forceinline__ float opt_load(const void* p, int i, float dflt) {
-  return p ? to_f<TW>(((const TW*)p)[i]) : dflt;
-}
-template <int V> __device__ __forceinline__ void load_table(float (&r)[V], const float* p) {
-#pragma unroll
-  for (int i = 0; i < V; i += 4) *(float4*)(r + i) = *(const float4*)(p + i);
+  for (int i = 0; i < 8; i++) e[i] = from_f<T>(v[i]);
+  Raw8<T> r;
+  __builtin_memcpy(&r, e, sizeof(r));
+  *(uint4*)p = r.a;
+  if constexpr (sizeof(T) == 4) *(uint4*)(p + 4) = r.b;
 }
 
-template <class T, class TW, int V, int G, bool BWD>
-__global__ __launch_bounds__(256) void qk_norm_rope_k(QkP p) {
-  constexpr int HPW = 64 / G;   // heads a wave handles at a time
+// Lanes of a wave hand values to each other through LDS, which a wave's accesses pass in order; this keeps the compiler from
+// moving one lane's read ahead of another's write.  No instruction comes of it.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// NL = lanes of a row, Dh / 8 (0: taken from the descriptor).  SEP: the roundings of separate passes are wanted (round_norm,
+// emulate_bf16); otherwise products are fused into the sums.
+template <class T, class TW, int NL, bool SEP, bool BWD>
+__global__ __launch_bounds__(256, 4) void qk_norm_rope_k(QkP p) {
+  constexpr int EX = 64 * 8, SUMS = 64 * 4;   // a wave's values handed to the other half of a head; partial sums (rows x 16)
+  __shared__ __attribute__((aligned(16))) float shared[4][EX + SUMS];
   const QkSec& s = p.s[blockIdx.y];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int j = lane % G, hl = lane / G, half = p.Dh >> 1;
-  const bool on = j * V < half;
-  const int d0 = on ? j * V : 0, d1 = d0 + half;
-  const float inv_n = 1.f / (float)p.Dh;
-  float w0[V], w1[V], b0[V], b1[V], gw0[V], gw1[V], gb0[V], gb1[V];
+  const int nl = NL ? NL : p.Dh >> 3, Dh = nl * 8, rpw = nl == 3 ? 16 : 64 / nl, rr = lane / nl, j = lane - rr * nl, d0 = 8 * j;
+  const bool on = rr < rpw;
+  float* ex = shared[wid] + (on ? rr : 0) * Dh;
+  float* sums = shared[wid] + EX + (on && rpw <= 16 ? rr : 0) * 16;
+  // the lane's two quads and where their partners lie, half a head (nl quads) away; a first-half quad takes -sin
+  const int qa = 2 * j, qb = 2 * j + 1;
+  const int pa = 4 * (qa < nl ? qa + nl : qa - nl), pb = 4 * (qb < nl ? qb + nl : qb - nl);
+  const float sga = qa < nl ? -1.f : 1.f, sgb = qb < nl ? -1.f : 1.f;
+  const float inv_n = 1.f / (float)Dh;
+  const bool has_b = !BWD && s.b != nullptr, has_table = s.table != nullptr;
+  float w[8], bias[8], gw[8], gb[8];
 #pragma unroll
-  for (int i = 0; i < V; i++) {
-    w0[i] = to_f<TW>(((const TW*)s.w)[d0 + i]); w1[i] = to_f<TW>(((const TW*)s.w)[d1 + i]);
-    b0[i] = BWD ? 0.f : opt_load<TW>(s.b, d0 + i, 0.f); b1[i] = BWD ? 0.f : opt_load<TW>(s.b, d1 + i, 0.f);
-    gw0[i] = gw1[i] = gb0[i] = gb1[i] = 0.f;
+  for (int i = 0; i < 8; i++) {
+    w[i] = on ? to_f<TW>(((const TW*)s.w)[d0 + i]) : 0.f;
+    bias[i] = has_b && on ? to_f<TW>(((const TW*)s.b)[d0 + i]) : 0.f;
+    gw[i] = gb[i] = 0.f;
   }
-  const int64_t tokens = (int64_t)p.B * s.L;
-  for (int64_t t = (int64_t)blockIdx.x * 4 + wid; t < tokens; t += (int64_t)gridDim.x * 4) {
-    const int64_t b = t / s.L;
-    const int l = (int)(t - b * s.L);
-    const bool rot = s.table != nullptr && l >= s.prefix;
-    float s0[V], s1[V], c0[V], c1[V];
-    if (rot) {
-      const float* tp = s.table + b * s.tok_stride + (int64_t)(l - s.prefix) * p.Dh;
-      load_table<V>(s0, tp + d0); load_table<V>(s1, tp + d1);
-      load_table<V>(c0, tp + s.cos_off + d0); load_table<V>(c1, tp + s.cos_off + d1);
-    }
-    const T* xt = (const T*)s.x + b * s.x_sb + (int64_t)l * s.x_ss;
-    const T* gt = BWD ? (const T*)s.g + b * s.g_sb + (int64_t)l * s.g_ss : nullptr;
-    T* yt = (T*)s.y + b * s.y_sb + (int64_t)l * s.y_ss;
-    for (int h0 = 0; h0 < s.H; h0 += HPW) {
-      const int h = h0 + hl;
-      const bool live = on && h < s.H;
-      float x0[V], x1[V], g0[V], g1[V];
-      if (live) {
-        load_n<T, V>(x0, xt + h * s.x_sh + d0); load_n<T, V>(x1, xt + h * s.x_sh + d1);
-        if (BWD) { load_n<T, V>(g0, gt + h * s.g_sh + d0); load_n<T, V>(g1, gt + h * s.g_sh + d1); }
-      } else {
+  // Sum over the lanes of a row, the same value in all of them: by shuffles where they are a power of two, else through LDS,
+  // in the lanes' order
+  auto row_sum = [&](float v) {
+    if (NL == 4 || NL == 8 || NL == 16) {
 #pragma unroll
-        for (int i = 0; i < V; i++) { x0[i] = x1[i] = 0.f; g0[i] = g1[i] = 0.f; }
+      for (int o = NL / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+      return v;
+    }
+    if (nl <= 2) return nl == 1 ? v : v + __shfl_xor(v, 1, 64);
+    wave_order();
+    if (on) sums[j] = v;   // at most 16 rows
+    wave_order();
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (4 * i < nl) {
+        const float4 q = *(const float4*)(sums + 4 * i);
+        t += 4 * i + 3 < nl ? (q.x + q.y) + (q.z + q.w) : 4 * i + 2 < nl ? q.x + q.y + q.z : 4 * i + 1 < nl ? q.x + q.y : q.x;
+      }
+    }
+    return t;
+  };
+  // A wave takes a run of tokens, the samples of a position one after the other, and of a token rpw heads at a time: the
+  // token's addresses are scalars, a lane only adds its head and position in it.
+  const int64_t tokens = (int64_t)p.B * s.L, nw = (int64_t)gridDim.x * 4, run = (tokens + nw - 1) / nw;
+  const int64_t t0 = run * ((int64_t)blockIdx.x * 4 + wid), t1 = t0 + run < tokens ? t0 + run : tokens;
+  if (t0 < t1) {
+    int l = (int)(t0 / p.B), b = (int)(t0 - (int64_t)l * p.B), u = 0, table_l = -1;
+    const int nu = (s.H + rpw - 1) / rpw;
+    const int xo = rr * (int)s.x_sh + d0, go = BWD ? rr * (int)s.g_sh + d0 : 0, yo = rr * (int)s.y_sh + d0;
+    auto fetch = [&](Raw8<T>& xr, Raw8<T>& gr, int l, int b, int u) {
+      if (on && u * rpw + rr < s.H) {
+        xr = load8<T>((const T*)s.x + b * s.x_sb + (int64_t)l * s.x_ss + (int64_t)u * rpw * s.x_sh + xo);
+        if (BWD) gr = load8<T>((const T*)s.g + b * s.g_sb + (int64_t)l * s.g_ss + (int64_t)u * rpw * s.g_sh + go);
+      }
+    };
+    float sn[8], cs[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) { sn[i] = 0.f; cs[i] = 1.f; }
+    Raw8<T> xr = {}, gr = {};
+    fetch(xr, gr, l, b, 0);
+    for (int64_t left = (t1 - t0) * nu; left > 0; left--) {
+      const int lc = l, bc = b, uc = u;
+      float x[8], g[8];
+      unpack8<T>(x, xr);
+      if (BWD) unpack8<T>(g, gr);
+      if (++u == nu) { u = 0; if (++b == p.B) { b = 0; l++; } }
+      if (left > 1) fetch(xr, gr, l, b, u);   // the next heads are asked for before these are worked on
+      const bool live = on && uc * rpw + rr < s.H;
+      const bool rot = has_table && lc >= s.prefix;
+      if (rot && (lc != table_l || s.tok_stride)) {
+        const float* tp = s.table + bc * s.tok_stride + (int64_t)(lc - s.prefix) * Dh + (on ? d0 : 0);
+        *(float4*)sn = *(const float4*)tp; *(float4*)(sn + 4) = *(const float4*)(tp + 4);
+        *(float4*)cs = *(const float4*)(tp + s.cos_off); *(float4*)(cs + 4) = *(const float4*)(tp + s.cos_off + 4);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (!BWD) sn[i] *= i < 4 ? sga : sgb;   // the sign of rotate_half goes with the sine
+        table_l = lc;
       }
       if (p.ln) {
         float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; i++) m += x0[i] + x1[i];
-        m = group_sum<G>(m) * inv_n;
+        for (int i = 0; i < 8; i++) m += x[i];
+        m = row_sum(m) * inv_n;
 #pragma unroll
-        for (int i = 0; i < V; i++) { x0[i] -= m; x1[i] -= m; }
+        for (int i = 0; i < 8; i++) x[i] -= m;
       }
       float q = 0.f;
-      if (live) {
 #pragma unroll
-        for (int i = 0; i < V; i++) { q = fmaf(x0[i], x0[i], q); q = fmaf(x1[i], x1[i], q); }
-      }
-      const float rstd = rsqrtf(group_sum<G>(q) * inv_n + p.eps);
+      for (int i = 0; i < 8; i++) q = fmaf(x[i], x[i], q);
+      const float rstd = __builtin_amdgcn_rsqf(row_sum(q) * inv_n + p.eps);   // 1 ulp
       if (!BWD) {
-        float y0[V], y1[V];
+        float y[8];
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-          float n0 = norm_apply(x0[i], rstd, w0[i], b0[i], s.b != nullptr), n1 = norm_apply(x1[i], rstd, w1[i], b1[i], s.b != nullptr);
-          if (p.round_norm) { n0 = round_as<T>(n0); n1 = round_as<T>(n1); }
-          y0[i] = rot ? rope_mix(n0, c0[i], -n1, s0[i], p.emu) : n0;
-          y1[i] = rot ? rope_mix(n1, c1[i], n0, s1[i], p.emu) : n1;
+        for (int i = 0; i < 8; i++) {
+          y[i] = SEP ? norm_apply(x[i], rstd, w[i], bias[i], has_b) : fmaf(x[i] * rstd, w[i], bias[i]);
+          if (SEP && p.round_norm) y[i] = round_as<T>(y[i]);
         }
-        if (live) { store_n<T, V>(yt + h * s.y_sh + d0, y0); store_n<T, V>(yt + h * s.y_sh + d1, y1); }
+        if (rot) {
+          wave_order();
+          if (on) {
+            *(float4*)(ex + d0) = make_float4(y[0], y[1], y[2], y[3]);
+            *(float4*)(ex + d0 + 4) = make_float4(y[4], y[5], y[6], y[7]);
+          }
+          wave_order();
+          float o[8];
+          *(float4*)o = *(const float4*)(ex + pa);
+          *(float4*)(o + 4) = *(const float4*)(ex + pb);
+#pragma unroll
+          for (int i = 0; i < 8; i++) y[i] = SEP ? rope_mix(y[i], cs[i], o[i], sn[i], p.emu) : fmaf(y[i], cs[i], o[i] * sn[i]);
+        }
+        if (live) store8<T>((T*)s.y + bc * s.y_sb + (int64_t)lc * s.y_ss + (int64_t)uc * rpw * s.y_sh + yo, y);
       } else {
+        if (rot) {   // the transposed rotation: the partner sends g sin
+          float t[8], o[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) t[i] = __fmul_rn(g[i], sn[i]);
+          wave_order();
+          if (on) {
+            *(float4*)(ex + d0) = make_float4(t[0], t[1], t[2], t[3]);
+            *(float4*)(ex + d0 + 4) = make_float4(t[4], t[5], t[6], t[7]);
+          }
+          wave_order();
+          *(float4*)o = *(const float4*)(ex + pa);
+          *(float4*)(o + 4) = *(const float4*)(ex + pb);
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float sg = i < 4 ? sga : sgb;   // -1 in the first half, which adds its partner's product
+            if (SEP) {
+              float a = __fmul_rn(g[i], cs[i]), c = o[i];
+              if (p.emu) { a = round_bf16(a); c = round_bf16(c); }
+              g[i] = __fadd_rn(a, -sg * c);
+              if (p.round_norm) g[i] = round_as<T>(g[i]);
+            } else {
+              g[i] = fmaf(g[i], cs[i], -sg * o[i]);
+            }
+          }
+        }
         float a = 0.f, c = 0.f;   // sums of u * xhat and of u
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-          float n0 = rot ? rope_mix(g0[i], c0[i], g1[i], s1[i], p.emu) : g0[i];
-          float n1 = rot ? rope_mix(g1[i], c1[i], -g0[i], s0[i], p.emu) : g1[i];
-          if (p.round_norm && rot) { n0 = round_as<T>(n0); n1 = round_as<T>(n1); }
-          x0[i] *= rstd; x1[i] *= rstd;
-          if (live) {
-            gw0[i] = fmaf(n0, x0[i], gw0[i]); gw1[i] = fmaf(n1, x1[i], gw1[i]);
-            gb0[i] += n0; gb1[i] += n1;
-            g0[i] = n0 * w0[i]; g1[i] = n1 * w1[i];
-            a = fmaf(g0[i], x0[i], a); a = fmaf(g1[i], x1[i], a);
-            c += g0[i] + g1[i];
-          }
+        for (int i = 0; i < 8; i++) {
+          x[i] *= rstd;
+          if (live) { gw[i] = fmaf(g[i], x[i], gw[i]); gb[i] += g[i]; }
+          g[i] *= w[i];
+          a = fmaf(g[i], x[i], a);
+          if (p.ln) c += g[i];
         }
-        a = group_sum<G>(a) * inv_n;
-        c = p.ln ? group_sum<G>(c) * inv_n : 0.f;
-        if (live) {
+        a = row_sum(a) * inv_n;
+        c = p.ln ? row_sum(c) * inv_n : 0.f;
 #pragma unroll
-          for (int i = 0; i < V; i++) {
-            g0[i] = (g0[i] - c - x0[i] * a) * rstd;
-            g1[i] = (g1[i] - c - x1[i] * a) * rstd;
-          }
-          store_n<T, V>(yt + h * s.y_sh + d0, g0); store_n<T, V>(yt + h * s.y_sh + d1, g1);
-        }
+        for (int i = 0; i < 8; i++) g[i] = (fmaf(-x[i], a, g[i]) - c) * rstd;
+        if (live) store8<T>((T*)s.y + bc * s.y_sb + (int64_t)lc * s.y_ss + (int64_t)uc * rpw * s.y_sh + yo, g);
       }
     }
   }
-  if (BWD && p.want_dw) {   // sums of the workgroup: groups of a wave by shuffles, waves through LDS, always in this order
-    __shared__ float red[4][2][128];
+  if (BWD && p.want_dw) {   // sums of the workgroup over the rows of its waves, always in this order: dw, then db
+    for (int which = 0; which < 2; which++) {
+      __syncthreads();
+      if (on) {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-#pragma unroll
-      for (int o = G; o < 64; o <<= 1) {
-        gw0[i] += __shfl_xor(gw0[i], o, 64); gw1[i] += __shfl_xor(gw1[i], o, 64);
-        gb0[i] += __shfl_xor(gb0[i], o, 64); gb1[i] += __shfl_xor(gb1[i], o, 64);
+        for (int i = 0; i < 8; i++) ex[d0 + i] = which ? gb[i] : gw[i];
       }
-      if (on && hl == 0) {
-        red[wid][0][d0 + i] = gw0[i]; red[wid][0][d1 + i] = gw1[i];
-        red[wid][1][d0 + i] = gb0[i]; red[wid][1][d1 + i] = gb1[i];
+      __syncthreads();
+      for (int d = threadIdx.x; d < Dh; d += 256) {
+        float t = 0.f;
+        for (int v = 0; v < 4; v++)
+          for (int r = 0; r < rpw; r++) t += shared[v][r * Dh + d];
+        p.partial[((int64_t)(blockIdx.y * 2 + which) * gridDim.x + blockIdx.x) * Dh + d] = t;
       }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * p.Dh; i += 256) {
-      const int which = i >= p.Dh, d = i - which * p.Dh;
-      p.partial[((int64_t)(blockIdx.y * 2 + which) * gridDim.x + blockIdx.x) * p.Dh + d] =
-          (red[0][which][d] + red[1][which][d]) + (red[2][which][d] + red[3][which][d]);
     }
   }
 }
 
-// dw / db of a section from the per-workgroup sums: block = (section, dw or db); 8 row groups x 128 columns
+// dw / db of a section from the per-workgroup sums: a workgroup per (section, dw or db) and 8 columns; 128 row groups, their
+// sums joined in a tree through LDS
 template <class TW> __global__ __launch_bounds__(1024) void qk_norm_rope_reduce_k(QkP p, int nblk) {
-  __shared__ float red[8][128];
-  const QkSec& s = p.s[blockIdx.x >> 1];
-  TW* out = (TW*)((blockIdx.x & 1) ? s.db : s.dw);
-  const int d = threadIdx.x & 127, r = threadIdx.x >> 7;
-  const float* src = p.partial + (int64_t)blockIdx.x * nblk * p.Dh;
+  __shared__ float red[128][8];
+  const int which = blockIdx.y, c = threadIdx.x & 7, r = threadIdx.x >> 3, d = (int)blockIdx.x * 8 + c;
+  const QkSec& s = p.s[which >> 1];
+  TW* out = (TW*)((which & 1) ? s.db : s.dw);
+  if (!out) return;
+  const float* src = p.partial + (int64_t)which * nblk * p.Dh + d;
   float a = 0.f;
-  if (out && d < p.Dh)
-    for (int i = r; i < nblk; i += 8) a += src[(int64_t)i * p.Dh + d];
-  red[r][d] = a;
-  __syncthreads();
-  if (out && r == 0 && d < p.Dh) {
-    float t = 0.f;
+  for (int i = r; i < nblk; i += 1024) {   // 8 rows in flight
+    float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) t += red[i][d];
-    out[d] = from_f<TW>(t);
+    for (int u = 0; u < 8; u++) x[u] = i + 128 * u < nblk ? src[(int64_t)(i + 128 * u) * p.Dh] : 0.f;
+    a += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
   }
+  red[r][c] = a;
+  __syncthreads();
+  for (int o = 64; o > 0; o >>= 1) {
+    if (r < o) red[r][c] += red[r + o][c];
+    __syncthreads();
+  }
+  if (r == 0) out[d] = from_f<TW>(red[0][c]);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -197,7 +272,7 @@ static int qk_blocks(const VitkQkNormRope* a, bool bwd) {
   int64_t tok = a->sec[0].L * a->B;
   if (a->sec[1].w && a->sec[1].L * a->B > tok) tok = a->sec[1].L * a->B;
   const int64_t want = ceil_div(tok, 4);
-  const int64_t cap = bwd ? 1024 : 16384;   // backward: one partial row per workgroup
+  const int64_t cap = bwd ? 1024 : 2048;   // 4 or 8 workgroups per CU; backward: one partial row per workgroup
   return (int)(want < cap ? (want < 1 ? 1 : want) : cap);
 }
 extern "C" size_t vitk_qk_norm_rope_workspace_bytes(const VitkQkNormRope* a) {
@@ -215,8 +290,7 @@ template <bool BWD> static int qk_norm_rope_run(const VitkQkNormRope* a, hipStre
   QkP p;
   p.B = (int)a->B; p.Dh = (int)a->Dh; p.eps = a->eps; p.ln = a->is_layernorm; p.round_norm = a->round_norm; p.emu = a->emulate_bf16;
   p.partial = (float*)a->workspace;
-  const int es = a->dtype == VITK_BF16 ? 2 : 4;
-  bool v8 = a->dtype == VITK_BF16 && a->Dh % 16 == 0;
+  const int es = a->dtype == VITK_BF16 ? 2 : 4, al = 16 / es;   // elements of 16 bytes
   bool want = false;
   int nsec = 0;
   for (int i = 0; i < 2; i++) {
@@ -228,19 +302,16 @@ template <bool BWD> static int qk_norm_rope_run(const VitkQkNormRope* a, hipStre
     VITK_REQUIRE(q.L >= 0 && q.H > 0 && q.L < (1ll << 31) && q.H < (1ll << 31), "%s: bad shape L=%lld H=%lld", name, (long long)q.L, (long long)q.H);
     VITK_REQUIRE(q.prefix >= 0 && q.prefix <= q.L, "%s: prefix=%lld outside [0, %lld]", name, (long long)q.prefix, (long long)q.L);
     VITK_REQUIRE(!q.table || ((uintptr_t)q.table & 15) == 0, "%s: the rotation table must be 16-byte aligned", name);
-    const int64_t st_[] = {q.x_sb, q.x_ss, q.x_sh, q.y_sb, q.y_ss, q.y_sh, BWD ? q.g_sb : 0, BWD ? q.g_ss : 0, BWD ? q.g_sh : 0};
+    const bool hs = q.H > 1, ls = q.L > 1, bs = a->B > 1;   // the stride of an axis of one element is never used
+    const int64_t st_[] = {bs ? q.x_sb : 0, ls ? q.x_ss : 0, hs ? q.x_sh : 0, bs ? q.y_sb : 0, ls ? q.y_ss : 0, hs ? q.y_sh : 0,
+                           BWD && bs ? q.g_sb : 0, BWD && ls ? q.g_ss : 0, BWD && hs ? q.g_sh : 0};
     const void* ps[] = {q.x, q.y, BWD ? q.g : q.x};
-    for (int64_t x : st_) {
-      VITK_REQUIRE(x % 4 == 0, "%s: strides must be multiples of 4 elements", name);
-      if (x % 8) v8 = false;
-    }
-    for (const void* x : ps) {
-      VITK_REQUIRE((uintptr_t)x % (4 * es) == 0, "%s: pointers must be aligned to 4 elements", name);
-      if ((uintptr_t)x % 16) v8 = false;
-    }
+    for (int64_t x : st_) VITK_REQUIRE(x % al == 0, "%s: strides must be multiples of 16 bytes", name);
+    for (int k : {2, 5, 8}) VITK_REQUIRE(st_[k] >= 0 && st_[k] < (1ll << 24), "%s: head stride %lld out of range", name, (long long)st_[k]);
+    for (const void* x : ps) VITK_REQUIRE((uintptr_t)x % 16 == 0, "%s: pointers must be 16-byte aligned", name);
     s.x = q.x; s.g = q.g; s.y = q.y; s.w = q.w; s.b = q.b; s.dw = q.dw; s.db = q.db; s.table = q.table;
-    s.x_sb = q.x_sb; s.x_ss = q.x_ss; s.x_sh = q.x_sh; s.g_sb = q.g_sb; s.g_ss = q.g_ss; s.g_sh = q.g_sh;
-    s.y_sb = q.y_sb; s.y_ss = q.y_ss; s.y_sh = q.y_sh;
+    s.x_sb = st_[0]; s.x_ss = st_[1]; s.x_sh = st_[2]; s.y_sb = st_[3]; s.y_ss = st_[4]; s.y_sh = st_[5];
+    s.g_sb = st_[6]; s.g_ss = st_[7]; s.g_sh = st_[8];
     const int64_t n = q.L - q.prefix;
     s.tok_stride = q.per_sample ? n * a->Dh : 0;
     s.cos_off = (q.per_sample ? a->B : 1) * n * a->Dh;
@@ -251,17 +322,24 @@ template <bool BWD> static int qk_norm_rope_run(const VitkQkNormRope* a, hipStre
   VITK_REQUIRE(!want || a->workspace, "%s: workspace required for the weight gradients", name);
   const int nb = qk_blocks(a, BWD);
   const dim3 grid((unsigned)nb, (unsigned)nsec), block(256);
-  const int lanes = (int)a->Dh / (v8 ? 16 : 8);   // lanes that hold a row
-#define QK_GO(T, TW, V, G) hipLaunchKernelGGL((qk_norm_rope_k<T, TW, V, G, BWD>), grid, block, 0, st, p)
-#define QK_G(T, TW, V) do { if (lanes <= 2) QK_GO(T, TW, V, 2); else if (lanes <= 4) QK_GO(T, TW, V, 4); else if (lanes <= 8) QK_GO(T, TW, V, 8); else QK_GO(T, TW, V, 16); } while (0)
-#define QK_W(T, V) do { if (a->w_dtype == VITK_F32) QK_G(T, float, V); else QK_G(T, bf16, V); } while (0)
-  if (a->dtype == VITK_F32) QK_W(float, 4);
-  else if (v8) QK_W(bf16, 8);
-  else QK_W(bf16, 4);
+  const bool sep = a->round_norm || a->emulate_bf16;
+#define QK_GO(T, TW, NL) do { \
+    if (sep) hipLaunchKernelGGL((qk_norm_rope_k<T, TW, NL, true, BWD>), grid, block, 0, st, p); \
+    else hipLaunchKernelGGL((qk_norm_rope_k<T, TW, NL, false, BWD>), grid, block, 0, st, p); } while (0)
+#define QK_N(T, TW) do { \
+    switch (a->Dh / 8) { \
+      case 4: QK_GO(T, TW, 4); break; case 8: QK_GO(T, TW, 8); break; case 10: QK_GO(T, TW, 10); break; \
+      case 11: QK_GO(T, TW, 11); break; case 12: QK_GO(T, TW, 12); break; case 16: QK_GO(T, TW, 16); break; \
+      default: QK_GO(T, TW, 0); } } while (0)
+  if (a->dtype == VITK_F32 && a->w_dtype == VITK_F32) QK_N(float, float);
+  else if (a->dtype == VITK_F32) QK_GO(float, bf16, 0);
+  else if (a->w_dtype == VITK_F32) QK_N(bf16, float);
+  else QK_N(bf16, bf16);
   VITK_LAUNCH_CHECK(name);
   if (BWD && want) {
-    if (a->w_dtype == VITK_F32) hipLaunchKernelGGL((qk_norm_rope_reduce_k<float>), dim3(2 * nsec), dim3(1024), 0, st, p, nb);
-    else hipLaunchKernelGGL((qk_norm_rope_reduce_k<bf16>), dim3(2 * nsec), dim3(1024), 0, st, p, nb);
+    const dim3 rgrid((unsigned)(a->Dh / 8), (unsigned)(2 * nsec));
+    if (a->w_dtype == VITK_F32) hipLaunchKernelGGL((qk_norm_rope_reduce_k<float>), rgrid, dim3(1024), 0, st, p, nb);
+    else hipLaunchKernelGGL((qk_norm_rope_reduce_k<bf16>), rgrid, dim3(1024), 0, st, p, nb);
     VITK_LAUNCH_CHECK(name);
   }
   return 0;

@@ -526,14 +526,6 @@ def can_qk_norm_rope(dtype: torch.dtype, Dh: int) -> bool:
     return Dh % 8 == 0 and 8 <= Dh <= 128 and dtype in (torch.float32, torch.bfloat16)
 
 
-def head_rows(t: Tensor) -> Tensor:
-    """``t`` [B, L, H, Dh] with d contiguous and heads on 4-element boundaries (a view that is not is copied once)."""
-    sb, ss, sh, sd = t.stride()
-    if sd == 1 and not (sb % 4 or ss % 4 or sh % 4 or t.data_ptr() % (4 * t.element_size())):
-        return t
-    return t.contiguous()
-
-
 def _qk_section(sec: L.VitkQkSection, x: Tensor, g: Optional[Tensor], y: Tensor, w: Tensor, b: Optional[Tensor],
                 dw: Optional[Tensor], db: Optional[Tensor], table: Optional[Tensor]) -> None:
     B, Ln, H, Dh = x.shape

@@ -476,11 +476,11 @@ class QkNormRopeFn(torch.autograd.Function):
         q, k, qw, kw, table_q, table_k = ctx.saved_tensors
         eps, layernorm, has_qb, has_kb = ctx.meta
         need = ctx.needs_input_grad
-        dq = torch.zeros_like(q) if dq is None else K.head_rows(dq)
+        dq = torch.zeros_like(q) if dq is None else K.attn_operand(dq)
         gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         gk = None
         if k is not None:
-            dk = torch.zeros_like(k) if dk is None else K.head_rows(dk)
+            dk = torch.zeros_like(k) if dk is None else K.attn_operand(dk)
             gk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         dw = K.qk_norm_rope_bwd((q, k), (dq, dk if k is not None else None), (gq, gk), (qw, kw), (table_q, table_k),
                                 eps, layernorm, (need[2], has_qb and need[4], need[3], has_kb and need[5]))
