@@ -70,7 +70,8 @@ template <class T, class TW, int NL, bool SEP, bool BWD>
 __global__ __launch_bounds__(256, 4) void qk_norm_rope_k(QkP p) {
   constexpr int EX = 64 * 8, SUMS = 64 * 4;   // a wave's values handed to the other half of a head; partial sums (rows x 16)
   __shared__ __attribute__((aligned(16))) float shared[4][EX + SUMS];
-  const QkSec& s = p.s[blockIdx.y];
+  const QkSec s = blockIdx.y == 0 ? p.s[0] : p.s[1];
+  const int H = s.H;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nl = NL ? NL : p.Dh >> 3, Dh = nl * 8, rpw = nl == 3 ? 16 : 64 / nl, rr = lane / nl, j = lane - rr * nl, d0 = 8 * j;
   const bool on = rr < rpw;
@@ -117,38 +118,61 @@ __global__ __launch_bounds__(256, 4) void qk_norm_rope_k(QkP p) {
   const int64_t t0 = run * ((int64_t)blockIdx.x * 4 + wid), t1 = t0 + run < tokens ? t0 + run : tokens;
   if (t0 < t1) {
     int l = (int)(t0 / p.B), b = (int)(t0 - (int64_t)l * p.B), u = 0, table_l = -1;
-    const int nu = (s.H + rpw - 1) / rpw;
+    const int nu = (H + rpw - 1) / rpw;
+    // Addresses move by three fixed steps: to the next heads of a token, to the next sample, to the next position
+    const int64_t xu = (int64_t)rpw * s.x_sh, yu = (int64_t)rpw * s.y_sh, gu = BWD ? (int64_t)rpw * s.g_sh : 0;
+    const int64_t xb = s.x_sb - (nu - 1) * xu, yb = s.y_sb - (nu - 1) * yu, gb_ = BWD ? s.g_sb - (nu - 1) * gu : 0;
+    const int64_t xl = s.x_ss - (p.B - 1) * s.x_sb - (nu - 1) * xu, yl = s.y_ss - (p.B - 1) * s.y_sb - (nu - 1) * yu;
+    const int64_t gl = BWD ? s.g_ss - (p.B - 1) * s.g_sb - (nu - 1) * gu : 0;
+    const T* xp = (const T*)s.x + b * s.x_sb + (int64_t)l * s.x_ss;
+    const T* gp = BWD ? (const T*)s.g + b * s.g_sb + (int64_t)l * s.g_ss : nullptr;
+    T* yp = (T*)s.y + b * s.y_sb + (int64_t)l * s.y_ss;
     const int xo = rr * (int)s.x_sh + d0, go = BWD ? rr * (int)s.g_sh + d0 : 0, yo = rr * (int)s.y_sh + d0;
-    auto fetch = [&](Raw8<T>& xr, Raw8<T>& gr, int l, int b, int u) {
-      if (on && u * rpw + rr < s.H) {
-        xr = load8<T>((const T*)s.x + b * s.x_sb + (int64_t)l * s.x_ss + (int64_t)u * rpw * s.x_sh + xo);
-        if (BWD) gr = load8<T>((const T*)s.g + b * s.g_sb + (int64_t)l * s.g_ss + (int64_t)u * rpw * s.g_sh + go);
+    const float* table = s.table;
+    const int64_t tok_stride = s.tok_stride, cos_off = s.cos_off;
+    const int prefix = s.prefix, B = p.B;
+    const bool ln = p.ln;
+    const float eps = p.eps;
+    auto fetch = [&](Raw8<T>& xr, Raw8<T>& gr, int u) {
+      if (on && u * rpw + rr < H) {
+        xr = load8<T>(xp + xo);
+        if (BWD) gr = load8<T>(gp + go);
       }
     };
     float sn[8], cs[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) { sn[i] = 0.f; cs[i] = 1.f; }
     Raw8<T> xr = {}, gr = {};
-    fetch(xr, gr, l, b, 0);
+    fetch(xr, gr, 0);
     for (int64_t left = (t1 - t0) * nu; left > 0; left--) {
       const int lc = l, bc = b, uc = u;
       float x[8], g[8];
       unpack8<T>(x, xr);
       if (BWD) unpack8<T>(g, gr);
-      if (++u == nu) { u = 0; if (++b == p.B) { b = 0; l++; } }
-      if (left > 1) fetch(xr, gr, l, b, u);   // the next heads are asked for before these are worked on
-      const bool live = on && uc * rpw + rr < s.H;
-      const bool rot = has_table && lc >= s.prefix;
-      if (rot && (lc != table_l || s.tok_stride)) {
-        const float* tp = s.table + bc * s.tok_stride + (int64_t)(lc - s.prefix) * Dh + (on ? d0 : 0);
+      T* const yc = yp;
+      if (++u < nu) {
+        xp += xu; yp += yu;
+        if (BWD) gp += gu;
+      } else {
+        u = 0;
+        const bool same = ++b < B;
+        if (!same) { b = 0; l++; }
+        xp += same ? xb : xl; yp += same ? yb : yl;
+        if (BWD) gp += same ? gb_ : gl;
+      }
+      if (left > 1) fetch(xr, gr, u);   // the next heads are asked for before these are worked on
+      const bool live = on && uc * rpw + rr < H;
+      const bool rot = has_table && lc >= prefix;
+      if (rot && (lc != table_l || tok_stride)) {
+        const float* tp = table + bc * tok_stride + (int64_t)(lc - prefix) * Dh + (on ? d0 : 0);
         *(float4*)sn = *(const float4*)tp; *(float4*)(sn + 4) = *(const float4*)(tp + 4);
-        *(float4*)cs = *(const float4*)(tp + s.cos_off); *(float4*)(cs + 4) = *(const float4*)(tp + s.cos_off + 4);
+        *(float4*)cs = *(const float4*)(tp + cos_off); *(float4*)(cs + 4) = *(const float4*)(tp + cos_off + 4);
 #pragma unroll
         for (int i = 0; i < 8; i++)
           if (!BWD) sn[i] *= i < 4 ? sga : sgb;   // the sign of rotate_half goes with the sine
         table_l = lc;
       }
-      if (p.ln) {
+      if (ln) {
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++) m += x[i];
@@ -159,7 +183,7 @@ __global__ __launch_bounds__(256, 4) void qk_norm_rope_k(QkP p) {
       float q = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; i++) q = fmaf(x[i], x[i], q);
-      const float rstd = __builtin_amdgcn_rsqf(row_sum(q) * inv_n + p.eps);   // 1 ulp
+      const float rstd = __builtin_amdgcn_rsqf(row_sum(q) * inv_n + eps);   // 1 ulp
       if (!BWD) {
         float y[8];
 #pragma unroll
@@ -180,7 +204,7 @@ __global__ __launch_bounds__(256, 4) void qk_norm_rope_k(QkP p) {
 #pragma unroll
           for (int i = 0; i < 8; i++) y[i] = SEP ? rope_mix(y[i], cs[i], o[i], sn[i], p.emu) : fmaf(y[i], cs[i], o[i] * sn[i]);
         }
-        if (live) store8<T>((T*)s.y + bc * s.y_sb + (int64_t)lc * s.y_ss + (int64_t)uc * rpw * s.y_sh + yo, y);
+        if (live) store8<T>(yc + yo, y);
       } else {
         if (rot) {   // the transposed rotation: the partner sends g sin
           float t[8], o[8];
@@ -214,13 +238,13 @@ __global__ __launch_bounds__(256, 4) void qk_norm_rope_k(QkP p) {
           if (live) { gw[i] = fmaf(g[i], x[i], gw[i]); gb[i] += g[i]; }
           g[i] *= w[i];
           a = fmaf(g[i], x[i], a);
-          if (p.ln) c += g[i];
+          if (ln) c += g[i];
         }
         a = row_sum(a) * inv_n;
-        c = p.ln ? row_sum(c) * inv_n : 0.f;
+        c = ln ? row_sum(c) * inv_n : 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++) g[i] = (fmaf(-x[i], a, g[i]) - c) * rstd;
-        if (live) store8<T>((T*)s.y + bc * s.y_sb + (int64_t)lc * s.y_ss + (int64_t)uc * rpw * s.y_sh + yo, g);
+        if (live) store8<T>(yc + yo, g);
       }
     }
   }
