@@ -10,6 +10,8 @@ struct VarP {
   const void *q, *k, *v, *dout;
   void *o, *dq, *dk, *dv;
   float *stat, *delta;         // [B, H, Lq, 2] (m, lr); [B, H, Lq] rowsum(dO O)
+  float* nl;                   // [B, H, Lq] -m c + lr
+  uint8_t* big;                // [B, H, nqt] some |m c| of the 32 rows is beyond BIG_EXP
   const int32_t* kv_len;
   const void* table;           // [buckets][H]
   const uint16_t* index;       // [Lq][Lk]
@@ -73,6 +75,77 @@ __device__ __forceinline__ HeadBlock var_block(const VarP& p, int nrows, int row
 template <bool BIAS> static inline unsigned var_grid(const VarP& p, int nrows, int rows_per_block) {
   if (!BIAS) return head_block_grid(p.B, p.H, nrows, rows_per_block);
   return xcd_grid((int64_t)p.H * ceil_div(nrows, rows_per_block) * p.B);
+}
+
+// ---- streamed tiles: 64 rows x DHP bf16 values, brought into LDS by DMA -----------------------------------------------------
+// A request moves 64 x 16 bytes to consecutive LDS addresses in lane order, so the rows are not padded; instead the source
+// address is permuted: 16-byte chunk c of row r lies at position c ^ u_swz(r).  With it the row-wise 16-byte reads (16 rows at
+// a time) and the transposing reads (4 rows x 64 bytes) of the fragments both spread over all banks.  Nothing passes through
+// registers on the way, which is what lets these kernels hold their accumulators without spilling: a spilled register's
+// reload waits behind every load in flight.  Rows at or beyond the descriptor's end arrive as zeros.
+template <int DHP> __device__ __forceinline__ int u_swz(int row) {
+  return DHP == 64 ? ((row >> 1) & 1) * 4 + ((row >> 2) & 3) : DHP == 96 ? (row >> 2) & 3 : (row & 3) * 4 + ((row >> 2) & 3);
+}
+template <int DHP> constexpr int u_tile() { return 64 * DHP * 2; }   // bytes
+// element j = tile[r0 + (lane & 31)][ks*16 + 8*(lane >> 5) + j]   (r0 a multiple of 32)
+template <int DHP> __device__ __forceinline__ bf16x8 u_rows(const char* s, int r0, int ks, int lane) {
+  const int rl = lane & 31, hi = lane >> 5, f = u_swz<DHP>(rl);
+  if (DHP == 96) return *(const bf16x8*)(s + rl * 192 + ((((ks & 1) * 2) | hi) ^ f) * 16 + (r0 * 192 + (ks >> 1) * 64));
+  return *(const bf16x8*)(s + r0 * DHP * 2 + ((rl * DHP * 2 + (hi ^ f) * 16) ^ (ks * 32)));
+}
+// element j = tile[r0 + 16*s2 + 8*(j>>2) + 4*(lane>>5) + (j&3)][c0 + (lane&31)]   (r0, c0 multiples of 32): see frag_cols
+template <int DHP> __device__ __forceinline__ bf16x8 u_cols(const char* s, int r0, int s2, int c0, int lane) {
+  const int hi = lane >> 5, l3 = lane & 3;
+  const int rowl = 4 * hi + ((lane & 15) >> 2), cl = 2 * ((lane >> 4) & 1) + (l3 >> 1), sub = (l3 & 1) * 8;
+  const int f_lo = u_swz<DHP>(rowl), f_hi = u_swz<DHP>(rowl + 8);   // adding 16 to a row leaves u_swz as it is
+  const char* t = s + (r0 + 16 * s2) * DHP * 2;
+  int lo = rowl * DHP * 2 + (cl ^ f_lo) * 16 + sub, hi8 = (rowl + 8) * DHP * 2 + (cl ^ f_hi) * 16 + sub;
+  if (DHP == 96) { lo += c0 * 2; hi8 += c0 * 2; }
+  else { lo ^= c0 * 2; hi8 ^= c0 * 2; }
+  const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(t + lo));
+  const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(t + hi8));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// The requests are issued from inline assembly: for a DMA it can see the compiler waits before every LDS read that follows.
+// They write LDS, no register; u_wait / the barrier behind it order them against the reads.
+__device__ __forceinline__ void u_dma16(__amdgpu_buffer_rsrc_t rs, uint32_t voff, uint32_t soff, uint32_t lds) {
+  uint32_t keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "s"(lds), "v"(voff), "s"(rs), "s"(soff) : "memory");
+}
+__device__ __forceinline__ void u_dma4(__amdgpu_buffer_rsrc_t rs, uint32_t voff, uint32_t soff, uint32_t lds) {
+  uint32_t keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "s"(lds), "v"(voff), "s"(rs), "s"(soff) : "memory");
+}
+// waits until at most N of the wave's memory requests are outstanding (they retire in the order of their issue)
+template <int N> __device__ __forceinline__ void u_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uintptr_t)(__attribute__((address_space(3))) const char*)p);
+}
+// One wave's share of a tile: DHP / 8 / NW requests
+template <int DHP, int NW> struct TileDma {
+  static constexpr int N = DHP / 8 / NW;
+  __amdgpu_buffer_rsrc_t rs;
+  uint32_t voff[N], tile_bytes, dst;
+};
+template <int DHP, int NW>
+__device__ __forceinline__ TileDma<DHP, NW> tile_dma(const bf16* g, int64_t ss, int S, int Dh, uint32_t dst, int wid, int lane) {
+  constexpr int CPR = DHP / 8, N = CPR / NW;
+  TileDma<DHP, NW> t;
+  t.rs = rows_rsrc(g, ss, S, Dh);
+  t.tile_bytes = (uint32_t)(64 * ss * 2);
+  t.dst = dst + (uint32_t)(wid * N * 1024);
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const int u = (wid * N + i) * 64 + lane, row = u / CPR, c = (u - row * CPR) ^ u_swz<DHP>(row);
+    t.voff[i] = c * 8 < Dh ? (uint32_t)((row * ss + c * 8) * 2) : OOB_OFF;
+  }
+  return t;
+}
+template <int DHP, int NW> __device__ __forceinline__ void tile_request(const TileDma<DHP, NW>& t, int tile, uint32_t buf_off) {
+#pragma unroll
+  for (int i = 0; i < TileDma<DHP, NW>::N; i++) u_dma16(t.rs, t.voff[i], (uint32_t)tile * t.tile_bytes, t.dst + buf_off + i * 1024);
 }
 
 // launches of the matrix-unit kernels (attn_var_fwd.hip, attn_var_bwd.hip); operands checked by the caller

@@ -419,7 +419,7 @@ static int var_dbias_splits(const VitkAttnVar* a) {
 static bool var_few(const VitkAttnVar* a) { return a->dtype == VITK_BF16 && a->Lq <= 32 && !(a->drop_p > 0.f); }
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-struct VarWs { size_t delta, bias_s, bias_t, dbias, pieces, part, pstat, total; int splits; };
+struct VarWs { size_t delta, nl, big, bias_s, bias_t, dbias, pieces, part, pstat, total; int splits; };
 static VarWs var_ws(const VitkAttnVar* a, bool bwd) {
   VarWs w = {};
   w.splits = 1;
@@ -436,6 +436,8 @@ static VarWs var_ws(const VitkAttnVar* a, bool bwd) {
     if (w.splits > 1) { w.part = take(w.splits * rows * a->Dh * 4); w.pstat = take(w.splits * rows * 8); }
   } else {
     w.delta = take(rows * 4);
+    w.nl = take(rows * 4);
+    w.big = take((size_t)(a->B * a->H * ceil_div(a->Lq, 32)));
     if (mfma && var_few(a)) w.part = take((size_t)ceil_div(a->Lk, 128) * rows * a->Dh * 4);
     if (a->dbias_table) {
       w.splits = mfma ? var_dbias_splits(a) : 1;
@@ -497,6 +499,8 @@ extern "C" int vitk_attn_var_bwd(const VitkAttnVar* desc, void* stream) {
   VITK_REQUIRE(w.total == 0 || (a->workspace && a->workspace_bytes >= (int64_t)w.total), "attn_var_bwd: workspace too small");
   char* ws = (char*)a->workspace;
   p.delta = (float*)(ws + w.delta);
+  p.nl = (float*)(ws + w.nl);
+  p.big = (uint8_t*)(ws + w.big);
   p.dbias = (float*)(ws + w.dbias);
   p.part = (float*)(ws + w.part);
   p.splits = w.splits;

@@ -19,7 +19,7 @@ __device__ __forceinline__ f32x16 init_tile(const bf16x8& lo, const bf16x8& hi, 
 }
 
 // ---- dQ -----------------------------------------------------------------------------------------------------------------
-template <int DHP, int HALVES, bool PARTIAL, bool BIAS, bool DROP, int KS, int VS>
+template <int DHP, int HALVES, bool PARTIAL, bool BIAS, bool DROP>
 __device__ __forceinline__ void var_dq_tile(const VarP& p, const char* sK, const char* sV, const bf16x8 (&qf)[DHP / 16],
                                             const bf16x8 (&gf)[DHP / 16], f32x16 (&sacc)[HALVES], f32x16 (&dqacc)[DHP / 32],
                                             float m, float nmc, bool big, float delta, float c, int k0, int len, uint32_t xrow,
@@ -28,11 +28,11 @@ __device__ __forceinline__ void var_dq_tile(const VarP& p, const char* sK, const
   const int rowoff = 4 * (lane >> 5);
 #pragma unroll
   for (int st = 0; st < HALVES; st++) {
-    f32x16 pacc = MFMA(frag_rows<VS, 0>(sV, st * 32, 0, lane), gf[0], zero, 0, 0, 0);
+    f32x16 pacc = zero;
 #pragma unroll
     for (int ks = 0; ks < DHP / 16; ks++) {
-      sacc[st] = MFMA(frag_rows<KS, 1>(sK, st * 32, ks, lane), qf[ks], sacc[st], 0, 0, 0);
-      if (ks) pacc = MFMA(frag_rows<VS, 0>(sV, st * 32, ks, lane), gf[ks], pacc, 0, 0, 0);
+      sacc[st] = MFMA(u_rows<DHP>(sK, st * 32, ks, lane), qf[ks], sacc[st], 0, 0, 0);
+      pacc = MFMA(u_rows<DHP>(sV, st * 32, ks, lane), gf[ks], pacc, 0, 0, 0);
     }
     if (BIAS && big) {
 #pragma unroll
@@ -61,7 +61,7 @@ __device__ __forceinline__ void var_dq_tile(const VarP& p, const char* sK, const
       const bf16x8 df = acc_to_frag(sacc[st], s2);
 #pragma unroll
       for (int dt = 0; dt < DHP / 32; dt++)
-        dqacc[dt] = MFMA(frag_cols<KS, 1>(sK, st * 32, s2, dt * 32, lane), df, dqacc[dt], 0, 0, 0);
+        dqacc[dt] = MFMA(u_cols<DHP>(sK, st * 32, s2, dt * 32, lane), df, dqacc[dt], 0, 0, 0);
     }
   }
 }
@@ -69,10 +69,8 @@ __device__ __forceinline__ void var_dq_tile(const VarP& p, const char* sK, const
 template <int DHP, bool BIAS, bool DROP> constexpr int var_dq_occ() { return (DHP <= 64 && !DROP && !BIAS) ? 3 : DHP <= 96 ? 2 : 1; }
 template <int DHP, int NW, bool BIAS, bool DROP>
 __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_dq_k(VarP p) {
-  constexpr int NT = NW * 64, CPR = DHP / 8, NCH = (64 * CPR + NT - 1) / NT;
-  constexpr int KS = Strides<DHP>::COLS, VS = Strides<DHP>::ROWS;   // K is read both ways (swizzled), V row-wise only
-  constexpr int TILE = 64 * KS + 64 * VS;
-  __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
+  constexpr int TILE = 2 * u_tile<DHP>(), NB = BIAS ? 2 : 3, REQ = 2 * TileDma<DHP, NW>::N;   // see var_fwd_k
+  __shared__ __attribute__((aligned(16))) char smem[NB * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, S = p.Lq;
   const HeadBlock hb = var_block<BIAS>(p, S, NW * 32);
   if (!hb.valid) return;
@@ -85,8 +83,13 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
   const bf16* vp = (const bf16*)p.v + b * p.v_sb + h * p.v_sh;
   const bf16* gp = (const bf16*)p.dout + b * p.g_sb + h * p.g_sh;
   const int len = key_count(p, b);
-  const TileSrc<NCH> ksrc = make_tilesrc<DHP, NT, NCH>(kp, p.k_ss, len, Dh, tid);
-  const TileSrc<NCH> vsrc = make_tilesrc<DHP, NT, NCH>(vp, p.v_ss, len, Dh, tid);
+  const uint32_t lds0 = lds_addr(smem);
+  const TileDma<DHP, NW> ksrc = tile_dma<DHP, NW>(kp, p.k_ss, len, Dh, lds0, wid, lane);
+  const TileDma<DHP, NW> vsrc = tile_dma<DHP, NW>(vp, p.v_ss, len, Dh, lds0 + u_tile<DHP>(), wid, lane);
+  auto request = [&](int t, int buf) {   // tiles beyond the keys arrive as zeros
+    tile_request(ksrc, t, buf * TILE);
+    tile_request(vsrc, t, buf * TILE);
+  };
   const int ntiles = (len + 63) >> 6, nfull = len >> 6;
   bf16x8 qf[DHP / 16], gf[DHP / 16], of[DHP / 16];
   load_stationary<DHP>(qf, qp, p.q_ss, qrow, S, Dh, lane);
@@ -103,108 +106,68 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
     for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(t * 4096 + i * 1024 + lane * 16)));
   };
   if (BIAS) load_bias(0);
-  uint4 rkA[NCH], rvA[NCH], rkB[NCH], rvB[NCH];
-  stage_load(rkA, ksrc, 0);
-  stage_load(rvA, vsrc, 0);
-  stage_load(rkB, ksrc, 1);
-  stage_load(rvB, vsrc, 1);
-  // delta = rowsum(dO * O), each half-wave holds half of the row; published for the kernels launched after this one
+  request(0, 0);
+  if (NB == 3) request(1, 1);
+  // delta = rowsum(dO * O), each half-wave holds half of the row
   float delta = 0.f;
 #pragma unroll
   for (int ks = 0; ks < DHP / 16; ks++)
 #pragma unroll
     for (int j = 0; j < 8; j++) delta += (float)of[ks][j] * (float)gf[ks][j];
   delta += __shfl_xor(delta, 32, 64);
-  if (qv && lane < 32) p.delta[srow] = delta;
   const float c = p.scale * LOG2E, nmc = -m * c;
   const bool big = BIAS && __any(fabsf(m * c) > BIG_EXP);
+  if (qv && lane < 32) {   // for the kernels launched after this one
+    p.delta[srow] = delta;
+    p.nl[srow] = nmc + lr;
+  }
+  if (BIAS && wave_on && lane == 0) p.big[(b * p.H + h) * p.nqt + qt] = big;
   const uint32_t rbase = var_drop_xrow(p, (uint64_t)srow, lane);
   const f32x16 zero = ZERO16;
   f32x16 dqacc[DHP / 32];
 #pragma unroll
   for (int dt = 0; dt < DHP / 32; dt++) dqacc[dt] = zero;
-  stage_store<DHP, NT, NCH, KS, true>(rkA, smem, tid);
-  stage_store<DHP, NT, NCH, VS, false>(rvA, smem + 64 * KS, tid);
+  u_wait<NB == 3 ? REQ : 0>();   // the stores above are in the count as well: a longer wait, never a shorter one
   __syncthreads();
-
-  auto step = [&](int t, uint4 (&nk)[NCH], uint4 (&nv)[NCH], uint4 (&fk)[NCH], uint4 (&fv)[NCH]) {
-    const char* sK = smem + (t & 1) * TILE;
-    const char* sV = sK + 64 * KS;
+  int buf = 0;
+  for (int t = 0; t < nfull; t++) {
+    const char* sK = smem + buf * TILE;
+    const int ahead = NB == 3 ? (buf == 0 ? 2 : buf - 1) : buf ^ 1;
     f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
-    if (BIAS) load_bias(t + 1);   // ahead of the K and V tiles: see var_fwd_k
-    stage_load(fk, ksrc, t + 2);
-    stage_load(fv, vsrc, t + 2);
-    if (wave_on) var_dq_tile<DHP, 2, false, BIAS, DROP, KS, VS>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, c, t * 64, len, rbase, lane);
-    char* nK = smem + ((t + 1) & 1) * TILE;
-    stage_store<DHP, NT, NCH, KS, true>(nk, nK, tid);
-    stage_store<DHP, NT, NCH, VS, false>(nv, nK + 64 * KS, tid);
+    if (BIAS) load_bias(t + 1);
+    request(t + NB - 1, ahead);
+    if (wave_on) var_dq_tile<DHP, 2, false, BIAS, DROP>(p, sK, sK + u_tile<DHP>(), qf, gf, sacc, dqacc, m, nmc, big, delta, c, t * 64, len, rbase, lane);
+    u_wait<NB == 3 ? REQ : 0>();
     __syncthreads();
-  };
-  for (int t = 0; t < nfull; t += 2) {
-    step(t, rkB, rvB, rkA, rvA);
-    if (t + 1 < nfull) step(t + 1, rkA, rvA, rkB, rvB);
+    buf = buf + 1 == NB ? 0 : buf + 1;
   }
   if (nfull < ntiles && wave_on) {
-    const char* sK = smem + (nfull & 1) * TILE;
-    const char* sV = sK + 64 * KS;
+    const char* sK = smem + buf * TILE;
+    const char* sV = sK + u_tile<DHP>();
     if (len - nfull * 64 > 32) {
       f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
-      var_dq_tile<DHP, 2, true, BIAS, DROP, KS, VS>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, c, nfull * 64, len, rbase, lane);
+      var_dq_tile<DHP, 2, true, BIAS, DROP>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, c, nfull * 64, len, rbase, lane);
     } else {
       f32x16 sacc[1] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale)};
-      var_dq_tile<DHP, 1, true, BIAS, DROP, KS, VS>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, c, nfull * 64, len, rbase, lane);
+      var_dq_tile<DHP, 1, true, BIAS, DROP>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, c, nfull * 64, len, rbase, lane);
     }
   }
+  u_wait<0>();   // nothing may arrive in LDS after the workgroup has left
   if (!qv) return;
   store_rows<DHP>((bf16*)p.dq + b * p.dq_sb + h * p.dq_sh + (int64_t)qrow * p.dq_ss, dqacc, p.scale * fast_exp2(lr), Dh, lane);
 }
 
-// ---- row constants of a 64-query tile, read by the kernels that stream queries ---------------------------------------------
-// sL: -m c + lr [64] (rows beyond Lq: -inf), delta [64]; with a bias also m [64], lr [64] and a flag: some |m c| > BIG_EXP.
-// Wave 0 fetches the statistics, wave 1 delta; every wave keeps what it fetched until store().
-struct RowConsts {
-  __amdgpu_buffer_rsrc_t srs, drs;
-  float a, b;
-};
-__device__ __forceinline__ void rc_open(RowConsts& rc, const VarP& p, int64_t sbase) {
-  rc.srs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.stat + 2 * sbase), 0, p.Lq * 8, 0x00020000);
-  rc.drs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.delta + sbase), 0, p.Lq * 4, 0x00020000);
-}
-__device__ __forceinline__ void rc_load(RowConsts& rc, int q0, int wid, int lane) {   // branch-free buffer loads
-  const uint32_t at = (uint32_t)(q0 + lane);
-  rc.a = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(wid == 0 ? rc.srs : rc.drs, wid == 0 ? at * 8u : wid == 1 ? at * 4u : OOB_OFF, 0, 0));
-  rc.b = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rc.srs, wid == 0 ? at * 8u + 4u : OOB_OFF, 0, 0));
-}
-template <bool BIAS>
-__device__ __forceinline__ void rc_store(const RowConsts& rc, float* sL, int q0, int Lq, float c, int wid, int lane) {
-  if (wid == 0) {
-    const bool ok = q0 + lane < Lq;
-    const float m = rc.a, lr = ok ? rc.b : -INFINITY;
-    sL[lane] = fmaf(-m, c, lr);
-    if (BIAS) {
-      sL[128 + lane] = m;
-      sL[192 + lane] = lr;
-      const bool big = __any(fabsf(m * c) > BIG_EXP);
-      if (lane == 0) sL[256] = big ? 1.f : 0.f;
-    }
-  } else if (wid == 1) {
-    sL[64 + lane] = rc.a;
-  }
-}
-template <bool BIAS> constexpr int rc_bytes() { return BIAS ? 1040 : 512; }
-
 // ---- dK, dV -----------------------------------------------------------------------------------------------------------------
-// P of a 32 x 32 tile (query r on the accumulator row, key on the lane) from its scores
+// Constants of a tile's 64 query rows: sL = nl = -m c + lr [64], delta [64], with a bias also (m, lr) [64] (zeros beyond Lq:
+// the rows of Q and dO are zeros there, and so is everything they add).  P of a 32 x 32 tile (query r on the accumulator row,
+// key on the lane) from its scores; `big`: the tile's rows hold an |m c| beyond BIG_EXP.
 template <bool BIAS>
-__device__ __forceinline__ void prob_rows(f32x16& sacc, const float* sL, int st, int rowoff, float c) {
-  const bool big = BIAS && __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sL[256])) != 0;
+__device__ __forceinline__ void prob_rows(f32x16& sacc, const float* sL, int st, int rowoff, float c, bool big) {
   if (BIAS && big) {
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const int ql = st * 32 + 8 * g + rowoff;
-      const f32x4 m4 = *(const f32x4*)(sL + 128 + ql), l4 = *(const f32x4*)(sL + 192 + ql);
-#pragma unroll
-      for (int j = 0; j < 4; j++) sacc[4 * g + j] = fast_exp2((sacc[4 * g + j] - m4[j]) * c + l4[j]);
+    for (int r = 0; r < 16; r++) {
+      const float* ml = sL + 128 + 2 * (st * 32 + acc_row(r) + rowoff);
+      sacc[r] = fast_exp2((sacc[r] - ml[0]) * c + ml[1]);
     }
   } else {
 #pragma unroll
@@ -214,6 +177,26 @@ __device__ __forceinline__ void prob_rows(f32x16& sacc, const float* sL, int st,
       for (int j = 0; j < 4; j++) sacc[4 * g + j] = fast_exp2(fmaf(sacc[4 * g + j], c, n4[j]));
     }
   }
+}
+template <bool BIAS> constexpr int row_bytes() { return BIAS ? 1024 : 512; }
+// One wave's request for the constants, 256 bytes: nl, delta and the two halves of (m, lr); without a bias waves 2 and 3
+// repeat the first two, so that every wave has the same number of requests.
+struct RowDma { __amdgpu_buffer_rsrc_t rs; uint32_t dst, row_bytes, off; };
+template <bool BIAS> __device__ __forceinline__ RowDma row_dma(const VarP& p, int64_t sbase, uint32_t dst, int wid) {
+  RowDma r;
+  const bool st = BIAS && wid >= 2;
+  const float* src = st ? p.stat + 2 * sbase : (wid & 1 ? p.delta : p.nl) + sbase;
+  r.row_bytes = st ? 8u : 4u;
+  r.off = st && wid == 3 ? 256u : 0u;
+  r.rs = __builtin_amdgcn_make_buffer_rsrc((void*)src, 0, p.Lq * (int)r.row_bytes, 0x00020000);
+  r.dst = dst + (uint32_t)(BIAS ? wid : wid & 1) * 256u;
+  return r;
+}
+__device__ __forceinline__ void row_request(const RowDma& r, int row0, uint32_t buf_off, int lane) {
+  u_dma4(r.rs, (uint32_t)lane * 4u + r.off, (uint32_t)row0 * r.row_bytes, r.dst + buf_off);
+}
+__device__ __forceinline__ bool tile_big(const VarP& p, int64_t bh, int qtile) {   // rows of 32-row tile qtile (wave-uniform)
+  return qtile < p.nqt && p.big[bh * p.nqt + qtile] != 0;
 }
 // dS (in pacc) and the P that multiplies dO (in sacc) of a 32 x 32 tile
 template <bool DROP>
@@ -260,11 +243,12 @@ __device__ __forceinline__ uint32_t drop_xkey(const VarP& p, const DropKey& d, i
   return (uint32_t)((uint64_t)(row0 + rowoff + (d.kodd ? 1 : 0)) * (var_drop_ld(p) >> 1)) * RNG_C1 + d.xk;
 }
 
-template <int DHP, int HALVES, bool BIAS, bool DROP, int QS>
+template <int DHP, int HALVES, bool BIAS, bool DROP>
 __device__ __forceinline__ void var_dkdv_tile(const VarP& p, const char* sQ, const char* sG, const float* sL,
                                               const bf16x8 (&kf)[DHP / 16], const bf16x8 (&vf)[DHP / 16], bf16x8 (&bf)[4],
                                               __amdgpu_buffer_rsrc_t brs, uint32_t bias_next, f32x16 (&dkacc)[DHP / 32],
-                                              f32x16 (&dvacc)[DHP / 32], float c, int64_t row0, const DropKey& dk, int lane) {
+                                              f32x16 (&dvacc)[DHP / 32], float c, int64_t bh, int q0, const DropKey& dk, int lane) {
+  const int64_t row0 = bh * p.Lq + q0;
   const f32x16 zero = ZERO16;
   const int rowoff = 4 * (lane >> 5);
   const uint32_t xkey = DROP ? drop_xkey(p, dk, row0, rowoff) : 0u;
@@ -278,10 +262,10 @@ __device__ __forceinline__ void var_dkdv_tile(const VarP& p, const char* sQ, con
     }
 #pragma unroll
     for (int ks = 0; ks < DHP / 16; ks++) {
-      sacc = MFMA(frag_rows<QS, 1>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
-      pacc = MFMA(frag_rows<QS, 1>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
+      sacc = MFMA(u_rows<DHP>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
+      pacc = MFMA(u_rows<DHP>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
     }
-    prob_rows<BIAS>(sacc, sL, st, rowoff, c);
+    prob_rows<BIAS>(sacc, sL, st, rowoff, c, BIAS && tile_big(p, bh, q0 / 32 + st));
     ds_rows<DROP>(p, sacc, pacc, sL, st, rowoff, xkey, dk.xstep, dk.kodd, dk.khalf);
 #pragma unroll
     for (int s2 = 0; s2 < 2; s2++) {
@@ -289,40 +273,43 @@ __device__ __forceinline__ void var_dkdv_tile(const VarP& p, const char* sQ, con
       const bf16x8 df = acc_to_frag(pacc, s2);
 #pragma unroll
       for (int dt = 0; dt < DHP / 32; dt++) {
-        dvacc[dt] = MFMA(frag_cols<QS, 1>(sG, st * 32, s2, dt * 32, lane), pf, dvacc[dt], 0, 0, 0);
-        dkacc[dt] = MFMA(frag_cols<QS, 1>(sQ, st * 32, s2, dt * 32, lane), df, dkacc[dt], 0, 0, 0);
+        dvacc[dt] = MFMA(u_cols<DHP>(sG, st * 32, s2, dt * 32, lane), pf, dvacc[dt], 0, 0, 0);
+        dkacc[dt] = MFMA(u_cols<DHP>(sQ, st * 32, s2, dt * 32, lane), df, dkacc[dt], 0, 0, 0);
       }
     }
+    // two halves in flight at once do not fit beside the accumulators of the larger heads
+    if (DHP > 64) __builtin_amdgcn_sched_barrier(0);
   }
 }
 
 template <int DHP, bool BIAS, bool DROP> constexpr int var_dkdv_occ() { return (DHP <= 64 || (DHP <= 96 && !DROP)) ? 2 : 1; }
 template <int DHP, int NW, bool BIAS, bool DROP>
 __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void var_dkdv_k(VarP p) {
-  constexpr int NT = NW * 64, CPR = DHP / 8, NCH = (64 * CPR + NT - 1) / NT;
-  constexpr int QS = Strides<DHP>::COLS;   // Q and dO tiles are read both ways (swizzled)
-  constexpr int TILE = 2 * 64 * QS + rc_bytes<BIAS>();
-  __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
+  static_assert(NW == 4, "row_dma");
+  constexpr int TILE = 2 * u_tile<DHP>() + row_bytes<BIAS>(), NB = BIAS ? 2 : 3, REQ = 2 * TileDma<DHP, NW>::N + 1;   // Q, dO, row constants; see var_fwd_k
+  __shared__ __attribute__((aligned(16))) char smem[NB * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, S = p.Lq;
   const HeadBlock hb = var_block<BIAS>(p, p.Lk, NW * 32);
   if (!hb.valid) return;
-  const int64_t b = hb.b, h = hb.h;
+  const int64_t b = hb.b, h = hb.h, bh = b * p.H + h;
   const int key0 = hb.xb * (NW * 32), krow = key0 + wid * 32 + (lane & 31);
   const int len = key_count(p, b);
   const bool wave_on = key0 + wid * 32 < len;
-  const bf16* qp = (const bf16*)p.q + b * p.q_sb + h * p.q_sh;
-  const bf16* gp = (const bf16*)p.dout + b * p.g_sb + h * p.g_sh;
-  const int64_t sbase = (b * p.H + h) * p.Lq;
   const f32x16 zero = ZERO16;
   f32x16 dkacc[DHP / 32], dvacc[DHP / 32];
 #pragma unroll
   for (int dt = 0; dt < DHP / 32; dt++) { dkacc[dt] = zero; dvacc[dt] = zero; }
   if (key0 < len) {   // otherwise all of the block's keys are padding
-    const TileSrc<NCH> qsrc = make_tilesrc<DHP, NT, NCH>(qp, p.q_ss, S, Dh, tid);
-    const TileSrc<NCH> gsrc = make_tilesrc<DHP, NT, NCH>(gp, p.g_ss, S, Dh, tid);
+    const uint32_t lds0 = lds_addr(smem);
+    const TileDma<DHP, NW> qsrc = tile_dma<DHP, NW>((const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, S, Dh, lds0, wid, lane);
+    const TileDma<DHP, NW> gsrc = tile_dma<DHP, NW>((const bf16*)p.dout + b * p.g_sb + h * p.g_sh, p.g_ss, S, Dh, lds0 + u_tile<DHP>(), wid, lane);
+    const RowDma rsrc = row_dma<BIAS>(p, bh * p.Lq, lds0 + 2 * u_tile<DHP>(), wid);
+    auto request = [&](int t, int buf) {   // tiles beyond the queries arrive as zeros
+      tile_request(qsrc, t, buf * TILE);
+      tile_request(gsrc, t, buf * TILE);
+      row_request(rsrc, t * 64, buf * TILE, lane);
+    };
     const int ntiles = (S + 63) >> 6, nfull = S >> 6;
-    RowConsts rc;
-    rc_open(rc, p, sbase);
     bf16x8 kf[DHP / 16], vf[DHP / 16];
     load_stationary<DHP>(kf, (const bf16*)p.k + b * p.k_sb + h * p.k_sh, p.k_ss, krow, len, Dh, lane);
     load_stationary<DHP>(vf, (const bf16*)p.v + b * p.v_sb + h * p.v_sh, p.v_ss, krow, len, Dh, lane);
@@ -330,43 +317,37 @@ __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void va
     const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc(
         BIAS ? (void*)(p.bias_t + ((int64_t)h * p.nkt_t + (wave_on ? kt : 0)) * p.nqt_t * 1024) : nullptr, 0, BIAS ? p.nqt_t * 2048 : 0, 0x00020000);
     bf16x8 bf[4];
-    auto load_bias = [&](int t) {
+    if (BIAS) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(t * 4096 + i * 1024 + lane * 16)));
-    };
+      for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(i * 1024 + lane * 16)));
+    }
     const float c = p.scale * LOG2E;
     const DropKey dkey = drop_key(p, krow);
-    uint4 rq[NCH], rg[NCH];
-    if (BIAS) load_bias(0);
-    stage_load(rq, qsrc, 0);
-    stage_load(rg, gsrc, 0);
-    rc_load(rc, 0, wid, lane);
-    stage_store<DHP, NT, NCH, QS, true>(rq, smem, tid);
-    stage_store<DHP, NT, NCH, QS, true>(rg, smem + 64 * QS, tid);
-    rc_store<BIAS>(rc, (float*)(smem + 2 * 64 * QS), 0, S, c, wid, lane);
+    request(0, 0);
+    if (NB == 3) request(1, 1);
+    u_wait<NB == 3 ? REQ : 0>();
     __syncthreads();
-    for (int t = 0; t < nfull; t++) {   // tile t + 1 travels while tile t is multiplied
-      const char* sQ = smem + (t & 1) * TILE;
-      const char* sG = sQ + 64 * QS;
-      const float* sL = (const float*)(sQ + 2 * 64 * QS);
-      stage_load(rq, qsrc, t + 1);   // tiles beyond the queries read as zeros
-      stage_load(rg, gsrc, t + 1);
-      rc_load(rc, (t + 1) * 64, wid, lane);
-      if (wave_on) var_dkdv_tile<DHP, 2, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, bf, brs, (uint32_t)(t + 1) * 4096u, dkacc, dvacc, c, sbase + t * 64, dkey, lane);
-      char* nQ = smem + ((t + 1) & 1) * TILE;
-      stage_store<DHP, NT, NCH, QS, true>(rq, nQ, tid);
-      stage_store<DHP, NT, NCH, QS, true>(rg, nQ + 64 * QS, tid);
-      rc_store<BIAS>(rc, (float*)(nQ + 2 * 64 * QS), (t + 1) * 64, S, c, wid, lane);
+    int buf = 0;
+    for (int t = 0; t < nfull; t++) {
+      const char* sQ = smem + buf * TILE;
+      const int ahead = NB == 3 ? (buf == 0 ? 2 : buf - 1) : buf ^ 1;
+      request(t + NB - 1, ahead);
+      if (wave_on)
+        var_dkdv_tile<DHP, 2, BIAS, DROP>(p, sQ, sQ + u_tile<DHP>(), (const float*)(sQ + 2 * u_tile<DHP>()), kf, vf, bf, brs,
+                                          (uint32_t)(t + 1) * 4096u, dkacc, dvacc, c, bh, t * 64, dkey, lane);
+      u_wait<NB == 3 ? REQ : 0>();
       __syncthreads();
+      buf = buf + 1 == NB ? 0 : buf + 1;
     }
     if (nfull < ntiles && wave_on) {
-      const char* sQ = smem + (nfull & 1) * TILE;
-      const char* sG = sQ + 64 * QS;
-      const float* sL = (const float*)(sQ + 2 * 64 * QS);
+      const char* sQ = smem + buf * TILE;
+      const char* sG = sQ + u_tile<DHP>();
+      const float* sL = (const float*)(sQ + 2 * u_tile<DHP>());
       const uint32_t none = OOB_OFF;
-      if (S - nfull * 64 > 32) var_dkdv_tile<DHP, 2, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, bf, brs, none, dkacc, dvacc, c, sbase + nfull * 64, dkey, lane);
-      else var_dkdv_tile<DHP, 1, BIAS, DROP, QS>(p, sQ, sG, sL, kf, vf, bf, brs, none, dkacc, dvacc, c, sbase + nfull * 64, dkey, lane);
+      if (S - nfull * 64 > 32) var_dkdv_tile<DHP, 2, BIAS, DROP>(p, sQ, sG, sL, kf, vf, bf, brs, none, dkacc, dvacc, c, bh, nfull * 64, dkey, lane);
+      else var_dkdv_tile<DHP, 1, BIAS, DROP>(p, sQ, sG, sL, kf, vf, bf, brs, none, dkacc, dvacc, c, bh, nfull * 64, dkey, lane);
     }
+    u_wait<0>();   // nothing may arrive in LDS after the workgroup has left
   }
   if (krow >= p.Lk) return;
   bf16* dvp = (bf16*)p.dv + b * p.dv_sb + h * p.dv_sh + (int64_t)krow * p.dv_ss;
@@ -387,9 +368,7 @@ __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void va
 // the next sample's keys and values during the last tile of a sample.
 template <int DHP, int QT, bool DROP>
 __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) {
-  constexpr int NT = 256, CPR = DHP / 8, NCH = (64 * CPR + NT - 1) / NT;
-  constexpr int QS = Strides<DHP>::ROWS;   // Q and dO tiles are read row-wise only
-  constexpr int TILE = 2 * 64 * QS + rc_bytes<true>();
+  constexpr int TILE = 2 * u_tile<DHP>() + row_bytes<true>();   // Q, dO, row constants
   __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh;
   const int nkb = (p.Lk + 127) / 128, nqb = (p.Lq + 64 * QT - 1) / (64 * QT);
@@ -416,31 +395,17 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
   const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.bias_t + ((int64_t)h * p.nkt_t + (tile_on ? kt : 0)) * p.nqt_t * 1024),
                                                                        0, tile_on ? p.nqt_t * 2048 : 0, 0x00020000);
   const DropKey dkey = drop_key(p, krow);
-  RowConsts rc;
-  uint4 rq[NCH], rg[NCH];
-  // this thread's chunks of a 64-row tile: the same offsets in every sample
-  uint32_t qoff[NCH], goff[NCH];
-#pragma unroll
-  for (int i = 0; i < NCH; i++) {
-    const int ch = tid + i * NT, row = ch / CPR, d = (ch % CPR) * 8;
-    const bool in = ch < 64 * CPR && d < Dh;
-    qoff[i] = in ? (uint32_t)((row * p.q_ss + d) * 2) : OOB_OFF;
-    goff[i] = in ? (uint32_t)((row * p.g_ss + d) * 2) : OOB_OFF;
-  }
-  auto load_tile = [&](int b, int qs) {   // 64 rows of Q, dO and their constants
-    const __amdgpu_buffer_rsrc_t qrs = rows_rsrc((const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, p.Lq, Dh);
-    const __amdgpu_buffer_rsrc_t grs = rows_rsrc((const bf16*)p.dout + b * p.g_sb + h * p.g_sh, p.g_ss, p.Lq, Dh);
-    const uint32_t qbase = (uint32_t)((q0 + qs * 64) * p.q_ss * 2), gbase = (uint32_t)((q0 + qs * 64) * p.g_ss * 2);
-#pragma unroll
-    for (int i = 0; i < NCH; i++) { rq[i] = buf_load16(qrs, qoff[i] + qbase); rg[i] = buf_load16(grs, goff[i] + gbase); }
-    rc_open(rc, p, ((int64_t)b * p.H + h) * p.Lq);
-    rc_load(rc, q0 + qs * 64, wid, lane);
-  };
-  auto store_tile = [&](int buf, int qs) {
-    char* s = smem + buf * TILE;
-    stage_store<DHP, NT, NCH, QS, false>(rq, s, tid);
-    stage_store<DHP, NT, NCH, QS, false>(rg, s + 64 * QS, tid);
-    rc_store<true>(rc, (float*)(s + 2 * 64 * QS), q0 + qs * 64, p.Lq, c, wid, lane);
+  const uint32_t lds0 = lds_addr(smem);
+  // the same offsets in every sample, another descriptor
+  TileDma<DHP, 4> qsrc = tile_dma<DHP, 4>((const bf16*)p.q, p.q_ss, p.Lq, Dh, lds0, wid, lane);
+  TileDma<DHP, 4> gsrc = tile_dma<DHP, 4>((const bf16*)p.dout, p.g_ss, p.Lq, Dh, lds0 + u_tile<DHP>(), wid, lane);
+  auto request = [&](int b, int qs, int buf) {   // 64 rows of Q, dO and their constants
+    qsrc.rs = rows_rsrc((const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, p.Lq, Dh);
+    gsrc.rs = rows_rsrc((const bf16*)p.dout + b * p.g_sb + h * p.g_sh, p.g_ss, p.Lq, Dh);
+    tile_request(qsrc, qb * QT + qs, buf * TILE);
+    tile_request(gsrc, qb * QT + qs, buf * TILE);
+    const RowDma rsrc = row_dma<true>(p, ((int64_t)b * p.H + h) * p.Lq, lds0 + 2 * u_tile<DHP>(), wid);
+    row_request(rsrc, q0 + qs * 64, buf * TILE, lane);
   };
   bf16x8 kf[DHP / 16], vf[DHP / 16], kn[DHP / 16], vn[DHP / 16];
   auto load_keys = [&](int b) {
@@ -452,44 +417,46 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
   int b = next_live(share * part), buf = 0;
   if (b < b_end) {
     load_keys(b);
-    load_tile(b, 0);
-    store_tile(0, 0);
+    request(b, 0, 0);
+    u_wait<0>();
     __syncthreads();
   }
   while (b < b_end) {
     const int len = key_count(p, b), bn = next_live(b + 1);
     const bool wave_on = key0 + wid * 32 < len, live = krow < len;
+    const int64_t bh = (int64_t)b * p.H + h;
 #pragma unroll
     for (int ks = 0; ks < DHP / 16; ks++) { kf[ks] = kn[ks]; vf[ks] = vn[ks]; }
 #pragma unroll
     for (int qs = 0; qs < QT; qs++) {
       if (qs == 1 && !second) break;
       const bool last = qs == QT - 1 || !second, more = !last || bn < b_end;
-      const int nb = last ? bn : b, nqs = last ? 0 : 1;
+      bf16x8 bf[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)((qb * QT + qs) * 4096 + i * 1024 + lane * 16)));
       if (last && more) load_keys(bn);
-      if (more) load_tile(nb, nqs);
+      if (more) request(last ? bn : b, last ? 0 : 1, buf ^ 1);
       if (wave_on) {
         const char* sQ = smem + buf * TILE;
-        const char* sG = sQ + 64 * QS;
-        const float* sL = (const float*)(sQ + 2 * 64 * QS);
-        const uint32_t xkey = DROP ? drop_xkey(p, dkey, ((int64_t)b * p.H + h) * p.Lq + q0 + qs * 64, rowoff) : 0u;
+        const char* sG = sQ + u_tile<DHP>();
+        const float* sL = (const float*)(sQ + 2 * u_tile<DHP>());
+        const uint32_t xkey = DROP ? drop_xkey(p, dkey, bh * p.Lq + q0 + qs * 64, rowoff) : 0u;
 #pragma unroll
         for (int st = 0; st < 2; st++) {
-          const uint32_t at = (uint32_t)(((qb * QT + qs) * 2 + st) * 2048 + lane * 16);
-          f32x16 sacc = init_tile<true>(__builtin_bit_cast(bf16x8, buf_load16(brs, at)), __builtin_bit_cast(bf16x8, buf_load16(brs, at + 1024)), p.inv_scale);
           f32x16 pacc = zero;
 #pragma unroll
-          for (int ks = 0; ks < DHP / 16; ks++) {
-            pacc = MFMA(frag_rows<QS, 0>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
-            sacc = MFMA(frag_rows<QS, 0>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
-          }
-          prob_rows<true>(sacc, sL, st, rowoff, c);
+          for (int ks = 0; ks < DHP / 16; ks++) pacc = MFMA(u_rows<DHP>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
+          f32x16 sacc = init_tile<true>(bf[2 * st], bf[2 * st + 1], p.inv_scale);
+#pragma unroll
+          for (int ks = 0; ks < DHP / 16; ks++) sacc = MFMA(u_rows<DHP>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
+          prob_rows<true>(sacc, sL, st, rowoff, c, tile_big(p, bh, (q0 + qs * 64) / 32 + st));
           ds_rows<DROP>(p, sacc, pacc, sL, st, rowoff, xkey, dkey.xstep, dkey.kodd, dkey.khalf);
 #pragma unroll
           for (int r = 0; r < 16; r++) acc[2 * qs + st][r] += live ? pacc[r] : 0.f;
+          __builtin_amdgcn_sched_barrier(0);   // as in var_dkdv_tile
         }
       }
-      if (more) store_tile(buf ^ 1, nqs);
+      u_wait<0>();
       __syncthreads();
       buf ^= 1;
     }
@@ -563,7 +530,10 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
     if (wid == 0) {
       frags_to_lds<DHP, QS>(qf, sQ, lane);
       if (lane < 32) { sC[0][lane] = nmc + lr; sC[1][lane] = delta; sC[2][lane] = m; sC[3][lane] = lr; }
-      if (hb.xb == 0 && qv && lane < 32) p.delta[srow] = delta;   // for the bias gradient
+      if (BIAS && hb.xb == 0) {   // for the bias gradient
+        if (qv && lane < 32) { p.delta[srow] = delta; p.nl[srow] = nmc + lr; }
+        if (lane == 0) p.big[b * p.H + h] = big;
+      }
     }
     if (wid == 1) frags_to_lds<DHP, QS>(gf, sG, lane);
     bf16x8 bs[2], bt[2];
@@ -645,8 +615,6 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
       for (int w = 0; w < 4; w++) a += red[(w * 32 + q) * (DHP + 4) + d];
       p.part[((int64_t)hb.xb * rows + (b * p.H + h) * p.Lq + q) * Dh + d] = a;
     }
-  } else if (hb.xb == 0 && wid == 0 && qv && lane < 32) {
-    p.delta[srow] = 0.f;   // a sample without keys: o = 0
   }
   if (krow >= p.Lk) return;
   if (krow >= len) {

@@ -1,8 +1,7 @@
 // Forward pass on the matrix units (bf16, v_mfma_f32_32x32x16_bf16) of attention with a relative position bias and / or key
 // counts, and the bias laid out for it.
 //
-//   workgroup = NW waves x 32 queries (Q in registers), 64-key tiles of K and V pass through LDS (double buffer, two tiles in
-//   flight); S'^T = K Q^T has the keys on the accumulator rows and the query on the lane, so the running maximum is a
+//   workgroup = NW waves x 32 queries (Q in registers), 64-key tiles of K and V arrive in LDS by DMA; S'^T = K Q^T has the keys on the accumulator rows and the query on the lane, so the running maximum is a
 //   register reduction and the probabilities are the next product's operand as they stand.  The bias enters as the INITIAL
 //   accumulator of the score product: it costs an unpacking and a multiplication by 1 / scale per element and nothing else.
 #include "attn_var.h"
@@ -83,7 +82,7 @@ __device__ __forceinline__ void var_init(f32x16 (&sacc)[HALVES], const bf16x8 (&
     for (int r = 0; r < 16; r++) sacc[st][r] = BIAS ? (float)bf[2 * st + (r >> 3)][r & 7] * inv_scale : 0.f;
 }
 // One 64-key tile (HALVES = 2) or its first 32 keys (HALVES = 1) against a wave's 32 queries; sacc starts as the bias.
-template <int DHP, int HALVES, bool PARTIAL, bool BIAS, bool DROP, int KS, int VS>
+template <int DHP, int HALVES, bool PARTIAL, bool BIAS, bool DROP>
 __device__ __forceinline__ void var_fwd_tile(const VarP& p, const char* sK, const char* sV, const bf16x8 (&qf)[DHP / 16],
                                              f32x16 (&sacc)[HALVES], f32x16 (&oacc)[DHP / 32], f32x16& lacc, float& m, float c,
                                              int k0, int len, uint32_t xrow, int lane) {
@@ -91,7 +90,7 @@ __device__ __forceinline__ void var_fwd_tile(const VarP& p, const char* sK, cons
 #pragma unroll
   for (int st = 0; st < HALVES; st++)
 #pragma unroll
-    for (int ks = 0; ks < DHP / 16; ks++) sacc[st] = MFMA(frag_rows<KS, 0>(sK, st * 32, ks, lane), qf[ks], sacc[st], 0, 0, 0);
+    for (int ks = 0; ks < DHP / 16; ks++) sacc[st] = MFMA(u_rows<DHP>(sK, st * 32, ks, lane), qf[ks], sacc[st], 0, 0, 0);
   if (PARTIAL) {   // keys at or beyond the count (only in the last half of the last tile)
 #pragma unroll
     for (int r = 0; r < 16; r++)
@@ -154,22 +153,23 @@ __device__ __forceinline__ void var_fwd_tile(const VarP& p, const char* sK, cons
       }
 #pragma unroll
       for (int dt = 0; dt < DHP / 32; dt++)
-        oacc[dt] = MFMA(frag_cols<VS, 0>(sV, st * 32, s2, dt * 32, lane), pf, oacc[dt], 0, 0, 0);
+        oacc[dt] = MFMA(u_cols<DHP>(sV, st * 32, s2, dt * 32, lane), pf, oacc[dt], 0, 0, 0);
     }
 }
 
 // waves per SIMD: what the registers of an instance allow without spilling
 template <int DHP, int NW, bool BIAS, bool DROP> constexpr int var_fwd_occ() {
-  return DHP <= 64 ? (NW == 4 && !BIAS ? 3 : 2) : (DHP <= 96 && NW == 4) ? 2 : 1;
+  return DHP <= 64 ? (!BIAS ? 3 : 2) : DHP <= 96 ? 2 : 1;
 }
 
 // SPLIT: the keys of a (sample, head) are shared by gridDim.y workgroups; each leaves O unnormalised in 32 bits with its m and
 // row sum, and var_combine_k joins them.
 template <int DHP, int NW, bool BIAS, bool DROP, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void var_fwd_k(VarP p) {
-  constexpr int NT = NW * 64, CPR = DHP / 8, NCH = (64 * CPR + NT - 1) / NT;
-  constexpr int KS = Strides<DHP>::ROWS, VS = Strides<DHP>::COLS, TILE = 64 * KS + 64 * VS;
-  __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
+  // Buffers: without a bias the requests are the loop's only memory operations, a tile is asked for two steps ahead and
+  // waited for with a count; with one the compiler's wait for a bias tile takes everything with it, so one step ahead.
+  constexpr int TILE = 2 * u_tile<DHP>(), NB = BIAS ? 2 : 3, REQ = 2 * TileDma<DHP, NW>::N;
+  __shared__ __attribute__((aligned(16))) char smem[NB * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, S = p.Lq;
   const HeadBlock hb = var_block<BIAS>(p, S, NW * 32);
   if (!hb.valid) return;
@@ -190,8 +190,13 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
     if (tile0 * 64 >= len_all) len = tile0 * 64;   // nothing left for this share
   }
   const int ntiles = (len + 63) >> 6, nfull = len >> 6;
-  const TileSrc<NCH> ksrc = make_tilesrc<DHP, NT, NCH>(kp, p.k_ss, len, Dh, tid);
-  const TileSrc<NCH> vsrc = make_tilesrc<DHP, NT, NCH>(vp, p.v_ss, len, Dh, tid);
+  const uint32_t lds0 = lds_addr(smem);
+  const TileDma<DHP, NW> ksrc = tile_dma<DHP, NW>(kp, p.k_ss, len, Dh, lds0, wid, lane);
+  const TileDma<DHP, NW> vsrc = tile_dma<DHP, NW>(vp, p.v_ss, len, Dh, lds0 + u_tile<DHP>(), wid, lane);
+  auto request = [&](int t, int buf) {   // tiles beyond the keys arrive as zeros
+    tile_request(ksrc, t, buf * TILE);
+    tile_request(vsrc, t, buf * TILE);
+  };
   bf16x8 qf[DHP / 16];
   load_stationary<DHP>(qf, qp, p.q_ss, qrow, S, Dh, lane);
   // bias tiles of this wave's query tile; key tiles beyond the row read as zeros
@@ -204,11 +209,8 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
     for (int i = 0; i < 4; i++) d[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(t * 4096 + i * 1024 + lane * 16)));
   };
   if (BIAS) load_bias(bf, tile0);
-  uint4 rkA[NCH], rvA[NCH], rkB[NCH], rvB[NCH];
-  stage_load(rkA, ksrc, tile0);
-  stage_load(rvA, vsrc, tile0);
-  stage_load(rkB, ksrc, tile0 + 1);   // tiles beyond the keys read as zeros, so prefetches need no condition
-  stage_load(rvB, vsrc, tile0 + 1);
+  request(tile0, 0);
+  if (NB == 3) request(tile0 + 1, 1);
   const f32x16 zero = ZERO16;
   f32x16 oacc[DHP / 32], lacc = zero;
 #pragma unroll
@@ -216,43 +218,35 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
   float m = -INFINITY;
   const float c = p.scale * LOG2E;
   const uint32_t rbase = var_drop_xrow(p, (uint64_t)(b * p.H + h) * p.Lq + (uint64_t)qrow, lane);
-  stage_store<DHP, NT, NCH, KS, false>(rkA, smem, tid);
-  stage_store<DHP, NT, NCH, VS, false>(rvA, smem + 64 * KS, tid);
+  u_wait<NB == 3 ? REQ : 0>();
   __syncthreads();
-
-  auto step = [&](int t, uint4 (&nk)[NCH], uint4 (&nv)[NCH], uint4 (&fk)[NCH], uint4 (&fv)[NCH]) {
-    const char* sK = smem + ((t - tile0) & 1) * TILE;
-    const char* sV = sK + 64 * KS;
-    // loads return in order: the next tile's bias is asked for ahead of the K and V tiles behind it, so that waiting for it
-    // leaves those in flight
+  int buf = 0;
+  for (int t = tile0; t < nfull; t++) {
+    const char* sK = smem + buf * TILE;
+    const int ahead = NB == 3 ? (buf == 0 ? 2 : buf - 1) : buf ^ 1;   // the buffer read in the step before
     f32x16 sacc[2];
     var_init<2, BIAS>(sacc, bf, p.inv_scale);
     if (BIAS) load_bias(bf, t + 1);
-    stage_load(fk, ksrc, t + 2);
-    stage_load(fv, vsrc, t + 2);
-    if (wave_on) var_fwd_tile<DHP, 2, false, BIAS, DROP, KS, VS>(p, sK, sV, qf, sacc, oacc, lacc, m, c, t * 64, len, rbase, lane);
-    char* nK = smem + ((t + 1 - tile0) & 1) * TILE;
-    stage_store<DHP, NT, NCH, KS, false>(nk, nK, tid);
-    stage_store<DHP, NT, NCH, VS, false>(nv, nK + 64 * KS, tid);
+    request(t + NB - 1, ahead);
+    if (wave_on) var_fwd_tile<DHP, 2, false, BIAS, DROP>(p, sK, sK + u_tile<DHP>(), qf, sacc, oacc, lacc, m, c, t * 64, len, rbase, lane);
+    u_wait<NB == 3 ? REQ : 0>();   // the next tile has arrived
     __syncthreads();
-  };
-  for (int t = tile0; t < nfull; t += 2) {
-    step(t, rkB, rvB, rkA, rvA);
-    if (t + 1 < nfull) step(t + 1, rkA, rvA, rkB, rvB);
+    buf = buf + 1 == NB ? 0 : buf + 1;
   }
   if (nfull < ntiles && nfull >= tile0 && wave_on) {
-    const char* sK = smem + ((nfull - tile0) & 1) * TILE;
-    const char* sV = sK + 64 * KS;
+    const char* sK = smem + buf * TILE;
+    const char* sV = sK + u_tile<DHP>();
     if (len - nfull * 64 > 32) {
       f32x16 sacc[2];
       var_init<2, BIAS>(sacc, bf, p.inv_scale);
-      var_fwd_tile<DHP, 2, true, BIAS, DROP, KS, VS>(p, sK, sV, qf, sacc, oacc, lacc, m, c, nfull * 64, len, rbase, lane);
+      var_fwd_tile<DHP, 2, true, BIAS, DROP>(p, sK, sV, qf, sacc, oacc, lacc, m, c, nfull * 64, len, rbase, lane);
     } else {
       f32x16 sacc[1];
       var_init<1, BIAS>(sacc, bf, p.inv_scale);
-      var_fwd_tile<DHP, 1, true, BIAS, DROP, KS, VS>(p, sK, sV, qf, sacc, oacc, lacc, m, c, nfull * 64, len, rbase, lane);
+      var_fwd_tile<DHP, 1, true, BIAS, DROP>(p, sK, sV, qf, sacc, oacc, lacc, m, c, nfull * 64, len, rbase, lane);
     }
   }
+  u_wait<0>();   // nothing may arrive in LDS after the workgroup has left
   if (qrow >= S) return;
   const float l = lacc[0];
   const int64_t srow = (b * p.H + h) * p.Lq + qrow;
