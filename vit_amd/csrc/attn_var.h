@@ -9,9 +9,8 @@
 struct VarP {
   const void *q, *k, *v, *dout;
   void *o, *dq, *dk, *dv;
-  float *stat, *delta;         // [B, H, Lq, 2] (m, lr); [B, H, Lq] rowsum(dO O)
+  float *stat, *delta;         // [B, H, Lq, 2] (m, lr); [B, H, Lq] rowsum(dO O), in the bf16 kernels with its sign turned
   float* nl;                   // [B, H, Lq] -m c + lr
-  uint8_t* big;                // [B, H, nqt] some |m c| of the 32 rows is beyond BIG_EXP
   const int32_t* kv_len;
   const void* table;           // [buckets][H]
   const uint16_t* index;       // [Lq][Lk]

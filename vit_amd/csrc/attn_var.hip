@@ -408,18 +408,20 @@ static int var_fwd_splits(const VitkAttnVar* a) {
   if (n > tiles / 4) n = tiles / 4;
   return (int)(n < 64 ? n : 64);
 }
-// Shares of the samples in the bias gradient: enough workgroups to fill the chip twice.
+// Shares of the samples in the bias gradient: float32 enough workgroups to fill the chip twice; bf16, where a workgroup
+// takes a CU for itself, as many as there are CUs at most (a 257th would run after the others).
 static int var_dbias_splits(const VitkAttnVar* a) {
-  const int rows = a->dtype == VITK_F32 ? 32 : 64;   // queries of a workgroup
+  const bool f32 = a->dtype == VITK_F32;
+  const int rows = f32 ? 32 : a->Dh <= 96 ? 128 : 64;   // queries of a workgroup
   const int64_t blocks = a->H * ceil_div(a->Lq, rows) * ceil_div(a->Lk, 128);
-  int64_t n = ceil_div(512, blocks);
+  int64_t n = f32 ? ceil_div(512, blocks) : 256 / blocks;
   if (n > a->B) n = a->B;
   return (int)(n < 1 ? 1 : n);
 }
 static bool var_few(const VitkAttnVar* a) { return a->dtype == VITK_BF16 && a->Lq <= 32 && !(a->drop_p > 0.f); }
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-struct VarWs { size_t delta, nl, big, bias_s, bias_t, dbias, pieces, part, pstat, total; int splits; };
+struct VarWs { size_t delta, nl, bias_s, bias_t, dbias, pieces, part, pstat, total; int splits; };
 static VarWs var_ws(const VitkAttnVar* a, bool bwd) {
   VarWs w = {};
   w.splits = 1;
@@ -437,7 +439,6 @@ static VarWs var_ws(const VitkAttnVar* a, bool bwd) {
   } else {
     w.delta = take(rows * 4);
     w.nl = take(rows * 4);
-    w.big = take((size_t)(a->B * a->H * ceil_div(a->Lq, 32)));
     if (mfma && var_few(a)) w.part = take((size_t)ceil_div(a->Lk, 128) * rows * a->Dh * 4);
     if (a->dbias_table) {
       w.splits = mfma ? var_dbias_splits(a) : 1;
@@ -500,7 +501,6 @@ extern "C" int vitk_attn_var_bwd(const VitkAttnVar* desc, void* stream) {
   char* ws = (char*)a->workspace;
   p.delta = (float*)(ws + w.delta);
   p.nl = (float*)(ws + w.nl);
-  p.big = (uint8_t*)(ws + w.big);
   p.dbias = (float*)(ws + w.dbias);
   p.part = (float*)(ws + w.part);
   p.splits = w.splits;

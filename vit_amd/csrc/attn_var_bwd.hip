@@ -118,10 +118,9 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
   const float c = p.scale * LOG2E, nmc = -m * c;
   const bool big = BIAS && __any(fabsf(m * c) > BIG_EXP);
   if (qv && lane < 32) {   // for the kernels launched after this one
-    p.delta[srow] = delta;
+    p.delta[srow] = -delta;
     p.nl[srow] = nmc + lr;
   }
-  if (BIAS && wave_on && lane == 0) p.big[(b * p.H + h) * p.nqt + qt] = big;
   const uint32_t rbase = var_drop_xrow(p, (uint64_t)srow, lane);
   const f32x16 zero = ZERO16;
   f32x16 dqacc[DHP / 32];
@@ -158,7 +157,7 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
 }
 
 // ---- dK, dV -----------------------------------------------------------------------------------------------------------------
-// Constants of a tile's 64 query rows: sL = nl = -m c + lr [64], delta [64], with a bias also (m, lr) [64] (zeros beyond Lq:
+// Constants of a tile's 64 query rows: sL = nl = -m c + lr [64], -delta [64], with a bias also (m, lr) [64] (zeros beyond Lq:
 // the rows of Q and dO are zeros there, and so is everything they add).  P of a 32 x 32 tile (query r on the accumulator row,
 // key on the lane) from its scores; `big`: the tile's rows hold an |m c| beyond BIG_EXP.
 template <bool BIAS>
@@ -195,8 +194,23 @@ template <bool BIAS> __device__ __forceinline__ RowDma row_dma(const VarP& p, in
 __device__ __forceinline__ void row_request(const RowDma& r, int row0, uint32_t buf_off, int lane) {
   u_dma4(r.rs, (uint32_t)lane * 4u + r.off, (uint32_t)row0 * r.row_bytes, r.dst + buf_off);
 }
-__device__ __forceinline__ bool tile_big(const VarP& p, int64_t bh, int qtile) {   // rows of 32-row tile qtile (wave-uniform)
-  return qtile < p.nqt && p.big[bh * p.nqt + qtile] != 0;
+// Which of the 64 rows hold an |m c| beyond BIG_EXP; from LDS: a load from memory here would wait for every request in flight
+// (the counter is one for all), a tile's time each step.
+template <bool BIAS> __device__ __forceinline__ uint64_t rows_big(const float* sL, float c, int lane) {
+  return BIAS ? __ballot(fabsf(sL[128 + 2 * lane] * c) > BIG_EXP) : 0ull;
+}
+// dP starts from -delta: P (dP - delta) is then one product (with dropout delta must not be scaled, and is subtracted later)
+template <bool DROP> __device__ __forceinline__ f32x16 init_dp(const float* sL, int st, int rowoff) {
+  f32x16 a = ZERO16;
+  if (!DROP) {
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const f32x4 d4 = *(const f32x4*)(sL + 64 + st * 32 + 8 * g + rowoff);
+#pragma unroll
+      for (int j = 0; j < 4; j++) a[4 * g + j] = d4[j];
+    }
+  }
+  return a;
 }
 // dS (in pacc) and the P that multiplies dO (in sacc) of a 32 x 32 tile
 template <bool DROP>
@@ -204,7 +218,8 @@ __device__ __forceinline__ void ds_rows(const VarP& p, f32x16& sacc, f32x16& pac
                                         uint32_t xkey, uint32_t xstep, bool kodd, int khalf) {
 #pragma unroll
   for (int g = 0; g < 4; g++) {
-    const f32x4 d4 = *(const f32x4*)(sL + 64 + st * 32 + 8 * g + rowoff);
+    f32x4 d4 = {0.f, 0.f, 0.f, 0.f};
+    if (DROP) d4 = *(const f32x4*)(sL + 64 + st * 32 + 8 * g + rowoff);
     uint32_t drops[4] = {0u, 0u, 0u, 0u};
     if (DROP) {   // neighbouring lanes share a pair's hash: each computes two rows' hashes and they swap (see attn.hip)
 #pragma unroll
@@ -226,7 +241,7 @@ __device__ __forceinline__ void ds_rows(const VarP& p, f32x16& sacc, f32x16& pac
         sacc[r] = keep ? pr * p.keep_scale : 0.f;
         dp = keep ? dp * p.keep_scale : 0.f;
       }
-      pacc[r] = pr * (dp - d4[j]);
+      pacc[r] = pr * (DROP ? dp + d4[j] : dp);
     }
   }
 }
@@ -249,13 +264,13 @@ __device__ __forceinline__ void var_dkdv_tile(const VarP& p, const char* sQ, con
                                               __amdgpu_buffer_rsrc_t brs, uint32_t bias_next, f32x16 (&dkacc)[DHP / 32],
                                               f32x16 (&dvacc)[DHP / 32], float c, int64_t bh, int q0, const DropKey& dk, int lane) {
   const int64_t row0 = bh * p.Lq + q0;
-  const f32x16 zero = ZERO16;
   const int rowoff = 4 * (lane >> 5);
   const uint32_t xkey = DROP ? drop_xkey(p, dk, row0, rowoff) : 0u;
+  const uint64_t big = rows_big<BIAS>(sL, c, lane);
 #pragma unroll
   for (int st = 0; st < HALVES; st++) {
     // a half's bias becomes its initial scores and the registers take the next tile's
-    f32x16 sacc = init_tile<BIAS>(bf[2 * st], bf[2 * st + 1], p.inv_scale), pacc = zero;
+    f32x16 sacc = init_tile<BIAS>(bf[2 * st], bf[2 * st + 1], p.inv_scale), pacc = init_dp<DROP>(sL, st, rowoff);
     if (BIAS) {
       bf[2 * st] = __builtin_bit_cast(bf16x8, buf_load16(brs, bias_next + (uint32_t)(st * 2048 + lane * 16)));
       bf[2 * st + 1] = __builtin_bit_cast(bf16x8, buf_load16(brs, bias_next + (uint32_t)(st * 2048 + 1024 + lane * 16)));
@@ -265,7 +280,7 @@ __device__ __forceinline__ void var_dkdv_tile(const VarP& p, const char* sQ, con
       sacc = MFMA(u_rows<DHP>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
       pacc = MFMA(u_rows<DHP>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
     }
-    prob_rows<BIAS>(sacc, sL, st, rowoff, c, BIAS && tile_big(p, bh, q0 / 32 + st));
+    prob_rows<BIAS>(sacc, sL, st, rowoff, c, (uint32_t)(big >> (32 * st)) != 0u);
     ds_rows<DROP>(p, sacc, pacc, sL, st, rowoff, xkey, dk.xstep, dk.kodd, dk.khalf);
 #pragma unroll
     for (int s2 = 0; s2 < 2; s2++) {
@@ -361,17 +376,19 @@ __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void va
 }
 
 // ---- bias gradient: dS summed over the samples ---------------------------------------------------------------------------------
-// A workgroup owns 128 keys (32 per wave, on the lanes) x 64 QT queries of a head and walks the samples of its share
-// (p.splits shares); dS of every sample is added to 2 QT accumulator tiles per wave and leaves as 32-bit values.  It forms S'
-// and dP once more, 4 of the 14 products of a training pass, which costs less than writing dS (2 bytes per sample, head and
-// pair) and reading it back.  Every load is asked for a step ahead: the next 64 rows of Q and dO while a tile is multiplied,
-// the next sample's keys and values during the last tile of a sample.
-template <int DHP, int QT, bool DROP>
-__global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) {
-  constexpr int TILE = 2 * u_tile<DHP>() + row_bytes<true>();   // Q, dO, row constants
-  __shared__ __attribute__((aligned(16))) char smem[2 * TILE];
+// A workgroup owns 128 keys x 64 WQ queries of a head, 32 x 64 per wave with the key on the lane, and walks the samples of its
+// share (p.splits shares); dS of every sample is added to two accumulator tiles per wave, in 32 bits, and leaves as 32-bit
+// values.  It forms S' and dP once more, 4 of the 14 products of a training pass, which costs less than writing dS (2 bytes
+// per sample, head and pair) and reading it back.  A sample brings 128 rows of K and V and 64 WQ of Q and dO, all by DMA a
+// sample ahead: the former go to registers, which frees their place at once, the latter have two places.
+template <int DHP> constexpr int dbias_wq() { return DHP <= 96 ? 2 : 1; }   // 128: Q and dO of 128 queries do not fit twice
+template <int DHP, int WQ, bool DROP>
+__global__ __launch_bounds__(WQ * 256, 1) void var_dbias_k(VarP p) {
+  constexpr int T = u_tile<DHP>(), KV = 4 * T, QG = WQ * (2 * T + row_bytes<true>());   // K, V; Q and dO and the row constants
+  __shared__ __attribute__((aligned(16))) char smem[KV + 2 * QG];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh;
-  const int nkb = (p.Lk + 127) / 128, nqb = (p.Lq + 64 * QT - 1) / (64 * QT);
+  const int wk = wid & 3, wq = wid >> 2;
+  const int nkb = (p.Lk + 127) / 128, nqb = (p.Lq + 64 * WQ - 1) / (64 * WQ);
   // Neighbours: panels of up to 8 key blocks, all query blocks of a panel, then the next panel of the head (and share): the
   // workgroups that run on an XCD at a time then read few rows between them, which stay in its L2.
   const int64_t it = xcd_item(blockIdx.x, (int64_t)nkb * nqb * p.splits * p.H);
@@ -380,92 +397,100 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
   const int part = (int)(hp % p.splits), h = (int)(hp / p.splits), in = (int)(it - hp * nkb * nqb);
   const int panel = in / (8 * nqb), width = min(8, nkb - panel * 8), rest = in - panel * 8 * nqb;
   const int kb = panel * 8 + rest % width, qb = rest / width;
-  const int key0 = kb * 128, q0 = qb * 64 * QT, krow = key0 + wid * 32 + (lane & 31);
+  const int key0 = kb * 128, q0 = (qb * WQ + wq) * 64, krow = key0 + wk * 32 + (lane & 31);
   const int share = (p.B + p.splits - 1) / p.splits;
   const int b_end = min(p.B, share * (part + 1));
   const float c = p.scale * LOG2E;
   const int rowoff = 4 * (lane >> 5);
   const f32x16 zero = ZERO16;
-  f32x16 acc[2 * QT];
-#pragma unroll
-  for (int i = 0; i < 2 * QT; i++) acc[i] = zero;
+  f32x16 acc[2] = {zero, zero};
   auto next_live = [&](int b) { while (b < b_end && key_count(p, b) <= key0) b++; return b; };
-  const int kt = key0 / 32 + wid;   // may lie beyond the last key tile: the descriptor then covers nothing
-  const bool tile_on = kt < p.nkt_t;
-  const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.bias_t + ((int64_t)h * p.nkt_t + (tile_on ? kt : 0)) * p.nqt_t * 1024),
-                                                                       0, tile_on ? p.nqt_t * 2048 : 0, 0x00020000);
+  const int kt = key0 / 32 + wk;   // may lie beyond the last key tile, as the queries may: the descriptor then covers nothing
+  const bool tile_on = kt < p.nkt_t && q0 < p.Lq;
+  const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(p.bias_t + (((int64_t)h * p.nkt_t + (tile_on ? kt : 0)) * p.nqt_t + (tile_on ? q0 / 32 : 0)) * 1024), 0, tile_on ? 4096 : 0, 0x00020000);
+  bf16x8 bf[4];   // the same for every sample
+#pragma unroll
+  for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(i * 1024 + lane * 16)));
   const DropKey dkey = drop_key(p, krow);
   const uint32_t lds0 = lds_addr(smem);
-  // the same offsets in every sample, another descriptor
-  TileDma<DHP, 4> qsrc = tile_dma<DHP, 4>((const bf16*)p.q, p.q_ss, p.Lq, Dh, lds0, wid, lane);
-  TileDma<DHP, 4> gsrc = tile_dma<DHP, 4>((const bf16*)p.dout, p.g_ss, p.Lq, Dh, lds0 + u_tile<DHP>(), wid, lane);
-  auto request = [&](int b, int qs, int buf) {   // 64 rows of Q, dO and their constants
+  // Four waves bring a 64-row tile: with WQ = 2 the waves of a half take one tile of each operand, with 1 all take both of K
+  // and V.  The same offsets in every sample, another descriptor.
+  const uint32_t qdst = lds0 + KV + wq * (2 * T + row_bytes<true>());
+  TileDma<DHP, 4> ksrc = tile_dma<DHP, 4>((const bf16*)p.k, p.k_ss, p.Lk, Dh, lds0 + wq * T, wk, lane);
+  TileDma<DHP, 4> vsrc = tile_dma<DHP, 4>((const bf16*)p.v, p.v_ss, p.Lk, Dh, lds0 + 2 * T + wq * T, wk, lane);
+  TileDma<DHP, 4> qsrc = tile_dma<DHP, 4>((const bf16*)p.q, p.q_ss, p.Lq, Dh, qdst, wk, lane);
+  TileDma<DHP, 4> gsrc = tile_dma<DHP, 4>((const bf16*)p.dout, p.g_ss, p.Lq, Dh, qdst + T, wk, lane);
+  auto request_keys = [&](int b) {
+    const int len = key_count(p, b);
+    ksrc.rs = rows_rsrc((const bf16*)p.k + b * p.k_sb + h * p.k_sh, p.k_ss, len, Dh);
+    vsrc.rs = rows_rsrc((const bf16*)p.v + b * p.v_sb + h * p.v_sh, p.v_ss, len, Dh);
+#pragma unroll
+    for (int i = 0; i < 2 / WQ; i++) {
+      tile_request(ksrc, kb * 2 + wq + i, i * T);
+      tile_request(vsrc, kb * 2 + wq + i, i * T);
+    }
+  };
+  auto request_rows = [&](int b, int buf) {
     qsrc.rs = rows_rsrc((const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, p.Lq, Dh);
     gsrc.rs = rows_rsrc((const bf16*)p.dout + b * p.g_sb + h * p.g_sh, p.g_ss, p.Lq, Dh);
-    tile_request(qsrc, qb * QT + qs, buf * TILE);
-    tile_request(gsrc, qb * QT + qs, buf * TILE);
-    const RowDma rsrc = row_dma<true>(p, ((int64_t)b * p.H + h) * p.Lq, lds0 + 2 * u_tile<DHP>(), wid);
-    row_request(rsrc, q0 + qs * 64, buf * TILE, lane);
+    tile_request(qsrc, qb * WQ + wq, buf * QG);
+    tile_request(gsrc, qb * WQ + wq, buf * QG);
+    row_request(row_dma<true>(p, ((int64_t)b * p.H + h) * p.Lq, qdst + 2 * T, wk), q0, buf * QG, lane);
   };
-  bf16x8 kf[DHP / 16], vf[DHP / 16], kn[DHP / 16], vn[DHP / 16];
-  auto load_keys = [&](int b) {
-    const int len = key_count(p, b);
-    load_stationary<DHP>(kn, (const bf16*)p.k + b * p.k_sb + h * p.k_sh, p.k_ss, krow, len, Dh, lane);
-    load_stationary<DHP>(vn, (const bf16*)p.v + b * p.v_sb + h * p.v_sh, p.v_ss, krow, len, Dh, lane);
-  };
-  const bool second = QT == 2 && q0 + 64 < p.Lq;   // the second 64-query tile has rows
   int b = next_live(share * part), buf = 0;
   if (b < b_end) {
-    load_keys(b);
-    request(b, 0, 0);
-    u_wait<0>();
-    __syncthreads();
+    request_keys(b);
+    request_rows(b, 0);
   }
   while (b < b_end) {
     const int len = key_count(p, b), bn = next_live(b + 1);
-    const bool wave_on = key0 + wid * 32 < len, live = krow < len;
+    const bool wave_on = q0 < p.Lq && key0 + wk * 32 < len, whole = key0 + wk * 32 + 32 <= len, live = krow < len;
     const int64_t bh = (int64_t)b * p.H + h;
+    u_wait<0>();
+    __syncthreads();
+    bf16x8 kf[DHP / 16], vf[DHP / 16];
+    {
+      const char* sK = smem + (wk >> 1) * T;
 #pragma unroll
-    for (int ks = 0; ks < DHP / 16; ks++) { kf[ks] = kn[ks]; vf[ks] = vn[ks]; }
+      for (int ks = 0; ks < DHP / 16; ks++) {
+        kf[ks] = u_rows<DHP>(sK, (wk & 1) * 32, ks, lane);
+        vf[ks] = u_rows<DHP>(sK + 2 * T, (wk & 1) * 32, ks, lane);
+      }
+    }
+    if (bn < b_end) request_rows(bn, buf ^ 1);
+    __syncthreads();   // every wave has its keys and values
+    if (bn < b_end) request_keys(bn);
+    if (wave_on) {
+      const char* sQ = smem + KV + buf * QG + wq * (2 * T + row_bytes<true>());
+      const char* sG = sQ + T;
+      const float* sL = (const float*)(sQ + 2 * T);
+      const uint32_t xkey = DROP ? drop_xkey(p, dkey, bh * p.Lq + q0, rowoff) : 0u;
+      const uint64_t big = rows_big<true>(sL, c, lane);
 #pragma unroll
-    for (int qs = 0; qs < QT; qs++) {
-      if (qs == 1 && !second) break;
-      const bool last = qs == QT - 1 || !second, more = !last || bn < b_end;
-      bf16x8 bf[4];
+      for (int st = 0; st < 2; st++) {
+        f32x16 sacc = init_tile<true>(bf[2 * st], bf[2 * st + 1], p.inv_scale), pacc = init_dp<DROP>(sL, st, rowoff);
 #pragma unroll
-      for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)((qb * QT + qs) * 4096 + i * 1024 + lane * 16)));
-      if (last && more) load_keys(bn);
-      if (more) request(last ? bn : b, last ? 0 : 1, buf ^ 1);
-      if (wave_on) {
-        const char* sQ = smem + buf * TILE;
-        const char* sG = sQ + u_tile<DHP>();
-        const float* sL = (const float*)(sQ + 2 * u_tile<DHP>());
-        const uint32_t xkey = DROP ? drop_xkey(p, dkey, bh * p.Lq + q0 + qs * 64, rowoff) : 0u;
+        for (int ks = 0; ks < DHP / 16; ks++) {
+          sacc = MFMA(u_rows<DHP>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
+          pacc = MFMA(u_rows<DHP>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
+        }
+        prob_rows<true>(sacc, sL, st, rowoff, c, (uint32_t)(big >> (32 * st)) != 0u);
+        if (DROP) ds_rows<true>(p, sacc, pacc, sL, st, rowoff, xkey, dkey.xstep, dkey.kodd, dkey.khalf);
 #pragma unroll
-        for (int st = 0; st < 2; st++) {
-          f32x16 pacc = zero;
-#pragma unroll
-          for (int ks = 0; ks < DHP / 16; ks++) pacc = MFMA(u_rows<DHP>(sG, st * 32, ks, lane), vf[ks], pacc, 0, 0, 0);
-          f32x16 sacc = init_tile<true>(bf[2 * st], bf[2 * st + 1], p.inv_scale);
-#pragma unroll
-          for (int ks = 0; ks < DHP / 16; ks++) sacc = MFMA(u_rows<DHP>(sQ, st * 32, ks, lane), kf[ks], sacc, 0, 0, 0);
-          prob_rows<true>(sacc, sL, st, rowoff, c, tile_big(p, bh, (q0 + qs * 64) / 32 + st));
-          ds_rows<DROP>(p, sacc, pacc, sL, st, rowoff, xkey, dkey.xstep, dkey.kodd, dkey.khalf);
-#pragma unroll
-          for (int r = 0; r < 16; r++) acc[2 * qs + st][r] += live ? pacc[r] : 0.f;
-          __builtin_amdgcn_sched_barrier(0);   // as in var_dkdv_tile
+        for (int r = 0; r < 16; r++) {
+          const float t = DROP ? acc[st][r] + pacc[r] : fmaf(sacc[r], pacc[r], acc[st][r]);
+          acc[st][r] = whole || live ? t : acc[st][r];
         }
       }
-      u_wait<0>();
-      __syncthreads();
-      buf ^= 1;
     }
+    buf ^= 1;
     b = bn;
   }
   if (krow >= p.Lk) return;
   float* out = p.dbias + ((int64_t)part * p.H + h) * p.Lq * p.Lk + krow;
 #pragma unroll
-  for (int i = 0; i < 2 * QT; i++)
+  for (int i = 0; i < 2; i++)
 #pragma unroll
     for (int r = 0; r < 16; r++) {
       const int row = q0 + i * 32 + acc_row(r) + rowoff;
@@ -531,8 +556,7 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
       frags_to_lds<DHP, QS>(qf, sQ, lane);
       if (lane < 32) { sC[0][lane] = nmc + lr; sC[1][lane] = delta; sC[2][lane] = m; sC[3][lane] = lr; }
       if (BIAS && hb.xb == 0) {   // for the bias gradient
-        if (qv && lane < 32) { p.delta[srow] = delta; p.nl[srow] = nmc + lr; }
-        if (lane == 0) p.big[b * p.H + h] = big;
+        if (qv && lane < 32) { p.delta[srow] = -delta; p.nl[srow] = nmc + lr; }
       }
     }
     if (wid == 1) frags_to_lds<DHP, QS>(gf, sG, lane);
@@ -659,9 +683,9 @@ template <int DHP, bool BIAS> static void dkdv_dh(const VarP& p, hipStream_t st)
   else hipLaunchKernelGGL((var_dkdv_k<DHP, 4, BIAS, false>), grid, dim3(256), 0, st, p);
 }
 template <int DHP, bool DROP> static void dbias_dh(const VarP& p, hipStream_t st) {
-  constexpr int QT = 1;   // 128 queries (QT = 2) spill: ViT-B/14, 64 samples, 191 us
-  const dim3 grid(xcd_grid(ceil_div(p.Lk, 128) * ceil_div(p.Lq, 64 * QT) * p.splits * p.H));
-  hipLaunchKernelGGL((var_dbias_k<DHP, QT, DROP>), grid, dim3(256), 0, st, p);
+  constexpr int WQ = dbias_wq<DHP>();
+  const dim3 grid(xcd_grid(ceil_div(p.Lk, 128) * ceil_div(p.Lq, 64 * WQ) * p.splits * p.H));
+  hipLaunchKernelGGL((var_dbias_k<DHP, WQ, DROP>), grid, dim3(WQ * 256), 0, st, p);
 }
 template <int DHP, bool BIAS> static void few_dh(const VarP& p, hipStream_t st) {
   hipLaunchKernelGGL((var_few_bwd_k<DHP, BIAS>), dim3(var_grid<BIAS>(p, p.Lk, 128)), dim3(256), 0, st, p);
