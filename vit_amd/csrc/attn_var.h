@@ -31,7 +31,8 @@ struct VarP {
 
 __device__ __forceinline__ int key_count(const VarP& p, int64_t b) {
   if (!p.kv_len) return p.Lk;
-  const int n = p.kv_len[b];
+  // a scalar load: a vector load would be waited for together with every request in flight
+  const int n = ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p.kv_len)[b];
   return n < 0 ? 0 : n > p.Lk ? p.Lk : n;
 }
 // Finite entries beyond the limit are pulled in so that S' and its multiples stay finite; -inf, +inf and NaN pass.
@@ -105,18 +106,18 @@ template <int DHP> __device__ __forceinline__ bf16x8 u_cols(const char* s, int r
   const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(t + hi8));
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 // The requests are issued from inline assembly: for a DMA it can see the compiler waits before every LDS read that follows.
 // They write LDS, no register; u_wait / the barrier behind it order them against the reads.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // m0 is reserved; nothing else in these kernels uses it
 __device__ __forceinline__ void u_dma16(__amdgpu_buffer_rsrc_t rs, uint32_t voff, uint32_t soff, uint32_t lds) {
-  uint32_t keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep) : "s"(lds), "v"(voff), "s"(rs), "s"(soff) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(uniform(lds)), "v"(voff), "s"(rs), "s"(uniform(soff)) : "memory", "m0");
 }
-__device__ __forceinline__ void u_dma4(__amdgpu_buffer_rsrc_t rs, uint32_t voff, uint32_t soff, uint32_t lds) {
-  uint32_t keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep) : "s"(lds), "v"(voff), "s"(rs), "s"(soff) : "memory");
+__device__ __forceinline__ void u_dma4(__amdgpu_buffer_rsrc_t rs, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(uniform(lds)), "v"(voff), "s"(rs) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // waits until at most N of the wave's memory requests are outstanding (they retire in the order of their issue)
 template <int N> __device__ __forceinline__ void u_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
@@ -127,6 +128,7 @@ template <int DHP, int NW> struct TileDma {
   static constexpr int N = DHP / 8 / NW;
   __amdgpu_buffer_rsrc_t rs;
   uint32_t voff[N], tile_bytes, dst;
+  int last;   // tile
 };
 template <int DHP, int NW>
 __device__ __forceinline__ TileDma<DHP, NW> tile_dma(const bf16* g, int64_t ss, int S, int Dh, uint32_t dst, int wid, int lane) {
@@ -135,6 +137,7 @@ __device__ __forceinline__ TileDma<DHP, NW> tile_dma(const bf16* g, int64_t ss, 
   t.rs = rows_rsrc(g, ss, S, Dh);
   t.tile_bytes = (uint32_t)(64 * ss * 2);
   t.dst = dst + (uint32_t)(wid * N * 1024);
+  t.last = (S - 1) >> 6;
 #pragma unroll
   for (int i = 0; i < N; i++) {
     const int u = (wid * N + i) * 64 + lane, row = u / CPR, c = (u - row * CPR) ^ u_swz<DHP>(row);
@@ -142,9 +145,12 @@ __device__ __forceinline__ TileDma<DHP, NW> tile_dma(const bf16* g, int64_t ss, 
   }
   return t;
 }
+// A tile beyond the last brings the last once more (no caller multiplies it): the scalar offset has to stay below the
+// descriptor's size, which the hardware reduces by it before it compares.
 template <int DHP, int NW> __device__ __forceinline__ void tile_request(const TileDma<DHP, NW>& t, int tile, uint32_t buf_off) {
+  const uint32_t soff = (uint32_t)max(min(tile, t.last), 0) * t.tile_bytes;
 #pragma unroll
-  for (int i = 0; i < TileDma<DHP, NW>::N; i++) u_dma16(t.rs, t.voff[i], (uint32_t)tile * t.tile_bytes, t.dst + buf_off + i * 1024);
+  for (int i = 0; i < TileDma<DHP, NW>::N; i++) u_dma16(t.rs, t.voff[i], soff, t.dst + buf_off + i * 1024);
 }
 
 // launches of the matrix-unit kernels (attn_var_fwd.hip, attn_var_bwd.hip); operands checked by the caller

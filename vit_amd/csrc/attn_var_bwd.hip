@@ -86,7 +86,7 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
   const uint32_t lds0 = lds_addr(smem);
   const TileDma<DHP, NW> ksrc = tile_dma<DHP, NW>(kp, p.k_ss, len, Dh, lds0, wid, lane);
   const TileDma<DHP, NW> vsrc = tile_dma<DHP, NW>(vp, p.v_ss, len, Dh, lds0 + u_tile<DHP>(), wid, lane);
-  auto request = [&](int t, int buf) {   // tiles beyond the keys arrive as zeros
+  auto request = [&](int t, int buf) {   
     tile_request(ksrc, t, buf * TILE);
     tile_request(vsrc, t, buf * TILE);
   };
@@ -192,7 +192,7 @@ template <bool BIAS> __device__ __forceinline__ RowDma row_dma(const VarP& p, in
   return r;
 }
 __device__ __forceinline__ void row_request(const RowDma& r, int row0, uint32_t buf_off, int lane) {
-  u_dma4(r.rs, (uint32_t)lane * 4u + r.off, (uint32_t)row0 * r.row_bytes, r.dst + buf_off);
+  u_dma4(r.rs, (uint32_t)row0 * r.row_bytes + (uint32_t)lane * 4u + r.off, r.dst + buf_off);
 }
 // Which of the 64 rows hold an |m c| beyond BIG_EXP; from LDS: a load from memory here would wait for every request in flight
 // (the counter is one for all), a tile's time each step.
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void va
     const TileDma<DHP, NW> qsrc = tile_dma<DHP, NW>((const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, S, Dh, lds0, wid, lane);
     const TileDma<DHP, NW> gsrc = tile_dma<DHP, NW>((const bf16*)p.dout + b * p.g_sb + h * p.g_sh, p.g_ss, S, Dh, lds0 + u_tile<DHP>(), wid, lane);
     const RowDma rsrc = row_dma<BIAS>(p, bh * p.Lq, lds0 + 2 * u_tile<DHP>(), wid);
-    auto request = [&](int t, int buf) {   // tiles beyond the queries arrive as zeros
+    auto request = [&](int t, int buf) {   
       tile_request(qsrc, t, buf * TILE);
       tile_request(gsrc, t, buf * TILE);
       row_request(rsrc, t * 64, buf * TILE, lane);
@@ -417,14 +417,22 @@ __global__ __launch_bounds__(WQ * 256, 1) void var_dbias_k(VarP p) {
   // Four waves bring a 64-row tile: with WQ = 2 the waves of a half take one tile of each operand, with 1 all take both of K
   // and V.  The same offsets in every sample, another descriptor.
   const uint32_t qdst = lds0 + KV + wq * (2 * T + row_bytes<true>());
-  TileDma<DHP, 4> ksrc = tile_dma<DHP, 4>((const bf16*)p.k, p.k_ss, p.Lk, Dh, lds0 + wq * T, wk, lane);
-  TileDma<DHP, 4> vsrc = tile_dma<DHP, 4>((const bf16*)p.v, p.v_ss, p.Lk, Dh, lds0 + 2 * T + wq * T, wk, lane);
-  TileDma<DHP, 4> qsrc = tile_dma<DHP, 4>((const bf16*)p.q, p.q_ss, p.Lq, Dh, qdst, wk, lane);
-  TileDma<DHP, 4> gsrc = tile_dma<DHP, 4>((const bf16*)p.dout, p.g_ss, p.Lq, Dh, qdst + T, wk, lane);
+  const bf16* kh = (const bf16*)p.k + h * p.k_sh;
+  const bf16* vh = (const bf16*)p.v + h * p.v_sh;
+  const bf16* qh = (const bf16*)p.q + h * p.q_sh;
+  const bf16* gh = (const bf16*)p.dout + h * p.g_sh;
+  TileDma<DHP, 4> ksrc = tile_dma<DHP, 4>(kh, p.k_ss, p.Lk, Dh, lds0 + wq * T, wk, lane);
+  TileDma<DHP, 4> vsrc = tile_dma<DHP, 4>(vh, p.v_ss, p.Lk, Dh, lds0 + 2 * T + wq * T, wk, lane);
+  TileDma<DHP, 4> qsrc = tile_dma<DHP, 4>(qh, p.q_ss, p.Lq, Dh, qdst, wk, lane);
+  TileDma<DHP, 4> gsrc = tile_dma<DHP, 4>(gh, p.g_ss, p.Lq, Dh, qdst + T, wk, lane);
+  RowDma rsrc = row_dma<true>(p, h * (int64_t)p.Lq, qdst + 2 * T, wk);
+  const float* rh = (wk >= 2 ? p.stat + 2 * (h * (int64_t)p.Lq) : (wk & 1 ? p.delta : p.nl) + h * (int64_t)p.Lq);
+  const uint32_t rstep = (uint32_t)(p.H * p.Lq) * (wk >= 2 ? 2u : 1u);   // floats from sample to sample
   auto request_keys = [&](int b) {
     const int len = key_count(p, b);
-    ksrc.rs = rows_rsrc((const bf16*)p.k + b * p.k_sb + h * p.k_sh, p.k_ss, len, Dh);
-    vsrc.rs = rows_rsrc((const bf16*)p.v + b * p.v_sb + h * p.v_sh, p.v_ss, len, Dh);
+    ksrc.rs = rows_rsrc(kh + (uint32_t)b * p.k_sb, p.k_ss, len, Dh);
+    vsrc.rs = rows_rsrc(vh + (uint32_t)b * p.v_sb, p.v_ss, len, Dh);
+    ksrc.last = vsrc.last = (len - 1) >> 6;
 #pragma unroll
     for (int i = 0; i < 2 / WQ; i++) {
       tile_request(ksrc, kb * 2 + wq + i, i * T);
@@ -432,11 +440,12 @@ __global__ __launch_bounds__(WQ * 256, 1) void var_dbias_k(VarP p) {
     }
   };
   auto request_rows = [&](int b, int buf) {
-    qsrc.rs = rows_rsrc((const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, p.Lq, Dh);
-    gsrc.rs = rows_rsrc((const bf16*)p.dout + b * p.g_sb + h * p.g_sh, p.g_ss, p.Lq, Dh);
+    qsrc.rs = rows_rsrc(qh + (uint32_t)b * p.q_sb, p.q_ss, p.Lq, Dh);
+    gsrc.rs = rows_rsrc(gh + (uint32_t)b * p.g_sb, p.g_ss, p.Lq, Dh);
     tile_request(qsrc, qb * WQ + wq, buf * QG);
     tile_request(gsrc, qb * WQ + wq, buf * QG);
-    row_request(row_dma<true>(p, ((int64_t)b * p.H + h) * p.Lq, qdst + 2 * T, wk), q0, buf * QG, lane);
+    rsrc.rs = __builtin_amdgcn_make_buffer_rsrc((void*)(rh + (uint64_t)(uint32_t)b * rstep), 0, p.Lq * (int)rsrc.row_bytes, 0x00020000);
+    row_request(rsrc, q0, buf * QG, lane);
   };
   int b = next_live(share * part), buf = 0;
   if (b < b_end) {

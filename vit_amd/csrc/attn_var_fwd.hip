@@ -193,7 +193,7 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
   const uint32_t lds0 = lds_addr(smem);
   const TileDma<DHP, NW> ksrc = tile_dma<DHP, NW>(kp, p.k_ss, len, Dh, lds0, wid, lane);
   const TileDma<DHP, NW> vsrc = tile_dma<DHP, NW>(vp, p.v_ss, len, Dh, lds0 + u_tile<DHP>(), wid, lane);
-  auto request = [&](int t, int buf) {   // tiles beyond the keys arrive as zeros
+  auto request = [&](int t, int buf) {
     tile_request(ksrc, t, buf * TILE);
     tile_request(vsrc, t, buf * TILE);
   };
