@@ -23,7 +23,7 @@ struct VarP {
   int B, H, Lq, Lk, Dh;
   int nqt, nkt;                // 32-row tiles of bias_s per head: nqt x nkt (nkt even); bias_t: nkt_t x nqt_t (nqt_t even)
   int nqt_t, nkt_t;
-  int splits;
+  int splits, buckets;
   uint64_t seed;
   float scale, inv_scale, bias_lim, keep_scale;
   uint32_t thr;

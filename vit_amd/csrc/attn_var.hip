@@ -278,17 +278,18 @@ __global__ __launch_bounds__(256) void var_piece_sum_k(const float* __restrict__
   if (pc >= npieces) return;
   const int b = piece[pc], e = piece[pc + 1], nh = min(4, H - h0);
   float a[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; s++) {
-    const float* src = dbias + ((int64_t)s * H + h0) * pairs;
-    for (int i = b + lane; i < e; i += 256) {
+  for (int i = b + lane; i < e; i += 256) {
+    int64_t at[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) at[u] = i + 64 * u < e ? order[i + 64 * u] : -1;
+#pragma unroll 2
+    for (int s = 0; s < splits; s++) {
+      const float* src = dbias + ((int64_t)s * H + h0) * pairs;
       float x[4][4];
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const bool in = i + 64 * u < e;
-        const int64_t at = in ? order[i + 64 * u] : 0;
+      for (int u = 0; u < 4; u++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) x[u][k] = in && k < nh ? src[k * pairs + at] : 0.f;
-      }
+        for (int k = 0; k < 4; k++) x[u][k] = at[u] >= 0 && k < nh ? src[k * pairs + at[u]] : 0.f;
 #pragma unroll
       for (int k = 0; k < 4; k++) a[k] += (x[0][k] + x[1][k]) + (x[2][k] + x[3][k]);
     }
@@ -332,7 +333,7 @@ static VarP make_varp(const VitkAttnVar* a) {
   p.B = (int)a->B; p.H = (int)a->H; p.Lq = (int)a->Lq; p.Lk = (int)a->Lk; p.Dh = (int)a->Dh;
   p.nqt = (int)ceil_div(a->Lq, 32); p.nkt = (int)ceil_div(a->Lk, 64) * 2;
   p.nkt_t = (int)ceil_div(a->Lk, 32); p.nqt_t = (int)ceil_div(a->Lq, 64) * 2;
-  p.splits = 1;
+  p.splits = 1; p.buckets = (int)a->num_buckets;
   p.seed = a->seed; p.scale = a->scale; p.inv_scale = 1.f / a->scale;
   p.bias_lim = 1e38f * a->scale < 1e37f ? 1e38f * a->scale : 1e37f;
   p.thr = a->drop_p > 0.f ? drop_threshold(a->drop_p) : 0;
@@ -346,7 +347,7 @@ static VitkAttnVar var_normal(const VitkAttnVar* a) {
     const bool key_side = i == 1 || i == 2 || i == 6 || i == 7;   // q, k, v, o, dout, dq, dk, dv
     if (n.B == 1) n.st[3 * i] = 0;
     if (n.H == 1) n.st[3 * i + 1] = 0;
-    if ((key_side ? n.Lk : n.Lq) == 1) n.st[3 * i + 2] = 0;
+    if ((key_side ? n.Lk : n.Lq) == 1) n.st[3 * i + 2] = (n.Dh + 7) & ~7;   // the next row lies behind the end: see var_mfma_ok
   }
   return n;
 }
@@ -365,6 +366,7 @@ static int var_validate(const VitkAttnVar* a, bool bwd) {
   VITK_REQUIRE(!a->bias_table == !a->bias_index, "attn_var: a bias needs its table and its index");
   if (a->bias_table) {
     VITK_REQUIRE(a->num_buckets > 0 && a->num_buckets <= 65536, "attn_var: num_buckets=%lld outside [1, 65536]", (long long)a->num_buckets);
+    VITK_REQUIRE(a->num_buckets * a->H < (1ll << 29), "attn_var: a bias table of %lld x %lld is not supported", (long long)a->num_buckets, (long long)a->H);
     VITK_REQUIRE(a->Lq * a->Lk < (1ll << 31), "attn_var: a bias over %lld x %lld pairs is not supported", (long long)a->Lq, (long long)a->Lk);
   }
   if (bwd) {
@@ -376,12 +378,13 @@ static int var_validate(const VitkAttnVar* a, bool bwd) {
   return 0;
 }
 // The matrix-unit kernels take head sizes that are multiples of 8, 16-byte aligned rows, and rows of one (sample, head)
-// within 32-bit byte offsets (the tiles asked for ahead of the last one included).
+// within 32-bit byte offsets (the tiles asked for ahead of the last one included).  Rows have to follow each other: the
+// kernels find the rows beyond the last by their addresses, so expanded or overlapping rows are not for them.
 static bool var_mfma_ok(const VitkAttnVar* a, bool bwd) {
   if (a->Dh % 8 || a->algo == 1 || a->Lk == 0) return false;
   const int es = a->dtype == VITK_BF16 ? 2 : 4;
   for (int i = 0; i < (bwd ? 24 : 12); i++)
-    if (a->st[i] * es % 16) return false;
+    if (a->st[i] * es % 16 || (i % 3 == 2 && a->st[i] < a->Dh)) return false;
   const void* ps[] = {a->q, a->k, a->v, a->o, a->dout, a->dq, a->dk, a->dv};
   for (int i = 0; i < (bwd ? 8 : 4); i++)
     if ((uintptr_t)ps[i] & 15) return false;

@@ -600,9 +600,10 @@ def qk_norm_rope_bwd(xs: tuple, gs: tuple, dxs: tuple, w: tuple, tables: tuple, 
 # attention with a relative position bias and / or key counts
 # ------------------------------------------------------------------------------------------------
 def attn_operand(t: Tensor) -> Tensor:
-    """``t`` [B, L, H, Dh] as the kernels take it: d contiguous, and rows on 16-byte boundaries where head_dim allows it
-    (the kernels on the matrix units load 16 bytes at a time; a view that is not laid out so is copied once)."""
-    if t.stride(3) == 1:
+    """``t`` [B, L, H, Dh] as the kernels take it: d contiguous, rows that do not overlap (an expanded dimension of rows does),
+    and on 16-byte boundaries where head_dim allows it (the kernels on the matrix units load 16 bytes at a time); a view that
+    is not laid out so is copied once."""
+    if t.stride(3) == 1 and (t.shape[1] <= 1 or t.stride(1) >= t.shape[3]):
         n = 16 // t.element_size()
         sb, ss, sh, _ = t.stride()
         if t.shape[3] % n or not (sb % n or ss % n or sh % n or t.data_ptr() % 16):
