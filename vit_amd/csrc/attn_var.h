@@ -153,8 +153,37 @@ template <int DHP, int NW> __device__ __forceinline__ void tile_request(const Ti
   for (int i = 0; i < TileDma<DHP, NW>::N; i++) u_dma16(t.rs, t.voff[i], soff, t.dst + buf_off + i * 1024);
 }
 
+// The same for a wave of its own: 32 rows.  Its LDS reads have to be over (u_wait_lds) before their place is asked for again.
+template <int DHP> struct WaveDma {
+  __amdgpu_buffer_rsrc_t rs;
+  uint32_t voff[DHP / 16], tile_bytes, dst;
+  int last;
+};
+template <int DHP> __device__ __forceinline__ WaveDma<DHP> wave_dma(const bf16* g, int64_t ss, int S, int Dh, uint32_t dst, int lane) {
+  constexpr int CPR = DHP / 8;
+  WaveDma<DHP> t;
+  t.rs = rows_rsrc(g, ss, S, Dh);
+  t.tile_bytes = (uint32_t)(32 * ss * 2);
+  t.dst = dst;
+  t.last = (S - 1) >> 5;
+#pragma unroll
+  for (int i = 0; i < DHP / 16; i++) {
+    const int u = i * 64 + lane, row = u / CPR, c = (u - row * CPR) ^ u_swz<DHP>(row);
+    t.voff[i] = c * 8 < Dh ? (uint32_t)((row * ss + c * 8) * 2) : OOB_OFF;
+  }
+  return t;
+}
+template <int DHP> __device__ __forceinline__ void wave_request(const WaveDma<DHP>& t, int tile, uint32_t buf_off) {
+  const uint32_t soff = (uint32_t)max(min(tile, t.last), 0) * t.tile_bytes;
+#pragma unroll
+  for (int i = 0; i < DHP / 16; i++) u_dma16(t.rs, t.voff[i], soff, t.dst + buf_off + i * 1024);
+}
+__device__ __forceinline__ void u_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // launches of the matrix-unit kernels (attn_var_fwd.hip, attn_var_bwd.hip); operands checked by the caller
 void var_launch_expand(const VarP& p, bool transposed, hipStream_t st);
+int var_few_heads(int64_t H);
+void var_launch_few_fwd(const VarP& p, bool bias, hipStream_t st);
 void var_launch_fwd(const VarP& p, bool bias, int nw, hipStream_t st);
 void var_launch_dq(const VarP& p, bool bias, hipStream_t st);
 void var_launch_dkdv(const VarP& p, bool bias, hipStream_t st);

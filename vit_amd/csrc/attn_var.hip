@@ -392,6 +392,8 @@ static bool var_mfma_ok(const VitkAttnVar* a, bool bwd) {
   if ((a->Lq + 256) * a->st[2] >= lim || (a->Lk + 256) * a->st[5] >= lim || (a->Lk + 256) * a->st[8] >= lim || (a->Lq + 256) * a->st[11] >= lim) return false;
   return !bwd || (a->Lq + 256) * a->st[14] < lim;
 }
+// Few queries: the kernels that read K and V once, with 32 keys per wave
+static bool var_few(const VitkAttnVar* a) { return a->dtype == VITK_BF16 && a->Lq <= 32 && !(a->drop_p > 0.f); }
 // Waves per workgroup, 32 query rows each: 4, or 2 where 64 rows hold all queries.
 static int var_nw(const VitkAttnVar* a) { return a->Lq <= 64 && !(a->drop_p > 0.f) ? 2 : 4; }
 // Workgroups that share the keys of a (sample, head) in the forward pass: 1 where the query blocks alone fill the chip
@@ -403,6 +405,13 @@ static int var_fwd_splits(const VitkAttnVar* a) {
     int64_t n = ceil_div(1024, waves);
     if (n > tiles / 2) n = tiles / 2;
     return (int)(n < 64 ? n : 64);
+  }
+  if (var_few(a)) {   // shares are waves, up to 4 of a workgroup: four rounds of the four waves a CU holds
+    const int64_t kw = 4 / var_few_heads(a->H);
+    int64_t n = 4096 / (a->B * a->H), most = ceil_div(a->Lk, 32) / 4;
+    if (n > most) n = most;
+    if (n > 64) n = 64;
+    return (int)(ceil_div(n < 1 ? 1 : n, kw) * kw);
   }
   if (a->drop_p > 0.f) return 1;
   const int64_t blocks = a->B * a->H * ceil_div(a->Lq, 32 * var_nw(a)), tiles = ceil_div(a->Lk, 64);
@@ -421,7 +430,6 @@ static int var_dbias_splits(const VitkAttnVar* a) {
   if (n > a->B) n = a->B;
   return (int)(n < 1 ? 1 : n);
 }
-static bool var_few(const VitkAttnVar* a) { return a->dtype == VITK_BF16 && a->Lq <= 32 && !(a->drop_p > 0.f); }
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 struct VarWs { size_t delta, nl, bias_s, bias_t, dbias, pieces, part, pstat, total; int splits; };
@@ -482,7 +490,8 @@ extern "C" int vitk_attn_var_fwd(const VitkAttnVar* desc, void* stream) {
         p.bias_s = (const bf16*)(ws + w.bias_s);
         var_launch_expand(p, false, st);
       }
-      var_launch_fwd(p, a->bias_table != nullptr, var_nw(a), st);
+      if (var_few(a)) var_launch_few_fwd(p, a->bias_table != nullptr, st);
+      else var_launch_fwd(p, a->bias_table != nullptr, var_nw(a), st);
     }
   } else {
     dim3 grid((unsigned)ceil_div(a->Lq, 64), (unsigned)a->H, (unsigned)a->B);

@@ -157,6 +157,33 @@ __device__ __forceinline__ void var_fwd_tile(const VarP& p, const char* sK, cons
     }
 }
 
+// A wave's 32 queries of head (b, h): the normalised rows and their statistics, or with SPLIT the shares for var_combine_k.
+template <int DHP, bool SPLIT>
+__device__ __forceinline__ void var_fwd_store(const VarP& p, const f32x16 (&oacc)[DHP / 32], float l, float m, int64_t b, int64_t h,
+                                              int qrow, int share, int lane) {
+  if (qrow >= p.Lq) return;
+  const int64_t srow = (b * p.H + h) * p.Lq + qrow;
+  if (SPLIT) {
+    const int64_t rows = (int64_t)p.B * p.H * p.Lq;
+    const int64_t prow = share * rows + srow;
+    float* dst = p.part + prow * p.Dh;
+#pragma unroll
+    for (int dt = 0; dt < DHP / 32; dt++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int d = dt * 32 + 8 * g + 4 * (lane >> 5);
+        if (d < p.Dh) *(float4*)(dst + d) = make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
+      }
+    if (lane < 32) { p.pstat[2 * prow] = m; p.pstat[2 * prow + 1] = l; }
+    return;
+  }
+  store_rows<DHP>((bf16*)p.o + b * p.o_sb + h * p.o_sh + (int64_t)qrow * p.o_ss, oacc, l == 0.f ? 0.f : 1.f / l, p.Dh, lane);
+  if (lane < 32) {
+    p.stat[2 * srow] = l == 0.f ? 0.f : m;
+    p.stat[2 * srow + 1] = l == 0.f ? -INFINITY : -__log2f(l);
+  }
+}
+
 // waves per SIMD: what the registers of an instance allow without spilling
 template <int DHP, int NW, bool BIAS, bool DROP> constexpr int var_fwd_occ() {
   return DHP <= 64 ? (!BIAS ? 3 : 2) : DHP <= 96 ? 2 : 1;
@@ -247,53 +274,103 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
     }
   }
   u_wait<0>();   // nothing may arrive in LDS after the workgroup has left
-  if (qrow >= S) return;
-  const float l = lacc[0];
-  const int64_t srow = (b * p.H + h) * p.Lq + qrow;
-  if (SPLIT) {
-    const int64_t rows = (int64_t)p.B * p.H * p.Lq;
-    const int64_t prow = (int64_t)blockIdx.y * rows + srow;
-    float* dst = p.part + prow * Dh;
-#pragma unroll
-    for (int dt = 0; dt < DHP / 32; dt++)
-#pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const int d = dt * 32 + 8 * g + 4 * (lane >> 5);
-        if (d < Dh) *(float4*)(dst + d) = make_float4(oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]);
-      }
-    if (lane < 32) { p.pstat[2 * prow] = m; p.pstat[2 * prow + 1] = l; }
-    return;
-  }
-  store_rows<DHP>((bf16*)p.o + b * p.o_sb + h * p.o_sh + (int64_t)qrow * p.o_ss, oacc, l == 0.f ? 0.f : 1.f / l, Dh, lane);
-  if (lane < 32) {
-    p.stat[2 * srow] = l == 0.f ? 0.f : m;
-    p.stat[2 * srow + 1] = l == 0.f ? -INFINITY : -__log2f(l);
-  }
+  var_fwd_store<DHP, SPLIT>(p, oacc, lacc[0], m, b, h, qrow, (int)blockIdx.y, lane);
 }
 
-// Joins the shares of a row: M = max m, O = sum 2^((m - M) c) O_s / sum 2^((m - M) c) l_s.  16 lanes per row.
+// Up to 32 queries: bound by K and V in, and what counts is how many bytes are on their way.  Every wave works for itself, on
+// a share of the keys of one head, with 32-key tiles in LDS of its own that it asks for NB - 1 steps ahead: no barrier.  The
+// HW heads of a workgroup are neighbours, and so are the workgroups of a sample's key range on an XCD: heads whose rows are
+// no multiple of a cache line share lines, which are then fetched once.
+template <int DHP> constexpr int few_buffers() { return DHP == 96 ? 3 : 2; }
+template <int DHP, int HW, bool BIAS, bool SPLIT>
+__global__ __launch_bounds__(256, (DHP <= 64 ? 2 : 1)) void var_few_fwd_k(VarP p) {
+  constexpr int T = 32 * DHP * 2, NB = few_buffers<DHP>(), REQ = 2 * TileDma<DHP, 2>::N, KW = 4 / HW;
+  __shared__ __attribute__((aligned(16))) char smem[4 * NB * 2 * T];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), Dh = p.Dh;
+  const int groups = p.H / HW, parts = p.splits / KW;   // of heads; of keys
+  const uint32_t i = blockIdx.x >> 3, g = uniform(i / groups) * 8 + (blockIdx.x & 7);
+  const int64_t b = uniform(g / parts), h = (int)(i % groups) * HW + wid % HW;
+  if (b >= p.B) return;
+  const int share = (int)(g - (uint32_t)b * parts) * KW + wid / HW;
+  const int len_all = key_count(p, b), per = uniform((uint32_t)(((len_all + 31) >> 5) + p.splits - 1) / (uint32_t)p.splits);
+  const int t0 = per * share, len = min(len_all, (t0 + per) * 32), nt = max((len + 31) >> 5, t0);   // keys [32 t0, len): none if t0 = nt
+  const int qrow = lane & 31;
+  const uint32_t lds0 = lds_addr(smem) + wid * (NB * 2 * T);
+  const bf16* kp = (const bf16*)p.k + b * p.k_sb + h * p.k_sh;
+  const bf16* vp = (const bf16*)p.v + b * p.v_sb + h * p.v_sh;
+  const WaveDma<DHP> ksrc = wave_dma<DHP>(kp, p.k_ss, len, Dh, lds0, lane), vsrc = wave_dma<DHP>(vp, p.v_ss, len, Dh, lds0 + T, lane);
+  const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc(BIAS ? (void*)(p.bias_s + h * p.nqt * p.nkt * 1024) : nullptr, 0, BIAS ? p.nkt * 2048 : 0, 0x00020000);
+  bf16x8 qf[DHP / 16], bf[4];
+  load_stationary<DHP>(qf, (const bf16*)p.q + b * p.q_sb + h * p.q_sh, p.q_ss, qrow, p.Lq, Dh, lane);
+  auto load_bias = [&](int t) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) bf[k] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(t * 2048 + k * 1024 + lane * 16)));
+  };
+  auto request = [&](int t, int buf) {
+    wave_request(ksrc, t, buf * 2 * T);
+    wave_request(vsrc, t, buf * 2 * T);
+  };
+  if (BIAS) load_bias(t0);
+#pragma unroll
+  for (int k = 0; k < NB - 1; k++) request(t0 + k, k);
+  const f32x16 zero = ZERO16;
+  f32x16 oacc[DHP / 32], lacc = zero;
+#pragma unroll
+  for (int dt = 0; dt < DHP / 32; dt++) oacc[dt] = zero;
+  float m = -INFINITY;
+  const float c = p.scale * LOG2E;
+  int buf = 0;
+  for (int t = t0; t < nt; t++) {
+    u_wait<(NB - 2) * REQ>();   // this tile has arrived
+    const char* sK = smem + (wid * NB + buf) * 2 * T;
+    f32x16 sacc[1];
+    var_init<1, BIAS>(sacc, bf, p.inv_scale);
+    if (BIAS) load_bias(t + 1);
+    u_wait_lds();   // the reads of the tile before, whose place the next one takes
+    request(t + NB - 1, buf == 0 ? NB - 1 : buf - 1);
+    if (t * 32 + 32 <= len) var_fwd_tile<DHP, 1, false, BIAS, false>(p, sK, sK + T, qf, sacc, oacc, lacc, m, c, t * 32, len, 0u, lane);
+    else var_fwd_tile<DHP, 1, true, BIAS, false>(p, sK, sK + T, qf, sacc, oacc, lacc, m, c, t * 32, len, 0u, lane);
+    buf = buf + 1 == NB ? 0 : buf + 1;
+  }
+  u_wait<0>();   // nothing may arrive in LDS after the workgroup has left
+  var_fwd_store<DHP, SPLIT>(p, oacc, lacc[0], m, b, h, qrow, share, lane);
+}
+
+// Joins the shares of a row: M = max m, O = sum 2^((m - M) c) O_s / sum 2^((m - M) c) l_s.  A wave per row: 16 lanes hold 8
+// values each, the four groups of 16 take every fourth share.
 template <class T> __global__ __launch_bounds__(256) void var_combine_k(VarP p) {
   const int64_t rows = (int64_t)p.B * p.H * p.Lq;
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int j = threadIdx.x & 15;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int j = threadIdx.x & 15, grp = (threadIdx.x >> 4) & 3;
   if (row >= rows) return;
   const float c = p.scale * LOG2E;
   float M = -INFINITY;
-  for (int s = 0; s < p.splits; s++) M = fmaxf(M, p.pstat[2 * (s * rows + row)]);
+#pragma unroll 4
+  for (int s = grp; s < p.splits; s += 4) M = fmaxf(M, p.pstat[2 * (s * rows + row)]);
+  M = fmaxf(M, __shfl_xor(M, 16, 64));
+  M = fmaxf(M, __shfl_xor(M, 32, 64));
   float l = 0.f, o[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) o[i] = 0.f;
   const bool on = j * 8 < p.Dh;
-  for (int s = 0; s < p.splits; s++) {
+#pragma unroll 4
+  for (int s = grp; s < p.splits; s += 4) {
     const int64_t at = s * rows + row;
     const float m = p.pstat[2 * at], w = m == M ? (M == -INFINITY ? 0.f : 1.f) : fast_exp2((m - M) * c);
     l = fmaf(w, p.pstat[2 * at + 1], l);
-    if (on && w != 0.f) {
+    if (on) {   // a share without keys holds zeros
       const float4 a = *(const float4*)(p.part + at * p.Dh + j * 8), b = *(const float4*)(p.part + at * p.Dh + j * 8 + 4);
       o[0] = fmaf(w, a.x, o[0]); o[1] = fmaf(w, a.y, o[1]); o[2] = fmaf(w, a.z, o[2]); o[3] = fmaf(w, a.w, o[3]);
       o[4] = fmaf(w, b.x, o[4]); o[5] = fmaf(w, b.y, o[5]); o[6] = fmaf(w, b.z, o[6]); o[7] = fmaf(w, b.w, o[7]);
     }
   }
+#pragma unroll
+  for (int x = 16; x < 64; x *= 2) {
+    l += __shfl_xor(l, x, 64);
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] += __shfl_xor(o[i], x, 64);
+  }
+  if (grp) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t i = row % p.Lq, h = (row / p.Lq) % p.H, b = row / ((int64_t)p.Lq * p.H);
   if (on) {
@@ -311,9 +388,28 @@ template <class T> __global__ __launch_bounds__(256) void var_combine_k(VarP p) 
 }
 
 void var_launch_combine(const VarP& p, bool f32, hipStream_t st) {
-  const dim3 grid((unsigned)ceil_div((int64_t)p.B * p.H * p.Lq, 16));
+  const dim3 grid((unsigned)ceil_div((int64_t)p.B * p.H * p.Lq, 4));
   if (f32) hipLaunchKernelGGL((var_combine_k<float>), grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL((var_combine_k<bf16>), grid, dim3(256), 0, st, p);
+}
+// Heads of a workgroup of var_few_fwd_k; its other waves share keys.
+int var_few_heads(int64_t H) { return H % 4 == 0 ? 4 : H % 2 == 0 ? 2 : 1; }
+template <int DHP, bool BIAS, int HW> static void few_fwd(const VarP& p, hipStream_t st) {
+  const dim3 grid((unsigned)(ceil_div((int64_t)p.B * (p.splits / (4 / HW)), 8) * 8 * (p.H / HW)));
+  if constexpr (HW == 4) {
+    if (p.splits == 1) {
+      hipLaunchKernelGGL((var_few_fwd_k<DHP, HW, BIAS, false>), grid, dim3(256), 0, st, p);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((var_few_fwd_k<DHP, HW, BIAS, true>), grid, dim3(256), 0, st, p);
+}
+template <int DHP, bool BIAS> static void few_fwd_dh(const VarP& p, hipStream_t st) {
+  const int hw = var_few_heads(p.H);
+  if (hw == 4) few_fwd<DHP, BIAS, 4>(p, st);
+  else if (hw == 2) few_fwd<DHP, BIAS, 2>(p, st);
+  else few_fwd<DHP, BIAS, 1>(p, st);
+  if (p.splits > 1) var_launch_combine(p, false, st);
 }
 template <int DHP, bool BIAS> static void fwd_dh(const VarP& p, int nw, hipStream_t st) {
   const dim3 grid(var_grid<BIAS>(p, p.Lq, nw * 32), (unsigned)p.splits);
@@ -327,6 +423,11 @@ template <int DHP, bool BIAS> static void fwd_dh(const VarP& p, int nw, hipStrea
     if (nw == 2) hipLaunchKernelGGL((var_fwd_k<DHP, 2, BIAS, false, false>), grid, dim3(128), 0, st, p);
     else hipLaunchKernelGGL((var_fwd_k<DHP, 4, BIAS, false, false>), grid, dim3(256), 0, st, p);
   }
+}
+void var_launch_few_fwd(const VarP& p, bool bias, hipStream_t st) {
+  if (p.Dh <= 64) { if (bias) few_fwd_dh<64, true>(p, st); else few_fwd_dh<64, false>(p, st); }
+  else if (p.Dh <= 96) { if (bias) few_fwd_dh<96, true>(p, st); else few_fwd_dh<96, false>(p, st); }
+  else { if (bias) few_fwd_dh<128, true>(p, st); else few_fwd_dh<128, false>(p, st); }
 }
 void var_launch_fwd(const VarP& p, bool bias, int nw, hipStream_t st) {
   if (p.Dh <= 64) { if (bias) fwd_dh<64, true>(p, nw, st); else fwd_dh<64, false>(p, nw, st); }
