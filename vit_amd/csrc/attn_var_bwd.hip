@@ -22,8 +22,8 @@ __device__ __forceinline__ f32x16 init_tile(const bf16x8& lo, const bf16x8& hi, 
 template <int DHP, int HALVES, bool PARTIAL, bool BIAS, bool DROP>
 __device__ __forceinline__ void var_dq_tile(const VarP& p, const char* sK, const char* sV, const bf16x8 (&qf)[DHP / 16],
                                             const bf16x8 (&gf)[DHP / 16], f32x16 (&sacc)[HALVES], f32x16 (&dqacc)[DHP / 32],
-                                            float m, float nmc, bool big, float delta, float c, int k0, int len, uint32_t xrow,
-                                            int lane) {
+                                            float m, float nmc, bool big, float delta, float& dsum, float c, int k0, int len,
+                                            uint32_t xrow, int lane) {
   const f32x16 zero = ZERO16;
   const int rowoff = 4 * (lane >> 5);
 #pragma unroll
@@ -62,6 +62,10 @@ __device__ __forceinline__ void var_dq_tile(const VarP& p, const char* sK, const
 #pragma unroll
       for (int dt = 0; dt < DHP / 32; dt++)
         dqacc[dt] = MFMA(u_cols<DHP>(sK, st * 32, s2, dt * 32, lane), df, dqacc[dt], 0, 0, 0);
+      if (BIAS) {
+#pragma unroll
+        for (int r = 8 * s2; r < 8 * s2 + 8; r += 2) dsum += sacc[st][r] + sacc[st][r + 1];
+      }
     }
   }
 }
@@ -117,10 +121,8 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
   delta += __shfl_xor(delta, 32, 64);
   const float c = p.scale * LOG2E, nmc = -m * c;
   const bool big = BIAS && __any(fabsf(m * c) > BIG_EXP);
-  if (qv && lane < 32) {   // for the kernels launched after this one
-    p.delta[srow] = -delta;
-    p.nl[srow] = nmc + lr;
-  }
+  if (qv && lane < 32) p.nl[srow] = nmc + lr;   // for the kernels launched after this one
+  float dsum = 0.f;
   const uint32_t rbase = var_drop_xrow(p, (uint64_t)srow, lane);
   const f32x16 zero = ZERO16;
   f32x16 dqacc[DHP / 32];
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
     f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
     if (BIAS) load_bias(t + 1);
     request(t + NB - 1, ahead);
-    if (wave_on) var_dq_tile<DHP, 2, false, BIAS, DROP>(p, sK, sK + u_tile<DHP>(), qf, gf, sacc, dqacc, m, nmc, big, delta, c, t * 64, len, rbase, lane);
+    if (wave_on) var_dq_tile<DHP, 2, false, BIAS, DROP>(p, sK, sK + u_tile<DHP>(), qf, gf, sacc, dqacc, m, nmc, big, delta, dsum, c, t * 64, len, rbase, lane);
     u_wait<NB == 3 ? REQ : 0>();
     __syncthreads();
     buf = buf + 1 == NB ? 0 : buf + 1;
@@ -145,14 +147,20 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
     const char* sV = sK + u_tile<DHP>();
     if (len - nfull * 64 > 32) {
       f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
-      var_dq_tile<DHP, 2, true, BIAS, DROP>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, c, nfull * 64, len, rbase, lane);
+      var_dq_tile<DHP, 2, true, BIAS, DROP>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, dsum, c, nfull * 64, len, rbase, lane);
     } else {
       f32x16 sacc[1] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale)};
-      var_dq_tile<DHP, 1, true, BIAS, DROP>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, c, nfull * 64, len, rbase, lane);
+      var_dq_tile<DHP, 1, true, BIAS, DROP>(p, sK, sV, qf, gf, sacc, dqacc, m, nmc, big, delta, dsum, c, nfull * 64, len, rbase, lane);
     }
   }
   u_wait<0>();   // nothing may arrive in LDS after the workgroup has left
+  // The rows of dS sum to zero; what they do sum to is the error that O's and P's rounding left in delta, and the kernels that
+  // follow get delta without it.  A bias shows it where its buckets hold most of a row's weight (ViT-g/14 at 1024 px with
+  // logarithmic buckets: relative error of dtable 2.5e-3 -> 1.7e-3, for 8% of this kernel's time); without one it stays
+  // below the rounding of dS.
+  if (BIAS) dsum += __shfl_xor(dsum, 32, 64);
   if (!qv) return;
+  if (lane < 32) p.delta[srow] = BIAS && lr != -INFINITY ? -fmaf(dsum, fast_exp2(lr), delta) : -delta;
   store_rows<DHP>((bf16*)p.dq + b * p.dq_sb + h * p.dq_sh + (int64_t)qrow * p.dq_ss, dqacc, p.scale * fast_exp2(lr), Dh, lane);
 }
 
@@ -524,6 +532,7 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
   constexpr int LDS = 6 * 32 * QS > RED ? 6 * 32 * QS : RED;
   __shared__ __attribute__((aligned(16))) char smem[LDS];   // K of each wave, Q, dO; then the dQ sums
   __shared__ __attribute__((aligned(16))) float sC[4][32];  // -m c + lr, delta, m, lr
+  __shared__ float sR[8][32];   // sums of P dP and of P of each wave's keys
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh, rowoff = 4 * (lane >> 5);
   const HeadBlock hb = var_block<BIAS>(p, p.Lk, 128);
   if (!hb.valid) return;
@@ -563,10 +572,7 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
     frags_to_lds<DHP, QS>(kf, sK, lane);
     if (wid == 0) {
       frags_to_lds<DHP, QS>(qf, sQ, lane);
-      if (lane < 32) { sC[0][lane] = nmc + lr; sC[1][lane] = delta; sC[2][lane] = m; sC[3][lane] = lr; }
-      if (BIAS && hb.xb == 0) {   // for the bias gradient
-        if (qv && lane < 32) { p.delta[srow] = -delta; p.nl[srow] = nmc + lr; }
-      }
+      if (lane < 32) { sC[0][lane] = nmc + lr; sC[2][lane] = m; sC[3][lane] = lr; }
     }
     if (wid == 1) frags_to_lds<DHP, QS>(gf, sG, lane);
     bf16x8 bs[2], bt[2];
@@ -577,6 +583,44 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
       const bf16* pt = p.bias_t + ((int64_t)h * p.nkt_t + (on ? kt : 0)) * p.nqt_t * 1024 + lane * 8;
       bs[0] = *(const bf16x8*)ps; bs[1] = *(const bf16x8*)(ps + 512);
       bt[0] = *(const bf16x8*)pt; bt[1] = *(const bf16x8*)(pt + 512);
+    }
+    __syncthreads();
+    // keys on the rows, query on the lane: P and dP, then dS for dQ
+    f32x16 st = init_tile<BIAS>(bs[0], bs[1], p.inv_scale), dt_ = zero;
+#pragma unroll
+    for (int ks = 0; ks < DHP / 16; ks++) {
+      st = MFMA(kf[ks], qf[ks], st, 0, 0, 0);
+      dt_ = MFMA(vf[ks], gf[ks], dt_, 0, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const float pr = BIAS && big ? fast_exp2((st[r] - m) * c) : fast_exp2(fmaf(st[r], c, nmc));
+      st[r] = key0 + wid * 32 + acc_row(r) + rowoff < len ? pr : 0.f;
+    }
+    // Where the workgroup holds all keys of the row, delta = sum P dP / sum P, free of O's rounding: with a handful of keys
+    // that rounding is much of what dS is made of (5 queries over 9 keys: error of dq 3.3e-3, 2.6e-3 so).
+    float num = 0.f, den = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; r++) { num += st[r] != 0.f ? st[r] * dt_[r] : 0.f; den += st[r]; }
+    num += __shfl_xor(num, 32, 64);
+    den += __shfl_xor(den, 32, 64);
+    if (lane < 32) { sR[wid][lane] = num; sR[4 + wid][lane] = den; }
+    __syncthreads();
+    if (len <= 128) {
+      const float dn = (sR[4][qrow] + sR[5][qrow]) + (sR[6][qrow] + sR[7][qrow]);
+      if (dn > 0.f && dn < INFINITY) delta = ((sR[0][qrow] + sR[1][qrow]) + (sR[2][qrow] + sR[3][qrow])) / dn;
+    }
+    if (wid == 0 && lane < 32) {
+      sC[1][lane] = delta;
+      if (BIAS && hb.xb == 0 && qv) { p.delta[srow] = -delta; p.nl[srow] = nmc + lr; }   // for the bias gradient
+    }
+#pragma unroll
+    for (int s2 = 0; s2 < 2; s2++) {
+#pragma unroll
+      for (int r = 8 * s2; r < 8 * s2 + 8; r++) dt_[r] = st[r] != 0.f ? st[r] * (dt_[r] - delta) : 0.f;
+      const bf16x8 df = acc_to_frag(dt_, s2);
+#pragma unroll
+      for (int dt = 0; dt < DHP / 32; dt++) dq[dt] = MFMA(frag_cols<QS, 1>(sK, 0, s2, dt * 32, lane), df, dq[dt], 0, 0, 0);
     }
     __syncthreads();
     // queries on the rows, key on the lane: P and dS for dV and dK
@@ -607,26 +651,6 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
           dv[dt] = MFMA(frag_cols<QS, 1>(sG, 0, s2, dt * 32, lane), pf, dv[dt], 0, 0, 0);
           dk[dt] = MFMA(frag_cols<QS, 1>(sQ, 0, s2, dt * 32, lane), df, dk[dt], 0, 0, 0);
         }
-      }
-    }
-    // keys on the rows, query on the lane: dS for dQ
-    {
-      f32x16 s = init_tile<BIAS>(bs[0], bs[1], p.inv_scale), d = zero;
-#pragma unroll
-      for (int ks = 0; ks < DHP / 16; ks++) {
-        s = MFMA(kf[ks], qf[ks], s, 0, 0, 0);
-        d = MFMA(vf[ks], gf[ks], d, 0, 0, 0);
-      }
-#pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const float pr = BIAS && big ? fast_exp2((s[r] - m) * c) : fast_exp2(fmaf(s[r], c, nmc));
-        d[r] = key0 + wid * 32 + acc_row(r) + rowoff < len ? pr * (d[r] - delta) : 0.f;
-      }
-#pragma unroll
-      for (int s2 = 0; s2 < 2; s2++) {
-        const bf16x8 df = acc_to_frag(d, s2);
-#pragma unroll
-        for (int dt = 0; dt < DHP / 32; dt++) dq[dt] = MFMA(frag_cols<QS, 1>(sK, 0, s2, dt * 32, lane), df, dq[dt], 0, 0, 0);
       }
     }
     // dQ of the four waves, summed in their order; a lane holds d = dt*32 + 8 g + rowoff + 0..3 of its query
