@@ -180,7 +180,14 @@ def ptr(t: Optional[Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream() -> int:
+    """Handle of the current device's current stream.  Without the Stream object that torch.cuda.current_stream() makes
+    (2.9 us a call, a tenth of a one-token launch) where torch has the accessor for it."""
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 

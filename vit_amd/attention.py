@@ -89,8 +89,8 @@ def qk_norm_rope(q: Tensor, k: Optional[Tensor], q_norm_weight: Tensor, k_norm_w
     if _wants_grad(q, k, q_norm_weight, k_norm_weight, q_norm_bias, k_norm_bias):
         return ops.QkNormRopeFn.apply(q, k, q_norm_weight, k_norm_weight, q_norm_bias, k_norm_bias, *tables, float(eps),
                                       bool(use_layer_norm))
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    qo = q.new_empty(q.shape)
+    ko = None if k is None else k.new_empty(k.shape)
     K.qk_norm_rope_fwd(q, k, qo, ko, (q_norm_weight, k_norm_weight), (q_norm_bias, k_norm_bias), tables, float(eps),
                        bool(use_layer_norm))
     return qo, ko

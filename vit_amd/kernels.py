@@ -611,6 +611,9 @@ def attn_operand(t: Tensor) -> Tensor:
     return t.contiguous()
 
 
+_ST24 = C.c_int64 * 24
+
+
 def _var_strides(ts) -> "C.Array":
     vals = []
     for t in ts:
@@ -619,7 +622,7 @@ def _var_strides(ts) -> "C.Array":
         else:
             sb, ss, sh, _ = t.stride()
             vals += (sb, sh, ss)
-    return (C.c_int64 * 24)(*vals)
+    return _ST24(*vals)
 
 
 def _var_desc(q: Tensor, k: Tensor, v: Tensor, o: Tensor, stat: Tensor, table: Optional[Tensor], buckets, kv_len: Optional[Tensor],
@@ -652,8 +655,8 @@ def attn_var_fwd(q: Tensor, k: Tensor, v: Tensor, *, table: Optional[Tensor] = N
     lib = L.load()
     L.require_gpu(q, k, v, table, kv_len, None if buckets is None else buckets.index16)
     B, Lq, H, Dh = q.shape
-    o = torch.empty((B, Lq, H, Dh), dtype=q.dtype, device=q.device) if out is None else out
-    stat = torch.empty((B, H, Lq, 2), dtype=torch.float32, device=q.device)
+    o = q.new_empty((B, Lq, H, Dh)) if out is None else out
+    stat = q.new_empty((B, H, Lq, 2), dtype=torch.float32)
     a = _var_desc(q, k, v, o, stat, table, buckets, kv_len, scale, drop_p, seed, algo)
     a.st = _var_strides((q, k, v, o, None, None, None, None))
     need = lib.vitk_attn_var_workspace_bytes(C.byref(a), 0)

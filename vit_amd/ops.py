@@ -463,8 +463,8 @@ class QkNormRopeFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, qw, kw, qb, kb, table_q, table_k, eps, layernorm):
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        qo = q.new_empty(q.shape)
+        ko = None if k is None else k.new_empty(k.shape)
         K.qk_norm_rope_fwd(q, k, qo, ko, (qw, kw), (qb, kb), (table_q, table_k), eps, layernorm)
         ctx.save_for_backward(q, k, qw, kw, table_q, table_k)
         ctx.meta = (eps, layernorm, qb is not None, kb is not None)
@@ -477,11 +477,11 @@ class QkNormRopeFn(torch.autograd.Function):
         eps, layernorm, has_qb, has_kb = ctx.meta
         need = ctx.needs_input_grad
         dq = torch.zeros_like(q) if dq is None else K.attn_operand(dq)
-        gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        gq = q.new_empty(q.shape)
         gk = None
         if k is not None:
             dk = torch.zeros_like(k) if dk is None else K.attn_operand(dk)
-            gk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            gk = k.new_empty(k.shape)
         dw = K.qk_norm_rope_bwd((q, k), (dq, dk if k is not None else None), (gq, gk), (qw, kw), (table_q, table_k),
                                 eps, layernorm, (need[2], has_qb and need[4], need[3], has_kb and need[5]))
         return (gq if need[0] else None, gk if need[1] else None, dw[0], dw[2], dw[1], dw[3], None, None, None, None)
@@ -505,7 +505,7 @@ class AttentionFn(torch.autograd.Function):
         buckets, scale, drop_p, seed, table_dtype = ctx.meta
         need = ctx.needs_input_grad
         dout = K.attn_operand(dout)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = (t.new_empty(t.shape) for t in (q, k, v))
         dtab = K.attn_var_bwd(q, k, v, o, lse, dout, dq=dq, dk=dk, dv=dv, table=tab, buckets=buckets, kv_len=kv_len, scale=scale,
                               drop_p=drop_p, seed=seed, dtable_dtype=table_dtype if need[3] else None)
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtab, None, None, None, None, None)
