@@ -534,3 +534,123 @@ def test_qk_norm_rope_in_place_strided_and_wide_batches():
         for i in range(2):
             check(x[:, :, i], want[i], "in place")
         assert torch.equal(buf[..., Dh:], rest)
+
+
+# ---- variants that only some sizes reach ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("H", [1, 2, 4, 6, 8, 12])
+@pytest.mark.parametrize("B,Lq,Lk", [(5, 2, 300), (5, 140, 150), (2, 70, 1100), (1, 300, 40)])
+def test_head_counts_shares_and_key_ranges(B, Lq, Lk, H, dtype):
+    """Head counts that lay the bias out 1, 2, 4 and 8 at a time and group 1, 2 and 4 heads of few queries; samples shared out
+    in the bias gradient; key ranges shared out in the forward pass; all with counts."""
+    q, k, v, dout = make(B, Lq, Lk, H, 64, dtype, H + Lq, packed=H % 4 == 0)
+    index = torch.randint(0, 21, (Lq, Lk), generator=torch.Generator().manual_seed(H))
+    table = torch.randn(21, H, generator=torch.Generator().manual_seed(1)).to(DEV, dtype)
+    lens = [Lk, Lk // 2, 0, Lk - 1, 33][:B]
+    got = run(q, k, v, dout, 0, bias_table=table, buckets=RelativeBuckets(index, 21).to(DEV),
+              kv_lengths=torch.tensor(lens, device=DEV, dtype=torch.int32))
+    want = reference(q, k, v, 64 ** -0.5, table.double().cpu()[index].permute(2, 0, 1), lens, dout)
+    want["dtable"] = bucket_sums(*want.pop("dS"), index, 21, dtype)
+    for n, w in want.items():
+        check(got[n], w, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,Lq,Lk,H,Dh", [(1100, 1, 40, 4, 32), (1100, 1, 40, 2, 64), (4200, 1, 33, 1, 64), (64, 40, 50, 8, 32), (64, 33, 200, 8, 96)])
+def test_many_samples(B, Lq, Lk, H, Dh, dtype):
+    """Enough samples that no axis is shared out; empty, single-key and full memories among them."""
+    q, k, v, dout = make(B, Lq, Lk, H, Dh, dtype, B, packed=True)
+    lens = torch.randint(0, Lk + 1, (B,), generator=torch.Generator().manual_seed(1))
+    lens[:3] = torch.tensor([0, 1, Lk])
+    got = run(q, k, v, dout, 0, kv_lengths=lens.to(DEV))
+    want = reference(q, k, v, Dh ** -0.5, None, lens.tolist(), dout)
+    want.pop("dS")
+    for n, w in want.items():
+        check(got[n], w, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Lq", [1, 40, 70])
+def test_expanded_operands(Lq, dtype):
+    """Queries expanded over rows (a stride of 0) and over samples, keys over heads, the output's gradient over everything:
+    rows beyond the last must not be read as more of them; gradients of what was expanded are sums."""
+    B, Lk, H, Dh = 3, 90, 4, 64
+    g = torch.Generator().manual_seed(Lq)
+    q1 = torch.randn(1, 1, H, Dh, generator=g).to(DEV, dtype).requires_grad_(True)
+    k1 = torch.randn(B, Lk, 1, Dh, generator=g).to(DEV, dtype).requires_grad_(True)
+    v = torch.randn(B, Lk, H, Dh, generator=g).to(DEV, dtype).requires_grad_(True)
+    d1 = torch.randn(1, 1, 1, Dh, generator=g).to(DEV, dtype)
+    lens = [90, 41, 0]
+    o = attention(q1.expand(B, Lq, H, Dh), k1.expand(B, Lk, H, Dh), v, kv_lengths=torch.tensor(lens, device=DEV))
+    dout = d1.expand(B, Lq, H, Dh)
+    got = torch.autograd.grad(o, (q1, k1, v), dout)
+    want = reference(q1.expand(B, Lq, H, Dh), k1.expand(B, Lk, H, Dh), v, Dh ** -0.5, None, lens, dout)
+    check(o, want["o"], "o")
+    check(got[2], want["dv"], "dv")
+    u = half_step(dtype)
+    for name, x, dims in (("dq", got[0], (0, 1)), ("dk", got[1], (2,))):
+        val, bound = want[name]
+        n = math.prod(val.shape[d] for d in dims)
+        # the sum over the expanded axes is torch's, in 32 bits, rounded once
+        total = (bound + n * U * val.abs()).sum(dims, keepdim=True) + u * val.sum(dims, keepdim=True).abs()
+        check(x, (val.sum(dims, keepdim=True), total), name)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,Lq,H", [(2, 1, 2), (3, 33, 1), (2, 130, 2), (70, 1, 8)])
+def test_dropout_gradients_for_any_row_count(B, Lq, H, dtype):
+    """As above, the mask read off V = unit vectors: one query (whose rows have no stride), some, many."""
+    p = 0.25
+    q, k, _, dout = make(B, Lq, 64, H, 64, dtype, 5 + Lq, packed=Lq % 2 == 0)
+    v = torch.eye(64, device=DEV, dtype=dtype)[None, :, None].expand(B, 64, H, 64).contiguous()
+    index = torch.randint(0, 9, (Lq, 64), generator=torch.Generator().manual_seed(2))
+    table = torch.randn(9, H, device=DEV, dtype=dtype)
+    torch.cuda.manual_seed(12)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, table)]
+    o = attention(*leaves[:3], bias_table=leaves[3], buckets=RelativeBuckets(index, 9).to(DEV), dropout=p, training=True)
+    grads = torch.autograd.grad(o, leaves, dout)
+    keep = (o.detach().double().cpu().transpose(1, 2) > 0).double() / (1 - p)
+    want = reference(q, k, v, 64 ** -0.5, table.double().cpu()[index].permute(2, 0, 1), None, dout, keep=keep)
+    want["dtable"] = bucket_sums(*want.pop("dS"), index, 9, dtype)
+    for name, t in zip(("o", "dq", "dk", "dv", "dtable"), (o, *grads)):
+        check(t, want[name], name)
+
+
+@pytest.mark.parametrize("algo", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Lq", [3, 100])
+def test_gradients_of_rows_at_the_lowest_value(Lq, dtype, algo):
+    """Beside the type's lowest value the scores vanish in 32 bits: such rows weigh their keys equally, as rows of zero queries
+    without a bias do, and their gradients (but dk, which multiplies the queries) are those."""
+    B, Lk, H, Dh = 2, 150, 2, 64
+    q, k, v, dout = make(B, Lq, Lk, H, Dh, dtype, 77, packed=True)
+    table = torch.full((2, H), torch.finfo(dtype).min).to(DEV, dtype)
+    index = torch.randint(0, 2, (Lq, Lk), generator=torch.Generator().manual_seed(3))
+    lens = [150, 67]
+    got = run(q, k, v, dout, algo, bias_table=table, buckets=RelativeBuckets(index, 2).to(DEV), kv_lengths=torch.tensor(lens, device=DEV))
+    want = reference(torch.zeros_like(q), k, v, Dh ** -0.5, None, lens, dout)
+    want["dtable"] = bucket_sums(*want.pop("dS"), index, 2, dtype)
+    for n in ("o", "dq", "dv", "dtable"):
+        check(got[n], want[n], n)
+    assert torch.isfinite(got["dk"]).all()
+
+
+def test_operands_elsewhere_are_refused():
+    q, k, v, dout = make(1, 4, 6, 2, 32, torch.bfloat16, 1, packed=True)
+    plan, table = RelativeBuckets(torch.zeros(4, 6, dtype=torch.long), 1), torch.zeros(1, 2, device=DEV, dtype=torch.bfloat16)
+    for args, kw in (((q, k.cpu(), v), {}), ((q, k, v), dict(kv_lengths=torch.tensor([3]))), ((q, k, v), dict(bias_table=table, buckets=plan)),
+                     ((q, k, v), dict(bias_table=table.cpu(), buckets=plan.to(DEV)))):
+        with pytest.raises((RuntimeError, ValueError)):
+            attention(*args, **kw)
+
+
+def test_backward_twice_and_retained_graphs():
+    """The saved tensors are not written: a second backward over the same graph gives the same gradients, also after other
+    calls have used the allocator's memory."""
+    q, k, v, dout = make(2, 50, 120, 2, 64, torch.bfloat16, 41, packed=True)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    o = attention(*leaves, kv_lengths=torch.tensor([120, 9], device=DEV))
+    first = torch.autograd.grad(o, leaves, dout, retain_graph=True)
+    run(*make(4, 90, 200, 2, 64, torch.bfloat16, 1, packed=True), 0, kv_lengths=torch.tensor([200, 1, 0, 30], device=DEV))
+    for a, b in zip(first, torch.autograd.grad(o, leaves, dout)):
+        assert torch.equal(a, b)
