@@ -337,7 +337,9 @@ int vitk_qk_norm_rope_bwd(const VitkQkNormRope* a, void* stream);
  * has no key left, or only keys with a bias of -inf, gives o = 0 and zero gradients.  Finite table entries beyond
  * +-min(1e37, 1e38 scale) count as that limit.  `stat` receives two values per row that bwd takes back: the maximum the
  * exponentials were taken with, in units of 1 / scale, and -log2 of their sum (0 and -inf for a row without keys).
- * Every operand has (batch, head, row) strides of its own, d contiguous.  head_dim <= 128.
+ * Every operand has (batch, head, row) strides of its own, d contiguous.  head_dim <= 128.  Rows that repeat or overlap (a
+ * row stride below head_dim), unaligned rows and head sizes that are no multiple of 8 go to the portable kernels.
+ * bias_index values are not checked: they have to be below num_buckets.
  * bwd: dbias_table [num_buckets, H] (or NULL) is summed over the pairs of a bucket in a fixed order given by the plan
  * order / piece / bucket_piece: `order` holds the pair numbers i * Lk + j sorted by bucket, piece p covers order[piece[p]
  * .. piece[p+1]) inside one bucket, bucket n owns the pieces bucket_piece[n] .. bucket_piece[n+1).

@@ -215,3 +215,22 @@ def test_entry_points_refuse_bad_descriptors():
     assert "multiple of 8" in err(lib.vitk_qk_norm_rope_fwd(ctypes.byref(n), None)) and "null" in err(lib.vitk_qk_norm_rope_bwd(None, None))
     n.Dh = 16
     assert "null pointer" in err(lib.vitk_qk_norm_rope_fwd(ctypes.byref(n), None))
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("B,Lq,Lk", [(0, 5, 500), (3, 0, 500), (3, 5, 0), (0, 0, 0), (0, 500, 500), (1, 1, 1)])
+def test_workspace_of_empty_problems(B, Lq, Lk, dtype):
+    """Sizes of zero pass every rule that shares an axis out: no division by the count of nothing."""
+    lib = _lib.load()
+    a = _lib.VitkAttnVar()
+    a.B, a.H, a.Lq, a.Lk, a.Dh, a.scale, a.dtype = B, 2, Lq, Lk, 64, 0.125, dtype
+    fake = 1 << 12   # never followed: these calls only count bytes
+    a.q = a.k = a.v = a.o = a.stat = a.dout = a.dq = a.dk = a.dv = fake
+    for i in range(24):
+        a.st[i] = 128
+    for table in (None, fake):
+        a.bias_table = a.bias_index = a.dbias_table = a.order = a.piece = a.bucket_piece = table
+        a.num_buckets = a.num_pieces = 3
+        for bwd in (0, 1):
+            n = lib.vitk_attn_var_workspace_bytes(ctypes.byref(a), bwd)
+            assert n == 0 or bwd or B * Lq * Lk > 0

@@ -383,7 +383,7 @@ static int var_validate(const VitkAttnVar* a, bool bwd) {
 // within 32-bit byte offsets (the tiles asked for ahead of the last one included).  Rows have to follow each other: the
 // kernels find the rows beyond the last by their addresses, so expanded or overlapping rows are not for them.
 static bool var_mfma_ok(const VitkAttnVar* a, bool bwd) {
-  if (a->Dh % 8 || a->algo == 1 || a->Lk == 0) return false;
+  if (a->Dh % 8 || a->algo == 1 || a->B * a->Lq * a->Lk == 0) return false;   // (the rules below divide by their counts)
   const int es = a->dtype == VITK_BF16 ? 2 : 4;
   for (int i = 0; i < (bwd ? 24 : 12); i++)
     if (a->st[i] * es % 16 || (i % 3 == 2 && a->st[i] < a->Dh)) return false;
