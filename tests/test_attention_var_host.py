@@ -234,3 +234,18 @@ def test_workspace_of_empty_problems(B, Lq, Lk, dtype):
         for bwd in (0, 1):
             n = lib.vitk_attn_var_workspace_bytes(ctypes.byref(a), bwd)
             assert n == 0 or bwd or B * Lq * Lk > 0
+
+
+def test_plans_of_captured_graphs_are_never_dropped(monkeypatch):
+    """A model keeps its last eight plans, and every plan that a graph was captured with: replays read its memory."""
+    model = ViTConfig(in_channels=3, patch_size=(8, 8), img_size=(32, 32), depth=1, hidden_size=64, ffn_hidden_size=128,
+                      num_attention_heads=2, pos_enc="relative", dtype=torch.float32).instantiate()
+    capturing = [True]
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    first = model.prepare_buckets((1, 2))
+    capturing[0] = False
+    plans = {g: model.prepare_buckets(g) for g in [(a, b) for a in (1, 2, 3) for b in (1, 2, 3, 4)] if g != (1, 2)}
+    assert model.prepare_buckets((1, 2)) is first
+    assert model.prepare_buckets((3, 4)) is plans[(3, 4)] and model.prepare_buckets((1, 1)) is not plans[(1, 1)]
+    assert len(model._bucket_plans) <= 9

@@ -70,6 +70,8 @@ def qk_norm_rope(q: Tensor, k: Optional[Tensor], q_norm_weight: Tensor, k_norm_w
     if not eps >= 0.0:
         raise ValueError(f"vit_amd: eps must not be negative, got {eps}")
     wdt = q_norm_weight.dtype
+    q_norm_weight, k_norm_weight, q_norm_bias, k_norm_bias = (None if t is None else t.contiguous() for t in (
+        q_norm_weight, k_norm_weight, q_norm_bias, k_norm_bias))
     for name, t in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight), ("q_norm_bias", q_norm_bias),
                     ("k_norm_bias", k_norm_bias)):
         if t is not None and (tuple(t.shape) != (Dh,) or t.dtype != wdt or wdt not in _DTYPES):

@@ -44,6 +44,7 @@ class ViT(nn.Module):
         kw = {"device": device, "dtype": config.dtype}
         self._config = config
         self._bucket_plans: dict = {}   # (token grid, device) -> RelativeBuckets
+        self._captured_plans: set = set()
         D = config.hidden_size
         stem_type = PatchEmbed2d if len(config.patch_size) == 2 else PatchEmbed3d
         self.stem = stem_type(config.in_channels, D, config.patch_size, config.img_size,
@@ -83,15 +84,19 @@ class ViT(nn.Module):
         return RelativeBuckets.grid_buckets(self.stem.tokenized_size(tuple(self._config.img_size)), self._num_prefix)
 
     def prepare_buckets(self, tokenized_size: Sequence[int]) -> RelativeBuckets:
-        """Plan of the relative position bias for a token grid up to the configured one; kept per grid and device."""
+        """Plan of the relative position bias for a token grid up to the configured one; the last eight are kept per grid and
+        device, and for good what a graph being captured uses (its replays read the plan's memory)."""
         full = tuple(self.stem.tokenized_size(tuple(self._config.img_size)))
         key = (tuple(tokenized_size), self.cls_tokens.device)
         plan = self._bucket_plans.get(key)
         if plan is None:
             plan = RelativeBuckets.grid(key[0], self._num_prefix, device=key[1], table_dims=full)
-            while len(self._bucket_plans) >= 8:
-                self._bucket_plans.pop(next(iter(self._bucket_plans)))
+            old = [k for k in self._bucket_plans if k not in self._captured_plans]
+            for k in old[:max(len(old) - 7, 0)]:
+                del self._bucket_plans[k]
             self._bucket_plans[key] = plan
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            self._captured_plans.add(key)
         return plan
 
     def _layer(self, layer_type, mlp_quantization_config, qkv_quantization_config, attn_quantization_config, device, dtype, **extra):
