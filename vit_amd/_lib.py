@@ -198,15 +198,19 @@ def require_gpu(*tensors: Optional[Tensor]) -> None:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError(
-                "vit_amd: the encoder kernels run on an MI355X (ROCm) device only; got a tensor on "
-                f"'{t.device}'. There is no CPU fallback."
-            )
         if cur is None:
-            cur = torch.cuda.current_device()
-        if t.device.index != cur:
-            raise RuntimeError(
-                f"vit_amd: tensor on '{t.device}' but the current device is cuda:{cur}; kernels are launched on the "
-                "current device's stream. Call torch.cuda.set_device(...) (or run under torch.cuda.device(...)) first."
-            )
+            cur = torch.cuda.current_device() if t.is_cuda else -2
+        if t.get_device() != cur:   # -1: host memory
+            _refuse_device(t)
+
+
+def _refuse_device(t: Tensor) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(
+            "vit_amd: the encoder kernels run on an MI355X (ROCm) device only; got a tensor on "
+            f"'{t.device}'. There is no CPU fallback."
+        )
+    raise RuntimeError(
+        f"vit_amd: tensor on '{t.device}' but the current device is cuda:{torch.cuda.current_device()}; kernels are launched on the "
+        "current device's stream. Call torch.cuda.set_device(...) (or run under torch.cuda.device(...)) first."
+    )

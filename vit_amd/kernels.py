@@ -590,7 +590,7 @@ def qk_norm_rope_bwd(xs: tuple, gs: tuple, dxs: tuple, w: tuple, tables: tuple, 
     a.B, a.Dh, a.eps, a.dtype, a.w_dtype = x.shape[0], x.shape[-1], eps, L.dt(x), L.dt(w[0])
     a.is_layernorm, a.round_norm, a.emulate_bf16 = int(layernorm), int(round_norm), int(emulate_bf16)
     if any(t is not None for t in outs):
-        ws = torch.empty(lib.vitk_qk_norm_rope_workspace_bytes(C.byref(a)), dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(lib.vitk_qk_norm_rope_workspace_bytes(C.byref(a)), dtype=torch.uint8)
         a.workspace = ws.data_ptr()
     L.check(lib.vitk_qk_norm_rope_bwd(C.byref(a), L.stream()))
     return tuple(outs)
@@ -603,10 +603,11 @@ def attn_operand(t: Tensor) -> Tensor:
     """``t`` [B, L, H, Dh] as the kernels take it: d contiguous, rows that do not overlap (an expanded dimension of rows does),
     and on 16-byte boundaries where head_dim allows it (the kernels on the matrix units load 16 bytes at a time); a view that
     is not laid out so is copied once."""
-    if t.stride(3) == 1 and (t.shape[1] <= 1 or t.stride(1) >= t.shape[3]):
+    sb, ss, sh, sd = t.stride()
+    _, rows, _, Dh = t.shape
+    if sd == 1 and (ss >= Dh or rows <= 1):
         n = 16 // t.element_size()
-        sb, ss, sh, _ = t.stride()
-        if t.shape[3] % n or not (sb % n or ss % n or sh % n or t.data_ptr() % 16):
+        if Dh % n or not ((sb | ss | sh) & (n - 1) or t.data_ptr() & 15):
             return t
     return t.contiguous()
 
@@ -616,12 +617,9 @@ _ST24 = C.c_int64 * 24
 
 def _var_strides(ts) -> "C.Array":
     vals = []
-    for t in ts:
-        if t is None:
-            vals += (0, 0, 0)
-        else:
-            sb, ss, sh, _ = t.stride()
-            vals += (sb, sh, ss)
+    for t in ts:   # the rest stays zero
+        sb, ss, sh, _ = t.stride()
+        vals += (sb, sh, ss)
     return _ST24(*vals)
 
 
@@ -631,8 +629,8 @@ def _var_desc(q: Tensor, k: Tensor, v: Tensor, o: Tensor, stat: Tensor, table: O
     Lk = k.shape[1]
     assert k.shape == (B, Lk, H, Dh) == v.shape and o.shape == q.shape and q.dtype == k.dtype == v.dtype == o.dtype
     assert q.stride(3) == k.stride(3) == v.stride(3) == o.stride(3) == 1
-    a = L.VitkAttnVar()
-    a.q, a.k, a.v, a.o, a.stat = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), stat.data_ptr()
+    a = L.VitkAttnVar(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr())
+    a.stat = stat.data_ptr()
     if kv_len is not None:
         assert kv_len.dtype == torch.int32 and kv_len.is_contiguous() and kv_len.numel() == B
         a.kv_len = kv_len.data_ptr()
@@ -658,10 +656,10 @@ def attn_var_fwd(q: Tensor, k: Tensor, v: Tensor, *, table: Optional[Tensor] = N
     o = q.new_empty((B, Lq, H, Dh)) if out is None else out
     stat = q.new_empty((B, H, Lq, 2), dtype=torch.float32)
     a = _var_desc(q, k, v, o, stat, table, buckets, kv_len, scale, drop_p, seed, algo)
-    a.st = _var_strides((q, k, v, o, None, None, None, None))
+    a.st = _var_strides((q, k, v, o))
     need = lib.vitk_attn_var_workspace_bytes(C.byref(a), 0)
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(need, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     L.check(lib.vitk_attn_var_fwd(C.byref(a), L.stream()))
     return o, stat
@@ -683,12 +681,12 @@ def attn_var_bwd(q: Tensor, k: Tensor, v: Tensor, o: Tensor, stat: Tensor, dout:
     a.st = _var_strides((q, k, v, o, dout, dq, dk, dv))
     dtable = None
     if dtable_dtype is not None:
-        dtable = torch.empty(table.shape, dtype=dtable_dtype, device=q.device)
+        dtable = table.new_empty(table.shape, dtype=dtable_dtype)
         a.dbias_table, a.dbias_dtype = dtable.data_ptr(), L.dt(dtable)
         a.order, a.piece, a.bucket_piece = buckets.order.data_ptr(), buckets.piece.data_ptr(), buckets.bucket_piece.data_ptr()
     need = lib.vitk_attn_var_workspace_bytes(C.byref(a), 1)
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(need, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     L.check(lib.vitk_attn_var_bwd(C.byref(a), L.stream()))
     return dtable
