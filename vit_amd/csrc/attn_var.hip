@@ -422,13 +422,13 @@ static int var_fwd_splits(const VitkAttnVar* a) {
   if (n > tiles / 4) n = tiles / 4;
   return (int)(n < 64 ? n : 64);
 }
-// Shares of the samples in the bias gradient: float32 enough workgroups to fill the chip twice; bf16, where a workgroup
-// takes a CU for itself, as many as there are CUs at most (a 257th would run after the others).
+// Shares of the samples in the bias gradient: float32 enough workgroups to fill the chip twice; bf16, where a CU holds two (one
+// with heads beyond 96), as many as run at once at most (the next would run after the others).
 static int var_dbias_splits(const VitkAttnVar* a) {
   const bool f32 = a->dtype == VITK_F32;
-  const int rows = f32 ? 32 : a->Dh <= 96 ? 128 : 64;   // queries of a workgroup
+  const int rows = f32 ? 32 : 64;   // queries of a workgroup
   const int64_t blocks = a->H * ceil_div(a->Lq, rows) * ceil_div(a->Lk, 128);
-  int64_t n = f32 ? ceil_div(512, blocks) : 256 / blocks;
+  int64_t n = f32 ? ceil_div(512, blocks) : (a->Dh <= 96 ? 512 : 256) / blocks;
   if (n > a->B) n = a->B;
   return (int)(n < 1 ? 1 : n);
 }

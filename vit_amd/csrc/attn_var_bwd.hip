@@ -2,13 +2,13 @@
 //
 //   var_dq_k    queries stationary (32 per wave), K and V stream: S'^T and dP^T with the query on the lane, dQ^T += K^T dS^T
 //   var_dkdv_k  keys stationary, Q and dO stream: S' and dP with the key on the lane, dV^T += dO^T P, dK^T += Q^T dS
-//   var_dbias_k pairs stationary (128 x 128 per workgroup), samples stream: dS summed over the samples in the accumulators, in
+//   var_dbias_k pairs stationary (128 x 64 per workgroup), samples stream: dS summed over the samples in the accumulators, in
 //               32 bits, one 32-bit value per pair and head out; no atomics, so the sums do not depend on the order of anything
 //   var_few_bwd_k up to 32 queries: keys stationary, everything in one pass over K and V (below)
 // Times: ViT-B/14, 64 samples x 12 heads of 64, 272 x 272 with bias: dQ 62, dK/dV 72, bias gradient 61 us; ViT-g/14 at 1024 px, 4 x
-// 16 heads of 88, 5329 x 5329 with bias: 1.27, 1.55, 2.29 ms; 300 queries over up to 4096 states, 16 x 16 heads of 64: dQ 129,
+// 16 heads of 88, 5329 x 5329 with bias: 1.27, 1.55, 2.09 ms; 300 queries over up to 4096 states, 16 x 16 heads of 64: dQ 129,
 // dK/dV 184 us.  All are bound by the vector units beside the matrix units (dK/dV: 8 vector instructions and an exponential
-// for the 4 products of a pair), the bias gradient also by LDS reads and by its steps' latency: one workgroup fills a CU.
+// for the 4 products of a pair), the bias gradient also by LDS reads and by its steps' latency.
 // P is formed again from the row statistics of the forward pass; delta = rowsum(dO O) comes from var_dq_k / var_few_bwd_k.
 #include "attn_var.h"
 
@@ -388,20 +388,22 @@ __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void va
 }
 
 // ---- bias gradient: dS summed over the samples ---------------------------------------------------------------------------------
-// A workgroup owns 128 keys x 64 WQ queries of a head, 32 x 64 per wave with the key on the lane, and walks the samples of its
+// A workgroup owns 128 keys x 64 queries of a head, 32 x 64 per wave with the key on the lane, and walks the samples of its
 // share (p.splits shares); dS of every sample is added to two accumulator tiles per wave, in 32 bits, and leaves as 32-bit
 // values.  It forms S' and dP once more, 4 of the 14 products of a training pass, which costs less than writing dS (2 bytes
-// per sample, head and pair) and reading it back.  128 x 64 pairs per workgroup with the keys in registers a sample ahead
-// took 131 us at ViT-B/14, this takes 61.  A sample brings 128 rows of K and V and 64 WQ of Q and dO, all by DMA a
-// sample ahead: the former go to registers, which frees their place at once, the latter have two places.
-template <int DHP> constexpr int dbias_wq() { return DHP <= 96 ? 2 : 1; }   // 128: Q and dO of 128 queries do not fit twice
-template <int DHP, int WQ, bool DROP>
-__global__ __launch_bounds__(WQ * 256, 1) void var_dbias_k(VarP p) {
-  constexpr int T = u_tile<DHP>(), KV = 4 * T, QG = WQ * (2 * T + row_bytes<true>());   // K, V; Q and dO and the row constants
-  __shared__ __attribute__((aligned(16))) char smem[KV + 2 * QG];
+// per sample, head and pair) and reading it back.  A sample brings 128 rows of K and V and 64 of Q and dO by DMA: the former
+// go to registers, which frees their place at once for the next sample's, the latter have NB places: two, or one where two
+// would not leave room for a second workgroup on the CU, which matters more (it works while this one starts, waits or
+// stores).  ViT-B/14: 131 us with the keys in registers a sample ahead instead of LDS, 61 us so; ViT-g/14 at 1024 px, 4 samples:
+// 2.29 ms with one workgroup of 128 queries and two places, 2.09 ms with two of 64.
+template <int DHP> constexpr int dbias_nb() { return DHP == 96 ? 1 : 2; }
+template <int DHP, bool DROP>
+__global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) {
+  constexpr int NB = dbias_nb<DHP>();
+  constexpr int T = u_tile<DHP>(), KV = 4 * T, QG = 2 * T + row_bytes<true>();   // K, V; Q and dO and the row constants
+  __shared__ __attribute__((aligned(16))) char smem[KV + NB * QG];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), Dh = p.Dh;
-  const int wk = wid & 3, wq = wid >> 2;
-  const int nkb = (p.Lk + 127) / 128, nqb = (p.Lq + 64 * WQ - 1) / (64 * WQ);
+  const int nkb = (p.Lk + 127) / 128, nqb = (p.Lq + 63) / 64;
   // Neighbours: panels of up to 8 key blocks, all query blocks of a panel, then the next panel of the head (and share): the
   // workgroups that run on an XCD at a time then read few rows between them, which stay in its L2.
   const int64_t it = xcd_item(blockIdx.x, (int64_t)nkb * nqb * p.splits * p.H);
@@ -410,7 +412,7 @@ __global__ __launch_bounds__(WQ * 256, 1) void var_dbias_k(VarP p) {
   const int part = (int)(hp % p.splits), h = (int)(hp / p.splits), in = (int)(it - hp * nkb * nqb);
   const int panel = in / (8 * nqb), width = min(8, nkb - panel * 8), rest = in - panel * 8 * nqb;
   const int kb = panel * 8 + rest % width, qb = rest / width;
-  const int key0 = kb * 128, q0 = (qb * WQ + wq) * 64, krow = key0 + wk * 32 + (lane & 31);
+  const int key0 = kb * 128, q0 = qb * 64, krow = key0 + wid * 32 + (lane & 31);
   const int share = (p.B + p.splits - 1) / p.splits;
   const int b_end = min(p.B, share * (part + 1));
   const float c = p.scale * LOG2E;
@@ -418,7 +420,7 @@ __global__ __launch_bounds__(WQ * 256, 1) void var_dbias_k(VarP p) {
   const f32x16 zero = ZERO16;
   f32x16 acc[2] = {zero, zero};
   auto next_live = [&](int b) { while (b < b_end && key_count(p, b) <= key0) b++; return b; };
-  const int kt = key0 / 32 + wk;   // may lie beyond the last key tile, as the queries may: the descriptor then covers nothing
+  const int kt = key0 / 32 + wid;   // may lie beyond the last key tile, as the queries may: the descriptor then covers nothing
   const bool tile_on = kt < p.nkt_t && q0 < p.Lq;
   const __amdgpu_buffer_rsrc_t brs = __builtin_amdgcn_make_buffer_rsrc(
       (void*)(p.bias_t + (((int64_t)h * p.nkt_t + (tile_on ? kt : 0)) * p.nqt_t + (tile_on ? q0 / 32 : 0)) * 1024), 0, tile_on ? 4096 : 0, 0x00020000);
@@ -427,36 +429,35 @@ __global__ __launch_bounds__(WQ * 256, 1) void var_dbias_k(VarP p) {
   for (int i = 0; i < 4; i++) bf[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(i * 1024 + lane * 16)));
   const DropKey dkey = drop_key(p, krow);
   const uint32_t lds0 = lds_addr(smem);
-  // Four waves bring a 64-row tile: with WQ = 2 the waves of a half take one tile of each operand, with 1 all take both of K
-  // and V.  The same offsets in every sample, another descriptor.
-  const uint32_t qdst = lds0 + KV + wq * (2 * T + row_bytes<true>());
+  // the same offsets in every sample, another descriptor
+  const uint32_t qdst = lds0 + KV;
   const bf16* kh = (const bf16*)p.k + h * p.k_sh;
   const bf16* vh = (const bf16*)p.v + h * p.v_sh;
   const bf16* qh = (const bf16*)p.q + h * p.q_sh;
   const bf16* gh = (const bf16*)p.dout + h * p.g_sh;
-  TileDma<DHP, 4> ksrc = tile_dma<DHP, 4>(kh, p.k_ss, p.Lk, Dh, lds0 + wq * T, wk, lane);
-  TileDma<DHP, 4> vsrc = tile_dma<DHP, 4>(vh, p.v_ss, p.Lk, Dh, lds0 + 2 * T + wq * T, wk, lane);
-  TileDma<DHP, 4> qsrc = tile_dma<DHP, 4>(qh, p.q_ss, p.Lq, Dh, qdst, wk, lane);
-  TileDma<DHP, 4> gsrc = tile_dma<DHP, 4>(gh, p.g_ss, p.Lq, Dh, qdst + T, wk, lane);
-  RowDma rsrc = row_dma<true>(p, h * (int64_t)p.Lq, qdst + 2 * T, wk);
-  const float* rh = (wk >= 2 ? p.stat + 2 * (h * (int64_t)p.Lq) : (wk & 1 ? p.delta : p.nl) + h * (int64_t)p.Lq);
-  const uint32_t rstep = (uint32_t)(p.H * p.Lq) * (wk >= 2 ? 2u : 1u);   // floats from sample to sample
+  TileDma<DHP, 4> ksrc = tile_dma<DHP, 4>(kh, p.k_ss, p.Lk, Dh, lds0, wid, lane);
+  TileDma<DHP, 4> vsrc = tile_dma<DHP, 4>(vh, p.v_ss, p.Lk, Dh, lds0 + 2 * T, wid, lane);
+  TileDma<DHP, 4> qsrc = tile_dma<DHP, 4>(qh, p.q_ss, p.Lq, Dh, qdst, wid, lane);
+  TileDma<DHP, 4> gsrc = tile_dma<DHP, 4>(gh, p.g_ss, p.Lq, Dh, qdst + T, wid, lane);
+  RowDma rsrc = row_dma<true>(p, h * (int64_t)p.Lq, qdst + 2 * T, wid);
+  const float* rh = (wid >= 2 ? p.stat + 2 * (h * (int64_t)p.Lq) : (wid & 1 ? p.delta : p.nl) + h * (int64_t)p.Lq);
+  const uint32_t rstep = (uint32_t)(p.H * p.Lq) * (wid >= 2 ? 2u : 1u);   // floats from sample to sample
   auto request_keys = [&](int b) {
     const int len = key_count(p, b);
     ksrc.rs = rows_rsrc(kh + (uint32_t)b * p.k_sb, p.k_ss, len, Dh);
     vsrc.rs = rows_rsrc(vh + (uint32_t)b * p.v_sb, p.v_ss, len, Dh);
     ksrc.last = vsrc.last = (len - 1) >> 6;
 #pragma unroll
-    for (int i = 0; i < 2 / WQ; i++) {
-      tile_request(ksrc, kb * 2 + wq + i, i * T);
-      tile_request(vsrc, kb * 2 + wq + i, i * T);
+    for (int i = 0; i < 2; i++) {
+      tile_request(ksrc, kb * 2 + i, i * T);
+      tile_request(vsrc, kb * 2 + i, i * T);
     }
   };
   auto request_rows = [&](int b, int buf) {
     qsrc.rs = rows_rsrc(qh + (uint32_t)b * p.q_sb, p.q_ss, p.Lq, Dh);
     gsrc.rs = rows_rsrc(gh + (uint32_t)b * p.g_sb, p.g_ss, p.Lq, Dh);
-    tile_request(qsrc, qb * WQ + wq, buf * QG);
-    tile_request(gsrc, qb * WQ + wq, buf * QG);
+    tile_request(qsrc, qb, buf * QG);
+    tile_request(gsrc, qb, buf * QG);
     rsrc.rs = __builtin_amdgcn_make_buffer_rsrc((void*)(rh + (uint64_t)(uint32_t)b * rstep), 0, p.Lq * (int)rsrc.row_bytes, 0x00020000);
     row_request(rsrc, q0, buf * QG, lane);
   };
@@ -467,24 +468,24 @@ __global__ __launch_bounds__(WQ * 256, 1) void var_dbias_k(VarP p) {
   }
   while (b < b_end) {
     const int len = key_count(p, b), bn = next_live(b + 1);
-    const bool wave_on = q0 < p.Lq && key0 + wk * 32 < len, whole = key0 + wk * 32 + 32 <= len, live = krow < len;
+    const bool wave_on = q0 < p.Lq && key0 + wid * 32 < len, whole = key0 + wid * 32 + 32 <= len, live = krow < len;
     const int64_t bh = (int64_t)b * p.H + h;
     u_wait<0>();
     __syncthreads();
     bf16x8 kf[DHP / 16], vf[DHP / 16];
     {
-      const char* sK = smem + (wk >> 1) * T;
+      const char* sK = smem + (wid >> 1) * T;
 #pragma unroll
       for (int ks = 0; ks < DHP / 16; ks++) {
-        kf[ks] = u_rows<DHP>(sK, (wk & 1) * 32, ks, lane);
-        vf[ks] = u_rows<DHP>(sK + 2 * T, (wk & 1) * 32, ks, lane);
+        kf[ks] = u_rows<DHP>(sK, (wid & 1) * 32, ks, lane);
+        vf[ks] = u_rows<DHP>(sK + 2 * T, (wid & 1) * 32, ks, lane);
       }
     }
-    if (bn < b_end) request_rows(bn, buf ^ 1);
+    if (NB == 2 && bn < b_end) request_rows(bn, buf ^ 1);
     __syncthreads();   // every wave has its keys and values
     if (bn < b_end) request_keys(bn);
     if (wave_on) {
-      const char* sQ = smem + KV + buf * QG + wq * (2 * T + row_bytes<true>());
+      const char* sQ = smem + KV + buf * QG;
       const char* sG = sQ + T;
       const float* sL = (const float*)(sQ + 2 * T);
       const uint32_t xkey = DROP ? drop_xkey(p, dkey, bh * p.Lq + q0, rowoff) : 0u;
@@ -506,7 +507,11 @@ __global__ __launch_bounds__(WQ * 256, 1) void var_dbias_k(VarP p) {
         }
       }
     }
-    buf ^= 1;
+    if (NB == 2) buf ^= 1;
+    else {
+      __syncthreads();
+      if (bn < b_end) request_rows(bn, 0);
+    }
     b = bn;
   }
   if (krow >= p.Lk) return;
@@ -722,9 +727,8 @@ template <int DHP, bool BIAS> static void dkdv_dh(const VarP& p, hipStream_t st)
   else hipLaunchKernelGGL((var_dkdv_k<DHP, 4, BIAS, false>), grid, dim3(256), 0, st, p);
 }
 template <int DHP, bool DROP> static void dbias_dh(const VarP& p, hipStream_t st) {
-  constexpr int WQ = dbias_wq<DHP>();
-  const dim3 grid(xcd_grid(ceil_div(p.Lk, 128) * ceil_div(p.Lq, 64 * WQ) * p.splits * p.H));
-  hipLaunchKernelGGL((var_dbias_k<DHP, WQ, DROP>), grid, dim3(WQ * 256), 0, st, p);
+  const dim3 grid(xcd_grid(ceil_div(p.Lk, 128) * ceil_div(p.Lq, 64) * p.splits * p.H));
+  hipLaunchKernelGGL((var_dbias_k<DHP, DROP>), grid, dim3(256), 0, st, p);
 }
 template <int DHP, bool BIAS> static void few_dh(const VarP& p, hipStream_t st) {
   hipLaunchKernelGGL((var_few_bwd_k<DHP, BIAS>), dim3(var_grid<BIAS>(p, p.Lk, 128)), dim3(256), 0, st, p);
