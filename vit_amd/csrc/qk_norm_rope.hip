@@ -11,7 +11,7 @@
 // row sums go through LDS.  Positions come before samples in a wave's run: their sines and cosines stay in registers.
 // Bound by HBM: x in, y out (forward), g and x in, dx out (backward).  Measured in bf16: ViT-H/14 at 224 px, 64 samples, 16 + 16
 // heads of 80: forward 36 us (4.7 TB/s), backward 71 us (3.6 TB/s; the reads of two tensors in one pass and the weight-gradient
-// sums); ViT-g/14 at 1024 px, 8 samples, heads of 88: 128 us (3.8 TB/s) and 202 us (3.6 TB/s), where a copy reaches 5.1 TB/s.
+// sums); ViT-g/14 at 1024 px, 8 samples, heads of 88: 128-134 us (3.7 TB/s) and 202-209 us (3.5 TB/s), where a copy reaches 5.1 TB/s.
 // One token of 12 + 12 heads takes 4 us, a launch.
 #include "common.h"
 
