@@ -115,57 +115,62 @@ __global__ __launch_bounds__(256, 4) void qk_norm_rope_k(QkP p) {
     }
     return t;
   };
-  // A wave takes a run of tokens, the samples of a position one after the other, and of a token rpw heads at a time: the
-  // token's addresses are scalars, a lane only adds its head and position in it.
-  const int64_t tokens = (int64_t)p.B * s.L, nw = (int64_t)gridDim.x * 4, run = (tokens + nw - 1) / nw;
-  const int64_t t0 = run * ((int64_t)blockIdx.x * 4 + wid), t1 = t0 + run < tokens ? t0 + run : tokens;
-  if (t0 < t1) {
-    int l = (int)(t0 / p.B), b = (int)(t0 - (int64_t)l * p.B), u = 0, table_l = -1;
-    const int nu = (H + rpw - 1) / rpw;
-    // Addresses move by three fixed steps: to the next heads of a token, to the next sample, to the next position
-    const int64_t xu = (int64_t)rpw * s.x_sh, yu = (int64_t)rpw * s.y_sh, gu = BWD ? (int64_t)rpw * s.g_sh : 0;
-    const int64_t xb = s.x_sb - (nu - 1) * xu, yb = s.y_sb - (nu - 1) * yu, gb_ = BWD ? s.g_sb - (nu - 1) * gu : 0;
-    const int64_t xl = s.x_ss - (p.B - 1) * s.x_sb - (nu - 1) * xu, yl = s.y_ss - (p.B - 1) * s.y_sb - (nu - 1) * yu;
-    const int64_t gl = BWD ? s.g_ss - (p.B - 1) * s.g_sb - (nu - 1) * gu : 0;
-    const T* xp = (const T*)s.x + b * s.x_sb + (int64_t)l * s.x_ss;
-    const T* gp = BWD ? (const T*)s.g + b * s.g_sb + (int64_t)l * s.g_ss : nullptr;
-    T* yp = (T*)s.y + b * s.y_sb + (int64_t)l * s.y_ss;
-    const int xo = rr * (int)s.x_sh + d0, go = BWD ? rr * (int)s.g_sh + d0 : 0, yo = rr * (int)s.y_sh + d0;
+  // Rows in the order position, sample, head: a wave takes a run of them, rpw at a time, so that all its lanes but those that
+  // no row fits in are busy (16 heads of 88 taken token by token: 5 + 5 + 5 + 1 of 5).  A row's place moves by a fixed step,
+  // corrected where the heads or the samples wrap; its sines and cosines stay until the position changes.
+  const int64_t rows = (int64_t)p.B * s.L * H, nw = (int64_t)gridDim.x * 4;
+  const int64_t run = ((rows + nw - 1) / nw + rpw - 1) / rpw * rpw;
+  const int64_t r0 = run * ((int64_t)blockIdx.x * 4 + wid), r1 = r0 + run < rows ? r0 + run : rows;
+  if (r0 < r1) {
+    const int B = p.B, step_t = rpw / H, sh = rpw - step_t * H, sl = step_t / B, sb = step_t - sl * B;   // rpw rows further
+    const int64_t xs = sl * s.x_ss + sb * s.x_sb + sh * s.x_sh, ys = sl * s.y_ss + sb * s.y_sb + sh * s.y_sh;
+    const int64_t xb = s.x_sb - H * s.x_sh, yb = s.y_sb - H * s.y_sh, xl = s.x_ss - B * s.x_sb, yl = s.y_ss - B * s.y_sb;
+    const int64_t gs = BWD ? sl * s.g_ss + sb * s.g_sb + sh * s.g_sh : 0, gb_ = BWD ? s.g_sb - H * s.g_sh : 0, gl = BWD ? s.g_ss - B * s.g_sb : 0;
+    const int64_t first = r0 + rr;
+    int64_t t = first / H;
+    int h = (int)(first - t * H), l = (int)(t / B), b = (int)(t - (int64_t)l * B), table_l = -1;
+    const T* xp = (const T*)s.x + b * s.x_sb + l * s.x_ss + h * s.x_sh + d0;
+    const T* gp = BWD ? (const T*)s.g + b * s.g_sb + l * s.g_ss + h * s.g_sh + d0 : nullptr;
+    T* yp = (T*)s.y + b * s.y_sb + l * s.y_ss + h * s.y_sh + d0;
     const float* table = s.table;
     const int64_t tok_stride = s.tok_stride, cos_off = s.cos_off;
-    const int prefix = s.prefix, B = p.B;
+    const int prefix = s.prefix;
     const bool ln = p.ln;
     const float eps = p.eps;
-    auto fetch = [&](Raw8<T>& xr, Raw8<T>& gr, int u) {
-      if (on && u * rpw + rr < H) {
-        xr = load8<T>(xp + xo);
-        if (BWD) gr = load8<T>(gp + go);
+    int left = on ? (int)min((int64_t)INT32_MAX, r1 - first) : 0;   // rows from the lane's on: none left where not above 0
+    auto fetch = [&](Raw8<T>& xr, Raw8<T>& gr) {
+      if (left > 0) {
+        xr = load8<T>(xp);
+        if (BWD) gr = load8<T>(gp);
       }
     };
     float sn[8], cs[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) { sn[i] = 0.f; cs[i] = 1.f; }
     Raw8<T> xr = {}, gr = {};
-    fetch(xr, gr, 0);
-    for (int64_t left = (t1 - t0) * nu; left > 0; left--) {
-      const int lc = l, bc = b, uc = u;
+    fetch(xr, gr);
+    for (int64_t n = r1 - r0; n > 0; n -= rpw) {
+      const int lc = l, bc = b;
+      const bool live = left > 0;
       float x[8], g[8];
       unpack8<T>(x, xr);
       if (BWD) unpack8<T>(g, gr);
       T* const yc = yp;
-      if (++u < nu) {
-        xp += xu; yp += yu;
-        if (BWD) gp += gu;
-      } else {
-        u = 0;
-        const bool same = ++b < B;
-        if (!same) { b = 0; l++; }
-        xp += same ? xb : xl; yp += same ? yb : yl;
-        if (BWD) gp += same ? gb_ : gl;
+      h += sh; b += sb; l += sl; left -= rpw;
+      xp += xs; yp += ys;
+      if (BWD) gp += gs;
+      if (h >= H) {
+        h -= H; b++;
+        xp += xb; yp += yb;
+        if (BWD) gp += gb_;
       }
-      if (left > 1) fetch(xr, gr, u);   // the next heads are asked for before these are worked on
-      const bool live = on && uc * rpw + rr < H;
-      const bool rot = has_table && lc >= prefix;
+      if (b >= B) {
+        b -= B; l++;
+        xp += xl; yp += yl;
+        if (BWD) gp += gl;
+      }
+      fetch(xr, gr);   // the next rows are asked for before these are worked on
+      const bool rot = has_table && lc >= prefix && live;
       if (rot && (lc != table_l || tok_stride)) {
         const float* tp = table + bc * tok_stride + (int64_t)(lc - prefix) * Dh + (on ? d0 : 0);
         *(float4*)sn = *(const float4*)tp; *(float4*)(sn + 4) = *(const float4*)(tp + 4);
@@ -207,7 +212,7 @@ __global__ __launch_bounds__(256, 4) void qk_norm_rope_k(QkP p) {
 #pragma unroll
           for (int i = 0; i < 8; i++) y[i] = SEP ? rope_mix(y[i], cs[i], o[i], sn[i], p.emu) : fmaf(y[i], cs[i], o[i] * sn[i]);
         }
-        if (live) store8<T>(yc + yo, y);
+        if (live) store8<T>(yc, y);
       } else {
         if (rot) {   // the transposed rotation: the partner sends g sin
           float t[8], o[8];
@@ -247,7 +252,7 @@ __global__ __launch_bounds__(256, 4) void qk_norm_rope_k(QkP p) {
         c = ln ? row_sum(c) * inv_n : 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++) g[i] = (fmaf(-x[i], a, g[i]) - c) * rstd;
-        if (live) store8<T>(yc + yo, g);
+        if (live) store8<T>(yc, g);
       }
     }
   }
