@@ -9,10 +9,10 @@
 // two passes.  A lane holds 8 consecutive values of a head (16 bytes in bf16), a wave as many whole rows as fit, so that its
 // loads and stores are one contiguous run where the rows are; the other half of the head that the rotation needs and the
 // row sums go through LDS.  Positions come before samples in a wave's run: their sines and cosines stay in registers.
-// Bound by HBM: x in, y out (forward), g and x in, dx out (backward).  Measured in bf16: ViT-H/14 at 224 px, 64 samples, 16 + 16
-// heads of 80: forward 36 us (4.7 TB/s), backward 71 us (3.6 TB/s; the reads of two tensors in one pass and the weight-gradient
-// sums); ViT-g/14 at 1024 px, 8 samples, heads of 88: 128-134 us (3.7 TB/s) and 202-209 us (3.5 TB/s), where a copy reaches 5.1 TB/s.
-// One token of 12 + 12 heads takes 4 us, a launch.
+// Bound by HBM: x in, y out (forward), g and x in, dx out (backward; its vector instructions come close).  Measured in bf16:
+// ViT-H/14 at 224 px, 64 samples, 16 + 16 heads of 80: forward 36 us (4.7 TB/s), backward 58 us (4.3 TB/s); ViT-g/14 at 1024 px, 8
+// samples, heads of 88: 102 us (4.7 TB/s) and 179 us (4.0 TB/s), where a copy reaches 5.1 TB/s; the weight gradients' partial
+// sums take 4-5 us more.  One token of 12 + 12 heads takes 4 us, a launch.
 #include "common.h"
 
 struct QkSec {        // one section: q or k
@@ -304,7 +304,9 @@ static int qk_blocks(const VitkQkNormRope* a, bool bwd) {
   int64_t tok = a->sec[0].L * a->B;
   if (a->sec[1].w && a->sec[1].L * a->B > tok) tok = a->sec[1].L * a->B;
   const int64_t want = ceil_div(tok, 4);
-  const int64_t cap = bwd ? 1024 : 2048;   // 4 or 8 workgroups per CU; backward: one partial row per workgroup
+  // As many workgroups of both sections as run at once (4 or 6 per CU), each with a longer run of rows: with twice as many, in
+  // two rounds, ViT-g/14 at 1024 px takes 111 / 188 us in place of 102 / 179.  Backward: a partial sum per workgroup.
+  const int64_t cap = (bwd ? 1024 : 1536) / (a->sec[1].w ? 2 : 1);
   return (int)(want < cap ? (want < 1 ? 1 : want) : cap);
 }
 extern "C" size_t vitk_qk_norm_rope_workspace_bytes(const VitkQkNormRope* a) {
