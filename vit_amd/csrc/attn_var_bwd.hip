@@ -628,10 +628,18 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
 #pragma unroll
     for (int s2 = 0; s2 < 2; s2++) {
 #pragma unroll
-      for (int r = 8 * s2; r < 8 * s2 + 8; r++) dt_[r] = st[r] != 0.f ? st[r] * (dt_[r] - delta) : 0.f;
-      const bf16x8 df = acc_to_frag(dt_, s2);
+      for (int r = 8 * s2; r < 8 * s2 + 8; r++) {
+        dt_[r] = st[r] != 0.f ? st[r] * (dt_[r] - delta) : 0.f;
+        st[r] = dt_[r] - (float)(bf16)dt_[r];
+      }
+      // dS as two bf16 operands, value and rest: the matrix units have time here, and dQ, a handful of rows, keeps its bits
+      const bf16x8 df = acc_to_frag(dt_, s2), dr = acc_to_frag(st, s2);
 #pragma unroll
-      for (int dt = 0; dt < DHP / 32; dt++) dq[dt] = MFMA(frag_cols<QS, 1>(sK, 0, s2, dt * 32, lane), df, dq[dt], 0, 0, 0);
+      for (int dt = 0; dt < DHP / 32; dt++) {
+        const bf16x8 kc = frag_cols<QS, 1>(sK, 0, s2, dt * 32, lane);
+        dq[dt] = MFMA(kc, df, dq[dt], 0, 0, 0);
+        dq[dt] = MFMA(kc, dr, dq[dt], 0, 0, 0);
+      }
     }
     __syncthreads();
     // queries on the rows, key on the lane: P and dS for dV and dK
