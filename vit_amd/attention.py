@@ -70,12 +70,16 @@ def qk_norm_rope(q: Tensor, k: Optional[Tensor], q_norm_weight: Tensor, k_norm_w
     if not eps >= 0.0:
         raise ValueError(f"vit_amd: eps must not be negative, got {eps}")
     wdt = q_norm_weight.dtype
-    q_norm_weight, k_norm_weight, q_norm_bias, k_norm_bias = (None if t is None else t.contiguous() for t in (
-        q_norm_weight, k_norm_weight, q_norm_bias, k_norm_bias))
-    for name, t in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight), ("q_norm_bias", q_norm_bias),
-                    ("k_norm_bias", k_norm_bias)):
-        if t is not None and (tuple(t.shape) != (Dh,) or t.dtype != wdt or wdt not in _DTYPES):
+    params = [q_norm_weight, k_norm_weight, q_norm_bias, k_norm_bias]
+    for i, t in enumerate(params):
+        if t is None:
+            continue
+        if t.shape != (Dh,) or t.dtype != wdt or wdt not in _DTYPES:
+            name = ("q_norm_weight", "k_norm_weight", "q_norm_bias", "k_norm_bias")[i]
             raise ValueError(f"vit_amd: {name} must be [{Dh}] {wdt} (float32 or bfloat16), got {tuple(t.shape)} {t.dtype}")
+        if not t.is_contiguous():
+            params[i] = t.contiguous()
+    q_norm_weight, k_norm_weight, q_norm_bias, k_norm_bias = params
     tables = []
     for name, x, rope in (("rope_q", q, rope_q), ("rope_k", k, rope_k)):
         if rope is None or x is None:
@@ -83,7 +87,7 @@ def qk_norm_rope(q: Tensor, k: Optional[Tensor], q_norm_weight: Tensor, k_norm_w
             continue
         B, Ln = x.shape[0], x.shape[1]
         n = rope.shape[-2] if rope.dim() >= 2 else -1
-        if tuple(rope.shape) not in ((2, n, Dh), (2, B, 1, n, Dh)) or n > Ln:
+        if (rope.shape != (2, n, Dh) and rope.shape != (2, B, 1, n, Dh)) or n > Ln:
             raise ValueError(f"vit_amd: {name} must be [2, N, {Dh}] or [2, {B}, 1, N, {Dh}] with N <= {Ln}, got {tuple(rope.shape)}")
         tables.append(rope if rope.dim() == 3 and rope.dtype == torch.float32 and rope.is_contiguous() and not rope.requires_grad
                       else ops._rope_table(rope, None, B, B, q.dtype)[0])
@@ -94,7 +98,7 @@ def qk_norm_rope(q: Tensor, k: Optional[Tensor], q_norm_weight: Tensor, k_norm_w
     qo = q.new_empty(q.shape)
     ko = None if k is None else k.new_empty(k.shape)
     K.qk_norm_rope_fwd(q, k, qo, ko, (q_norm_weight, k_norm_weight), (q_norm_bias, k_norm_bias), tables, float(eps),
-                       bool(use_layer_norm))
+                       bool(use_layer_norm), checked=True)
     return qo, ko
 
 

@@ -537,7 +537,10 @@ def _qk_section(sec: L.VitkQkSection, x: Tensor, g: Optional[Tensor], y: Tensor,
     if g is not None:
         sec.g = g.data_ptr()
         sec.g_sb, sec.g_ss, sec.g_sh, _ = g.stride()
-    sec.dw, sec.db = L.ptr(dw), L.ptr(db)
+    if dw is not None:
+        sec.dw = dw.data_ptr()
+    if db is not None:
+        sec.db = db.data_ptr()
     sec.L, sec.H = Ln, H
     if table is not None:   # fp32 [2, N, Dh] or [2, B, N, Dh], contiguous (ops._rope_table)
         sec.table, sec.prefix, sec.per_sample = table.data_ptr(), Ln - table.shape[-2], int(table.dim() == 4)
@@ -556,16 +559,19 @@ def _qk_check(x: Tensor, w: Tensor, b: Optional[Tensor], table: Optional[Tensor]
 
 
 def qk_norm_rope_fwd(q: Tensor, k: Optional[Tensor], q_out: Tensor, k_out: Optional[Tensor], w: tuple, b: tuple, tables: tuple,
-                     eps: float, layernorm: bool, round_norm: bool = False, emulate_bf16: bool = False) -> None:
+                     eps: float, layernorm: bool, round_norm: bool = False, emulate_bf16: bool = False,
+                     checked: bool = False) -> None:
     """q [B, Lq, H, Dh] (and k [B, Lk, Hk, Dh]) -> q_out, k_out, same shapes, any strides with d contiguous: every head
-    normalised, scaled by w = (w_q, w_k), shifted by b, and rotated with tables = (table_q, table_k)."""
+    normalised, scaled by w = (w_q, w_k), shifted by b, and rotated with tables = (table_q, table_k).  ``checked``: the caller
+    has looked at shapes, types and layouts."""
     lib = L.load()
     L.require_gpu(q, k, q_out, k_out, *w, *b, *tables)
     a = L.VitkQkNormRope()
     for i, (x, y) in enumerate(((q, q_out), (k, k_out))):
         if x is not None:
-            _qk_check(x, w[i], b[i], tables[i])
-            assert y.dtype == x.dtype == q.dtype and y.shape == x.shape and y.stride(-1) == 1
+            if not checked:
+                _qk_check(x, w[i], b[i], tables[i])
+                assert y.dtype == x.dtype == q.dtype and y.shape == x.shape and y.stride(-1) == 1
             _qk_section(a.sec[i], x, None, y, w[i], b[i], None, None, tables[i])
     a.B, a.Dh, a.eps, a.dtype, a.w_dtype = q.shape[0], q.shape[-1], eps, L.dt(q), L.dt(w[0])
     a.is_layernorm, a.round_norm, a.emulate_bf16 = int(layernorm), int(round_norm), int(emulate_bf16)

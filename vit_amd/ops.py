@@ -465,7 +465,7 @@ class QkNormRopeFn(torch.autograd.Function):
     def forward(ctx, q, k, qw, kw, qb, kb, table_q, table_k, eps, layernorm):
         qo = q.new_empty(q.shape)
         ko = None if k is None else k.new_empty(k.shape)
-        K.qk_norm_rope_fwd(q, k, qo, ko, (qw, kw), (qb, kb), (table_q, table_k), eps, layernorm)
+        K.qk_norm_rope_fwd(q, k, qo, ko, (qw, kw), (qb, kb), (table_q, table_k), eps, layernorm, checked=True)
         ctx.save_for_backward(q, k, qw, kw, table_q, table_k)
         ctx.meta = (eps, layernorm, qb is not None, kb is not None)
         return qo, ko
