@@ -23,16 +23,16 @@ __device__ __forceinline__ f32x16 init_tile(const bf16x8& lo, const bf16x8& hi, 
 }
 
 // ---- dQ -----------------------------------------------------------------------------------------------------------------
-template <int DHP, int HALVES, bool PARTIAL, bool BIAS, bool DROP>
+// WHOLE: the tile holds all keys of the rows, and delta = sum P dP / sum P replaces rowsum(dO O), whose rounding is much of what
+// dS is made of when the keys are few (5 keys: error of dq 3.0e-3, 2.4e-3 so).
+template <int DHP, int HALVES, bool PARTIAL, bool BIAS, bool DROP, bool WHOLE = false>
 __device__ __forceinline__ void var_dq_tile(const VarP& p, const char* sK, const char* sV, const bf16x8 (&qf)[DHP / 16],
                                             const bf16x8 (&gf)[DHP / 16], f32x16 (&sacc)[HALVES], f32x16 (&dqacc)[DHP / 32],
-                                            float m, float nmc, bool big, float delta, float& dsum, float c, int k0, int len,
+                                            float m, float nmc, bool big, float& delta, float& dsum, float c, int k0, int len,
                                             uint32_t xrow, int lane) {
   const f32x16 zero = ZERO16;
   const int rowoff = 4 * (lane >> 5);
-#pragma unroll
-  for (int st = 0; st < HALVES; st++) {
-    f32x16 pacc = zero;
+  auto scores = [&](int st, f32x16& pacc) {   // P in sacc, dP (dropout applied) in pacc
 #pragma unroll
     for (int ks = 0; ks < DHP / 16; ks++) {
       sacc[st] = MFMA(u_rows<DHP>(sK, st * 32, ks, lane), qf[ks], sacc[st], 0, 0, 0);
@@ -52,13 +52,14 @@ __device__ __forceinline__ void var_dq_tile(const VarP& p, const char* sK, const
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const int r = 4 * g + j;
-        float pr = sacc[st][r];
-        if (PARTIAL && st == HALVES - 1) pr = k0 + st * 32 + acc_row(r) + rowoff < len ? pr : 0.f;
-        float dp = pacc[r];
-        if (DROP) dp = dr[j] >= p.thr ? dp * p.keep_scale : 0.f;
-        sacc[st][r] = pr * (dp - delta);
+        if (PARTIAL && st == HALVES - 1) sacc[st][r] = k0 + st * 32 + acc_row(r) + rowoff < len ? sacc[st][r] : 0.f;
+        if (DROP) pacc[r] = dr[j] >= p.thr ? pacc[r] * p.keep_scale : 0.f;
       }
     }
+  };
+  auto grads = [&](int st, const f32x16& pacc) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) sacc[st][r] *= pacc[r] - delta;
     // dS is rounded to bf16 to be an operand (half a step, 2^-8); its row factor 1 / sum is applied to the 32-bit result
 #pragma unroll
     for (int s2 = 0; s2 < 2; s2++) {
@@ -66,10 +67,33 @@ __device__ __forceinline__ void var_dq_tile(const VarP& p, const char* sK, const
 #pragma unroll
       for (int dt = 0; dt < DHP / 32; dt++)
         dqacc[dt] = MFMA(u_cols<DHP>(sK, st * 32, s2, dt * 32, lane), df, dqacc[dt], 0, 0, 0);
-      if (BIAS) {
+      if (BIAS && !WHOLE) {
 #pragma unroll
         for (int r = 8 * s2; r < 8 * s2 + 8; r += 2) dsum += sacc[st][r] + sacc[st][r + 1];
       }
+    }
+  };
+  if constexpr (WHOLE) {
+    f32x16 pacc[HALVES];
+    float num = 0.f, den = 0.f;
+#pragma unroll
+    for (int st = 0; st < HALVES; st++) {
+      pacc[st] = zero;
+      scores(st, pacc[st]);
+#pragma unroll
+      for (int r = 0; r < 16; r++) { num = fmaf(sacc[st][r], pacc[st][r], num); den += sacc[st][r]; }
+    }
+    num += __shfl_xor(num, 32, 64);
+    den += __shfl_xor(den, 32, 64);
+    if (den > 0.f && den < INFINITY) delta = num / den;
+#pragma unroll
+    for (int st = 0; st < HALVES; st++) grads(st, pacc[st]);
+  } else {
+#pragma unroll
+    for (int st = 0; st < HALVES; st++) {
+      f32x16 pacc = zero;
+      scores(st, pacc);
+      grads(st, pacc);
     }
   }
 }
@@ -135,7 +159,8 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
   u_wait<NB == 3 ? REQ : 0>();   // the stores above are in the count as well: a longer wait, never a shorter one
   __syncthreads();
   int buf = 0;
-  for (int t = 0; t < nfull; t++) {
+  const bool whole = ntiles == 1;
+  for (int t = 0; t < nfull && !whole; t++) {
     const char* sK = smem + buf * TILE;
     const int ahead = NB == 3 ? (buf == 0 ? 2 : buf - 1) : buf ^ 1;
     f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
@@ -146,7 +171,15 @@ __global__ __launch_bounds__(NW * 64, (var_dq_occ<DHP, BIAS, DROP>())) void var_
     __syncthreads();
     buf = buf + 1 == NB ? 0 : buf + 1;
   }
-  if (nfull < ntiles && wave_on) {
+  if (whole && wave_on) {
+    if (len > 32) {
+      f32x16 sacc[2] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale), init_tile<BIAS>(bf[2], bf[3], p.inv_scale)};
+      var_dq_tile<DHP, 2, true, BIAS, DROP, true>(p, smem, smem + u_tile<DHP>(), qf, gf, sacc, dqacc, m, nmc, big, delta, dsum, c, 0, len, rbase, lane);
+    } else {
+      f32x16 sacc[1] = {init_tile<BIAS>(bf[0], bf[1], p.inv_scale)};
+      var_dq_tile<DHP, 1, true, BIAS, DROP, true>(p, smem, smem + u_tile<DHP>(), qf, gf, sacc, dqacc, m, nmc, big, delta, dsum, c, 0, len, rbase, lane);
+    }
+  } else if (nfull < ntiles && wave_on) {
     const char* sK = smem + buf * TILE;
     const char* sV = sK + u_tile<DHP>();
     if (len - nfull * 64 > 32) {
@@ -526,7 +559,7 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
 }
 
 // ---- up to 32 queries -------------------------------------------------------------------------------------------------------------
-// Bound by K, V in and dK, dV out (256 samples x 12 heads of 64, one query over up to 272 states: 89 us for 320 MB, 3.6 TB/s), so
+// Bound by K, V in and dK, dV out (256 samples x 12 heads of 64, one query over up to 272 states: 91 us for 320 MB, 3.5 TB/s), so
 // K and V are read once: a wave holds 32 keys, forms S' and dP both ways (the query rows'
 // fragments serve as either operand), and writes dK, dV of its keys; dQ^T += K^T dS^T of the workgroup's 128 keys goes to
 // p.part and is summed over the key blocks, in their order, by var_few_sum_k.
@@ -632,7 +665,8 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
         dt_[r] = st[r] != 0.f ? st[r] * (dt_[r] - delta) : 0.f;
         st[r] = dt_[r] - (float)(bf16)dt_[r];
       }
-      // dS as two bf16 operands, value and rest: the matrix units have time here, and dQ, a handful of rows, keeps its bits
+      // dS (P and dS below) as two bf16 operands, value and rest: the matrix units have time here, and the gradients keep the
+      // bits of 32-bit arithmetic up to their own rounding (88 -> 92 us at the case above)
       const bf16x8 df = acc_to_frag(dt_, s2), dr = acc_to_frag(st, s2);
 #pragma unroll
       for (int dt = 0; dt < DHP / 32; dt++) {
@@ -666,9 +700,15 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_few_bwd_k(VarP p
       for (int s2 = 0; s2 < 2; s2++) {
         const bf16x8 pf = acc_to_frag(s, s2), df = acc_to_frag(d, s2);
 #pragma unroll
+        for (int r = 8 * s2; r < 8 * s2 + 8; r++) { s[r] -= (float)(bf16)s[r]; d[r] -= (float)(bf16)d[r]; }
+        const bf16x8 pr = acc_to_frag(s, s2), dr = acc_to_frag(d, s2);
+#pragma unroll
         for (int dt = 0; dt < DHP / 32; dt++) {
-          dv[dt] = MFMA(frag_cols<QS, 1>(sG, 0, s2, dt * 32, lane), pf, dv[dt], 0, 0, 0);
-          dk[dt] = MFMA(frag_cols<QS, 1>(sQ, 0, s2, dt * 32, lane), df, dk[dt], 0, 0, 0);
+          const bf16x8 gc = frag_cols<QS, 1>(sG, 0, s2, dt * 32, lane), qc = frag_cols<QS, 1>(sQ, 0, s2, dt * 32, lane);
+          dv[dt] = MFMA(gc, pf, dv[dt], 0, 0, 0);
+          dv[dt] = MFMA(gc, pr, dv[dt], 0, 0, 0);
+          dk[dt] = MFMA(qc, df, dk[dt], 0, 0, 0);
+          dk[dt] = MFMA(qc, dr, dk[dt], 0, 0, 0);
         }
       }
     }
