@@ -5,8 +5,8 @@
 //   var_dbias_k pairs stationary (128 x 64 per workgroup), samples stream: dS summed over the samples in the accumulators, in
 //               32 bits, one 32-bit value per pair and head out; no atomics, so the sums do not depend on the order of anything
 //   var_few_bwd_k up to 32 queries: keys stationary, everything in one pass over K and V (below)
-// Times: ViT-B/14, 64 samples x 12 heads of 64, 272 x 272 with bias: dQ 62, dK/dV 72, bias gradient 61 us; ViT-g/14 at 1024 px, 4 x
-// 16 heads of 88, 5329 x 5329 with bias: 1.27, 1.56, 2.14 ms; 300 queries over up to 4096 states, 16 x 16 heads of 64: dQ 129,
+// Times: ViT-B/14, 64 samples x 12 heads of 64, 272 x 272 with bias: dQ 64, dK/dV 72, bias gradient 61 us; ViT-g/14 at 1024 px, 4 x
+// 16 heads of 88, 5329 x 5329 with bias: 1.20, 1.46, 2.08 ms; 300 queries over up to 4096 states, 16 x 16 heads of 64: dQ 129,
 // dK/dV 184 us.  All are bound by the vector units beside the matrix units (dK/dV: 8 vector instructions and an exponential
 // for the 4 products of a pair), the bias gradient also by LDS reads and by its steps' latency.
 // P is formed again from the row statistics of the forward pass; delta = rowsum(dO O) comes from var_dq_k / var_few_bwd_k.
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(NW * 64, (var_dkdv_occ<DHP, BIAS, DROP>())) void va
 // go to registers, which frees their place at once for the next sample's, the latter have NB places: two, or one where two
 // would not leave room for a second workgroup on the CU, which matters more (it works while this one starts, waits or
 // stores).  ViT-B/14: 131 us with the keys in registers a sample ahead instead of LDS, 61 us so; ViT-g/14 at 1024 px, 4 samples:
-// 2.29 ms with one workgroup of 128 queries and two places, 2.14 ms with two of 64.
+// 2.29 ms with one workgroup of 128 queries and two places, 2.08-2.14 ms with two of 64.
 template <int DHP> constexpr int dbias_nb() { return DHP == 96 ? 1 : 2; }
 template <int DHP, bool DROP>
 __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) {

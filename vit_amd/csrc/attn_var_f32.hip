@@ -9,8 +9,8 @@
 // An element of S costs 4 Dh operations at 256 per cycle and CU, 16 times the bf16 rate, so everything else (exponentials,
 // bias gathered from table and index where it is used, dropout) stays under the matrix units' time.  Streamed tiles hold 32
 // rows, in LDS, the next one on its way in registers.  ViT-S/16, 8 samples x 6 heads of 64, 197 x 197 with bias: forward 25 + 7,
-// dQ 30, dK/dV 33, bias gradient 20 us (one wave per 32 rows without sharing: dQ 58, dK/dV 68); 4 x 12 heads, 77 queries over up
-// to 577 states: 17 + 6, 26, 25 us (dQ 84 unshared).
+// dQ 32, dK/dV 33, bias gradient 20 us (one wave per 32 rows without sharing: dQ 58, dK/dV 68); 4 x 12 heads, 77 queries over up
+// to 577 states: 18 + 6, 28, 25 us (dQ 84 unshared).
 #include "attn_var.h"
 
 #define MFMA32 __builtin_amdgcn_mfma_f32_32x32x2f32

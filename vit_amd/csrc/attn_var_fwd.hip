@@ -7,8 +7,8 @@
 //   an unpacking and a multiplication by 1 / scale per element and nothing else.
 //   Bound by the vector units beside the matrix units (about 9 vector instructions and one exponential per score).  ViT-B/14,
 //   64 samples x 12 heads of 64, 272 x 272 with bias: 51 us; ViT-g/14 at 1024 px, 4 samples x 16 heads of 88, 5329 x 5329 with
-//   bias: 1.09 ms, 587 TFLOP/s (640 as the heads are padded to 96); 300 queries over up to 4096 states, 16 x 16 heads of
-//   64: 106 us.
+//   bias: 1.01 ms, 634 TFLOP/s (691 as the heads are padded to 96); 300 queries over up to 4096 states, 16 x 16 heads of
+//   64: 107 us.
 #include "attn_var.h"
 
 // ---- bias in accumulator order ----------------------------------------------------------------------------------------
