@@ -181,7 +181,7 @@ template <int DHP> __device__ __forceinline__ void wave_request(const WaveDma<DH
 __device__ __forceinline__ void u_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // launches of the matrix-unit kernels (attn_var_fwd.hip, attn_var_bwd.hip); operands checked by the caller
-void var_launch_expand(const VarP& p, bool transposed, hipStream_t st);
+void var_launch_expand(const VarP& p, bool both, hipStream_t st);   // bias_s, or bias_s and bias_t
 int var_few_heads(int64_t H);
 void var_launch_few_fwd(const VarP& p, bool bias, hipStream_t st);
 void var_launch_fwd(const VarP& p, bool bias, int nw, hipStream_t st);

@@ -530,7 +530,6 @@ extern "C" int vitk_attn_var_bwd(const VitkAttnVar* desc, void* stream) {
     if (bias) {
       p.bias_s = (const bf16*)(ws + w.bias_s);
       p.bias_t = (const bf16*)(ws + w.bias_t);
-      var_launch_expand(p, false, st);
       var_launch_expand(p, true, st);
     }
     if (var_few(a)) {

@@ -18,7 +18,7 @@
 // tile]; TR = true: queries on the rows, key on the lane (dK/dV, bias gradient), [H][key tile][query tile].  Gathering once
 // per pair and head here, instead of once per pair, head and sample inside the attention, takes the gather (an LDS or L2
 // access with its own address per element) out of the inner loops.  Bound by its stores (16 heads x 5329 x 5329: 216 us, 4.2 TB/s;
-// transposed 292 us).  HV heads are read per access.
+// both layouts 400 us, 4.5 TB/s, where a launch each took 508).  HV heads are read per access.
 template <int HV> struct HeadVec;
 template <> struct HeadVec<8> { typedef uint4 t; };
 template <> struct HeadVec<4> { typedef uint2 t; };
@@ -26,13 +26,10 @@ template <> struct HeadVec<2> { typedef uint32_t t; };
 template <> struct HeadVec<1> { typedef uint16_t t; };
 
 template <int HV, bool TR>
-__global__ __launch_bounds__(256) void var_expand_k(VarP p, bf16* __restrict__ out) {
+__device__ __forceinline__ void expand_tile(const VarP& p, int lt, int rt, bf16* __restrict__ out) {   // tile along the lanes, along the rows
   const int half = (threadIdx.x >> 6) & 1, lane = threadIdx.x & 63, hi = lane >> 5;
-  const int nlt = TR ? p.nkt_t : p.nqt, nrt = TR ? p.nqt_t : p.nkt;   // tiles along the lanes, along the rows
-  const int64_t tiles = (int64_t)nlt * nrt;
-  const int64_t tile = (int64_t)blockIdx.x * 2 + (threadIdx.x >> 7);
-  if (tile >= tiles) return;
-  const int lt = (int)(tile / nrt), rt = (int)(tile - (int64_t)lt * nrt);
+  const int nlt = TR ? p.nkt_t : p.nqt, nrt = TR ? p.nqt_t : p.nkt;
+  const int64_t tiles = (int64_t)nlt * nrt, tile = (int64_t)lt * nrt + rt;
   const int at_lane = lt * 32 + (lane & 31);
   int n[8];
   bool ok[8];
@@ -63,19 +60,29 @@ __global__ __launch_bounds__(256) void var_expand_k(VarP p, bf16* __restrict__ o
     }
   }
 }
-template <bool TR> static void expand_t(const VarP& p, hipStream_t st) {
-  const int64_t tiles = TR ? (int64_t)p.nkt_t * p.nqt_t : (int64_t)p.nqt * p.nkt;
-  const dim3 grid((unsigned)ceil_div(tiles, 2)), block(256);
-  bf16* out = (bf16*)(TR ? p.bias_t : p.bias_s);
-  const uintptr_t at = (uintptr_t)p.table;
-  if (p.H % 8 == 0 && at % 16 == 0) hipLaunchKernelGGL((var_expand_k<8, TR>), grid, block, 0, st, p, out);
-  else if (p.H % 4 == 0 && at % 8 == 0) hipLaunchKernelGGL((var_expand_k<4, TR>), grid, block, 0, st, p, out);
-  else if (p.H % 2 == 0 && at % 4 == 0) hipLaunchKernelGGL((var_expand_k<2, TR>), grid, block, 0, st, p, out);
-  else hipLaunchKernelGGL((var_expand_k<1, TR>), grid, block, 0, st, p, out);
+// bias_s alone (forward): two waves a tile, two tiles a workgroup.  BOTH (backward): a workgroup lays the same 32 x 32 pairs out
+// both ways, two waves each; nqt_t >= nqt, nkt >= nkt_t.
+template <int HV, bool BOTH> __global__ __launch_bounds__(256) void var_expand_k(VarP p) {
+  const int which = threadIdx.x >> 7, nq = BOTH ? p.nqt_t : p.nqt;
+  const int64_t tile = BOTH ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 2 + which;
+  if (tile >= (int64_t)nq * p.nkt) return;
+  const int qt = (int)(tile / p.nkt), kt = (int)(tile - (int64_t)qt * p.nkt);
+  if (BOTH && which) {
+    if (kt < p.nkt_t) expand_tile<HV, true>(p, kt, qt, (bf16*)p.bias_t);
+  } else if (qt < p.nqt) {
+    expand_tile<HV, false>(p, qt, kt, (bf16*)p.bias_s);
+  }
 }
-void var_launch_expand(const VarP& p, bool transposed, hipStream_t st) {
-  if (transposed) expand_t<true>(p, st);
-  else expand_t<false>(p, st);
+template <int HV> static void expand_h(const VarP& p, bool both, hipStream_t st) {
+  if (both) hipLaunchKernelGGL((var_expand_k<HV, true>), dim3((unsigned)((int64_t)p.nqt_t * p.nkt)), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((var_expand_k<HV, false>), dim3((unsigned)ceil_div((int64_t)p.nqt * p.nkt, 2)), dim3(256), 0, st, p);
+}
+void var_launch_expand(const VarP& p, bool both, hipStream_t st) {
+  const uintptr_t at = (uintptr_t)p.table;
+  if (p.H % 8 == 0 && at % 16 == 0) expand_h<8>(p, both, st);
+  else if (p.H % 4 == 0 && at % 8 == 0) expand_h<4>(p, both, st);
+  else if (p.H % 2 == 0 && at % 4 == 0) expand_h<2>(p, both, st);
+  else expand_h<1>(p, both, st);
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
