@@ -5,6 +5,7 @@ import itertools
 import math
 import os
 import re
+import subprocess
 
 import pytest
 import torch
@@ -249,3 +250,49 @@ def test_plans_of_captured_graphs_are_never_dropped(monkeypatch):
     assert model.prepare_buckets((1, 2)) is first
     assert model.prepare_buckets((3, 4)) is plans[(3, 4)] and model.prepare_buckets((1, 1)) is not plans[(1, 1)]
     assert len(model._bucket_plans) <= 9
+
+
+SHARES = r"""
+#include "attn_share.h"
+#include <cstdio>
+#include <initializer_list>
+static int fail(int n, int tile, int shares, int y) { std::printf("keys %d tile %d share %d of %d\n", n, tile, y, shares); return 1; }
+static int look(int n, int tile, int shares) {
+  const int tiles = (n + tile - 1) / tile;
+  int at = 0, least = tiles, most = 0;
+  for (int y = 0; y < shares; y++) {
+    const KeyShare s = key_share(n, tile, shares, y);
+    // the tiles follow each other, their keys are covered, and no descriptor reaches behind the last key
+    if (s.t0 != at || s.t1 < s.t0 || s.end > n || s.end < 0) return fail(n, tile, shares, y);
+    if (s.end != (s.t1 * tile < n ? s.t1 * tile : n)) return fail(n, tile, shares, y);
+    if (s.t1 > s.t0 && (s.end <= (s.t1 - 1) * tile)) return fail(n, tile, shares, y);   // its last tile has a key
+    at = s.t1;
+    least = s.t1 - s.t0 < least ? s.t1 - s.t0 : least;
+    most = s.t1 - s.t0 > most ? s.t1 - s.t0 : most;
+  }
+  return at != tiles || most - least > 1 ? fail(n, tile, shares, -1) : 0;
+}
+int main() {
+  const int tile[] = {32, 64}, large[] = {65537, 999999, (1 << 24) - 1};
+  for (int t : tile)
+    for (int shares = 1; shares <= 64; shares++) {
+      for (int tiles = 0; tiles <= 700; tiles++)
+        for (int n : {tiles * t - t + 1, tiles * t - 1, tiles * t})
+          if (n >= 0 && look(n, t, shares)) return 1;
+      for (int n : large)
+        if (look(n, t, shares)) return 1;
+    }
+  std::puts("covered");
+}
+"""
+
+
+def test_key_shares_cover_every_key_once_and_nothing_behind_the_last(tmp_path):
+    """The arithmetic by which workgroups share a sample's keys, compiled for the host from the kernels' own header: all tile
+    counts and shares; shares without tiles are among them (more shares than tiles)."""
+    src = tmp_path / "shares.cc"
+    src.write_text(SHARES)
+    out = str(tmp_path / "shares")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I", os.path.join(ROOT, "vit_amd", "csrc"), str(src), "-o", out], check=True)
+    done = subprocess.run([out], capture_output=True, text=True, timeout=60)
+    assert done.returncode == 0 and done.stdout == "covered\n", done.stdout

@@ -654,3 +654,29 @@ def test_backward_twice_and_retained_graphs():
     run(*make(4, 90, 200, 2, 64, torch.bfloat16, 1, packed=True), 0, kv_lengths=torch.tensor([200, 1, 0, 30], device=DEV))
     for a, b in zip(first, torch.autograd.grad(o, leaves, dout)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,Lq,Lk,H,Dh,bias,counts", [
+    (1, 100, 4097, 3, 64, False, None), (1, 100, 4097, 3, 64, True, None), (1, 40, 2305, 1, 96, False, None),
+    (1, 130, 1031, 2, 128, True, None), (2, 70, 2000, 1, 64, False, [2000, 130]), (2, 48, 700, 2, 64, False, [64, 700]),
+    (1, 5, 1500, 1, 88, True, [1500])])
+def test_key_shares_that_do_not_divide_the_tiles(B, Lq, Lk, H, Dh, bias, counts, dtype):
+    """Few rows over long memories, tile counts that the shares do not divide, counts that leave shares without any tile; the
+    memory is a tensor of its own, nothing lies behind it."""
+    g = torch.Generator().manual_seed(Lk)
+    q, k, v, dout = [torch.randn(B, n, H, Dh, generator=g).to(DEV, dtype) for n in (Lq, Lk, Lk, Lq)]
+    kw = {} if counts is None else dict(kv_lengths=torch.tensor(counts, device=DEV))
+    full = None
+    if bias:
+        index = torch.randint(0, 30, (Lq, Lk), generator=g)
+        table = torch.randn(30, H, generator=g).to(DEV, dtype)
+        kw.update(bias_table=table, buckets=RelativeBuckets(index, 30).to(DEV))
+        full = table.double().cpu()[index].permute(2, 0, 1)
+    got = run(q, k, v, dout, 0, **kw)
+    want = reference(q, k, v, Dh ** -0.5, full, counts, dout)
+    dS = want.pop("dS")
+    if bias:
+        want["dtable"] = bucket_sums(*dS, index, 30, dtype)
+    for n, w in want.items():
+        check(got[n], w, n)

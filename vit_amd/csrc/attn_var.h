@@ -4,6 +4,7 @@
 // Row statistics kept for the backward pass: m (the reference maximum the exponentials were taken with) and lr = -log2 of
 // their sum; a row that nothing is left for has m = 0, lr = -inf, so that every probability of it comes out 0.
 #pragma once
+#include "attn_share.h"
 #include "attn_tile.h"
 
 struct VarP {

@@ -119,16 +119,8 @@ __global__ __launch_bounds__(NW * 64) void f32_fwd_k(VarP p) {
   const int64_t b = hb.b, h = hb.h;
   const int q0 = hb.xb * (NW * 32) + wid * 32, qrow = q0 + (lane & 31), rowoff = 4 * (lane >> 5);
   const bool wave_on = q0 < S;
-  const int len_all = key_count(p, b);
-  int t0 = 0, len = len_all;
-  if (SPLIT) {
-    const int per = (((len_all + 31) >> 5) + p.splits - 1) / p.splits;
-    t0 = per * (int)blockIdx.y;
-    const int end = (t0 + per) * 32;
-    if (end < len) len = end;
-    if (t0 * 32 >= len_all) len = t0 * 32;
-  }
-  const int nt = (len + 31) >> 5;
+  const KeyShare share = key_share(key_count(p, b), 32, SPLIT ? p.splits : 1, SPLIT ? (int)blockIdx.y : 0);
+  const int t0 = share.t0, len = share.end, nt = share.t1;
   const __amdgpu_buffer_rsrc_t krs = rows_rsrc32((const float*)p.k + b * p.k_sb + h * p.k_sh, p.k_ss, len, Dh);
   const __amdgpu_buffer_rsrc_t vrs = rows_rsrc32((const float*)p.v + b * p.v_sb + h * p.v_sh, p.v_ss, len, Dh);
   f32x4 qf[DHP / 8], rk[NCH], rv[NCH];
@@ -140,8 +132,10 @@ __global__ __launch_bounds__(NW * 64) void f32_fwd_k(VarP p) {
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * LOG2E;
   const uint32_t xrow = var_drop_xrow(p, (uint64_t)(b * p.H + h) * p.Lq + (uint64_t)qrow, lane);
-  f32_load<DHP, NT, NCH>(rk, krs, p.k_ss, t0 * 32, Dh, tid);
-  f32_load<DHP, NT, NCH>(rv, vrs, p.v_ss, t0 * 32, Dh, tid);
+  if (t0 < nt) {
+    f32_load<DHP, NT, NCH>(rk, krs, p.k_ss, t0 * 32, Dh, tid);
+    f32_load<DHP, NT, NCH>(rv, vrs, p.v_ss, t0 * 32, Dh, tid);
+  }
   for (int t = t0; t < nt; t++) {
     __syncthreads();
     f32_store<DHP, NT, NCH>(rk, sK, tid);

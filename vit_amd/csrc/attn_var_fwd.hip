@@ -219,17 +219,9 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
   const bf16* qp = (const bf16*)p.q + b * p.q_sb + h * p.q_sh;
   const bf16* kp = (const bf16*)p.k + b * p.k_sb + h * p.k_sh;
   const bf16* vp = (const bf16*)p.v + b * p.v_sb + h * p.v_sh;
-  const int len_all = key_count(p, b);
   // this workgroup's keys: [64 tile0, len)
-  int tile0 = 0, len = len_all;
-  if (SPLIT) {
-    const int per = (((len_all + 63) >> 6) + p.splits - 1) / p.splits;
-    tile0 = per * (int)blockIdx.y;
-    const int end = (tile0 + per) * 64;
-    if (end < len) len = end;
-    if (tile0 * 64 >= len_all) len = tile0 * 64;   // nothing left for this share
-  }
-  const int ntiles = (len + 63) >> 6, nfull = len >> 6;
+  const KeyShare share = key_share(key_count(p, b), 64, SPLIT ? p.splits : 1, SPLIT ? (int)blockIdx.y : 0);
+  const int tile0 = share.t0, len = share.end, ntiles = share.t1, nfull = tile0 < ntiles ? len >> 6 : ntiles;
   const uint32_t lds0 = lds_addr(smem);
   const TileDma<DHP, NW> ksrc = tile_dma<DHP, NW>(kp, p.k_ss, len, Dh, lds0, wid, lane);
   const TileDma<DHP, NW> vsrc = tile_dma<DHP, NW>(vp, p.v_ss, len, Dh, lds0 + u_tile<DHP>(), wid, lane);
@@ -249,8 +241,10 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
     for (int i = 0; i < 4; i++) d[i] = __builtin_bit_cast(bf16x8, buf_load16(brs, (uint32_t)(t * 4096 + i * 1024 + lane * 16)));
   };
   if (BIAS) load_bias(bf, tile0);
-  request(tile0, 0);
-  if (NB == 3) request(tile0 + 1, 1);
+  if (tile0 < ntiles) {   // requests beyond the last tile bring the last once more
+    request(tile0, 0);
+    if (NB == 3) request(tile0 + 1, 1);
+  }
   const f32x16 zero = ZERO16;
   f32x16 oacc[DHP / 32], lacc = zero;
 #pragma unroll
@@ -273,7 +267,7 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
     __syncthreads();
     buf = buf + 1 == NB ? 0 : buf + 1;
   }
-  if (nfull < ntiles && nfull >= tile0 && wave_on) {
+  if (nfull < ntiles && wave_on) {
     const char* sK = smem + buf * TILE;
     const char* sV = sK + u_tile<DHP>();
     if (len - nfull * 64 > 32) {
@@ -307,8 +301,8 @@ __global__ __launch_bounds__(256, (DHP <= 64 ? 2 : 1)) void var_few_fwd_k(VarP p
   const int64_t b = uniform(g / parts), h = (int)(i % groups) * HW + wid % HW;
   if (b >= p.B) return;
   const int share = (int)(g - (uint32_t)b * parts) * KW + wid / HW;
-  const int len_all = key_count(p, b), per = uniform((uint32_t)(((len_all + 31) >> 5) + p.splits - 1) / (uint32_t)p.splits);
-  const int t0 = per * share, len = min(len_all, (t0 + per) * 32), nt = max((len + 31) >> 5, t0);   // keys [32 t0, len): none if t0 = nt
+  const KeyShare part = key_share(key_count(p, b), 32, p.splits, share);
+  const int t0 = (int)uniform(part.t0), nt = (int)uniform(part.t1), len = (int)uniform(part.end);   // keys [32 t0, len)
   const int qrow = lane & 31;
   const uint32_t lds0 = lds_addr(smem) + wid * (NB * 2 * T);
   const bf16* kp = (const bf16*)p.k + b * p.k_sb + h * p.k_sh;
@@ -326,8 +320,10 @@ __global__ __launch_bounds__(256, (DHP <= 64 ? 2 : 1)) void var_few_fwd_k(VarP p
     wave_request(vsrc, t, buf * 2 * T);
   };
   if (BIAS) load_bias(t0);
+  if (t0 < nt) {
 #pragma unroll
-  for (int k = 0; k < NB - 1; k++) request(t0 + k, k);
+    for (int k = 0; k < NB - 1; k++) request(t0 + k, k);
+  }
   const f32x16 zero = ZERO16;
   f32x16 oacc[DHP / 32], lacc = zero;
 #pragma unroll
