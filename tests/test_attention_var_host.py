@@ -10,7 +10,7 @@ import subprocess
 import pytest
 import torch
 
-from vit_amd import KVMemory, RelativeBuckets, ViTConfig, _lib, qk_norm_rope
+from vit_amd import KVMemory, RelativeBuckets, ViTConfig, _lib, kernels, qk_norm_rope
 from vit_amd.attention import CrossAttention, SelfAttention, attention
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -296,3 +296,26 @@ def test_key_shares_cover_every_key_once_and_nothing_behind_the_last(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I", os.path.join(ROOT, "vit_amd", "csrc"), str(src), "-o", out], check=True)
     done = subprocess.run([out], capture_output=True, text=True, timeout=60)
     assert done.returncode == 0 and done.stdout == "covered\n", done.stdout
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_operands_start_on_16_byte_boundaries(dtype):
+    """Contiguous or not, what starts or steps off a boundary is copied; everything else is passed on as it is, axes of one
+    element with any stride among it."""
+    flat = torch.arange(1 + 2 * 5 * 3 * 64, dtype=torch.float32).to(dtype)
+    for off in range(9):
+        t = flat[off:off + 2 * 5 * 2 * 64].view(2, 5, 2, 64)
+        got = kernels.attn_operand(t)
+        assert got.data_ptr() % 16 == 0 and torch.equal(got, t)
+        assert (got is t) == (off * t.element_size() % 16 == 0)
+    wide = torch.zeros(2, 5, 3, 68, dtype=dtype)[..., :64]
+    got = kernels.attn_operand(wide)
+    assert (got is wide) == (dtype == torch.float32) and all(s * got.element_size() % 16 == 0 for s in got.stride()[:3])
+    one = flat[:64].as_strided((1, 1, 1, 64), (3, 5, 7, 1))
+    assert kernels.attn_operand(one) is one
+    odd = flat[1:1 + 2 * 5 * 3 * 20].view(2, 5, 3, 20)[..., :12 if dtype == torch.bfloat16 else 10]
+    assert kernels.attn_operand(odd) is odd   # head sizes that no 16-byte access fits
+    leaf = flat[1:129].view(1, 2, 1, 64).clone().requires_grad_(True)
+    shifted = torch.cat([leaf.new_zeros(1), leaf.reshape(-1)])[1:].view(1, 2, 1, 64)
+    kernels.attn_operand(shifted).square().sum().backward()
+    assert torch.equal(leaf.grad, 2 * leaf.detach())

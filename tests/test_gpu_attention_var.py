@@ -680,3 +680,33 @@ def test_key_shares_that_do_not_divide_the_tiles(B, Lq, Lk, H, Dh, bias, counts,
         want["dtable"] = bucket_sums(*dS, index, 30, dtype)
     for n, w in want.items():
         check(got[n], w, n)
+
+
+def shifted(t, n=1):
+    """The same values, contiguous, n elements behind a 16-byte boundary."""
+    flat = torch.empty(t.numel() + 16, device=t.device, dtype=t.dtype)
+    out = flat[n:n + t.numel()].view(t.shape)
+    out.copy_(t)
+    assert out.is_contiguous() and out.data_ptr() % 16
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_contiguous_operands_off_the_boundary(dtype):
+    """Contiguous tensors at an odd storage offset, and output gradients like them, give what aligned copies give, bit for bit."""
+    q, k, v, dout = [t.contiguous() for t in make(2, 40, 100, 2, 64, dtype, 4, packed=True)]
+    lens = torch.tensor([100, 37], device=DEV)
+    want = run(q, k, v, dout, 0, kv_lengths=lens)
+    got = run(shifted(q), shifted(k, 3), shifted(v), shifted(dout), 0, kv_lengths=lens)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+    w = (1 + torch.arange(64, device=DEV) / 64).to(dtype)
+
+    def norms(q, k, dq, dk):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, w, w)]
+        out = qk_norm_rope(*leaves, rope_q=rope_table(40, 64, 1), rope_k=rope_table(90, 64, 2))
+        return [*out, *torch.autograd.grad(out, leaves, [dq, dk])]
+
+    dk = torch.randn_like(k)
+    for a, b in zip(norms(shifted(q), shifted(k), shifted(dout), shifted(dk, 5)), norms(q, k, dout, dk)):
+        assert torch.equal(a, b)

@@ -608,14 +608,20 @@ def qk_norm_rope_bwd(xs: tuple, gs: tuple, dxs: tuple, w: tuple, tables: tuple, 
 def attn_operand(t: Tensor) -> Tensor:
     """``t`` [B, L, H, Dh] as the kernels take it: d contiguous, rows that do not overlap (an expanded dimension of rows does),
     and on 16-byte boundaries where head_dim allows it (the kernels on the matrix units load 16 bytes at a time); a view that
-    is not laid out so is copied once."""
+    is not laid out so is copied once, a contiguous one that starts off the boundary included."""
     sb, ss, sh, sd = t.stride()
-    _, rows, _, Dh = t.shape
+    B, rows, H, Dh = t.shape
     if sd == 1 and (ss >= Dh or rows <= 1):
         n = 16 // t.element_size()
-        if Dh % n or not ((sb | ss | sh) & (n - 1) or t.data_ptr() & 15):
+        if Dh % n:
             return t
-    return t.contiguous()
+        if not t.data_ptr() & 15:
+            if not (sb | ss | sh) & (n - 1):
+                return t
+            # the stride of an axis of one element is never used
+            if not ((sb if B > 1 else 0) | (ss if rows > 1 else 0) | (sh if H > 1 else 0)) & (n - 1):
+                return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 _ST24 = C.c_int64 * 24
