@@ -10,7 +10,7 @@ import subprocess
 import pytest
 import torch
 
-from vit_amd import KVMemory, RelativeBuckets, ViTConfig, _lib, kernels, qk_norm_rope
+from vit_amd import KVMemory, RelativeBuckets, ViTConfig, _lib, kernels, ops, qk_norm_rope
 from vit_amd.attention import CrossAttention, SelfAttention, attention
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -319,3 +319,15 @@ def test_operands_start_on_16_byte_boundaries(dtype):
     shifted = torch.cat([leaf.new_zeros(1), leaf.reshape(-1)])[1:].view(1, 2, 1, 64)
     kernels.attn_operand(shifted).square().sum().backward()
     assert torch.equal(leaf.grad, 2 * leaf.detach())
+
+
+def test_rotation_tables_start_on_16_byte_boundaries():
+    for shape, keep in (((2, 5, 16), None), ((2, 3, 1, 5, 16), None), ((2, 3, 1, 5, 16), torch.tensor([2, 0]))):
+        n = math.prod(shape)
+        rope = torch.arange(n + 1.0)[1:].view(shape)
+        assert rope.is_contiguous() and rope.data_ptr() % 16
+        table, _ = ops._rope_table(rope, keep, 3, 3 if keep is None else 2, torch.float32)
+        want = rope if len(shape) == 3 else rope[:, :, 0] if keep is None else rope[:, keep, 0]
+        assert table.data_ptr() % 16 == 0 and torch.equal(table, want)
+    aligned = torch.zeros(2, 5, 16)
+    assert ops._rope_table(aligned, None, 3, 3, torch.float32)[0].data_ptr() == aligned.data_ptr()

@@ -283,3 +283,25 @@ def test_training_step_of_a_decoder_captures_into_a_graph():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), rep
+
+
+def test_layers_take_rotation_tables_off_the_boundary():
+    """A contiguous float32 table one element behind a boundary, through the layers that normalise and rotate in one pass."""
+    D, H, S = 160, 2, 11
+    g = torch.Generator().manual_seed(1)
+    ang = torch.rand(S, 80, generator=g) * 6
+    rope = torch.stack([ang.sin(), ang.cos()]).to(DEV)
+    off = torch.empty(rope.numel() + 1, device=DEV)[1:].view(rope.shape).copy_(rope)
+    assert off.is_contiguous() and off.data_ptr() % 16
+    layer = randomize(TransformerDecoderLayer(D, 2 * D, H, 0.0, 0.0, qk_normalization=True, device=DEV, dtype=torch.bfloat16,
+                                              activation="silu")).train()
+    x, kv = torch.randn(2, S, D, generator=g).to(DEV, torch.bfloat16), torch.randn(2, S, D, generator=g).to(DEV, torch.bfloat16)
+
+    def go(rope):
+        layer.zero_grad()
+        y = layer(x, kv, rope_q=rope, rope_k=rope)
+        y.float().square().mean().backward()
+        return [y] + [p.grad.clone() for p in layer.parameters()]
+
+    for a, b in zip(go(off), go(rope)):
+        assert torch.equal(a, b)

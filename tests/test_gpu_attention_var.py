@@ -710,3 +710,12 @@ def test_contiguous_operands_off_the_boundary(dtype):
     dk = torch.randn_like(k)
     for a, b in zip(norms(shifted(q), shifted(k), shifted(dout), shifted(dk, 5)), norms(q, k, dout, dk)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("batch", [None, 2])
+def test_rotation_tables_off_the_boundary(batch):
+    q, k, _, _ = make(2, 9, 9, 2, 80, torch.bfloat16, 4, packed=True)
+    w = torch.ones(80, device=DEV)
+    t = rope_table(8, 80, 3, batch)
+    for a, b in zip(qk_norm_rope(q, k, w, w, rope_q=shifted(t), rope_k=shifted(t, 2)), qk_norm_rope(q, k, w, w, rope_q=t, rope_k=t)):
+        assert torch.equal(a, b)

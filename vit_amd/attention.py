@@ -90,7 +90,7 @@ def qk_norm_rope(q: Tensor, k: Optional[Tensor], q_norm_weight: Tensor, k_norm_w
         if (rope.shape != (2, n, Dh) and rope.shape != (2, B, 1, n, Dh)) or n > Ln:
             raise ValueError(f"vit_amd: {name} must be [2, N, {Dh}] or [2, {B}, 1, N, {Dh}] with N <= {Ln}, got {tuple(rope.shape)}")
         tables.append(rope if rope.dim() == 3 and rope.dtype == torch.float32 and rope.is_contiguous() and not rope.requires_grad
-                      else ops._rope_table(rope, None, B, B, q.dtype)[0])
+                      and not rope.data_ptr() & 15 else ops._rope_table(rope, None, B, B, q.dtype)[0])
     q, k = K.attn_operand(q), None if k is None else K.attn_operand(k)
     if _wants_grad(q, k, q_norm_weight, k_norm_weight, q_norm_bias, k_norm_bias):
         return ops.QkNormRopeFn.apply(q, k, q_norm_weight, k_norm_weight, q_norm_bias, k_norm_bias, *tables, float(eps),

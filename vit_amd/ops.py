@@ -411,7 +411,8 @@ def _residual_grad(dnew2: Tensor, tc: torch.dtype, gamma: Optional[Tensor], rows
 
 def _rope_table(rope: Optional[Tensor], keep_idx: Optional[Tensor], B: int, Bk: int, tc: torch.dtype):
     """(fp32 table for the rope kernels, emulate-bf16 flag).  [2, N, Dh] is shared by all samples; [2, B, 1, N', Dh] holds
-    one table per sample (masked tokens, vit/vit.py:522-527) and follows a drop-path subset (vit/transformer.py:41-46)."""
+    one table per sample (masked tokens, vit/vit.py:522-527) and follows a drop-path subset (vit/transformer.py:41-46).
+    The table starts on a 16-byte boundary: one that does not is copied."""
     if rope is None:
         return None, False
     emu = rope.dtype == torch.bfloat16 and tc == torch.bfloat16
@@ -426,6 +427,8 @@ def _rope_table(rope: Optional[Tensor], keep_idx: Optional[Tensor], B: int, Bk: 
         table = rope.detach().to(torch.float32).contiguous()
     else:
         raise ValueError(f"vit_amd: RoPE table must be [2, N, Dh] or [2, B, 1, N, Dh], got {tuple(rope.shape)}")
+    if table.data_ptr() & 15:
+        table = table.clone()
     return table, emu
 
 
