@@ -719,3 +719,26 @@ def test_rotation_tables_off_the_boundary(batch):
     t = rope_table(8, 80, 3, batch)
     for a, b in zip(qk_norm_rope(q, k, w, w, rope_q=shifted(t), rope_k=shifted(t, 2)), qk_norm_rope(q, k, w, w, rope_q=t, rope_k=t)):
         assert torch.equal(a, b)
+
+
+def test_head_norms_of_heads_far_apart():
+    """[B, H, L, Dh] laid out, heads 2^24 elements and more apart: forward and backward as for heads side by side."""
+    B, L, H, Dh = 2, 6, 3, 64
+    sh = 2 ** 24 + 64
+    buf = torch.empty(B * H * sh, device=DEV, dtype=torch.bfloat16)
+    far = buf.as_strided((B, L, H, Dh), (H * sh, Dh, sh, 1))
+    g = torch.Generator().manual_seed(2)
+    far.copy_(torch.randn(B, L, H, Dh, generator=g))
+    near, w, t = far.contiguous(), torch.ones(Dh, device=DEV), rope_table(L, Dh, 5)
+    dy = torch.randn(B, L, H, Dh, generator=g).to(DEV, torch.bfloat16)
+    dfar = torch.empty_like(buf).as_strided(far.shape, far.stride()).copy_(dy)
+    outs = []
+    for x, d in ((near, dy), (far, dfar)):
+        x = x.detach().requires_grad_(True)
+        y, none = qk_norm_rope(x, None, w, rope_q=t)
+        outs.append((y, *torch.autograd.grad(y, x, d)))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    want = norm_rope_reference(near, w, None, t, False, 1e-5, dy)
+    check(outs[1][0], want["y"], "y")
+    check(outs[1][1], want["dx"], "dx")
