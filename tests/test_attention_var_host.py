@@ -331,3 +331,15 @@ def test_rotation_tables_start_on_16_byte_boundaries():
         assert table.data_ptr() % 16 == 0 and torch.equal(table, want)
     aligned = torch.zeros(2, 5, 16)
     assert ops._rope_table(aligned, None, 3, 3, torch.float32)[0].data_ptr() == aligned.data_ptr()
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 16), (2, 2, 1, 3, 16)])
+def test_rotation_tables_that_ask_for_a_gradient_are_refused(shape):
+    """They would get none; where no gradients are taken, and detached, they pass (as far as the missing GPU)."""
+    q, w, rope = torch.zeros(2, 3, 4, 16), torch.ones(16), torch.zeros(shape, requires_grad=True)
+    for kw in (dict(rope_q=rope), dict(k=q, k_norm_weight=w, rope_k=rope)):
+        with pytest.raises(ValueError, match="constant table"):
+            qk_norm_rope(q, kw.pop("k", None), w, **kw)
+    for context, table in ((torch.no_grad(), rope), (torch.enable_grad(), rope.detach())):
+        with context, pytest.raises(RuntimeError, match="no CPU fallback|MI355X"):
+            qk_norm_rope(q, None, w, rope_q=table)

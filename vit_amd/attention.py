@@ -58,7 +58,8 @@ def qk_norm_rope(q: Tensor, k: Optional[Tensor], q_norm_weight: Tensor, k_norm_w
     pass over both (vit/attention.py:25-41 and vit/rope.py:139-163); returns (q, k).  ``k`` may be None (a decoder step
     that rotates its query only).  Weights and biases are [Dh]; a table [2, N, Dh] or [2, B, 1, N, Dh] (sin, cos) rotates
     the last N rows.  Any strides with contiguous heads; head_dim a multiple of 8, at most 128; float32 or bfloat16.
-    Arithmetic is float32, rounded once at the store.  Differentiable in q, k, the weights and the biases."""
+    Arithmetic is float32, rounded once at the store.  Differentiable in q, k, the weights and the biases; the tables are
+    constants, and one that asks for a gradient is refused."""
     _heads("q", q)
     Dh = q.shape[3]
     if k is not None:
@@ -89,6 +90,8 @@ def qk_norm_rope(q: Tensor, k: Optional[Tensor], q_norm_weight: Tensor, k_norm_w
         n = rope.shape[-2] if rope.dim() >= 2 else -1
         if (rope.shape != (2, n, Dh) and rope.shape != (2, B, 1, n, Dh)) or n > Ln:
             raise ValueError(f"vit_amd: {name} must be [2, N, {Dh}] or [2, {B}, 1, N, {Dh}] with N <= {Ln}, got {tuple(rope.shape)}")
+        if _wants_grad(rope):
+            raise ValueError(f"vit_amd: {name} is a constant table, its gradient is not computed; pass {name}.detach()")
         tables.append(rope if rope.dim() == 3 and rope.dtype == torch.float32 and rope.is_contiguous() and not rope.requires_grad
                       and not rope.data_ptr() & 15 else ops._rope_table(rope, None, B, B, q.dtype)[0])
     q, k = K.attn_operand(q), None if k is None else K.attn_operand(k)
