@@ -296,6 +296,11 @@ int vitk_fourier_features_bwd(const float* grid, const float* w, const void* g, 
  * aligned).  Called with the dropped samples before the residual epilogue (or the norm backward) writes the kept ones. */
 int vitk_copy_samples(const void* src, void* dst, const int64_t* idx, int64_t n, int64_t sample_bytes, void* stream);
 
+/* dst [B, L] rows of row_bytes = src for the rows l < kv_len[b] (counts below 0 are 0), zeros for the others.  src may be dst:
+ * the rows before the counts are then neither read nor written.  Padding of a memory before something that sums over all of its
+ * rows (a weight gradient multiplies padded rows by zeros, which NaN and infinities survive). */
+int vitk_zero_padding(const void* src, void* dst, const int32_t* kv_len, int64_t B, int64_t L, int64_t row_bytes, void* stream);
+
 /* ---- per-head normalisation of q and k with the rotation in the same pass ---------------------------------------------
  * vit/attention.py:25-41 (applied at :95-105) followed by vit/rope.py:139-163, and the backward of the two together.
  *   xhat = (x - mean) * rstd (RMSNorm: mean 0, eps inside the root), n = xhat * w (+ b),

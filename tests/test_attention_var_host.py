@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from vit_amd import KVMemory, RelativeBuckets, ViTConfig, _lib, kernels, ops, qk_norm_rope
-from vit_amd.attention import CrossAttention, SelfAttention, attention
+from vit_amd.attention import CrossAttention, SelfAttention, attention, attention_q_kv_packed
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -343,3 +343,24 @@ def test_rotation_tables_that_ask_for_a_gradient_are_refused(shape):
     for context, table in ((torch.no_grad(), rope), (torch.enable_grad(), rope.detach())):
         with context, pytest.raises(RuntimeError, match="no CPU fallback|MI355X"):
             qk_norm_rope(q, None, w, rope_q=table)
+
+
+def test_zero_padding_refusals():
+    lib = _lib.load()
+    for args, match in (((None, None, None, 1, 1, 3), "bad shape"), ((None, None, None, -1, 1, 4), "bad shape"), ((None, None, None, 1, 1, 4), "null"),
+                        ((4097, 4096, 4096, 1, 1, 4), "aligned")):
+        assert lib.vitk_zero_padding(*args, None) != 0 and match in lib.vitk_last_error().decode()
+    assert lib.vitk_zero_padding(None, None, None, 0, 5, 4, None) == 0 and lib.vitk_zero_padding(None, None, None, 5, 0, 4, None) == 0
+
+
+def test_head_norms_of_padded_rows_need_an_eps():
+    """A padded row is cleared before its gradient is formed; without an eps the norm of zeros is no number."""
+    q, kv, w = torch.zeros(2, 3, 32), torch.zeros(2, 4, 32), torch.zeros(32, 32, requires_grad=True)
+    ones = torch.ones(16)
+    args = (w, None, torch.zeros(64, 32), None, torch.ones(32), None, False, 16, w, None, None, 1e-5, ones, None, ones, None, False)
+    lens = torch.tensor([4, 1])
+    for eps, wkv_grad, error in ((0.0, True, ValueError), (1e-5, True, RuntimeError), (0.0, False, RuntimeError)):
+        a = list(args)
+        a[2] = torch.zeros(64, 32, requires_grad=wkv_grad)
+        with pytest.raises(error, match="qk_eps" if error is ValueError else "no CPU fallback|MI355X"):
+            attention_q_kv_packed(q, kv, *a, eps, True, 0.0, 0.0, True, kv_lengths=lens)

@@ -305,3 +305,57 @@ def test_layers_take_rotation_tables_off_the_boundary():
 
     for a, b in zip(go(off), go(rope)):
         assert torch.equal(a, b)
+
+
+BAD = [float("nan"), float("inf"), -float("inf")]
+
+
+@pytest.mark.parametrize("dtype,autocast", MODES, ids=MODE_IDS)
+@pytest.mark.parametrize("Dh,qk_norm,norm", [(64, False, "rmsnorm"), (80, True, "rmsnorm"), (32, True, "layernorm"), (12, True, "rmsnorm")])
+def test_training_does_not_see_what_padding_holds(dtype, autocast, Dh, qk_norm, norm):
+    """Padded rows of a memory that hold NaN and infinities: outputs, the weights' gradients and those of the inputs are the
+    ones of a memory padded with ones, bit for bit, with and without drop-path's choice of samples; the memory is not written."""
+    D, H, Lq, Lk, B = 2 * Dh, 2, 9, 70, 6
+    lens = [70, 1, 33, 0, 64, 69]
+    g = torch.Generator().manual_seed(1)
+    x, kv = torch.randn(B, Lq, D, generator=g).to(DEV, dtype), torch.randn(B, Lk, D, generator=g).to(DEV, dtype)
+    ones, bad = kv.clone(), kv.clone()
+    for b, n in enumerate(lens):
+        ones[b, n:] = 1.0
+        bad[b, n:] = BAD[b % 3]
+    for drop in (0.0, 0.5):
+        layer = randomize(TransformerDecoderLayer(D, 2 * D, H, 0.0, 0.0, norm_type=norm, qk_normalization=qk_norm, device=DEV, dtype=dtype,
+                                                  activation="silu", drop_path_rate=drop)).train()
+
+        def go(kv):
+            layer.zero_grad()
+            torch.manual_seed(7)
+            xg, kvg = x.clone().requires_grad_(True), kv.clone().requires_grad_(True)
+            before = kvg.detach().clone()
+            with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+                y = layer(xg, kvg, kv_lengths=torch.tensor(lens, device=DEV))
+            y.float().square().mean().backward()
+            assert torch.equal(kvg.detach().view(torch.uint8), before.view(torch.uint8))
+            return [y, xg.grad, kvg.grad] + [p.grad.clone() for p in layer.parameters()]
+
+        for i, (a, b) in enumerate(zip(go(bad), go(ones))):
+            assert torch.isfinite(a).all() and torch.equal(a, b), (drop, i)
+
+
+@pytest.mark.parametrize("frozen", [False, True])
+def test_pooling_trains_on_padding_that_holds_anything(frozen):
+    """The pooling head over states without a gradient of their own (a frozen encoder's) and with one."""
+    D, H, L = 128, 2, 300
+    lens = torch.tensor([300, 0, 17, 299], device=DEV)
+    head = randomize(AttentivePoolHead(D, 10, H, device=DEV, dtype=torch.bfloat16)).train()
+    x = torch.randn(4, L, D, generator=torch.Generator().manual_seed(3)).to(DEV, torch.bfloat16)
+    grads = []
+    for fill in (1.0, float("nan")):
+        for b in range(4):
+            x[b, int(lens[b]):] = fill
+        head.zero_grad()
+        xg = x.clone().requires_grad_(not frozen)
+        head(xg, lens).float().square().sum().backward()
+        grads.append([p.grad.clone() for p in head.parameters()] + ([] if frozen else [xg.grad]))
+    for a, b in zip(*grads):
+        assert torch.isfinite(b).all() and torch.equal(a, b)

@@ -742,3 +742,21 @@ def test_head_norms_of_heads_far_apart():
     want = norm_rope_reference(near, w, None, t, False, 1e-5, dy)
     check(outs[1][0], want["y"], "y")
     check(outs[1][1], want["dx"], "dx")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,L,W,off", [(1, 1, 1, 0), (5, 70, 128, 0), (5, 33, 30, 0), (3, 40, 17, 0), (4, 300, 64, 1), (700, 9, 256, 0)])
+def test_padding_is_cleared(B, L, W, off, dtype):
+    """Out of place and in place, units of 16, 4 and 2 bytes; rows before the counts keep their bits, NaN among them."""
+    g = torch.Generator().manual_seed(L)
+    flat = torch.randn(B * L * W + off, generator=g).to(DEV, dtype)
+    x = flat[off:].view(B * L, W)
+    x[::3] = float("nan")
+    lens = torch.randint(-2, L + 3, (B,), generator=g, dtype=torch.int32)
+    lens[0] = L
+    live = (torch.arange(L)[None] < lens[:, None]).reshape(-1, 1).to(DEV)
+    want = torch.where(live, x, torch.zeros_like(x))
+    before = x.clone()
+    got = K.zero_padding(x, lens.to(DEV), torch.full_like(before, 7.0))
+    assert torch.equal(got.view(torch.uint8), want.view(torch.uint8)) and torch.equal(x.view(torch.uint8), before.view(torch.uint8))
+    assert K.zero_padding(x, lens.to(DEV), x) is x and torch.equal(x.view(torch.uint8), want.view(torch.uint8))

@@ -21,7 +21,7 @@ EXPORTS = [
     "vitk_gemm", "vitk_gemm_workspace_bytes", "vitk_attn_fwd", "vitk_attn_bwd", "vitk_attn_weights", "vitk_rope_qk", "vitk_rope_rows", "vitk_debug_hold_cus", "vitk_act_fwd",
     "vitk_act_bwd", "vitk_im2col", "vitk_col2im", "vitk_colsum", "vitk_colsum_static", "vitk_colsum_workspace_bytes", "vitk_scale_cast",
     "vitk_scale_cast_dgamma", "vitk_scale_cast_dgamma_workspace_bytes",
-    "vitk_prefix_fill", "vitk_copy_samples", "vitk_fourier_features", "vitk_fourier_features_bwd",
+    "vitk_prefix_fill", "vitk_copy_samples", "vitk_zero_padding", "vitk_fourier_features", "vitk_fourier_features_bwd",
     "vitk_qk_norm_rope_fwd", "vitk_qk_norm_rope_bwd", "vitk_qk_norm_rope_workspace_bytes",
     "vitk_attn_var_fwd", "vitk_attn_var_bwd", "vitk_attn_var_workspace_bytes",
 ]
@@ -149,6 +149,7 @@ def load() -> C.CDLL:
         "vitk_scale_cast_dgamma": [vp, i32, i64, vp, vp, vp, i32, vp, i32, vp, i64, i64, f32, f32, u64, vp, vp],
         "vitk_prefix_fill": [vp, i64, vp, i64, i32, vp, i32, i64, i64, i64, vp],
         "vitk_copy_samples": [vp, vp, vp, i64, i64, vp],
+        "vitk_zero_padding": [vp, vp, vp, i64, i64, i64, vp],
         "vitk_fourier_features": [vp, vp, vp, i32, i64, i64, i64, vp],
         "vitk_fourier_features_bwd": [vp, vp, vp, i32, vp, i64, i64, i64, vp],
     }

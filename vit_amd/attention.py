@@ -265,7 +265,7 @@ def attention_q_kv_packed(q, kv, w_q, b_q, w_kv, b_kv, w_norm, b_norm, use_layer
                           qk_normalization, attention_dropout, dropout, training, rope_q=None, rope_k=None, *,
                           kv_lengths=None) -> Tensor:
     """Same positional signature as the reference function (vit/attention.py:218-280).  ``kv_lengths`` [B]: the keys each
-    sample of ``kv`` has; rows behind them are padding."""
+    sample of ``kv`` has; rows behind them are padding, whatever they hold: no output and no gradient depends on them."""
     if attn_mask is not None:
         raise NotImplementedError("vit_amd: attention masks are not built")
     if qk_normalization:
@@ -274,6 +274,9 @@ def attention_q_kv_packed(q, kv, w_q, b_q, w_kv, b_kv, w_norm, b_norm, use_layer
         q_norm_weight = q_norm_bias = k_norm_weight = k_norm_bias = None
     opt = _sublayer_opts(head_dim=head_dim, eps=eps, layernorm=use_layer_norm, attention_dropout=attention_dropout,
                          dropout=dropout, training=training, residual=False, qk_eps=qk_eps, qk_layernorm=qk_use_layer_norm)
+    opt["zero_padding"] = kv_lengths is not None and _wants_grad(kv, w_kv, b_kv, k_norm_weight, k_norm_bias)
+    if opt["zero_padding"] and qk_normalization and not qk_eps > 0.0:
+        raise ValueError("vit_amd: kv_lengths with head norms need qk_eps above 0 where gradients are taken (the norm of a padded row)")
     return ops.CrossAttentionFn.apply(q, kv, w_norm, b_norm, w_q, b_q, w_kv, b_kv, w_out, b_out, q_norm_weight, q_norm_bias,
                                       k_norm_weight, k_norm_bias, None, None, rope_q, rope_k, opt, _key_counts(kv_lengths, kv.shape[0]))
 
@@ -341,6 +344,7 @@ class CrossAttention(nn.Module):
         opt = _sublayer_opts(head_dim=self._head_dim, eps=self.norm.eps or 1e-5, layernorm=self._use_layer_norm,
                              attention_dropout=self.attention_dropout.p, dropout=self.dropout.p, training=self.training,
                              residual=True, alpha=alpha, qk_eps=qk_eps, qk_layernorm=self._use_layer_norm)
+        opt["zero_padding"] = kv_lengths is not None and _wants_grad(kv, self.kv_proj.weight, self.kv_proj.bias, kw_, kb)
         return ops.CrossAttentionFn.apply(x, kv, self.norm.weight, get_norm_bias(self.norm), self.q_proj.weight,
                                           self.q_proj.bias, self.kv_proj.weight, self.kv_proj.bias, self.out_proj.weight,
                                           self.out_proj.bias, qw, qb, kw_, kb, gamma, keep_idx, rope_q, rope_k, opt,
@@ -423,7 +427,7 @@ class AttentivePool(nn.Module):
         self.cross_attention.reset_parameters()
 
     def forward(self, x: Tensor, lengths: Optional[Tensor] = None) -> Tensor:
-        """``lengths`` [B]: the tokens each sample has; rows of x behind them are padding."""
+        """``lengths`` [B]: the tokens each sample has; rows of x behind them are padding, whatever they hold."""
         y = self.cross_attention(self.query.expand(x.shape[0], -1, -1), x, kv_lengths=lengths)
         return y.squeeze(1) if y.shape[1] == 1 else y
 

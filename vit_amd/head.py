@@ -54,7 +54,7 @@ class AttentivePoolHead(nn.Module):
         self.proj.reset_parameters()
 
     def forward(self, x: Tensor, lengths: Optional[Tensor] = None) -> Tensor:
-        """``lengths`` [B]: the tokens each sample has; rows of x behind them are padding."""
+        """``lengths`` [B]: the tokens each sample has; rows of x behind them are padding, whatever they hold."""
         return self.proj(self.pool(x, lengths))
 
     def forward_weights(self, x: Tensor) -> Tensor:

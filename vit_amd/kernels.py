@@ -505,6 +505,20 @@ def copy_samples_(dst: Tensor, src: Tensor, idx: Tensor, sample_elems: int) -> T
     return dst
 
 
+def zero_padding(x: Tensor, kv_len: Tensor, out: Tensor) -> Tensor:
+    """out = the rows of x [B * L, W] that lie before their sample's count (int32 [B]), zeros in place of the others; ``out`` may
+    be x itself, whose live rows are then left alone."""
+    lib = L.load()
+    L.require_gpu(x, kv_len, out)
+    B, rows = kv_len.numel(), x.shape[0]
+    assert x.is_contiguous() and out.is_contiguous() and out.shape == x.shape and out.dtype == x.dtype and (rows % B == 0 if B else rows == 0)
+    assert kv_len.dtype == torch.int32 and kv_len.is_contiguous()
+    if rows:
+        L.check(lib.vitk_zero_padding(x.data_ptr(), out.data_ptr(), kv_len.data_ptr(), B, rows // B, x.shape[1] * x.element_size(),
+                                      L.stream()))
+    return out
+
+
 def prefix_fill_(out: Tensor, cls_tokens: Tensor, register_tokens: Tensor) -> Tensor:
     """Rows 0 .. ncls + nreg - 1 of every sample of out [B, S, D] <- cls [1, ncls, D], register tokens [1, nreg, D]."""
     lib = L.load()

@@ -689,7 +689,10 @@ class AttentionSublayerFn(torch.autograd.Function):
 class CrossAttentionFn(torch.autograd.Function):
     """q -> q (+) alpha * gamma * dropout(out_proj(SDPA(q_proj(norm(q)), kv_proj(kv))))   (vit/attention.py:112-162,
     :218-280; the residual form is the cross sub-layer of vit/transformer.py:262-284 and :367-384).  Lq queries attend
-    to Lk keys; the norm is on the query side only.  ``keep_idx`` (drop-path) selects samples of q and of kv alike."""
+    to Lk keys; the norm is on the query side only.  ``keep_idx`` (drop-path) selects samples of q and of kv alike.
+    ``kv_len`` counts the rows of kv each sample has.  The attention never reads the others, but a weight's gradient sums over all
+    rows, and the zeros that padded rows contribute would not survive a NaN there: opt["zero_padding"] (a gradient on the side of kv is
+    wanted) clears what holds such rows, in the copy of kv where the call makes one, else in a copy made for the gradient."""
 
     @staticmethod
     def forward(ctx, q, kv, norm_w, norm_b, w_q, b_q, w_kv, b_kv, w_out, b_out, qn_w, qn_b, kn_w, kn_b, gamma, keep_idx,
@@ -716,16 +719,22 @@ class CrossAttentionFn(torch.autograd.Function):
                                     opt["layernorm"], tc, rows)
         kv_kept = kv.detach() if keep_idx is None else kv.detach().index_select(0, keep_idx)   # vit/transformer.py:49-54
         kv2 = _cast(kv_kept.reshape(Mk, D), tc)
+        if kv_len is not None and keep_idx is not None:
+            kv_len = kv_len.index_select(0, keep_idx)
+        zero_padding = kv_len is not None and opt["zero_padding"]
+        own_kv = kv2.data_ptr() != kv.data_ptr()   # cast, gathered or made contiguous: not the caller's memory
+        if zero_padding and own_kv:
+            K.zero_padding(kv2, kv_len, kv2)
         wq, bq, wkv, bkv, wo, bo = (_cast(t, tc) for t in (w_q, b_q, w_kv, b_kv, w_out, b_out))
         qp = torch.empty((Mq, D), dtype=tc, device=q.device)
         K.gemm(qn, wq, trans_a=False, trans_b=False, M=Mq, N=D, K=D, out=qp, bias=bq)
         kvp = torch.empty((Mk, 2 * D), dtype=tc, device=q.device)
         K.gemm(kv2, wkv, trans_a=False, trans_b=False, M=Mk, N=2 * D, K=D, out=kvp, bias=bkv)
+        if zero_padding and not own_kv and qn_w is not None:   # the key norm's gradient sums over all rows, too
+            K.zero_padding(kvp, kv_len, kvp)
         qk_saved = (None,) * 6
         tq, emu_q = _rope_table(rope_q, keep_idx, B, Bk, tc)   # vit/attention.py:156-159
         tk, emu_k = _rope_table(rope_k, keep_idx, B, Bk, tc)
-        if kv_len is not None and keep_idx is not None:
-            kv_len = kv_len.index_select(0, keep_idx)
         # per-head normalisation and rotation of q and k in one pass into buffers of their own (v stays in the projection)
         emus = {e for t, e in ((tq, emu_q), (tk, emu_k)) if t is not None}
         fuse_pass = qn_w is not None and K.can_qk_norm_rope(tc, Dh) and qn_w.dtype == kn_w.dtype and len(emus) < 2
@@ -774,6 +783,7 @@ class CrossAttentionFn(torch.autograd.Function):
                               tq, tk, kv_len, *qk_saved)
         ctx.emu = (emu_q, emu_k)
         ctx.fuse_pass = fuse_pass
+        ctx.pads_kv = zero_padding and not own_kv   # kv2 is the caller's, padding and all
         ctx.meta = (B, Bk, Lq, Lk, D, H, Dh, tc, tr, p_attn, p_hid, seed_a, seed_h, opt, q.dtype, kv.dtype, w_q.dtype,
                     norm_b is not None, b_q is not None, b_kv is not None, b_out is not None, qn_b is not None,
                     kn_b is not None)
@@ -825,6 +835,8 @@ class CrossAttentionFn(torch.autograd.Function):
                                         need[12], has_knb and need[13])
             dkvp[:, :D].copy_(dk_pre.view(Mk, D))
         dqn_in, dwq, dbq = _linear_bwd(dqp, qn, wq, True, need[4], has_bq and need[5], wdtype)
+        if ctx.pads_kv and need[6]:
+            kv2 = K.zero_padding(kv2, kv_len, torch.empty_like(kv2))
         dkv_in, dwkv, dbkv = _linear_bwd(dkvp, kv2, wkv, need[1], need[6], has_bkv and need[7], wdtype)
         if residual:
             if rows is None:

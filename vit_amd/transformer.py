@@ -160,7 +160,7 @@ class TransformerDecoderLayer(nn.Module):
     def forward(self, x: Tensor, kv: Union[Tensor, KVMemory], rope_q: Optional[Tensor] = None,
                 rope_k: Optional[Tensor] = None, kv_lengths: Optional[Tensor] = None,
                 buckets: Optional[RelativeBuckets] = None) -> Tensor:
-        """``kv_lengths`` [B]: the rows of ``kv`` each sample has, the others are padding.  ``kv`` may be what
+        """``kv_lengths`` [B]: the rows of ``kv`` each sample has, the others are padding, whatever they hold.  ``kv`` may be what
         ``cross_attention.project_kv`` made of it (inference).  ``buckets``: the relative position bias of x's tokens."""
         idx, scale = _select_keep_indices(x, self.drop_path_rate, self.training)
         x = self.self_attention.fused_residual(x, rope_q, getattr(self.layer_scale_attn, "gamma", None), idx, scale, buckets)
