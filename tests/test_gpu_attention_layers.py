@@ -359,3 +359,35 @@ def test_pooling_trains_on_padding_that_holds_anything(frozen):
         grads.append([p.grad.clone() for p in head.parameters()] + ([] if frozen else [xg.grad]))
     for a, b in zip(*grads):
         assert torch.isfinite(b).all() and torch.equal(a, b)
+
+
+def relative_vit(**kw):
+    cfg = dict(in_channels=3, patch_size=(8, 8), img_size=(96, 96), depth=1, hidden_size=128, ffn_hidden_size=256, num_attention_heads=2,
+               pos_enc="relative", dtype=torch.bfloat16, hidden_dropout=0.0, attention_dropout=0.0)
+    return ViTConfig(**{**cfg, **kw}).instantiate(device=DEV).eval()
+
+
+def test_dropped_plans_keep_their_memory_until_their_streams_are_through():
+    """A plan made on one stream and used on another, dropped by eight newer grids while that work is still waiting: what is
+    allocated meanwhile does not get its memory; once the work is done, it does."""
+    model = relative_vit()
+    model.prepare_buckets((12, 12))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(side):
+        model(torch.randn(1, 3, 96, 96, device=DEV, dtype=torch.bfloat16))
+        torch.cuda._sleep(400_000_000)   # some tenths of a second
+    plan = model.prepare_buckets((12, 12))
+    place = {t.data_ptr(): t.numel() * t.element_size() for t in (plan.index16, plan.order)}
+    del plan
+    busy = not side.query()
+    for n in range(1, 9):
+        model.prepare_buckets((1, n))
+    assert ((12, 12), model.cls_tokens.device) not in model._bucket_plans
+    held = [torch.empty(16384, device=DEV, dtype=torch.uint8) for _ in range(2000)]
+    still = not side.query()
+    if busy and still:
+        for t in held:
+            assert not any(at < t.data_ptr() + t.numel() and t.data_ptr() < at + n for at, n in place.items())
+    torch.cuda.synchronize()
+    assert busy and still, "the side stream was through too early to tell"

@@ -166,6 +166,12 @@ class RelativeBuckets:
         new.__dict__.update({k: v.to(device) if isinstance(v, Tensor) else v for k, v in self.__dict__.items()})
         return new
 
+    def record_stream(self, stream) -> None:
+        """``Tensor.record_stream`` for the plan: its memory is not given away before what ``stream`` has been asked to do until
+        the plan is dropped."""
+        for t in (self.index16, self.order, self.piece, self.bucket_piece):
+            t.record_stream(stream)
+
     @classmethod
     def grid(cls, dims: Sequence[int], num_prefix_tokens: int = 0, device=None, table_dims: Optional[Sequence[int]] = None):
         """Tokens of a grid behind ``num_prefix_tokens`` prefix tokens: a bucket for every offset between two grid tokens of

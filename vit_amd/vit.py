@@ -85,9 +85,11 @@ class ViT(nn.Module):
 
     def prepare_buckets(self, tokenized_size: Sequence[int]) -> RelativeBuckets:
         """Plan of the relative position bias for a token grid up to the configured one; the last eight are kept per grid and
-        device, and for good what a graph being captured uses (its replays read the plan's memory)."""
+        device, and for good what a graph being captured uses (its replays read the plan's memory).  A plan that is dropped keeps
+        its memory until the streams it was used on are through with it."""
         full = tuple(self.stem.tokenized_size(tuple(self._config.img_size)))
         key = (tuple(tokenized_size), self.cls_tokens.device)
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         plan = self._bucket_plans.get(key)
         if plan is None:
             plan = RelativeBuckets.grid(key[0], self._num_prefix, device=key[1], table_dims=full)
@@ -95,8 +97,10 @@ class ViT(nn.Module):
             for k in old[:max(len(old) - 7, 0)]:
                 del self._bucket_plans[k]
             self._bucket_plans[key] = plan
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        if capturing:
             self._captured_plans.add(key)
+        elif plan.device.type == "cuda":
+            plan.record_stream(torch.cuda.current_stream(plan.device))
         return plan
 
     def _layer(self, layer_type, mlp_quantization_config, qkv_quantization_config, attn_quantization_config, device, dtype, **extra):
