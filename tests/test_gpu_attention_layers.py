@@ -391,3 +391,23 @@ def test_dropped_plans_keep_their_memory_until_their_streams_are_through():
             assert not any(at < t.data_ptr() + t.numel() and t.data_ptr() < at + n for at, n in place.items())
     torch.cuda.synchronize()
     assert busy and still, "the side stream was through too early to tell"
+
+
+def test_a_plan_is_not_made_during_capture():
+    model = relative_vit()
+    x = torch.randn(2, 3, 64, 96, device=DEV, dtype=torch.bfloat16)
+    with torch.no_grad():
+        model(torch.randn(2, 3, 96, 96, device=DEV, dtype=torch.bfloat16))
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                model(x)
+        want = model(x).dense_features.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = model(x).dense_features
+        for _ in range(2):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)

@@ -86,12 +86,16 @@ class ViT(nn.Module):
     def prepare_buckets(self, tokenized_size: Sequence[int]) -> RelativeBuckets:
         """Plan of the relative position bias for a token grid up to the configured one; the last eight are kept per grid and
         device, and for good what a graph being captured uses (its replays read the plan's memory).  A plan that is dropped keeps
-        its memory until the streams it was used on are through with it."""
+        its memory until the streams it was used on are through with it.  Making one reads back to the host, so that a graph's
+        capture needs its plan to be there: call this, or the model, with the same grid before."""
         full = tuple(self.stem.tokenized_size(tuple(self._config.img_size)))
         key = (tuple(tokenized_size), self.cls_tokens.device)
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         plan = self._bucket_plans.get(key)
         if plan is None:
+            if capturing and key[1].type == "cuda":
+                raise RuntimeError(f"vit_amd: the plan of the relative position bias for a grid of {key[0]} cannot be made while a graph is "
+                                   "captured; call prepare_buckets (or the model) with this grid first")
             plan = RelativeBuckets.grid(key[0], self._num_prefix, device=key[1], table_dims=full)
             old = [k for k in self._bucket_plans if k not in self._captured_plans]
             for k in old[:max(len(old) - 7, 0)]:
