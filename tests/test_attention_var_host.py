@@ -12,6 +12,7 @@ import torch
 
 from vit_amd import KVMemory, RelativeBuckets, ViTConfig, _lib, kernels, ops, qk_norm_rope
 from vit_amd.attention import CrossAttention, SelfAttention, attention, attention_q_kv_packed
+from vit_amd.transformer import TransformerEncoderLayer
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -364,3 +365,35 @@ def test_head_norms_of_padded_rows_need_an_eps():
         a[2] = torch.zeros(64, 32, requires_grad=wkv_grad)
         with pytest.raises(error, match="qk_eps" if error is ValueError else "no CPU fallback|MI355X"):
             attention_q_kv_packed(q, kv, *a, eps, True, 0.0, 0.0, True, kv_lengths=lens)
+
+
+@pytest.mark.parametrize("ckpt", [False, True])
+@pytest.mark.parametrize("pos_enc", ["none", "relative"])
+def test_blocks_without_a_relative_bias_are_called_as_ever(pos_enc, ckpt):
+    """A model whose blocks override forward(x, rope) runs; with a relative bias they get its plan."""
+    seen = []
+
+    class Block(TransformerEncoderLayer):
+        def forward(self, x, rope=None):
+            seen.append(None)
+            return x + 1
+
+    class BiasBlock(TransformerEncoderLayer):
+        def forward(self, x, rope=None, buckets=None):
+            seen.append(buckets)
+            return x + 1
+
+    class Stem(torch.nn.Module):
+        def tokenized_size(self, size):
+            return tuple(s // 8 for s in size)
+
+        def forward(self, x, prefix=None):
+            return torch.zeros(1, 12, 64, requires_grad=True)
+
+    model = ViTConfig(in_channels=3, patch_size=(8, 8), img_size=(32, 24), depth=2, hidden_size=64, ffn_hidden_size=128,
+                      num_attention_heads=2, pos_enc=pos_enc, dtype=torch.float32, activation_checkpointing=ckpt).instantiate().train()
+    model.stem = Stem()
+    model.blocks = torch.nn.ModuleList([(BiasBlock if pos_enc == "relative" else Block)(64, 128, 2) for _ in range(2)])
+    out = model(torch.zeros(1, 3, 32, 24), output_norm=False)
+    assert bool((out.dense_features == 2).all())
+    assert [s if s is None else s.shape for s in seen] == [None if pos_enc == "none" else (12, 12)] * 2

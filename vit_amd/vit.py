@@ -213,10 +213,12 @@ class ViT(nn.Module):
         rope = self.prepare_rope(grid, mask, rope_seed) if self.rope is not None else None
         for block in self.blocks:
             assert isinstance(block, TransformerEncoderLayer)
+            # only blocks with a relative bias are called with its plan: others need not know the argument
+            extra = {} if buckets is None else {"buckets": buckets}
             if c.activation_checkpointing and self.training:
-                x = checkpoint(block, x, rope, buckets, use_reentrant=False)
+                x = checkpoint(block, x, rope, use_reentrant=False, **extra)
             else:
-                x = block(x, rope=rope, buckets=buckets)
+                x = block(x, rope=rope, **extra)
         if output_norm:
             x = self.output_norm(x)
         return ViTFeatures(x, c.num_register_tokens, c.num_cls_tokens, grid)
