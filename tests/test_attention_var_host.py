@@ -397,3 +397,15 @@ def test_blocks_without_a_relative_bias_are_called_as_ever(pos_enc, ckpt):
     out = model(torch.zeros(1, 3, 32, 24), output_norm=False)
     assert bool((out.dense_features == 2).all())
     assert [s if s is None else s.shape for s in seen] == [None if pos_enc == "none" else (12, 12)] * 2
+
+
+def test_plans_are_made_under_any_default_device():
+    """The index decides where a plan lives, not torch's default device (meta stands for a GPU here)."""
+    index = torch.randint(0, 9, (20, 30), generator=torch.Generator().manual_seed(1))
+    made = lambda: (RelativeBuckets(index, 9), RelativeBuckets.grid((3, 4), 2, device="cpu"), RelativeBuckets.log_distance(20, 30, device="cpu"))
+    want = made()
+    with torch.device("meta"):
+        got = made()
+    for a, b in zip(got, want):
+        for n in ("index16", "order", "piece", "bucket_piece"):
+            assert torch.equal(getattr(a, n), getattr(b, n)), n

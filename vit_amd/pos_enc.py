@@ -149,8 +149,8 @@ class RelativeBuckets:
         pieces = (counts + length - 1) // length
         bucket_piece = torch.cat([pieces.new_zeros(1), pieces.cumsum(0)])
         starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
-        owner = torch.repeat_interleave(torch.arange(num_buckets), pieces)          # bucket of every piece
-        within = torch.arange(int(bucket_piece[-1])) - bucket_piece[owner]
+        owner = torch.repeat_interleave(torch.arange(num_buckets, device="cpu"), pieces)          # bucket of every piece
+        within = torch.arange(int(bucket_piece[-1]), device="cpu") - bucket_piece[owner]
         piece = torch.cat([starts[owner] + within * length, starts[-1:]])
         self.num_pieces = int(bucket_piece[-1])
         self.piece = piece.to(torch.int32).to(index.device)
@@ -181,17 +181,17 @@ class RelativeBuckets:
         table_dims = tuple(int(d) for d in (table_dims or dims))
         if len(dims) != len(table_dims) or any(d < 1 or d > t for d, t in zip(dims, table_dims)):
             raise ValueError(f"a table for grids up to {table_dims} does not cover a {dims} grid")
-        pos = torch.stack(torch.meshgrid([torch.arange(d) for d in dims], indexing="ij"), dim=-1).view(-1, len(dims))
+        pos = torch.stack(torch.meshgrid([torch.arange(d, device="cpu") for d in dims], indexing="ij"), dim=-1).view(-1, len(dims))
         num = cls.grid_buckets(table_dims, num_prefix_tokens)
-        idx = torch.zeros((pos.shape[0], pos.shape[0]), dtype=torch.int64)
+        idx = torch.zeros((pos.shape[0], pos.shape[0]), dtype=torch.int64, device="cpu")
         for axis, t in enumerate(table_dims):
             idx = idx * (2 * t - 1) + (pos[:, None, axis] - pos[None, :, axis] + t - 1)
         n = int(num_prefix_tokens)
         if n:
-            full = torch.empty((n + pos.shape[0],) * 2, dtype=torch.int64)
+            full = torch.empty((n + pos.shape[0],) * 2, dtype=torch.int64, device="cpu")
             full[n:, n:], full[:n, n:], full[n:, :n], full[:n, :n] = idx, num - 3, num - 2, num - 1
             idx = full
-        return cls(idx.to(device) if device is not None else idx, num)
+        return cls(idx.to(torch.get_default_device() if device is None else device), num)
 
     @staticmethod
     def grid_buckets(table_dims: Sequence[int], num_prefix_tokens: int = 0) -> int:
@@ -207,7 +207,8 @@ class RelativeBuckets:
             raise ValueError(f"log_distance needs num_buckets a multiple of 4 and max_distance > num_buckets / 4, got "
                              f"{num_buckets}, {max_distance}")
         far = max(num_queries, num_keys)
-        d = torch.arange(max(far, 1), dtype=torch.float64)
+        device = torch.get_default_device() if device is None else device
+        d = torch.arange(max(far, 1), dtype=torch.float64, device="cpu")
         log = exact + torch.floor(torch.log(d.clamp_min(1) / exact) / math.log(max_distance / exact) * (half - exact) + 1e-9)
         table = torch.where(d < exact, d, log.clamp_max(half - 1)).to(torch.int64).to(device)
         rel = torch.arange(num_keys, device=device)[None, :] - torch.arange(num_queries, device=device)[:, None]
