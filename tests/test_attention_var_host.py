@@ -1,9 +1,11 @@
 """Host side of the relative position bias, the key counts and the per-head normalisation pass: bucket plans against brute
 force, and the refusals, which need no GPU."""
+import copy
 import ctypes
 import itertools
 import math
 import os
+import pickle
 import re
 import subprocess
 
@@ -409,3 +411,16 @@ def test_plans_are_made_under_any_default_device():
     for a, b in zip(got, want):
         for n in ("index16", "order", "piece", "bucket_piece"):
             assert torch.equal(getattr(a, n), getattr(b, n)), n
+
+
+def test_copies_and_saved_models_carry_no_plans():
+    model = ViTConfig(in_channels=3, patch_size=(8, 8), img_size=(256, 256), depth=1, hidden_size=64, ffn_hidden_size=128,
+                      num_attention_heads=2, pos_enc="relative", dtype=torch.float32).instantiate()
+    size = lambda: len(pickle.dumps(model))
+    before = size()
+    plan = model.prepare_buckets((32, 32))
+    assert size() - before < 4096 and model.prepare_buckets((32, 32)) is plan
+    for other in (copy.deepcopy(model), pickle.loads(pickle.dumps(model))):
+        assert other._bucket_plans == {} and other._captured_plans == set() and other.prepare_buckets((32, 32)) is not plan
+        assert all(torch.equal(a, b) for a, b in zip(other.state_dict().values(), model.state_dict().values()))
+    assert model.prepare_buckets((32, 32)) is plan

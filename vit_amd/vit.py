@@ -68,6 +68,11 @@ class ViT(nn.Module):
         self.self_attention_requires_grad_(config.self_attention_requires_grad)
         self.heads = nn.ModuleDict({name: self.create_head(name, hc, device=device) for name, hc in config.heads.items()})
 
+    def __getstate__(self) -> dict:
+        """A copy or a saved module makes its plans itself: these are as large as the pairs, belong to one device, and their
+        tensors would follow a map_location that their keys do not."""
+        return {**self.__dict__, "_bucket_plans": {}, "_captured_plans": set()}
+
     # ---- construction helpers ------------------------------------------------------------------
     @property
     def config(self) -> ViTConfig:
