@@ -760,3 +760,44 @@ def test_padding_is_cleared(B, L, W, off, dtype):
     got = K.zero_padding(x, lens.to(DEV), torch.full_like(before, 7.0))
     assert torch.equal(got.view(torch.uint8), want.view(torch.uint8)) and torch.equal(x.view(torch.uint8), before.view(torch.uint8))
     assert K.zero_padding(x, lens.to(DEV), x) is x and torch.equal(x.view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("algo", [0, 1])
+@pytest.mark.parametrize("Lq,Lk,nb,counts", [(4, 1000, 4, None), (32, 300, 2, [300, 129]), (1, 700, 3, [128, 700]), (40, 500, 2, [500, 65])])
+def test_table_gradients_do_not_see_the_rounding_of_the_output(Lq, Lk, nb, counts, algo):
+    """bf16 operands, a float32 table, values with a common offset: what O's rounding to bf16 leaves in delta would add up over
+    every bucket that holds much of a row.  Bound of an entry, sums over samples and rows i, and keys j of the bucket:
+      * the row sums are those of numerators rounded to bf16: every probability of a row off by one factor 1 + eta, |eta| <= u
+        + (Lk + 8) U, which reaches the entry through |sum_j dS_ij| alone;
+      * otherwise 32-bit errors: rho of a probability (the exponential's argument, as above), Dh U |G| |V| of dP, and of
+        delta = sum P dP / sum P what these and a sum of Lk leave, or for more than 32 rows and in the portable kernels (delta
+        from O, less the sum of dS) eta times the rounding of O on top: u |G| |O|."""
+    B, H, Dh = 2, 2, 64
+    q, k, v, dout = make(B, Lq, Lk, H, Dh, torch.bfloat16, Lq + Lk, packed=False)
+    v = (v.float() + 4.0).bfloat16()
+    index = torch.randint(0, nb, (Lq, Lk), generator=torch.Generator().manual_seed(3))
+    table = torch.randn(nb, H, generator=torch.Generator().manual_seed(4)).bfloat16().float().to(DEV)
+    kw = {} if counts is None else dict(kv_lengths=torch.tensor(counts, device=DEV))
+    got = run(q, k, v, dout, algo, bias_table=table, buckets=RelativeBuckets(index, nb).to(DEV), **kw)["dtable"].double().cpu()
+    Q, Kk, V, G = [t.double().cpu().transpose(1, 2) for t in (q, k, v, dout)]
+    dead = torch.zeros(B, 1, 1, Lk, dtype=torch.bool) if counts is None else (torch.arange(Lk)[None] >= torch.tensor(counts)[:, None])[:, None, None]
+    bias = table.double().cpu()[index].permute(2, 0, 1)
+    s = (Dh ** -0.5 * Q @ Kk.transpose(-1, -2) + bias).masked_fill(dead, -math.inf)
+    P = s.softmax(-1)
+    top = s.amax(-1, keepdim=True).abs()
+    rho = (Dh + 8) * U * (Dh ** -0.5 * Q.abs() @ Kk.abs().transpose(-1, -2) + bias.abs() + top + 1.0)
+    rho = 2 * rho + 2 * rho.amax(-1, keepdim=True) + 8 * U
+    dP = G @ V.transpose(-1, -2)
+    delta = (P * dP).sum(-1, keepdim=True)
+    dS = P * (dP - delta)
+    u = half_step(torch.bfloat16)
+    eta = u + (Lk + 8) * U
+    edp = (Dh + 4) * U * (G.abs() @ V.abs().transpose(-1, -2))
+    ed = (2 * rho * dS.abs() + P * edp).sum(-1, keepdim=True) + (Lk + 8) * U * (P * dP.abs()).sum(-1, keepdim=True)
+    ed = ed + 2 * eta * u * (G.abs() * (P @ V).abs()).sum(-1, keepdim=True)
+    fine = (rho * dS.abs() + P * (edp + ed)) * (1 + 1 / 16) + min(B * Lq * Lk, 4096) * U * dS.abs()
+    for n in range(nb):
+        m = (index == n).double()
+        val = (dS * m).sum((0, 2, 3))
+        bound = (eta * (dS * m).sum(-1).abs()).sum((0, 2)) + (fine * m).sum((0, 2, 3)) + 2 * U * val.abs()
+        check(got[n], (val, bound), f"bucket {n}")

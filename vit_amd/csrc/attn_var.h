@@ -18,7 +18,8 @@ struct VarP {
   const bf16 *bias_s, *bias_t; // the bias laid out in accumulator order (var_expand_k), keys or queries on the rows
   float* dbias;                // [splits][H][Lq][Lk]
   float* part;                 // split forward: [splits][B, H, Lq][Dh]; few-query backward: [blocks][B, H, Lq][Dh]
-  float* pstat;                // split forward: [splits][B, H, Lq][2] (m, sum)
+  float* pstat;                // split forward: [splits][B, H, Lq][2] (m, sum); few-query backward with a table's gradient:
+                               // [blocks][B, H, Lq][2] (sum P dP, sum P), otherwise NULL
   int64_t q_sb, q_sh, q_ss, k_sb, k_sh, k_ss, v_sb, v_sh, v_ss, o_sb, o_sh, o_ss, g_sb, g_sh, g_ss;
   int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
   int B, H, Lq, Lk, Dh;

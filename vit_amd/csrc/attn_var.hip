@@ -131,6 +131,7 @@ __global__ __launch_bounds__(256) void var_dq_simple_k(VarP p) {
   const int64_t srow = (b * p.H + h) * p.Lq + qrow;
   const float m = qv ? p.stat[2 * srow] : 0.f, lr = qv ? p.stat[2 * srow + 1] : 0.f, delta = qv ? p.delta[srow] : 0.f;
   const float c = p.scale * LOG2E;
+  float dsum = 0.f;
   const uint64_t rbase = (uint64_t)srow * var_drop_ld(p);
   for (int64_t k0 = 0; k0 < len; k0 += VT) {
     __syncthreads();
@@ -151,6 +152,7 @@ __global__ __launch_bounds__(256) void var_dq_simple_k(VarP p) {
       const float pr = exp2f(__fmul_rn(s - m, c) + lr);
       if (p.thr) dp = rng_u32(p.seed, rbase + (uint64_t)(k0 + kk)) >= p.thr ? dp * p.keep_scale : 0.f;
       const float ds = pr * (dp - delta);
+      dsum += ds;
 #pragma unroll
       for (int i = 0; i < VMAXI; i++) {
         const int d = part + 4 * i;
@@ -159,6 +161,9 @@ __global__ __launch_bounds__(256) void var_dq_simple_k(VarP p) {
     }
   }
   if (!qv) return;
+  // The rows of dS sum to zero; what they do sum to is what O's rounding left in delta, and a bucket of the bias gradient would
+  // add it up: the kernels that follow get delta without it.
+  if (p.table && part == 0) p.delta[srow] = delta + dsum;
   T* op = (T*)p.dq + b * p.dq_sb + h * p.dq_sh + qrow * p.dq_ss;
 #pragma unroll
   for (int i = 0; i < VMAXI; i++) {
@@ -452,7 +457,10 @@ static VarWs var_ws(const VitkAttnVar* a, bool bwd) {
   } else {
     w.delta = take(rows * 4);
     w.nl = take(rows * 4);
-    if (mfma && var_few(a)) w.part = take((size_t)ceil_div(a->Lk, 128) * rows * a->Dh * 4);
+    if (mfma && var_few(a)) {
+      w.part = take((size_t)ceil_div(a->Lk, 128) * rows * a->Dh * 4);
+      if (a->dbias_table) w.pstat = take((size_t)ceil_div(a->Lk, 128) * rows * 8);
+    }
     if (a->dbias_table) {
       w.splits = mfma ? var_dbias_splits(a) : 1;
       w.dbias = take((size_t)w.splits * a->H * a->Lq * a->Lk * 4);
@@ -533,6 +541,7 @@ extern "C" int vitk_attn_var_bwd(const VitkAttnVar* desc, void* stream) {
       var_launch_expand(p, true, st);
     }
     if (var_few(a)) {
+      if (a->dbias_table) p.pstat = (float*)(ws + w.pstat);
       var_launch_few_bwd(p, bias, st);
     } else {
       var_launch_dq(p, bias, st);     // writes delta
