@@ -801,3 +801,90 @@ def test_table_gradients_do_not_see_the_rounding_of_the_output(Lq, Lk, nb, count
         val = (dS * m).sum((0, 2, 3))
         bound = (eta * (dS * m).sum(-1).abs()).sum((0, 2)) + (fine * m).sum((0, 2, 3)) + 2 * U * val.abs()
         check(got[n], (val, bound), f"bucket {n}")
+
+
+def dropout_call(q, k, v, dout, p, algo, **kw):
+    torch.cuda.manual_seed(31)
+    table = kw.pop("bias_table", None)
+    old = K.set_algo(algo)
+    try:
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v) + (() if table is None else (table,))]
+        o = attention(*leaves[:3], bias_table=None if table is None else leaves[3], dropout=p, training=True, **kw)
+        return dict(zip(("o", "dq", "dk", "dv", "dtable"), (o, *torch.autograd.grad(o, leaves, dout))))
+    finally:
+        K.set_algo(old)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("Lq,Lk,H,Dh,bias,counts", [
+    (90, 65, 2, 64, True, False), (3, 129, 2, 64, True, False), (150, 197, 1, 80, True, True), (40, 300, 2, 64, False, True),
+    (1, 577, 3, 88, False, True), (197, 197, 2, 128, True, False), (300, 130, 1, 96, True, True), (33, 64, 1, 32, False, False)])
+def test_dropout_beyond_one_tile_of_keys(Lq, Lk, H, Dh, bias, counts, dtype):
+    """Odd key counts, key tiles behind the first, several blocks of rows and of keys, counts: the mask is read off the forward
+    passes of one seed with unit vectors for 64 keys (or Dh, if fewer) at a time as the values; the gradients are those of that
+    very mask, in both kernel families; 1 - p of the live probabilities are kept."""
+    B, p = 2, 0.3
+    q, k, v, dout = make(B, Lq, Lk, H, Dh, dtype, Lq + Lk, packed=Lq % 2 == 0)
+    lens = [Lk, Lk // 2 + 1] if counts else [Lk] * B
+    kw = dict(kv_lengths=torch.tensor(lens, device=DEV)) if counts else {}
+    full = index = None
+    if bias:
+        index = torch.randint(0, 9, (Lq, Lk), generator=torch.Generator().manual_seed(2))
+        kw.update(bias_table=torch.randn(9, H, generator=torch.Generator().manual_seed(3)).to(DEV, dtype), buckets=RelativeBuckets(index, 9).to(DEV))
+        full = kw["bias_table"].double().cpu()[index].permute(2, 0, 1)
+
+    def mask(algo):
+        cols = []
+        width = min(64, Dh)
+        for k0 in range(0, Lk, width):
+            unit = torch.zeros(B, Lk, H, Dh, device=DEV, dtype=dtype)
+            n = min(width, Lk - k0)
+            unit[:, k0:k0 + n, :, :n] = torch.eye(n, device=DEV, dtype=dtype)[None, :, None]
+            o = dropout_call(q, k, unit, dout, p, algo, **kw)["o"]
+            cols.append((o.detach() > 0).cpu().transpose(1, 2)[..., :n])
+        return torch.cat(cols, -1)
+
+    keep = mask(0)
+    live = (torch.arange(Lk)[None] < torch.tensor(lens)[:, None])[:, None, None].expand(B, H, Lq, Lk)
+    assert not keep[~live].any()
+    n = int(live.sum())
+    assert abs(keep[live].double().mean().item() - (1 - p)) < 5 * math.sqrt(p * (1 - p) / n) + 1e-3
+    assert torch.equal(mask(1), keep)   # both kernel families draw the same mask
+    want = reference(q, k, v, Dh ** -0.5, full, lens, dout, keep=keep.double() / (1 - p))
+    dS = want.pop("dS")
+    if bias:
+        want["dtable"] = bucket_sums(*dS, index, 9, dtype)
+    for algo in (0, 1):
+        got = dropout_call(q, k, v, dout, p, algo, **kw)
+        for name, w in want.items():
+            check(got[name], w, f"{name}, algo {algo}")
+
+
+def test_every_dropout_call_draws_a_seed_of_its_own():
+    q, k, v, dout = make(1, 40, 64, 1, 64, torch.bfloat16, 3, packed=True)
+    torch.cuda.manual_seed(5)
+    first, second = (attention(q, k, v, dropout=0.5, training=True) for _ in range(2))
+    torch.cuda.manual_seed(5)
+    again = attention(q, k, v, dropout=0.5, training=True)
+    assert torch.equal(first, again) and not torch.equal(first, second)
+    gen = torch.cuda.default_generators[torch.cuda.current_device()]
+    before = gen.get_state()
+    attention(q, k, v, dropout=0.5, training=False)
+    attention(q, k, v, training=True)
+    assert torch.equal(gen.get_state(), before)   # nothing is drawn where nothing is dropped
+
+
+@pytest.mark.parametrize("algo", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,Lq,Lk,H,Dh", [(2, 1, 300, 4, 128), (2, 17, 200, 1, 128), (1, 48, 700, 2, 64), (1, 48, 700, 2, 128), (2, 9, 130, 3, 120)])
+def test_wide_heads_of_few_queries_and_two_waves_that_share_keys(B, Lq, Lk, H, Dh, dtype, algo):
+    """Head sizes above 96 with up to 32 queries (other buffer counts), 33 to 64 queries over enough keys to be shared out."""
+    q, k, v, dout = make(B, Lq, Lk, H, Dh, dtype, Lq * 5 + Lk, packed=Dh == 64)
+    index = torch.randint(0, 11, (Lq, Lk), generator=torch.Generator().manual_seed(Lk))
+    table = torch.randn(11, H, generator=torch.Generator().manual_seed(Lq)).to(DEV, dtype)
+    lens = [Lk - 1, 140][:B]
+    got = run(q, k, v, dout, algo, bias_table=table, buckets=RelativeBuckets(index, 11).to(DEV), kv_lengths=torch.tensor(lens, device=DEV))
+    want = reference(q, k, v, Dh ** -0.5, table.double().cpu()[index].permute(2, 0, 1), lens, dout)
+    want["dtable"] = bucket_sums(*want.pop("dS"), index, 11, dtype)
+    for n, w in want.items():
+        check(got[n], w, n)
