@@ -411,3 +411,26 @@ def test_a_plan_is_not_made_during_capture():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("layer_type", [SelfAttention, CrossAttention])
+def test_head_norm_weights_may_be_strided(layer_type):
+    """Norm weights that are every second element of something, through the layers that normalise and rotate in one pass."""
+    D, H, S = 160, 2, 11
+    plain = randomize(layer_type(D, H, 0.0, 0.0, qk_normalization=True, device=DEV, dtype=torch.bfloat16, norm_type="layernorm"))
+    strided = copy.deepcopy(plain)
+    for norm in (strided.q_norm, strided.k_norm):
+        for n in ("weight", "bias"):
+            wide = torch.zeros(160, device=DEV, dtype=torch.bfloat16)[::2]
+            setattr(norm, n, torch.nn.Parameter(wide.copy_(getattr(norm, n).detach())))
+            assert not getattr(norm, n).is_contiguous()
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(2, S, D, generator=g).to(DEV, torch.bfloat16)
+    args = (x,) if layer_type is SelfAttention else (x, torch.randn(2, 20, D, generator=g).to(DEV, torch.bfloat16))
+    outs = []
+    for layer in (strided, plain):
+        y = layer(*args)
+        y.float().square().mean().backward()
+        outs.append([y] + [p.grad for p in layer.parameters()])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)

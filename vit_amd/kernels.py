@@ -540,6 +540,10 @@ def can_qk_norm_rope(dtype: torch.dtype, Dh: int) -> bool:
     return Dh % 8 == 0 and 8 <= Dh <= 128 and dtype in (torch.float32, torch.bfloat16)
 
 
+def _cs(ts: tuple) -> tuple:
+    return tuple(None if t is None else _c(t) for t in ts)
+
+
 def _qk_section(sec: L.VitkQkSection, x: Tensor, g: Optional[Tensor], y: Tensor, w: Tensor, b: Optional[Tensor],
                 dw: Optional[Tensor], db: Optional[Tensor], table: Optional[Tensor]) -> None:
     B, Ln, H, Dh = x.shape
@@ -580,6 +584,8 @@ def qk_norm_rope_fwd(q: Tensor, k: Optional[Tensor], q_out: Tensor, k_out: Optio
     has looked at shapes, types and layouts."""
     lib = L.load()
     L.require_gpu(q, k, q_out, k_out, *w, *b, *tables)
+    if not checked:
+        w, b = _cs(w), _cs(b)
     a = L.VitkQkNormRope()
     for i, (x, y) in enumerate(((q, q_out), (k, k_out))):
         if x is not None:
@@ -598,6 +604,7 @@ def qk_norm_rope_bwd(xs: tuple, gs: tuple, dxs: tuple, w: tuple, tables: tuple, 
     xs go (may be gs).  ``want`` = flags of (dw_q, db_q, dw_k, db_k); returns those four (or None) in the weights' dtype."""
     lib = L.load()
     L.require_gpu(*xs, *gs, *dxs, *w, *tables)
+    w = _cs(w)
     a = L.VitkQkNormRope()
     outs = [torch.empty_like(w[i // 2]) if f and xs[i // 2] is not None else None for i, f in enumerate(want)]
     for i in range(2):
