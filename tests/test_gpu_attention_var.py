@@ -888,3 +888,18 @@ def test_wide_heads_of_few_queries_and_two_waves_that_share_keys(B, Lq, Lk, H, D
     want["dtable"] = bucket_sums(*want.pop("dS"), index, 11, dtype)
     for n, w in want.items():
         check(got[n], w, n)
+
+
+def test_dropout_is_refused_during_capture():
+    """Its seed comes from the host: a replay would drop the same probabilities every time."""
+    q, k, v, _ = make(1, 40, 64, 1, 64, torch.bfloat16, 3, packed=True)
+    with pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            attention(q, k, v, dropout=0.5, training=True)
+    want = attention(q, k, v)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = attention(q, k, v, dropout=0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)

@@ -115,6 +115,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, bias_table: Optional[Tensor] =
     ``kv_lengths`` [B] (int32 or int64) counts the keys each sample has; keys behind them are padding: never read, zero
     gradient.  A query that no key is left for gives zeros.  ``scale`` defaults to Dh ** -0.5.
     Any strides with contiguous heads, head_dim <= 128, float32 or bfloat16; Lq and Lk are independent, one query included.
+    Head sizes that are no multiple of 8 run portable kernels, which take about a hundred times as long.  A bias needs memory
+    while a call runs, per pair and head: 2 bytes in bfloat16, 4 in its backward, and 4 more (for each share of the samples, where
+    their number is split to fill the chip) where the table's gradient is wanted, which float32 needs alone.
     Differentiable once in q, k, v and the table.  Tensors belong to the current device and stream."""
     _heads("q", q)
     _heads("k", k, q)

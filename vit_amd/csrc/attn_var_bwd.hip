@@ -5,10 +5,11 @@
 //   var_dbias_k pairs stationary (128 x 64 per workgroup), samples stream: dS summed over the samples in the accumulators, in
 //               32 bits, one 32-bit value per pair and head out; no atomics, so the sums do not depend on the order of anything
 //   var_few_bwd_k up to 32 queries: keys stationary, everything in one pass over K and V (below)
-// Times: ViT-B/14, 64 samples x 12 heads of 64, 272 x 272 with bias: dQ 64, dK/dV 72, bias gradient 61 us; ViT-g/14 at 1024 px, 4 x
-// 16 heads of 88, 5329 x 5329 with bias: 1.20, 1.46, 2.08 ms; 300 queries over up to 4096 states, 16 x 16 heads of 64: dQ 129,
-// dK/dV 184 us.  All are bound by the vector units beside the matrix units (dK/dV: 8 vector instructions and an exponential
-// for the 4 products of a pair), the bias gradient also by LDS reads and by its steps' latency.
+// Times: ViT-B/14, 64 samples x 12 heads of 64, 272 x 272 with bias: dQ 62, dK/dV 71, bias gradient 60 us; ViT-g/14 at 1024 px, 4 x
+// 16 heads of 88, 5329 x 5329 with bias: 1.25, 1.51, 2.10 ms; 300 queries over up to 4096 states, 16 x 16 heads of 64: dQ and
+// dK/dV 280 us together (126 and 181 with a profiler attached).  All are bound by the latency of a wave's chain through a tile,
+// which two or three waves per SIMD do not cover: matrix units 15-45 % busy (bias gradient 11-15), vector instructions issued in
+// 29-44 % of the cycles (18-23), waves waiting 31-47 % of their time, LDS bank conflicts next to none.
 // P is formed again from the row statistics of the forward pass; delta = rowsum(dO O) comes from var_dq_k / var_few_bwd_k.
 #include "attn_var.h"
 
@@ -559,10 +560,11 @@ __global__ __launch_bounds__(256, (DHP <= 96 ? 2 : 1)) void var_dbias_k(VarP p) 
 }
 
 // ---- up to 32 queries -------------------------------------------------------------------------------------------------------------
-// Bound by K, V in and dK, dV out (256 samples x 12 heads of 64, one query over up to 272 states: 91 us for 320 MB, 3.5 TB/s), so
-// K and V are read once: a wave holds 32 keys, forms S' and dP both ways (the query rows'
-// fragments serve as either operand), and writes dK, dV of its keys; dQ^T += K^T dS^T of the workgroup's 128 keys goes to
-// p.part and is summed over the key blocks, in their order, by var_few_sum_k.
+// Bound by K, V in and dK, dV out (256 samples x 12 heads of 64, one query over up to 272 states: 90 us for 320 MB, 3.5 TB/s:
+// nothing is on its way while a workgroup computes, vector instructions are issued in 43 % of the cycles), so K and V are read
+// once: a wave holds 32 keys, forms S' and dP both ways (the query rows' fragments serve as either operand), and writes dK, dV of
+// its keys; dQ^T += K^T dS^T of the workgroup's 128 keys goes to p.part and is summed over the key blocks, in their order, by
+// var_few_sum_k.
 template <int DHP, int STRIDE>
 __device__ __forceinline__ void frags_to_lds(const bf16x8 (&f)[DHP / 16], char* s, int lane) {
   const int row = lane & 31, hi = lane >> 5;

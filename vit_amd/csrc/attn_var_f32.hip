@@ -6,11 +6,12 @@
 //     LDS read serves four products;
 //   * the contraction over accumulator rows takes register r of both halves, rows acc_row(r) and acc_row(r) + 4: P and dS are
 //     the next product's operand as they stand.
-// An element of S costs 4 Dh operations at 256 per cycle and CU, 16 times the bf16 rate, so everything else (exponentials,
-// bias gathered from table and index where it is used, dropout) stays under the matrix units' time.  Streamed tiles hold 32
-// rows, in LDS, the next one on its way in registers.  ViT-S/16, 8 samples x 6 heads of 64, 197 x 197 with bias: forward 25 + 7,
-// dQ 32, dK/dV 33, bias gradient 20 us (one wave per 32 rows without sharing: dQ 58, dK/dV 68); 4 x 12 heads, 77 queries over up
-// to 577 states: 18 + 6, 28, 25 us (dQ 84 unshared).
+// An element of S costs 4 Dh operations at 256 per cycle and CU, a sixteenth of the bf16 rate, so everything else (exponentials,
+// bias gathered from table and index where it is used, dropout) has room beside the matrix units.  Streamed tiles hold 32
+// rows, in LDS, the next one on its way in registers.  ViT-S/16, 8 samples x 6 heads of 64, 197 x 197 with bias: forward 26 + 8,
+// dQ 30, dK/dV 33, bias gradient 20 us (one wave per 32 rows without sharing: dQ 58, dK/dV 68); 4 x 12 heads, 77 queries over up
+// to 577 states: 20 + 6, 27, 28 us (dQ 84 unshared).  At these sizes it is latency that counts, of the gathers, loads and products
+// of one tile after the other: matrix units 10-16 % busy, vector instructions issued in 3-9 % of the cycles, 0.4-0.9 waves per SIMD.
 #include "attn_var.h"
 
 #define MFMA32 __builtin_amdgcn_mfma_f32_32x32x2f32

@@ -5,10 +5,12 @@
 //   on the accumulator rows and the query on the lane, so the running maximum is a register reduction and the probabilities
 //   are the next product's operand as they stand.  The bias enters as the INITIAL accumulator of the score product: it costs
 //   an unpacking and a multiplication by 1 / scale per element and nothing else.
-//   Bound by the vector units beside the matrix units (about 9 vector instructions and one exponential per score).  ViT-B/14,
-//   64 samples x 12 heads of 64, 272 x 272 with bias: 51 us; ViT-g/14 at 1024 px, 4 samples x 16 heads of 88, 5329 x 5329 with
-//   bias: 1.01 ms, 634 TFLOP/s (691 as the heads are padded to 96); 300 queries over up to 4096 states, 16 x 16 heads of
-//   64: 107 us.
+//   Bound by the latency of a wave's chain through a tile (products, maximum, exponentials, conversion, products), which two or
+//   three waves per SIMD do not cover: matrix units 15-35 % busy, vector instructions issued in 32-42 % of the cycles, waves
+//   waiting 37-52 % of their time, no LDS bank conflicts (counters of the three cases that follow).  ViT-B/14, 64 samples x 12
+//   heads of 64, 272 x 272 with bias: 50 us; ViT-g/14 at 1024 px, 4 samples x 16 heads of 88, 5329 x 5329 with bias: 1.03 ms,
+//   620 TFLOP/s (676 as the heads are padded to 96); 300 queries over up to 4096 states, 16 x 16 heads of 64: 90 us.  One
+//   sample, 100 queries over 4097 states, 12 heads of 64: 16 shares of the keys, 20 us with their joining.
 #include "attn_var.h"
 
 // ---- bias in accumulator order ----------------------------------------------------------------------------------------
@@ -288,7 +290,7 @@ __global__ __launch_bounds__(NW * 64, (var_fwd_occ<DHP, NW, BIAS, DROP>())) void
 // a share of the keys of one head, with 32-key tiles in LDS of its own that it asks for NB - 1 steps ahead: no barrier.  The
 // HW heads of a workgroup are neighbours, and so are the workgroups of a sample's key range on an XCD: heads whose rows are
 // no multiple of a cache line share lines, which are then fetched once.  One query over up to 5329 states, 16 samples x 16 heads
-// of 88: 68 us for the 300 MB of K and V it needs (4.4 TB/s) and 5 us to join 16 shares, where workgroups of one head with
+// of 88: 66 us for the 300 MB of K and V it needs (4.5 TB/s) and 5 us to join 16 shares, where workgroups of one head with
 // common tiles took 104 + 5; 256 samples x 12 heads of 64 over up to 272 states: 25 us (36 before).
 template <int DHP> constexpr int few_buffers() { return DHP == 96 ? 3 : 2; }
 template <int DHP, int HW, bool BIAS, bool SPLIT>

@@ -10,9 +10,15 @@
 // loads and stores are one contiguous run where the rows are; the other half of the head that the rotation needs and the
 // row sums go through LDS.  Positions come before samples in a wave's run: their sines and cosines stay in registers.
 // Bound by HBM: x in, y out (forward), g and x in, dx out (backward; its vector instructions come close).  Measured in bf16:
-// ViT-H/14 at 224 px, 64 samples, 16 + 16 heads of 80: forward 36 us (4.7 TB/s), backward 58 us (4.3 TB/s); ViT-g/14 at 1024 px, 8
-// samples, heads of 88: 102 us (4.7 TB/s) and 179 us (4.0 TB/s), where a copy reaches 5.1 TB/s; the weight gradients' partial
+// ViT-H/14 at 224 px, 64 samples, 16 + 16 heads of 80: forward 35 us (4.7 TB/s), backward 58 us (4.3 TB/s); ViT-g/14 at 1024 px, 8
+// samples, heads of 88: 102 us (4.7 TB/s) and 180 us (4.0 TB/s), where a copy reaches 5.1 TB/s; the weight gradients' partial
 // sums take 4-5 us more.  One token of 12 + 12 heads takes 4 us, a launch.
+// Instances: head sizes 32, 64, 96, 128 and those of the larger ViTs (80, 88) know their lanes per row when compiled, which folds
+// the row sums; the others, and float32 rows with bf16 weights, take the same code with the count in a register.  64 samples x
+// 257 tokens, 16 + 16 heads, forward / training, instance against general form: heads of 32 in bf16 20 / 42 against 22 / 48 us,
+// 64: 29 / 64 against 32 / 72, 80: 37 / 93 against 39 / 101, 88: 40 / 113 against 42 / 120, 96: 43 / 120 against 44 / 126, 128: 58 / 139 against 62 / 152; float32
+// 64: 60 / 136 against 69 / 149, 96: no difference, 128: 124 / 272 against 151 / 297.  Sizes between them stay near their
+// neighbours' bandwidth without an instance (72: 36 / 88, 104: 49 / 143, 120: 60 / 155 us).
 #include "common.h"
 
 struct QkSec {        // one section: q or k
